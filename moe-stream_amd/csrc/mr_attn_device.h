@@ -1,0 +1,73 @@
+// mr_attn_device.h -- device helpers of the attention-side kernels.
+#pragma once
+
+#include "mr_attn.h"
+#include "mr_device.h"
+
+namespace mr {
+
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// Two f32 to adjacent f16 (bf16), rounded to nearest even.
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+  const f16x2 v = {(_Float16)a, (_Float16)b};
+  return __builtin_bit_cast(uint32_t, v);
+}
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  const bf16x2 v = {(__bf16)a, (__bf16)b};
+  return __builtin_bit_cast(uint32_t, v);
+}
+__device__ __forceinline__ f32x2 unpack_f16(uint32_t w) {
+  const f16x2 v = __builtin_bit_cast(f16x2, w);
+  return f32x2{(float)v.x, (float)v.y};
+}
+__device__ __forceinline__ f32x2 unpack_bf16(uint32_t w) { return f32x2{bits_f32(w << 16), bits_f32(w & 0xFFFF0000u)}; }
+
+// Four adjacent elements at element offset i of an array of type `dtype` (the same for all lanes).
+__device__ __forceinline__ f32x4 load4(const void* p, uint32_t dtype, uint64_t i) {
+  if (dtype == MR_F32) return *reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + i);
+  const u32x2 w = *reinterpret_cast<const u32x2*>(static_cast<const uint16_t*>(p) + i);
+  const f32x2 a = dtype == MR_F16 ? unpack_f16(w.x) : unpack_bf16(w.x);
+  const f32x2 b = dtype == MR_F16 ? unpack_f16(w.y) : unpack_bf16(w.y);
+  return f32x4{a.x, a.y, b.x, b.y};
+}
+__device__ __forceinline__ void store4(void* p, uint32_t dtype, uint64_t i, f32x4 v) {
+  if (dtype == MR_F32) {
+    *reinterpret_cast<f32x4*>(static_cast<float*>(p) + i) = v;
+    return;
+  }
+  const u32x2 w = dtype == MR_F16 ? u32x2{pack_f16(v.x, v.y), pack_f16(v.z, v.w)}
+                                  : u32x2{pack_bf16(v.x, v.y), pack_bf16(v.z, v.w)};
+  *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p) + i) = w;
+}
+
+// Value of a doubled e2m1 code (0..15), halved on use: {0,1,2,3,4,6,8,12}.
+__device__ __forceinline__ float fp4_value(uint32_t c) {
+  const uint32_t m = c & 7u;
+  const float a = m < 5u ? 0.5f * (float)m : (m == 5u ? 3.f : m == 6u ? 4.f : 6.f);
+  return c & 8u ? -a : a;
+}
+// 2^e of a scale byte.
+template <int FMT>
+__device__ __forceinline__ float scale_value(uint32_t b) {
+  return FMT == MR_KV_MXFP4 ? bits_f32(b << 23) : h2f(b << 8);
+}
+
+// Element d of token s of a chunk.
+template <int FMT, int D>
+__device__ __forceinline__ float kv_value(const uint8_t* chunk, bool key, int s, int d) {
+  using L = KvLayout<FMT, D>;
+  const uint8_t* p = chunk + (key ? L::k_off(s, d) : L::v_off(s, d));
+  if (FMT == MR_KV_F16) return h2f(*reinterpret_cast<const uint16_t*>(p));
+  const float sc = scale_value<FMT>(chunk[key ? L::ks_off(s, d >> 5) : L::vs_off(s, d >> 5)]);
+  if (FMT == MR_KV_MXINT8) return sc * (float)*reinterpret_cast<const int8_t*>(p);
+  const bool high = key ? d & 1 : d & 16;
+  return sc * fp4_value(high ? *p >> 4 : *p & 15u);
+}
+
+}  // namespace mr

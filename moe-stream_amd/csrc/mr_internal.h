@@ -107,6 +107,10 @@ struct mr_ctx {
   // mr_ctx_create; nullptr with static_err set when the lookup failed.
   void* static_scratch = nullptr;
   hipError_t static_err = hipSuccess;
+  // Error word of the attention-side calls (moe_rocm_attn.h), allocated with the context; read by
+  // mr_sync once such a call was made.
+  uint32_t* attn_err = nullptr;
+  bool attn_used = false;
   hipEvent_t ev0 = nullptr, ev1 = nullptr;
   bool capturing = false;
   mr::Prof prof;

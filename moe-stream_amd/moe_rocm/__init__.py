@@ -123,11 +123,16 @@ _SIGS = {
     "mr_profile_reset": (C.c_int, [_vp]),
 }
 
-for _name, (_res, _args) in _SIGS.items():
-    _fn = getattr(_lib, _name)
-    _fn.restype = _res
-    _fn.argtypes = _args
 
+
+def _register(sigs: dict) -> None:
+    for name, (res, args) in sigs.items():
+        fn = getattr(_lib, name)
+        fn.restype, fn.argtypes = res, args
+    _SIGS.update(sigs)
+
+
+_register(dict(_SIGS))
 lib = _lib
 
 
@@ -185,6 +190,10 @@ class Context:
 
     def set_option(self, option: int, value: int) -> None:
         self.check(_lib.mr_ctx_set_option(self.h, option, value))
+
+    def set_stream(self, stream: int) -> None:
+        """Enqueue the context's work on this hipStream_t (an address; 0: the default stream) from now on."""
+        self.check(_lib.mr_ctx_set_stream(self.h, stream))
 
     # -- memory ---------------------------------------------------------------
     def alloc(self, nbytes: int) -> "DeviceBuffer":
@@ -499,3 +508,8 @@ def matrix_bytes(ggml_type: int, rows: int, cols: int) -> int:
 
 def exported_symbols() -> list[str]:
     return sorted(_SIGS)
+
+
+from .attn import (BF16, F16, F32, KV_F16, KV_MXFP4, KV_MXINT8, ROPE_HALF, ROPE_INTERLEAVED,  # noqa: E402,F401
+                   ROPE_LINEAR, ROPE_PLAIN, ROPE_YARN, ROPE_YARN_EXACT, Heads, KvCache, Rope, attn_prefill,
+                   qk_norm_rope)

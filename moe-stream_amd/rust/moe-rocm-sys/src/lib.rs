@@ -10,6 +10,9 @@
 
 use core::ffi::{c_char, c_int, c_void};
 
+/// include/moe_rocm_attn.h
+pub mod attn;
+
 // ---- status codes
 pub const MR_OK: c_int = 0;
 pub const MR_E_INVAL: c_int = -1;
