@@ -1,65 +1,249 @@
 // mr_attn_prefill.hip -- causal attention over packed prompts.
+//
+// One pass over the keys with the running maximum m and sum l of each row's softmax:
+//   S = K Q^T (keys down, rows across), p = 2^(S c - m), O = 2^(m_old - m) O + V^T p,  c = scale log2 e.
+// Both products are 32x32x16 matrix instructions. With the keys down, a lane holds the scores of one
+// row, 16 of each 32 keys, so that maximum, sum and p need one exchange between two lanes; and p is
+// already where the second product wants its right operand, if that product counts its keys in the
+// order the first one left them in (16 c + 4 h + 0..3, then 16 c + 8 + 4 h + 0..3 for lane half h).
+// V^T in that order is what the transposing LDS read returns: four adjacent keys of one column.
 #include "mr_attn_device.h"
 
 namespace mr {
 
 namespace {
 
-// One wave for a query row and head. blockIdx.x counts the rows; the row's sequence is found in cu_q.
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kRows = 128;  // query rows of a workgroup: 4 waves of 32
+constexpr int kKeys = 64;   // keys of a step
+
+template <bool BF>
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (BF)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+template <bool BF>
+__device__ __forceinline__ uint32_t pack16(float a, float b) {
+  return BF ? pack_bf16(a, b) : pack_f16(a, b);
+}
+
+// Where 16-byte piece `c` of a tile's row lies in LDS, in pieces of the row. Rows are a multiple of the
+// 64 banks or half of it: without the exclusive or, the 8 rows of a read's phase would share banks.
 template <int D>
-__global__ __launch_bounds__(64) void k_attn_prefill(Heads q, Heads k, Heads v, Heads out, int nq, int nk, int n_seqs,
-                                                     const int32_t* __restrict__ cu_q, const int32_t* __restrict__ cu_k,
-                                                     AttnOpts o, uint32_t* err) {
-  __shared__ float qs[D], ps[64];
-  const int row = blockIdx.x, h = blockIdx.y, lane = threadIdx.x, hk = h / (q.n / k.n);
-  auto clamp = [](int x, int hi) { return min(max(x, 0), hi); };
-  int seq = -1;
-  for (int s = 0; s < n_seqs && seq < 0; ++s) {
-    if (cu_q[s] != clamp(cu_q[s], nq) || cu_q[s + 1] != clamp(cu_q[s + 1], nq) || cu_q[s + 1] < cu_q[s] ||
-        cu_k[s] != clamp(cu_k[s], nk) || cu_k[s + 1] != clamp(cu_k[s + 1], nk) || cu_k[s + 1] < cu_k[s])
-      if (lane == 0) atomicOr(err, kErrOffset);
-    if (row >= clamp(cu_q[s], nq) && row < clamp(cu_q[s + 1], nq)) seq = s;
-  }
-  if (seq < 0) return;
-  const int q1 = clamp(cu_q[seq + 1], nq), k0 = clamp(cu_k[seq], nk), k1 = clamp(cu_k[seq + 1], nk);
-  for (int d = lane * 4; d < D; d += 256) {
-    const f32x4 x = load4(q.p, q.dtype, (uint64_t)row * q.ts + (uint64_t)h * q.hs + d);
-    qs[d] = x.x, qs[d + 1] = x.y, qs[d + 2] = x.z, qs[d + 3] = x.w;
-  }
-  __syncthreads();
-  float m = o.sinks ? o.sinks[h] : -INFINITY, l = o.sinks ? 1.f : 0.f, acc[D / 64] = {};
-  const int64_t last = (int64_t)k1 - (q1 - row), first = max((int64_t)k0, o.window ? last + 1 - (int64_t)o.window : 0);
-  for (int64_t j0 = first; j0 <= last; j0 += 64) {
-    const int64_t key = j0 + lane;
-    float s = -INFINITY;
-    if (key <= last) {
-      s = 0.f;
-      for (int d = 0; d < D; d += 4) {
-        const f32x4 x = load4(k.p, k.dtype, (uint64_t)key * k.ts + (uint64_t)hk * k.hs + d);
-        s += x.x * qs[d] + x.y * qs[d + 1] + x.z * qs[d + 2] + x.w * qs[d + 3];
-      }
-      s *= o.scale;
+__device__ __forceinline__ int k_piece(int row, int c) {
+  return D == 64 ? c ^ ((row >> 1) & 7) : c ^ (row & 15);
+}
+// The transposing read takes 4 adjacent rows and 64 adjacent bytes of each in a phase.
+template <int D>
+__device__ __forceinline__ int v_piece(int row, int c) {
+  return D == 64 ? c ^ (((row >> 1) & 1) * 4) : c ^ ((row & 3) * 4);
+}
+
+// 16 bytes a lane from global memory straight to LDS, lane i's to dst + 16 i (dst: the same for all lanes).
+// Not the compiler's builtin: after that it waits for all of them before each LDS read that it cannot tell
+// apart, here for the next step's tile in the middle of this one. The caller waits (vmcnt) and synchronises.
+__device__ __forceinline__ void load_lds16(const void* src, const void* dst) {
+  const uint32_t to = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)dst);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(src) : "memory", "m0");
+}
+
+struct PrefillArgs {
+  Heads q, k, v, out;
+  int nq, nk, n_seqs, n_tiles;
+  const int32_t *cu_q, *cu_k;
+  AttnOpts o;
+  uint32_t* err;
+};
+
+// The sequence and first row of row tile `tile`: sequences in turn, each in whole tiles. Offsets are
+// clamped into the rows; `report` also looks at all of them. Returns false behind the last tile.
+struct Place {
+  int q0, q1, k0, k1;  // the sequence's rows
+  int row;             // the tile's first row
+};
+__device__ __forceinline__ bool find_tile(const PrefillArgs& a, int tile, bool report, Place& p) {
+  const int lane = threadIdx.x & 63;
+  auto in = [](int x, int hi) { return min(max(x, 0), hi); };
+  int before = 0, found = -1, found_before = 0;
+  for (int s0 = 0; s0 < a.n_seqs; s0 += 64) {
+    const int s = s0 + lane;
+    int n = 0;
+    bool bad = false;
+    if (s < a.n_seqs) {
+      const int x = a.cu_q[s], y = a.cu_q[s + 1], kx = a.cu_k[s], ky = a.cu_k[s + 1];
+      bad = x < 0 || y < x || y > a.nq || kx < 0 || ky < kx || ky > a.nk;
+      n = max(0, in(y, a.nq) - in(x, a.nq));
+      n = (n + kRows - 1) / kRows;
     }
-    const float top = fmaxf(m, wave_max(s));
-    const float p = s == -INFINITY ? 0.f : expf(s - top), f = m == -INFINITY ? 0.f : expf(m - top);
-    l = l * f + wave_sum(p), m = top;
-    ps[lane] = p;
-    __syncthreads();
-    for (int i = 0; i < D / 64; ++i) {
-      acc[i] *= f;
-      for (int j = 0; j < 64 && j0 + j <= last; ++j) {
-        const uint16_t w = static_cast<const uint16_t*>(v.p)[(uint64_t)(j0 + j) * v.ts + (uint64_t)hk * v.hs + lane + 64 * i];
-        acc[i] += ps[j] * (v.dtype == MR_F16 ? h2f(w) : bits_f32((uint32_t)w << 16));
-      }
+    if (report && __any(bad) && lane == 0) atomicOr(a.err, kErrOffset);
+    int sum = n;
+    for (int o = 1; o < 64; o *= 2) {
+      const int t = __shfl_up(sum, o, kWave);
+      if (lane >= o) sum += t;
     }
+    const uint64_t past = __ballot(before + sum > tile);
+    if (past && found < 0) {
+      const int l = __ffsll((unsigned long long)past) - 1;
+      found = s0 + l;
+      found_before = before + __shfl(sum - n, l, kWave);
+      if (!report) break;
+    }
+    before += __shfl(sum, 63, kWave);
+  }
+  if (found < 0) return false;
+  p.q0 = in(a.cu_q[found], a.nq), p.q1 = in(a.cu_q[found + 1], a.nq);
+  p.k0 = in(a.cu_k[found], a.nk), p.k1 = max(p.k0, in(a.cu_k[found + 1], a.nk));
+  const int tiles = (p.q1 - p.q0 + kRows - 1) / kRows;
+  p.row = p.q0 + (tiles - 1 - (tile - found_before)) * kRows;  // the longest rows first
+  return true;
+}
+
+template <int D, bool BF>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_prefill(PrefillArgs a) {
+  constexpr int P = D / 8, ND = D / 32;  // 16-byte pieces of a row; 32-wide tiles of a head
+  constexpr int kTile = kKeys * D;       // elements of a key or value tile
+  __shared__ __attribute__((aligned(16))) uint16_t lds[4 * kTile];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 31, half = lane >> 5;
+
+  // Workgroups go to the 8 XCDs in turn. Each XCD gets a contiguous share of the (head, tile) pairs, so that
+  // the query heads that share keys find them in one L2.
+  const int units = a.n_tiles * (int)a.q.n, per = (units + 7) / 8;
+  const int unit = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= per || unit >= units) return;
+  const int h = unit / a.n_tiles, hk = h / (int)(a.q.n / a.k.n);
+  Place pl;
+  if (!find_tile(a, unit % a.n_tiles, unit == 0, pl)) return;
+
+  // keys [first, last] of the tile's rows; a row r sees those up to r + diff, from r + diff - window + 1 on
+  const int diff = pl.k1 - pl.q1;
+  const int row = pl.row + wave * 32 + n;  // this lane's query row
+  const bool live = row < pl.q1;
+  const int last_row = min(pl.row + kRows, pl.q1) - 1;
+  const int last = last_row + diff;  // < k1
+  int first = pl.k0;
+  if (a.o.window) first = (int)max((int64_t)first, (int64_t)pl.row + diff + 1 - (int64_t)a.o.window);
+  const int see_last = row + diff;
+  const int64_t see_first = a.o.window ? max((int64_t)pl.k0, (int64_t)see_last + 1 - (int64_t)a.o.window) : pl.k0;
+
+  const float c = fabsf(a.o.scale) * 1.44269504088896340736f;
+  u32x4 qf[D / 16];
+  {
+    const uint16_t* qp = static_cast<const uint16_t*>(a.q.p) + (uint64_t)min(row, pl.q1 - 1) * a.q.ts + (uint64_t)h * a.q.hs;
+    const uint32_t flip = a.o.scale < 0.f ? 0x80008000u : 0u;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) qf[i] = *reinterpret_cast<const u32x4*>(qp + 16 * i + 8 * half) ^ flip;
+  }
+
+  const uint16_t* kp = static_cast<const uint16_t*>(a.k.p) + (uint64_t)hk * a.k.hs;
+  const uint16_t* vp = static_cast<const uint16_t*>(a.v.p) + (uint64_t)hk * a.v.hs;
+  // Copies the 64 keys from k0 on into buffer b; rows behind the last key repeat it (they are masked).
+  auto fetch = [&](int k0, int b) {
+    uint16_t* kd = lds + b * 2 * kTile;
+    uint16_t* vd = kd + kTile;
+#pragma unroll
+    for (int i = 0; i < kTile / 8 / 256; ++i) {
+      const int piece = (i * 4 + wave) * 64 + lane, r = piece / P, cp = piece % P;
+      const uint64_t key = (uint64_t)min(k0 + r, last);
+      const uint16_t* ks = kp + key * a.k.ts + 8 * k_piece<D>(r, cp);
+      const uint16_t* vs = vp + key * a.v.ts + 8 * v_piece<D>(r, cp);
+      load_lds16(ks, kd + (i * 4 + wave) * 512);
+      load_lds16(vs, vd + (i * 4 + wave) * 512);
+    }
+  };
+
+  f32x16 acc[ND];
+#pragma unroll
+  for (int t = 0; t < ND; ++t) acc[t] = f32x16{};
+  float m = -INFINITY, l = 0.f;
+  if (a.o.sinks) {
+    m = a.o.sinks[h] * 1.44269504088896340736f;
+    l = half == 0 && m != -INFINITY ? 1.f : 0.f;  // the two halves of a row are added at the end
+  }
+
+  int b = 0;
+  if (first <= last) fetch(first, 0);
+  for (int k0 = first; k0 <= last; k0 += kKeys, b ^= 1) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
+    if (k0 + kKeys <= last) fetch(k0 + kKeys, b ^ 1);
+    const uint16_t* kt = lds + b * 2 * kTile;
+    const uint16_t* vt = kt + kTile;
+
+    f32x16 s[2] = {};
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        const int r = 32 * t + n;
+        const u32x4 kf = *reinterpret_cast<const u32x4*>(kt + r * D + 8 * k_piece<D>(r, 2 * i + half));
+        s[t] = mfma32<BF>(kf, qf[i], s[t]);
+      }
+    // whether every row of the wave sees every key of the step
+    const bool whole = k0 + kKeys - 1 <= pl.row + wave * 32 + diff && k0 >= see_first;
+    const bool masked = !__all(whole);
+    if (masked) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int key = k0 + 32 * t + 8 * (i >> 2) + 4 * half + (i & 3);
+          if (key > see_last || key < see_first) s[t][i] = -INFINITY;
+        }
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int i = 1; i < 32; ++i) top = fmaxf(top, s[i >> 4][i & 15]);
+    top = max_xor32(top) * c;
+    const float m1 = fmaxf(m, top);
+    if (__any(m1 > m)) {
+      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m1);
+      l *= f;
+#pragma unroll
+      for (int t = 0; t < ND; ++t) acc[t] *= f;
+      m = m1;
+    }
+    const float base = m == -INFINITY ? 0.f : m;
+    u32x4 pf[4];
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+      const float p0 = __builtin_amdgcn_exp2f(fmaf(s[i >> 4][i & 15], c, -base));
+      const float p1 = __builtin_amdgcn_exp2f(fmaf(s[i >> 4][(i & 15) + 1], c, -base));
+      l += p0 + p1;
+      pf[i >> 3][(i >> 1) & 3] = pack16<BF>(p0, p1);
+    }
+    // V^T: lane 16 g + i of a read takes row (i >> 2), elements 4 (i & 3).. and gets column i of four rows
+#pragma unroll
+    for (int t = 0; t < ND; ++t)
+#pragma unroll
+      for (int cc = 0; cc < 4; ++cc) {
+        u32x4 vf;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int r = 16 * cc + 8 * j + 4 * half + ((lane & 15) >> 2), e = 32 * t + (lane & 16) + 4 * (lane & 3);
+          const uint16_t* src = vt + r * D + 8 * v_piece<D>(r, e >> 3) + (e & 7);
+          const i16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)src);
+          const u32x2 w2 = __builtin_bit_cast(u32x2, w);
+          vf[2 * j] = w2.x, vf[2 * j + 1] = w2.y;
+        }
+        acc[t] = mfma32<BF>(vf, pf[cc], acc[t]);
+      }
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  uint16_t* dst = static_cast<uint16_t*>(out.p) + (uint64_t)row * out.ts + (uint64_t)h * out.hs;
-  for (int i = 0; i < D / 64; ++i) {
-    const float x = acc[i] * inv;
-    dst[lane + 64 * i] = (uint16_t)(out.dtype == MR_F16 ? pack_f16(x, 0.f) : pack_bf16(x, 0.f));
-  }
+
+  l = add_xor32(l);
+  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : NAN;
+  if (!live) return;
+  uint16_t* dst = static_cast<uint16_t*>(a.out.p) + (uint64_t)row * a.out.ts + (uint64_t)h * a.out.hs;
+#pragma unroll
+  for (int t = 0; t < ND; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const u32x2 w = {pack16<BF>(acc[t][i] * inv, acc[t][i + 1] * inv), pack16<BF>(acc[t][i + 2] * inv, acc[t][i + 3] * inv)};
+      *reinterpret_cast<u32x2*>(dst + 32 * t + 8 * (i >> 2) + 4 * half) = w;
+    }
 }
 
 }  // namespace
@@ -68,10 +252,16 @@ hipError_t launch_attn_prefill(const Launch& K, uint32_t D, const Heads& q, uint
                                uint32_t nk, uint32_t n_seqs, const int32_t* cu_q, const int32_t* cu_k, const AttnOpts& o,
                                const Heads& out, uint32_t* err) {
   ProfScope ps(K, "attn_prefill");
-  const dim3 g(nq, q.n);
-  if (D == 64) hipLaunchKernelGGL((k_attn_prefill<64>), g, dim3(64), 0, K.s, q, k, v, out, (int)nq, (int)nk, (int)n_seqs, cu_q, cu_k, o, err);
-  if (D == 128) hipLaunchKernelGGL((k_attn_prefill<128>), g, dim3(64), 0, K.s, q, k, v, out, (int)nq, (int)nk, (int)n_seqs, cu_q, cu_k, o, err);
-  if (D == 256) hipLaunchKernelGGL((k_attn_prefill<256>), g, dim3(64), 0, K.s, q, k, v, out, (int)nq, (int)nk, (int)n_seqs, cu_q, cu_k, o, err);
+  // every sequence ends with at most one tile that is not full
+  const uint64_t tiles = std::min<uint64_t>((uint64_t)nq / kRows + n_seqs, nq);
+  const uint64_t units = tiles * q.n;
+  if (units > 0x7FFFFF00ull) return hipErrorInvalidConfiguration;
+  PrefillArgs a{q, k, v, out, (int)nq, (int)nk, (int)n_seqs, (int)tiles, cu_q, cu_k, o, err};
+  const dim3 g((unsigned)((units + 7) / 8 * 8)), blk(256);
+  const bool bf = q.dtype == MR_BF16;
+  if (D == 64) hipLaunchKernelGGL((bf ? k_attn_prefill<64, true> : k_attn_prefill<64, false>), g, blk, 0, K.s, a);
+  if (D == 128) hipLaunchKernelGGL((bf ? k_attn_prefill<128, true> : k_attn_prefill<128, false>), g, blk, 0, K.s, a);
+  if (D == 256) hipLaunchKernelGGL((bf ? k_attn_prefill<256, true> : k_attn_prefill<256, false>), g, blk, 0, K.s, a);
   return hipGetLastError();
 }
 
