@@ -102,21 +102,19 @@ __device__ __forceinline__ bool find_tile(const PrefillArgs& a, int tile, bool r
   return true;
 }
 
-template <int D, bool BF>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_prefill(PrefillArgs a) {
+// One tile of rows and one head. p is 0 where a row does not see a key, but 0 * inf and 0 * NaN are NaN: a tile
+// that ends with such a sum returns false and is done over with `CAREFUL`, where values that are not finite
+// are taken out of the steps that some row sees in part, and added at the end to the rows that see them.
+template <int D, bool BF, bool CAREFUL>
+__device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds, int unit) {
   constexpr int P = D / 8, ND = D / 32;  // 16-byte pieces of a row; 32-wide tiles of a head
   constexpr int kTile = kKeys * D;       // elements of a key or value tile
-  __shared__ __attribute__((aligned(16))) uint16_t lds[4 * kTile];
+  constexpr uint32_t kTop = BF ? 0x7F80u : 0x7C00u;  // the exponent of infinities and NaN
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 31, half = lane >> 5;
 
-  // Workgroups go to the 8 XCDs in turn. Each XCD gets a contiguous share of the (head, tile) pairs, so that
-  // the query heads that share keys find them in one L2.
-  const int units = a.n_tiles * (int)a.q.n, per = (units + 7) / 8;
-  const int unit = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  if ((int)(blockIdx.x >> 3) >= per || unit >= units) return;
   const int h = unit / a.n_tiles, hk = h / (int)(a.q.n / a.k.n);
   Place pl;
-  if (!find_tile(a, unit % a.n_tiles, unit == 0, pl)) return;
+  if (!find_tile(a, unit % a.n_tiles, unit == 0 && !CAREFUL, pl)) return true;
 
   // keys [first, last] of the tile's rows; a row r sees those up to r + diff, from r + diff - window + 1 on
   const int diff = pl.k1 - pl.q1;
@@ -155,6 +153,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_prefill(PrefillA
     }
   };
 
+  // whether some row of the workgroup does not see some key of the step
+  const int64_t all_first = a.o.window ? (int64_t)last + 1 - (int64_t)a.o.window : pl.k0;
+  auto edge = [&](int k0) { return k0 < all_first || k0 + kKeys - 1 > pl.row + diff; };
+
   f32x16 acc[ND];
 #pragma unroll
   for (int t = 0; t < ND; ++t) acc[t] = f32x16{};
@@ -164,14 +166,18 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_prefill(PrefillA
     l = half == 0 && m != -INFINITY ? 1.f : 0.f;  // the two halves of a row are added at the end
   }
 
-  int b = 0;
   if (first <= last) fetch(first, 0);
-  for (int k0 = first; k0 <= last; k0 += kKeys, b ^= 1) {
+  for (int k0 = first, b = 0; k0 <= last; k0 += kKeys, b ^= 1) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (k0 + kKeys <= last) fetch(k0 + kKeys, b ^ 1);
     const uint16_t* kt = lds + b * 2 * kTile;
-    const uint16_t* vt = kt + kTile;
+    uint16_t* vt = lds + b * 2 * kTile + kTile;
+    if (CAREFUL && edge(k0)) {
+      for (int i = threadIdx.x; i < kTile; i += 256)
+        if ((vt[i] & kTop) == kTop) vt[i] = 0;
+      __syncthreads();
+    }
 
     f32x16 s[2] = {};
 #pragma unroll
@@ -216,34 +222,76 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_prefill(PrefillA
       pf[i >> 3][(i >> 1) & 3] = pack16<BF>(p0, p1);
     }
     // V^T: lane 16 g + i of a read takes row (i >> 2), elements 4 (i & 3).. and gets column i of four rows
+    auto values = [&](int t, int cc) {
+      u32x4 vf;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int r = 16 * cc + 8 * j + 4 * half + ((lane & 15) >> 2), e = 32 * t + (lane & 16) + 4 * (lane & 3);
+        const uint16_t* src = vt + r * D + 8 * v_piece<D>(r, e >> 3) + (e & 7);
+        const i16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)src);
+        const u32x2 w2 = __builtin_bit_cast(u32x2, w);
+        vf[2 * j] = w2.x, vf[2 * j + 1] = w2.y;
+      }
+      return vf;
+    };
 #pragma unroll
     for (int t = 0; t < ND; ++t)
 #pragma unroll
-      for (int cc = 0; cc < 4; ++cc) {
-        u32x4 vf;
+      for (int cc = 0; cc < 4; ++cc) acc[t] = mfma32<BF>(values(t, cc), pf[cc], acc[t]);
+  }
+
+  if (!CAREFUL) {
+    bool odd = false;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int r = 16 * cc + 8 * j + 4 * half + ((lane & 15) >> 2), e = 32 * t + (lane & 16) + 4 * (lane & 3);
-          const uint16_t* src = vt + r * D + 8 * v_piece<D>(r, e >> 3) + (e & 7);
-          const i16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)src);
-          const u32x2 w2 = __builtin_bit_cast(u32x2, w);
-          vf[2 * j] = w2.x, vf[2 * j + 1] = w2.y;
-        }
-        acc[t] = mfma32<BF>(vf, pf[cc], acc[t]);
-      }
+    for (int t = 0; t < ND; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) odd |= !(fabsf(acc[t][i]) < INFINITY);
+    if (__syncthreads_or(odd)) return false;
   }
 
   l = add_xor32(l);
   const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : NAN;
-  if (!live) return;
-  uint16_t* dst = static_cast<uint16_t*>(a.out.p) + (uint64_t)row * a.out.ts + (uint64_t)h * a.out.hs;
+  if (live) {
+    uint16_t* dst = static_cast<uint16_t*>(a.out.p) + (uint64_t)row * a.out.ts + (uint64_t)h * a.out.hs;
 #pragma unroll
-  for (int t = 0; t < ND; ++t)
+    for (int t = 0; t < ND; ++t)
 #pragma unroll
-    for (int i = 0; i < 16; i += 4) {
-      const u32x2 w = {pack16<BF>(acc[t][i] * inv, acc[t][i + 1] * inv), pack16<BF>(acc[t][i + 2] * inv, acc[t][i + 3] * inv)};
-      *reinterpret_cast<u32x2*>(dst + 32 * t + 8 * (i >> 2) + 4 * half) = w;
+      for (int i = 0; i < 16; i += 4) {
+        const u32x2 w = {pack16<BF>(acc[t][i] * inv, acc[t][i + 1] * inv), pack16<BF>(acc[t][i + 2] * inv, acc[t][i + 3] * inv)};
+        *reinterpret_cast<u32x2*>(dst + 32 * t + 8 * (i >> 2) + 4 * half) = w;
+      }
+  }
+  if (CAREFUL) {
+    __syncthreads();  // the rows are written
+    const int d = threadIdx.x % D;
+    for (int k0 = first; k0 <= last; k0 += kKeys) {
+      if (!edge(k0)) continue;
+      for (int key = k0; key < min(k0 + kKeys, last + 1); ++key) {
+        const uint16_t x = vp[(uint64_t)key * a.v.ts + d];
+        if ((x & kTop) != kTop) continue;
+        for (int r = pl.row + threadIdx.x / D; r <= last_row; r += 256 / D) {
+          if (key > r + diff || (a.o.window && key <= (int64_t)r + diff - (int64_t)a.o.window)) continue;
+          uint16_t* dst = static_cast<uint16_t*>(a.out.p) + (uint64_t)r * a.out.ts + (uint64_t)h * a.out.hs + d;
+          const float y = BF ? bits_f32((uint32_t)*dst << 16) + bits_f32((uint32_t)x << 16) : h2f(*dst) + h2f(x);
+          *dst = (uint16_t)pack16<BF>(y, 0.f);
+        }
+      }
     }
+  }
+  return true;
+}
+
+template <int D, bool BF>
+__global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void k_attn_prefill(PrefillArgs a) {
+  __shared__ __attribute__((aligned(16))) uint16_t lds[4 * kKeys * D];
+  // Workgroups go to the 8 XCDs in turn. Each XCD gets a contiguous share of the (head, tile) pairs, so that
+  // the query heads that share keys find them in one L2.
+  const int units = a.n_tiles * (int)a.q.n, per = (units + 7) / 8;
+  int unit = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= per || unit >= units) return;
+  if (attend_tile<D, BF, false>(a, lds, unit)) return;
+  asm volatile("" : "+s"(unit));  // nothing of the first pass stays in registers for the second
+  attend_tile<D, BF, true>(a, lds, unit);
 }
 
 }  // namespace

@@ -442,6 +442,42 @@ def test_prefill_scores_of_any_size(gpu_ctx):
         prompts(gpu_ctx, 64, 1, 2, dtype, [150], [150], window=20, sinks=[300.0, -300.0], spread=6.0, seed=4)
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_prefill_infinities_and_nan_where_rows_do_not_look(gpu_ctx, D, dtype):
+    """Keys and values that are not finite, at positions before some rows' windows and after others: rows that do not
+    see them are as without them, rows that do are NaN, or an infinity where only values of one sign are."""
+    dtype, n, window = TYPES[dtype], 200, 50
+    rng = np.random.default_rng(D)
+    q, k, v = (R.rounded(rng.normal(size=(n, 1, D)), dtype) for _ in range(3))
+    clean_k, clean_v = k.copy(), v.copy()
+    k[150, 0, 3] = np.nan
+    v[20, 0, 5], v[20, 0, 7], v[70, 0, 1], v[71, 0, 1], v[199, 0, :] = np.inf, -np.inf, np.inf, -np.inf, np.nan
+    v[45, 0, D - 1] = np.nan
+    dq, dk, dv, out = (R.Rows(gpu_ctx, a, dtype, n, 1, D) for a in (q, k, v, None))
+    cu = R.i32(gpu_ctx, [0, n])
+    M.attn_prefill(gpu_ctx, D, dq.heads, dk.heads, dv.heads, n, n, 1, cu, cu, out.heads, window=window)
+    gpu_ctx.sync()
+    got = out.get()[:, 0]
+    for r in range(n):
+        sees = lambda j: max(0, r - window + 1) <= j <= r  # noqa: E731
+        y, av, ss, cnt = R.attend(q[r, 0], clean_k[:, 0], clean_v[:, 0], D ** -0.5, max(0, r - window + 1), r)
+        y = y.copy()
+        if sees(20):
+            y[5], y[7] = np.inf, -np.inf
+        y[1] = np.nan if sees(70) and sees(71) else np.inf if sees(70) else -np.inf if sees(71) else y[1]
+        y[D - 1] = np.nan if sees(45) else y[D - 1]
+        if sees(150) or sees(199):
+            y[:] = np.nan
+        tol = R.attention_bound(np.where(np.isfinite(y), y, 0), av, ss, cnt, D, dtype, R.HALF[dtype])
+        fine = np.isfinite(y)
+        assert (np.isnan(got[r]) == np.isnan(y)).all(), (r, got[r], y)
+        assert (got[r][np.isinf(y)] == y[np.isinf(y)]).all(), r
+        assert (np.abs(got[r] - y)[fine] <= tol[fine]).all(), r
+    for b in (dq, dk, dv, out, cu):
+        b.free()
+
+
 @pytest.mark.parametrize("cu_q,cu_k", [([0, 40, 999], [0, 40, 90]), ([0, 50, 30], [0, 50, 90]), ([-9, 40, 90], [0, 40, 90]),
                                        ([0, 40, 90], [0, 40, 2 ** 31 - 1]), ([0, 40, 90], [0, 60, 50]),
                                        ([0, 40, 90], [-2 ** 31, 40, 90])])
