@@ -359,6 +359,7 @@ void mr_ctx_destroy(mr_ctx* c) {
     if (c->scratch.base) (void)hipFree(c->scratch.base);
     for (void* r : c->retired) (void)hipFree(r);
     if (c->attn_err) (void)hipFree(c->attn_err);
+    if (c->attn_scratch) (void)hipFree(c->attn_scratch);
     if (c->ev0) (void)hipEventDestroy(c->ev0);
     if (c->ev1) (void)hipEventDestroy(c->ev1);
     for (hipEvent_t ev : c->prof.pool) (void)hipEventDestroy(ev);

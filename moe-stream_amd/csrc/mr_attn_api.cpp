@@ -245,7 +245,9 @@ int mr_kv_create(mr_ctx* c, const mr_kv_desc* desc, mr_kv** out) {
   if (c->device >= 0) {
     rc = bind(c);
     if (!rc) {
-      hipError_t e = hipMalloc(&kv->base, kv->bytes);
+      hipError_t e = hipSuccess;
+      if (!c->attn_scratch) e = hipMalloc(&c->attn_scratch, mr::attn_decode_scratch_bytes());
+      if (e == hipSuccess) e = hipMalloc(&kv->base, kv->bytes);
       if (e == hipSuccess) e = mr::launch_zero(mr::Launch{c->stream, nullptr}, kv->base, kv->bytes);
       if (e != hipSuccess) rc = hip_fail(c, e, "cache pages");
     }
@@ -324,7 +326,7 @@ int mr_attn_decode(mr_ctx* c, const mr_kv* kv, const mr_heads* q, uint32_t B, co
   if ((rc = bind(c))) return rc;
   c->attn_used = true;
   const hipError_t e = mr::launch_attn_decode(c->launch(), pages(kv), kv->d.format, D, hq, B, seq_len, block_table,
-                                              max_pages, o, ho, c->attn_err);
+                                              max_pages, o, ho, c->attn_err, c->attn_scratch);
   return e == hipSuccess ? MR_OK : hip_fail(c, e, "attn_decode launch");
 }
 

@@ -1,81 +1,441 @@
 // mr_attn_decode.hip -- attention of one query token per sequence over the paged cache.
+//
+// The cache is read once: 2 D FMT / 8 bytes (and the scales) a token and key head, and 4 D operations for each
+// query head on them, so memory bounds it. The query heads that share a key head (up to 16) are the columns of
+// 16x16x32 f16 matrix instructions, S = K Q^T and O = V^T P; the cached values are f16 numbers, so turning
+// codes into operands rounds nothing. Pages lie in the order in which the lanes read them (KvLayout): no LDS,
+// no barrier and no exchange of elements between lanes; a wave takes chunks of 64 tokens by itself.
+//
+// The sequences' chunks are dealt out to the workgroups in parts of one size, so that a long sequence next to
+// short ones is spread over many CUs; the parts of a sequence are joined by a second launch.
 #include "mr_attn_device.h"
 
 namespace mr {
 
 namespace {
 
-// One wave for a sequence and query head: a lane takes a key of each 64 and, for the sum, D/64
-// elements of the values.
-template <int FMT, int D>
-__global__ __launch_bounds__(64) void k_attn_decode(KvPages kv, Heads q, Heads out, const int32_t* __restrict__ len,
-                                                    const int32_t* __restrict__ table, uint32_t max_pages, AttnOpts o,
-                                                    uint32_t* err) {
-  __shared__ float qs[D], ps[64];
-  const int b = blockIdx.x, h = blockIdx.y, lane = threadIdx.x, hk = h / (q.n / kv.n_heads);
-  const int64_t cap = (int64_t)max_pages << kv.page_shift;
-  const int64_t raw = len[b], n = raw < 0 ? 0 : raw > cap ? cap : raw;
-  if (raw != n && lane == 0) atomicOr(err, kErrLength);
-  for (int d = lane * 4; d < D; d += 256) {
-    const f32x4 v = load4(q.p, q.dtype, (uint64_t)b * q.ts + (uint64_t)h * q.hs + d);
-    qs[d] = v.x, qs[d + 1] = v.y, qs[d + 2] = v.z, qs[d + 3] = v.w;
-  }
-  __syncthreads();
-  float m = o.sinks ? o.sinks[h] : -INFINITY, l = o.sinks ? 1.f : 0.f, acc[D / 64] = {};
-  const int64_t first = o.window && n > o.window ? n - o.window : 0;
-  for (int64_t k0 = first & ~63ll; k0 < n; k0 += 64) {
-    const int32_t page = table[(uint64_t)b * max_pages + (k0 >> kv.page_shift)];
-    const bool there = page >= 0 && (uint32_t)page < kv.n_pages;
-    if (!there) {
-      if (lane == 0) atomicOr(err, kErrPage);
-      continue;
-    }
-    const uint8_t* chunk = kv.at(page, hk, (uint32_t)((k0 & ((1ll << kv.page_shift) - 1)) >> 6));
-    const int64_t key = k0 + lane;
-    float s = -INFINITY;
-    if (key >= first && key < n) {
-      s = 0.f;
-      for (int d = 0; d < D; ++d) s += qs[d] * kv_value<FMT, D>(chunk, true, lane, d);
-      s *= o.scale;
-    }
-    const float top = fmaxf(m, wave_max(s));
-    const float p = s == -INFINITY ? 0.f : expf(s - top), f = m == -INFINITY ? 0.f : expf(m - top);
-    l = l * f + wave_sum(p), m = top;
-    ps[lane] = p;
-    __syncthreads();
-    for (int i = 0; i < D / 64; ++i) {
-      acc[i] *= f;
-      for (int j = 0; j < 64; ++j) acc[i] += ps[j] * kv_value<FMT, D>(chunk, false, j, lane + 64 * i);
-    }
-    __syncthreads();
-  }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  uint16_t* dst = static_cast<uint16_t*>(out.p) + (uint64_t)b * out.ts + (uint64_t)h * out.hs;
-  for (int i = 0; i < D / 64; ++i) {
-    const float v = acc[i] * inv;
-    dst[lane + 64 * i] = (uint16_t)(out.dtype == MR_F16 ? pack_f16(v, 0.f) : pack_bf16(v, 0.f));
-  }
+struct DecodeArgs {
+  KvPages kv;
+  Heads q, out;
+  const int32_t *len, *table;
+  uint32_t max_pages, n_seqs;
+  uint32_t heads;      // query heads of a key head
+  uint32_t head_tiles; // tiles of 16 of them
+  uint32_t parts;      // parts all chunks are dealt out in, about
+  AttnOpts o;
+  uint32_t* err;
+  float* part;         // [slot][key head][head tile][16][D] sums, then [slot][..][16][2] maximum and sum
+};
+
+constexpr int kWaves = 4;
+constexpr uint32_t kMinPart = kWaves;  // chunks of a part at least: one for each wave
+
+// Which tokens of sequence b are seen, in chunks.
+struct Span {
+  int n, first;     // length, first token seen
+  int c0, chunks;   // first chunk, number of chunks
+};
+__device__ __forceinline__ Span span_of(const DecodeArgs& a, uint32_t b) {
+  const int64_t cap = (int64_t)a.max_pages << a.kv.page_shift;
+  Span s;
+  s.n = (int)min(max((int64_t)a.len[b], (int64_t)0), cap);
+  s.first = a.o.window && (uint32_t)s.n > a.o.window ? s.n - (int)a.o.window : 0;
+  s.c0 = s.first >> 6;
+  s.chunks = s.n ? ((s.n - 1) >> 6) + 1 - s.c0 : 0;
+  return s;
 }
 
-template <int FMT>
-hipError_t decode_fmt(const Launch& K, const KvPages& kv, uint32_t D, const Heads& q, uint32_t B, const int32_t* len,
-                      const int32_t* table, uint32_t max_pages, const AttnOpts& o, const Heads& out, uint32_t* err) {
-  const dim3 g(B, q.n);
-  if (D == 64) hipLaunchKernelGGL((k_attn_decode<FMT, 64>), g, dim3(64), 0, K.s, kv, q, out, len, table, max_pages, o, err);
-  if (D == 128) hipLaunchKernelGGL((k_attn_decode<FMT, 128>), g, dim3(64), 0, K.s, kv, q, out, len, table, max_pages, o, err);
-  if (D == 256) hipLaunchKernelGGL((k_attn_decode<FMT, 256>), g, dim3(64), 0, K.s, kv, q, out, len, table, max_pages, o, err);
-  return hipGetLastError();
+// The sequence and part of index `i` among all parts (split_only: of the sequences of several parts, in
+// which case the part is 0). Parts of p chunks; a sequence of no more than p chunks is one part, one of no
+// chunks too. slot: the number of parts of split sequences in front.
+struct Part {
+  uint32_t b, part, parts, slot, size;
+};
+__device__ __forceinline__ uint32_t wave_total(uint32_t v) {
+  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, kWave);
+  return v;
 }
+__device__ __forceinline__ bool find_part(const DecodeArgs& a, uint32_t i, bool split_only, Part& r) {
+  const int lane = threadIdx.x & 63;
+  uint32_t all = 0;
+  for (uint32_t b0 = 0; b0 < a.n_seqs; b0 += 64) all += b0 + lane < a.n_seqs ? span_of(a, b0 + lane).chunks : 0;
+  all = wave_total(all);
+  r.size = max(kMinPart, (all + a.parts - 1) / a.parts);
+  uint32_t before = 0, slots = 0;
+  for (uint32_t b0 = 0; b0 < a.n_seqs; b0 += 64) {
+    uint32_t n = 0, split = 0;
+    if (b0 + lane < a.n_seqs) {
+      n = max(1u, ((uint32_t)span_of(a, b0 + lane).chunks + r.size - 1) / r.size);
+      split = n > 1 ? n : 0;
+    }
+    const uint32_t count = split_only ? split > 0 : n;
+    uint32_t sum = count, ssum = split;
+    for (int o = 1; o < 64; o *= 2) {
+      const uint32_t t = __shfl_up(sum, o, kWave), u = __shfl_up(ssum, o, kWave);
+      if (lane >= o) sum += t, ssum += u;
+    }
+    const uint64_t past = __ballot(before + sum > i);
+    if (past) {
+      const int l = __ffsll((unsigned long long)past) - 1;
+      r.b = b0 + l;
+      r.parts = __shfl(n, l, kWave);
+      const uint32_t part = i - before - __shfl(sum - count, l, kWave);
+      r.part = split_only ? 0 : part;
+      r.slot = slots + __shfl(ssum - split, l, kWave);
+      return true;
+    }
+    before += __shfl(sum, 63, kWave);
+    slots += __shfl(ssum, 63, kWave);
+  }
+  return false;
+}
+
+__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// Two of an MXFP4 word's codes (byte `sel`) as f16, times 2^(e) of scale byte `e` (in bits 23.. of sc).
+template <int SEL>
+__device__ __forceinline__ uint32_t fp4_pair(uint32_t w, uint32_t sc) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, bits_f32(sc), SEL));
+}
+// Byte `sel` of w at bits 23..30 (an f32 power of two from its exponent).
+__device__ __forceinline__ uint32_t exp_bits(uint32_t w, int sel) { return (w >> (8 * sel) & 0xFFu) << 23; }
+
+// Two bytes (signed, of a word with its sign bits flipped) as f16: 0x6400 | u is 1024 + u.
+__device__ __forceinline__ f16x2 int8_pair(uint32_t flipped, int pair) {
+  const uint32_t w = __builtin_amdgcn_perm(0x64646464u, flipped, pair ? 0x07030602u : 0x05010400u);
+  return __builtin_bit_cast(f16x2, w) - f16x2{(_Float16)1152.f, (_Float16)1152.f};
+}
+
+template <int FMT, int D>
+struct Chunk {
+  static constexpr int NP = D * FMT / 128;  // 16-byte pieces a lane has of the keys, and of the values
+  static constexpr int NKS = FMT == MR_KV_F16 ? 0 : D == 256 ? 2 : 1, NVS = FMT == MR_KV_F16 ? 0 : D / 32;
+  u32x4 k[NP], v[NP];
+  uint32_t ks[NKS ? NKS : 1];
+  u32x4 vs[NVS ? NVS : 1];  // [G][block][j] bytes: D / 2 in all
+
+  __device__ __forceinline__ void load_k(const uint8_t* p, int lane) {
+    using L = KvLayout<FMT, D>;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) k[i] = *reinterpret_cast<const u32x4*>(p + i * 1024 + lane * 16);
+    if constexpr (FMT != MR_KV_F16) {
+      const int m = lane & 15, g = lane >> 4;
+#pragma unroll
+      for (int i = 0; i < NKS; ++i) {
+        const int blk = D == 64 ? g >> 1 : D == 128 ? g : 2 * g + i;
+        ks[i] = *reinterpret_cast<const uint32_t*>(p + L::kKs + (blk * 16 + m) * 4);
+      }
+    }
+  }
+  __device__ __forceinline__ void load_v(const uint8_t* p, int lane) {
+    using L = KvLayout<FMT, D>;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) v[i] = *reinterpret_cast<const u32x4*>(p + L::kV + i * 1024 + lane * 16);
+    if constexpr (FMT != MR_KV_F16) {
+#pragma unroll
+      for (int i = 0; i < NVS; ++i) vs[i] = *reinterpret_cast<const u32x4*>(p + L::kVs + (lane >> 4) * (D / 2) + 16 * i);
+    }
+  }
+  // Elements 8 i .. 8 i + 7 of the lane's quarter of key 16 t + m.
+  __device__ __forceinline__ u32x4 key(int t, int i) const {
+    if constexpr (FMT == MR_KV_F16) return k[t * (D / 32) + i];
+    const uint32_t s = ks[D == 256 ? i >> 2 : 0];
+    if constexpr (FMT == MR_KV_MXFP4) {
+      const int w = t * (D / 32) + i;
+      const uint32_t c = k[w >> 2][w & 3], e = exp_bits(s, t);
+      return u32x4{fp4_pair<0>(c, e), fp4_pair<1>(c, e), fp4_pair<2>(c, e), fp4_pair<3>(c, e)};
+    } else {
+      const int w = 2 * (t * (D / 32) + i);
+      const uint32_t c0 = k[w >> 2][w & 3] ^ 0x80808080u, c1 = k[w >> 2][(w & 3) + 1] ^ 0x80808080u;
+      const uint32_t b = s >> (8 * t) & 0xFFu;
+      const f16x2 e = __builtin_bit_cast(f16x2, b << 8 | b << 24);
+      return u32x4{__builtin_bit_cast(uint32_t, int8_pair(c0, 0) * e), __builtin_bit_cast(uint32_t, int8_pair(c0, 1) * e),
+                   __builtin_bit_cast(uint32_t, int8_pair(c1, 0) * e), __builtin_bit_cast(uint32_t, int8_pair(c1, 1) * e)};
+    }
+  }
+  // Element m of tiles 2 b and 2 b + 1 (of 16) for the 8 tokens of the lane in group G.
+  __device__ __forceinline__ void value(int G, int b, u32x4& lo, u32x4& hi) const {
+    if constexpr (FMT == MR_KV_F16) {
+      lo = v[G * (D / 16) + 2 * b], hi = v[G * (D / 16) + 2 * b + 1];
+      return;
+    }
+    const int sw = 2 * (G * (D / 32) + b);
+    const uint32_t s0 = vs[sw >> 2][sw & 3], s1 = vs[sw >> 2][(sw & 3) + 1];
+    if constexpr (FMT == MR_KV_MXFP4) {
+      const uint32_t c0 = v[sw >> 2][sw & 3], c1 = v[sw >> 2][(sw & 3) + 1];
+      const uint32_t p[8] = {fp4_pair<0>(c0, exp_bits(s0, 0)), fp4_pair<1>(c0, exp_bits(s0, 1)),
+                             fp4_pair<2>(c0, exp_bits(s0, 2)), fp4_pair<3>(c0, exp_bits(s0, 3)),
+                             fp4_pair<0>(c1, exp_bits(s1, 0)), fp4_pair<1>(c1, exp_bits(s1, 1)),
+                             fp4_pair<2>(c1, exp_bits(s1, 2)), fp4_pair<3>(c1, exp_bits(s1, 3))};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        lo[j] = __builtin_amdgcn_perm(p[2 * j + 1], p[2 * j], 0x05040100u);
+        hi[j] = __builtin_amdgcn_perm(p[2 * j + 1], p[2 * j], 0x07060302u);
+      }
+    } else {
+      // scale bytes j, j + 1 as the high bytes of two f16
+      const f16x2 e[4] = {__builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0u, s0, 0x010C000Cu)),
+                          __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0u, s0, 0x030C020Cu)),
+                          __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0u, s1, 0x010C000Cu)),
+                          __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0u, s1, 0x030C020Cu))};
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int w = 2 * (G * (D / 16) + 2 * b + x);
+        const uint32_t c0 = v[w >> 2][w & 3] ^ 0x80808080u, c1 = v[w >> 2][(w & 3) + 1] ^ 0x80808080u;
+        (x ? hi : lo) = u32x4{__builtin_bit_cast(uint32_t, int8_pair(c0, 0) * e[0]), __builtin_bit_cast(uint32_t, int8_pair(c0, 1) * e[1]),
+                              __builtin_bit_cast(uint32_t, int8_pair(c1, 0) * e[2]), __builtin_bit_cast(uint32_t, int8_pair(c1, 1) * e[3])};
+      }
+    }
+  }
+};
+
+template <int FMT, int D>
+__global__ __launch_bounds__(64 * kWaves) void k_attn_decode(DecodeArgs a) {
+  constexpr int NT = D / 16;
+  __shared__ __attribute__((aligned(16))) float sums[kWaves / 2][16 * D];
+  __shared__ float stats[kWaves / 2][16][2];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  Part pt;
+  if (!find_part(a, blockIdx.x, false, pt)) return;
+  const Span sp = span_of(a, pt.b);
+  if (threadIdx.x == 0 && blockIdx.y == 0 && pt.part == 0 && sp.n != a.len[pt.b]) atomicOr(a.err, kErrLength);
+  const uint32_t hk = blockIdx.y / a.head_tiles, h0 = 16 * (blockIdx.y % a.head_tiles);  // first query head within the group
+  const uint32_t heads = min(16u, a.heads - h0);
+  const uint32_t hq = hk * a.heads + h0 + min((uint32_t)n, heads - 1);  // this lane's query head (the last one repeated)
+
+  // The query as f16, scaled by a power of two so that its largest element lies in [2^14, 2^15): exact for
+  // f16, and for bf16 all but what lies 2^-30 below the largest.
+  u32x4 qf[D / 32];
+  float c;
+  {
+    const uint64_t o = (uint64_t)pt.b * a.q.ts + (uint64_t)hq * a.q.hs + g * (D / 4);
+    f32x4 x[D / 16];
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      x[i] = load4(a.q.p, a.q.dtype, o + 4 * i);
+      top = fmaxf(fmaxf(fmaxf(top, fabsf(x[i].x)), fmaxf(fabsf(x[i].y), fabsf(x[i].z))), fabsf(x[i].w));
+    }
+    top = max_xor16(max_xor32(top));
+    const int e = top > 0.f ? ilogbf(fminf(top, 3.0e38f)) - 14 : 0;
+    const float sign = a.o.scale < 0.f ? -1.f : 1.f;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      float y[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = ldexpf(x[2 * i + (j >> 2)][j & 3], -e) * sign;
+      qf[i] = u32x4{pack_f16(y[0], y[1]), pack_f16(y[2], y[3]), pack_f16(y[4], y[5]), pack_f16(y[6], y[7])};
+    }
+    // above zero: a masked score times c stays -inf
+    c = fmaxf(ldexpf(fabsf(a.o.scale) * 1.44269504088896340736f, e), 0x1p-126f);
+  }
+
+  f32x4 acc[NT] = {};
+  float m = -INFINITY, l = 0.f;
+  const int begin = sp.c0 + (int)(pt.part * pt.size), end = min(begin + (int)pt.size, sp.c0 + sp.chunks);
+  const int cpp = 1 << (a.kv.page_shift - 6);
+  // this wave's chunks: begin + wave, + kWaves, ..; lane i has the page of the i-th of the next 64
+  auto page_of = [&](int chunk) -> int {
+    if (chunk >= end) return -1;
+    const int p = a.table[(uint64_t)pt.b * a.max_pages + (uint32_t)(chunk >> (a.kv.page_shift - 6))];
+    if (p >= 0 && (uint32_t)p < a.kv.n_pages) return p;
+    atomicOr(a.err, kErrPage);
+    return -1;
+  };
+  auto address = [&](int page, int chunk) { return a.kv.at(page < 0 ? 0 : page, hk, chunk & (cpp - 1)); };
+  Chunk<FMT, D> ch;
+  int pages = -1, page = -1;
+  for (int i = 0, cidx = begin + wave; cidx < end; ++i, cidx += kWaves) {
+    if ((i & 63) == 0) {
+      pages = page_of(cidx + kWaves * lane);
+      page = __builtin_amdgcn_readlane(pages, 0);
+      ch.load_k(address(page, cidx), lane);
+    }
+    const bool there = page >= 0;
+    ch.load_v(address(page, cidx), lane);
+    f32x4 s[4] = {};
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) s[t] = mfma16(ch.key(t, j), qf[j], s[t]);
+    if ((i & 63) != 63 && cidx + kWaves < end) {
+      page = __builtin_amdgcn_readlane(pages, (i + 1) & 63);
+      ch.load_k(address(page, cidx + kWaves), lane);
+    }
+    const int k0 = cidx << 6;
+    if (!there || k0 < sp.first || k0 + 64 > sp.n) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int key = k0 + 16 * t + 4 * g + j;
+          if (!there || key < sp.first || key >= sp.n) s[t][j] = -INFINITY;
+        }
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int t = 0; t < 16; ++t) top = fmaxf(top, s[t >> 2][t & 3]);
+    top = max_xor16(max_xor32(top)) * c;
+    const float m1 = fmaxf(m, top);
+    if (__any(m1 > m)) {
+      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m1);
+      l *= f;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) acc[t] *= f;
+      m = m1;
+    }
+    const float base = m == -INFINITY ? 0.f : m;
+    u32x4 pf[2];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      float p[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) p[j] = __builtin_amdgcn_exp2f(fmaf(s[t][j], c, -base)), l += p[j];
+      pf[t >> 1][2 * (t & 1)] = pack_f16(p[0], p[1]), pf[t >> 1][2 * (t & 1) + 1] = pack_f16(p[2], p[3]);
+    }
+#pragma unroll
+    for (int G = 0; G < 2; ++G)
+#pragma unroll
+      for (int b = 0; b < D / 32; ++b) {
+        u32x4 lo, hi;
+        ch.value(G, b, lo, hi);
+        acc[2 * b] = mfma16(lo, pf[G], acc[2 * b]);
+        acc[2 * b + 1] = mfma16(hi, pf[G], acc[2 * b + 1]);
+      }
+  }
+  l = add_xor16(add_xor32(l));
+
+  // The waves' results are joined in pairs: (0, 2) and (1, 3), then (0, 1). acc: element 16 t + 4 g + j of head n.
+#pragma unroll
+  for (int w = kWaves / 2; w >= 1; w /= 2) {
+    if (wave >= w && wave < 2 * w) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) *reinterpret_cast<f32x4*>(&sums[wave - w][n * D + 16 * t + 4 * g]) = acc[t];
+      if (g == 0) stats[wave - w][n][0] = m, stats[wave - w][n][1] = l;
+    }
+    __syncthreads();
+    if (wave < w) {
+      const float m2 = stats[wave][n][0], l2 = stats[wave][n][1], m1 = fmaxf(m, m2);
+      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m1);
+      const float f2 = m2 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m2 - m1);
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+        acc[t] = acc[t] * f + *reinterpret_cast<const f32x4*>(&sums[wave][n * D + 16 * t + 4 * g]) * f2;
+      l = l * f + l2 * f2, m = m1;
+    }
+    __syncthreads();
+  }
+  if (wave > 0 || (uint32_t)n >= heads) return;
+  if (pt.parts > 1) {
+    const uint64_t unit = ((uint64_t)(pt.slot + pt.part) * gridDim.y + blockIdx.y) * 16 + n;
+    float* dst = a.part + unit * D;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) *reinterpret_cast<f32x4*>(dst + 16 * t + 4 * g) = acc[t];
+    float* st = a.part + (uint64_t)2 * a.parts * gridDim.y * 16 * D + unit * 2;
+    if (g == 0) st[0] = m, st[1] = l;
+    return;
+  }
+  if (a.o.sinks) {
+    const float sink = a.o.sinks[hq] * 1.44269504088896340736f, m1 = fmaxf(m, sink);
+    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m1);
+    l = l * f + (sink == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sink - m1));
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[t] *= f;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+    store4(a.out.p, a.out.dtype, (uint64_t)pt.b * a.out.ts + (uint64_t)hq * a.out.hs + 16 * t + 4 * g, acc[t] * inv);
+}
+
+// Joins the parts of split sequence blockIdx.x for one query head: a quarter of the parts to a wave in turn,
+// in order, then the waves.
+template <int D>
+__global__ __launch_bounds__(256) void k_attn_join(DecodeArgs a) {
+  constexpr int E = D / 64;
+  __shared__ float sums[4][D], stats[4][2];
+  Part pt;
+  if (!find_part(a, blockIdx.x, true, pt)) return;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const uint32_t h = blockIdx.y, hk = h / a.heads, in = h % a.heads, units = a.kv.n_heads * a.head_tiles;
+  const uint64_t unit0 = ((uint64_t)pt.slot * units + hk * a.head_tiles + in / 16) * 16 + in % 16;
+  const float* stat = a.part + (uint64_t)2 * a.parts * units * 16 * D;
+  float m = -INFINITY, l = 0.f, acc[E] = {};
+  for (uint32_t p = wave; p < pt.parts; p += 4) {
+    const uint64_t u = unit0 + (uint64_t)p * units * 16;
+    const float m2 = stat[2 * u], l2 = stat[2 * u + 1], m1 = fmaxf(m, m2);
+    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m1);
+    const float f2 = m2 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m2 - m1);
+#pragma unroll
+    for (int i = 0; i < E; ++i) acc[i] = acc[i] * f + a.part[u * D + lane + 64 * i] * f2;
+    l = l * f + l2 * f2, m = m1;
+  }
+#pragma unroll
+  for (int i = 0; i < E; ++i) sums[wave][lane + 64 * i] = acc[i];
+  if (lane == 0) stats[wave][0] = m, stats[wave][1] = l;
+  __syncthreads();
+  if ((int)threadIdx.x >= D) return;
+  m = a.o.sinks ? a.o.sinks[h] * 1.44269504088896340736f : -INFINITY;
+  for (int w = 0; w < 4; ++w) m = fmaxf(m, stats[w][0]);
+  const float base = m == -INFINITY ? 0.f : m;
+  float s = 0.f;
+  l = a.o.sinks ? __builtin_amdgcn_exp2f(a.o.sinks[h] * 1.44269504088896340736f - base) : 0.f;
+  for (int w = 0; w < 4; ++w) {
+    const float f = __builtin_amdgcn_exp2f(stats[w][0] - base);
+    s += sums[w][threadIdx.x] * f, l += stats[w][1] * f;
+  }
+  const float v = l == 0.f ? 0.f : s / l;
+  uint16_t* dst = static_cast<uint16_t*>(a.out.p) + (uint64_t)pt.b * a.out.ts + (uint64_t)h * a.out.hs + threadIdx.x;
+  *dst = (uint16_t)(a.out.dtype == MR_F16 ? pack_f16(v, 0.f) : pack_bf16(v, 0.f));
+}
+
+template <int FMT, int D>
+void decode(hipStream_t s, const DecodeArgs& a, dim3 g) {
+  hipLaunchKernelGGL((k_attn_decode<FMT, D>), g, dim3(64 * kWaves), 0, s, a);
+}
+template <int FMT>
+void decode_fmt(hipStream_t s, uint32_t D, const DecodeArgs& a, dim3 g) {
+  if (D == 64) decode<FMT, 64>(s, a, g);
+  if (D == 128) decode<FMT, 128>(s, a, g);
+  if (D == 256) decode<FMT, 256>(s, a, g);
+}
+
+constexpr uint32_t kPartUnits = 1024;  // parts times key heads and head tiles: four workgroups to a CU
 
 }  // namespace
 
+uint64_t attn_decode_scratch_bytes() { return 2ull * kPartUnits * 16 * (256 + 2) * sizeof(float); }
+
 hipError_t launch_attn_decode(const Launch& K, const KvPages& kv, uint32_t format, uint32_t D, const Heads& q, uint32_t B,
                               const int32_t* len, const int32_t* table, uint32_t max_pages, const AttnOpts& o,
-                              const Heads& out, uint32_t* err) {
-  ProfScope ps(K, "attn_decode");
-  if (format == MR_KV_F16) return decode_fmt<MR_KV_F16>(K, kv, D, q, B, len, table, max_pages, o, out, err);
-  if (format == MR_KV_MXINT8) return decode_fmt<MR_KV_MXINT8>(K, kv, D, q, B, len, table, max_pages, o, out, err);
-  return decode_fmt<MR_KV_MXFP4>(K, kv, D, q, B, len, table, max_pages, o, out, err);
+                              const Heads& out, uint32_t* err, float* scratch) {
+  DecodeArgs a{kv, q, out, len, table, max_pages, B, q.n / kv.n_heads, 0, 0, o, err, scratch};
+  a.head_tiles = (a.heads + 15) / 16;
+  const uint32_t units = kv.n_heads * a.head_tiles;
+  // chunks a sequence can have: no more parts than they allow
+  const uint64_t cap = (uint64_t)max_pages << (kv.page_shift - 6);
+  const uint64_t chunks = o.window ? std::min<uint64_t>(cap, (o.window + 62ull) / 64 + 1) : cap;
+  a.parts = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(kPartUnits / units, (uint64_t)B * ((chunks + kMinPart - 1) / kMinPart)));
+  const bool split = a.parts > 1 && chunks > kMinPart;
+  // a sequence's last part need not be full
+  const dim3 g(split ? a.parts + B : B, units);
+  {
+    ProfScope ps(K, "attn_decode");
+    if (format == MR_KV_F16) decode_fmt<MR_KV_F16>(K.s, D, a, g);
+    if (format == MR_KV_MXINT8) decode_fmt<MR_KV_MXINT8>(K.s, D, a, g);
+    if (format == MR_KV_MXFP4) decode_fmt<MR_KV_MXFP4>(K.s, D, a, g);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || !split) return e;
+  }
+  ProfScope ps(K, "attn_join");
+  // a split sequence has more than half of its parts full
+  const dim3 j(std::min(B, a.parts), q.n);
+  if (D == 64) hipLaunchKernelGGL((k_attn_join<64>), j, dim3(256), 0, K.s, a);
+  if (D == 128) hipLaunchKernelGGL((k_attn_join<128>), j, dim3(256), 0, K.s, a);
+  if (D == 256) hipLaunchKernelGGL((k_attn_join<256>), j, dim3(256), 0, K.s, a);
+  return hipGetLastError();
 }
 
 }  // namespace mr

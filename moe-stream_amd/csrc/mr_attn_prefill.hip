@@ -127,7 +127,7 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
   const int see_last = row + diff;
   const int64_t see_first = a.o.window ? max((int64_t)pl.k0, (int64_t)see_last + 1 - (int64_t)a.o.window) : pl.k0;
 
-  const float c = fabsf(a.o.scale) * 1.44269504088896340736f;
+  const float c = fmaxf(fabsf(a.o.scale) * 1.44269504088896340736f, 0x1p-126f);  // above zero: a masked score stays -inf
   u32x4 qf[D / 16];
   {
     const uint16_t* qp = static_cast<const uint16_t*>(a.q.p) + (uint64_t)min(row, pl.q1 - 1) * a.q.ts + (uint64_t)h * a.q.hs;

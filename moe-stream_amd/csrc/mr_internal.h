@@ -111,6 +111,8 @@ struct mr_ctx {
   // mr_sync once such a call was made.
   uint32_t* attn_err = nullptr;
   bool attn_used = false;
+  // Partial results of mr_attn_decode, of one size for all calls; allocated with the first cache.
+  float* attn_scratch = nullptr;
   hipEvent_t ev0 = nullptr, ev1 = nullptr;
   bool capturing = false;
   mr::Prof prof;
