@@ -97,7 +97,7 @@ hipError_t launch_kv_read(const Launch& K, const KvPages& kv, uint32_t format, u
                           const int32_t* slots, const Heads& k, const Heads& v, uint32_t* err);
 hipError_t launch_attn_decode(const Launch& K, const KvPages& kv, uint32_t format, uint32_t D, const Heads& q, uint32_t B,
                               const int32_t* len, const int32_t* table, uint32_t max_pages, const AttnOpts& o,
-                              const Heads& out, uint32_t* err, float* scratch);
+                              const Heads& out, uint32_t* err, float* scratch, int n_cu);
 // Scratch of launch_attn_decode, at any size.
 uint64_t attn_decode_scratch_bytes();
 hipError_t launch_attn_prefill(const Launch& K, uint32_t D, const Heads& q, uint32_t nq, const Heads& k, const Heads& v,

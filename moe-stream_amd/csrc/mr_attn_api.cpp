@@ -326,7 +326,7 @@ int mr_attn_decode(mr_ctx* c, const mr_kv* kv, const mr_heads* q, uint32_t B, co
   if ((rc = bind(c))) return rc;
   c->attn_used = true;
   const hipError_t e = mr::launch_attn_decode(c->launch(), pages(kv), kv->d.format, D, hq, B, seq_len, block_table,
-                                              max_pages, o, ho, c->attn_err, c->attn_scratch);
+                                              max_pages, o, ho, c->attn_err, c->attn_scratch, c->n_cu);
   return e == hipSuccess ? MR_OK : hip_fail(c, e, "attn_decode launch");
 }
 

@@ -21,24 +21,30 @@ struct DecodeArgs {
   uint32_t max_pages, n_seqs;
   uint32_t heads;      // query heads of a key head
   uint32_t head_tiles; // tiles of 16 of them
-  uint32_t parts;      // parts all chunks are dealt out in, about
+  uint32_t parts;      // full parts that all chunks are dealt out in at most; 1: a sequence a part
+  uint32_t room;       // parts that the CUs hold at once
   AttnOpts o;
   uint32_t* err;
   float* part;         // [slot][key head][head tile][16][D] sums, then [slot][..][16][2] maximum and sum
 };
 
 constexpr int kWaves = 4;
-constexpr uint32_t kMinPart = kWaves;  // chunks of a part at least: one for each wave
+constexpr uint32_t kPartUnits = 1024;  // most parts, times key heads and head tiles
+constexpr uint32_t kMinPart = kWaves;       // chunks of a part at least: one for each wave
+constexpr uint32_t kGoodPart = 4 * kWaves;  // chunks that make up for a part's beginning and end
 
 // Which tokens of sequence b are seen, in chunks.
 struct Span {
   int n, first;     // length, first token seen
   int c0, chunks;   // first chunk, number of chunks
+  int bad;          // the length was out of range
 };
 __device__ __forceinline__ Span span_of(const DecodeArgs& a, uint32_t b) {
   const int64_t cap = (int64_t)a.max_pages << a.kv.page_shift;
   Span s;
-  s.n = (int)min(max((int64_t)a.len[b], (int64_t)0), cap);
+  const int64_t len = a.len[b];
+  s.n = (int)min(max(len, (int64_t)0), cap);
+  s.bad = s.n != len;
   s.first = a.o.window && (uint32_t)s.n > a.o.window ? s.n - (int)a.o.window : 0;
   s.c0 = s.first >> 6;
   s.chunks = s.n ? ((s.n - 1) >> 6) + 1 - s.c0 : 0;
@@ -46,46 +52,55 @@ __device__ __forceinline__ Span span_of(const DecodeArgs& a, uint32_t b) {
 }
 
 // The sequence and part of index `i` among all parts (split_only: of the sequences of several parts, in
-// which case the part is 0). Parts of p chunks; a sequence of no more than p chunks is one part, one of no
-// chunks too. slot: the number of parts of split sequences in front.
+// which case the part is 0). Parts of `size` chunks; a sequence of no more than that is one part, one of no
+// chunks too. slot: the number of parts of split sequences in front. A lane looks at a sequence; the lengths of
+// up to 64 are read once.
 struct Part {
   uint32_t b, part, parts, slot, size;
+  Span sp;
 };
 __device__ __forceinline__ uint32_t wave_total(uint32_t v) {
   for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, kWave);
   return v;
 }
 __device__ __forceinline__ bool find_part(const DecodeArgs& a, uint32_t i, bool split_only, Part& r) {
-  const int lane = threadIdx.x & 63;
-  uint32_t all = 0;
-  for (uint32_t b0 = 0; b0 < a.n_seqs; b0 += 64) all += b0 + lane < a.n_seqs ? span_of(a, b0 + lane).chunks : 0;
+  const uint32_t lane = threadIdx.x & 63;
+  if (a.parts == 1) {
+    if (split_only || i >= a.n_seqs) return false;
+    r = Part{i, 0, 1, 0, 0x7FFFFFFFu, span_of(a, i)};
+    return true;
+  }
+  auto span = [&](uint32_t b) { return b < a.n_seqs ? span_of(a, b) : Span{}; };
+  Span s = span(lane);
+  uint32_t all = s.chunks;
+  for (uint32_t b0 = 64; b0 < a.n_seqs; b0 += 64) all += span(b0 + lane).chunks;
   all = wave_total(all);
-  r.size = max(kMinPart, (all + a.parts - 1) / a.parts);
+  // parts of kGoodPart chunks where that makes no fewer than the CUs hold at once, and no more than `parts`
+  r.size = max(max(kMinPart, (all + a.parts - 1) / a.parts), min(kGoodPart, (all + a.room - 1) / a.room));
   uint32_t before = 0, slots = 0;
   for (uint32_t b0 = 0; b0 < a.n_seqs; b0 += 64) {
-    uint32_t n = 0, split = 0;
-    if (b0 + lane < a.n_seqs) {
-      n = max(1u, ((uint32_t)span_of(a, b0 + lane).chunks + r.size - 1) / r.size);
-      split = n > 1 ? n : 0;
-    }
-    const uint32_t count = split_only ? split > 0 : n;
+    if (b0) s = span(b0 + lane);
+    const uint32_t n = b0 + lane < a.n_seqs ? max(1u, ((uint32_t)s.chunks + r.size - 1) / r.size) : 0;
+    const uint32_t split = n > 1 ? n : 0, count = split_only ? split > 0 : n;
     uint32_t sum = count, ssum = split;
-    for (int o = 1; o < 64; o *= 2) {
-      const uint32_t t = __shfl_up(sum, o, kWave), u = __shfl_up(ssum, o, kWave);
-      if (lane >= o) sum += t, ssum += u;
-    }
+    if (a.n_seqs > 1)
+      for (int o = 1; o < 64; o *= 2) {
+        const uint32_t t = __shfl_up(sum, o, kWave), u = __shfl_up(ssum, o, kWave);
+        if ((int)lane >= o) sum += t, ssum += u;
+      }
     const uint64_t past = __ballot(before + sum > i);
     if (past) {
       const int l = __ffsll((unsigned long long)past) - 1;
       r.b = b0 + l;
-      r.parts = __shfl(n, l, kWave);
-      const uint32_t part = i - before - __shfl(sum - count, l, kWave);
-      r.part = split_only ? 0 : part;
-      r.slot = slots + __shfl(ssum - split, l, kWave);
+      r.parts = __builtin_amdgcn_readlane(n, l);
+      r.part = split_only ? 0 : i - before - __builtin_amdgcn_readlane(sum - count, l);
+      r.slot = slots + __builtin_amdgcn_readlane(ssum - split, l);
+      r.sp = Span{__builtin_amdgcn_readlane(s.n, l), __builtin_amdgcn_readlane(s.first, l), __builtin_amdgcn_readlane(s.c0, l),
+                  __builtin_amdgcn_readlane(s.chunks, l), __builtin_amdgcn_readlane(s.bad, l)};
       return true;
     }
-    before += __shfl(sum, 63, kWave);
-    slots += __shfl(ssum, 63, kWave);
+    before += __builtin_amdgcn_readlane(sum, 63);
+    slots += __builtin_amdgcn_readlane(ssum, 63);
   }
   return false;
 }
@@ -94,13 +109,13 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// Two of an MXFP4 word's codes (byte `sel`) as f16, times 2^(e) of scale byte `e` (in bits 23.. of sc).
+// Two of an MXFP4 word's codes (byte `sel`) as f16, times the power of two in the exponent field of sc.
 template <int SEL>
 __device__ __forceinline__ uint32_t fp4_pair(uint32_t w, uint32_t sc) {
   return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, bits_f32(sc), SEL));
 }
-// Byte `sel` of w at bits 23..30 (an f32 power of two from its exponent).
-__device__ __forceinline__ uint32_t exp_bits(uint32_t w, int sel) { return (w >> (8 * sel) & 0xFFu) << 23; }
+// Byte `sel` of w in the exponent field; the conversion takes no notice of the other bits.
+__device__ __forceinline__ uint32_t exp_bits(uint32_t w, int sel) { return sel == 3 ? w >> 1 : w << (23 - 8 * sel); }
 
 // Two bytes (signed, of a word with its sign bits flipped) as f16: 0x6400 | u is 1024 + u.
 __device__ __forceinline__ f16x2 int8_pair(uint32_t flipped, int pair) {
@@ -129,13 +144,14 @@ struct Chunk {
       }
     }
   }
-  __device__ __forceinline__ void load_v(const uint8_t* p, int lane) {
+  // The values of group G (32 tokens).
+  __device__ __forceinline__ void load_v(const uint8_t* p, int lane, int G) {
     using L = KvLayout<FMT, D>;
 #pragma unroll
-    for (int i = 0; i < NP; ++i) v[i] = *reinterpret_cast<const u32x4*>(p + L::kV + i * 1024 + lane * 16);
+    for (int i = G * NP / 2; i < (G + 1) * NP / 2; ++i) v[i] = *reinterpret_cast<const u32x4*>(p + L::kV + i * 1024 + lane * 16);
     if constexpr (FMT != MR_KV_F16) {
 #pragma unroll
-      for (int i = 0; i < NVS; ++i) vs[i] = *reinterpret_cast<const u32x4*>(p + L::kVs + (lane >> 4) * (D / 2) + 16 * i);
+      for (int i = G * NVS / 2; i < (G + 1) * NVS / 2; ++i) vs[i] = *reinterpret_cast<const u32x4*>(p + L::kVs + (lane >> 4) * (D / 2) + 16 * i);
     }
   }
   // Elements 8 i .. 8 i + 7 of the lane's quarter of key 16 t + m.
@@ -191,16 +207,25 @@ struct Chunk {
   }
 };
 
+// Waves of a SIMD, as many as the registers of a chunk and of the sums leave room for, and whether the next
+// chunk's keys are on their way while this one's values are used; both measured (DECODE_TABLE).
 template <int FMT, int D>
-__global__ __launch_bounds__(64 * kWaves) void k_attn_decode(DecodeArgs a) {
+struct Tuning {
+  static constexpr int kPerSimd = D == 64 ? (FMT == 16 ? 3 : 4) : D == 128 ? (FMT == 4 ? 3 : 2) : FMT == 16 ? 1 : 2;
+  static constexpr bool kAhead = !(D == 256 && FMT == 8);
+};
+
+template <int FMT, int D>
+__global__ __launch_bounds__(64 * kWaves, (Tuning<FMT, D>::kPerSimd)) void k_attn_decode(DecodeArgs a) {
   constexpr int NT = D / 16;
+  constexpr bool kAhead = Tuning<FMT, D>::kAhead;
   __shared__ __attribute__((aligned(16))) float sums[kWaves / 2][16 * D];
   __shared__ float stats[kWaves / 2][16][2];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   Part pt;
   if (!find_part(a, blockIdx.x, false, pt)) return;
-  const Span sp = span_of(a, pt.b);
-  if (threadIdx.x == 0 && blockIdx.y == 0 && pt.part == 0 && sp.n != a.len[pt.b]) atomicOr(a.err, kErrLength);
+  const Span sp = pt.sp;
+  if (threadIdx.x == 0 && blockIdx.y == 0 && pt.part == 0 && sp.bad) atomicOr(a.err, kErrLength);
   const uint32_t hk = blockIdx.y / a.head_tiles, h0 = 16 * (blockIdx.y % a.head_tiles);  // first query head within the group
   const uint32_t heads = min(16u, a.heads - h0);
   const uint32_t hq = hk * a.heads + h0 + min((uint32_t)n, heads - 1);  // this lane's query head (the last one repeated)
@@ -234,7 +259,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_attn_decode(DecodeArgs a) {
 
   f32x4 acc[NT] = {};
   float m = -INFINITY, l = 0.f;
-  const int begin = sp.c0 + (int)(pt.part * pt.size), end = min(begin + (int)pt.size, sp.c0 + sp.chunks);
+  const int begin = sp.c0 + (int)(pt.part * pt.size), end = sp.c0 + (int)min((uint32_t)sp.chunks, (pt.part + 1) * pt.size);
   const int cpp = 1 << (a.kv.page_shift - 6);
   // this wave's chunks: begin + wave, + kWaves, ..; lane i has the page of the i-th of the next 64
   auto page_of = [&](int chunk) -> int {
@@ -251,18 +276,22 @@ __global__ __launch_bounds__(64 * kWaves) void k_attn_decode(DecodeArgs a) {
     if ((i & 63) == 0) {
       pages = page_of(cidx + kWaves * lane);
       page = __builtin_amdgcn_readlane(pages, 0);
-      ch.load_k(address(page, cidx), lane);
+      if (kAhead) ch.load_k(address(page, cidx), lane);
     }
     const bool there = page >= 0;
-    ch.load_v(address(page, cidx), lane);
+    const uint8_t* chunk = address(page, cidx);
+    if (!kAhead) ch.load_k(chunk, lane);
+    ch.load_v(chunk, lane, 0);
+    if (kAhead) ch.load_v(chunk, lane, 1);
     f32x4 s[4] = {};
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
       for (int j = 0; j < D / 32; ++j) s[t] = mfma16(ch.key(t, j), qf[j], s[t]);
+    if (!kAhead) ch.load_v(chunk, lane, 1);
     if ((i & 63) != 63 && cidx + kWaves < end) {
       page = __builtin_amdgcn_readlane(pages, (i + 1) & 63);
-      ch.load_k(address(page, cidx + kWaves), lane);
+      if (kAhead) ch.load_k(address(page, cidx + kWaves), lane);
     }
     const int k0 = cidx << 6;
     if (!there || k0 < sp.first || k0 + 64 > sp.n) {
@@ -350,59 +379,67 @@ __global__ __launch_bounds__(64 * kWaves) void k_attn_decode(DecodeArgs a) {
     store4(a.out.p, a.out.dtype, (uint64_t)pt.b * a.out.ts + (uint64_t)hq * a.out.hs + 16 * t + 4 * g, acc[t] * inv);
 }
 
-// Joins the parts of split sequence blockIdx.x for one query head: a quarter of the parts to a wave in turn,
-// in order, then the waves.
+// Joins the parts of split sequence blockIdx.x for one query head: first all parts' weights, then the weighted
+// sums, D/4 lanes to a part and kJoin / (D/4) parts at a time, many loads in flight (a running maximum would
+// make each part wait for the one before: 36 us for 391 parts of 256, instead of JOIN_US).
+constexpr int kJoin = 256;
 template <int D>
-__global__ __launch_bounds__(256) void k_attn_join(DecodeArgs a) {
-  constexpr int E = D / 64;
-  __shared__ float sums[4][D], stats[4][2];
+__global__ __launch_bounds__(kJoin) void k_attn_join(DecodeArgs a) {
+  constexpr int L = D / 4, G = kJoin / L;
+  __shared__ __attribute__((aligned(16))) float sums[G * D];
+  __shared__ float weight[kPartUnits], wave_m[kJoin / 64], wave_l[kJoin / 64];
   Part pt;
   if (!find_part(a, blockIdx.x, true, pt)) return;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const uint32_t h = blockIdx.y, hk = h / a.heads, in = h % a.heads, units = a.kv.n_heads * a.head_tiles;
   const uint64_t unit0 = ((uint64_t)pt.slot * units + hk * a.head_tiles + in / 16) * 16 + in % 16;
   const float* stat = a.part + (uint64_t)2 * a.parts * units * 16 * D;
-  float m = -INFINITY, l = 0.f, acc[E] = {};
-  for (uint32_t p = wave; p < pt.parts; p += 4) {
-    const uint64_t u = unit0 + (uint64_t)p * units * 16;
-    const float m2 = stat[2 * u], l2 = stat[2 * u + 1], m1 = fmaxf(m, m2);
-    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m1);
-    const float f2 = m2 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m2 - m1);
+  float m[kPartUnits / kJoin], l = 0.f, top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < E; ++i) acc[i] = acc[i] * f + a.part[u * D + lane + 64 * i] * f2;
-    l = l * f + l2 * f2, m = m1;
+  for (int i = 0; i < (int)(kPartUnits / kJoin); ++i) {
+    const uint32_t p = tid + i * kJoin;
+    m[i] = p < pt.parts ? stat[2 * (unit0 + (uint64_t)p * units * 16)] : -INFINITY;
+    top = fmaxf(top, m[i]);
   }
-#pragma unroll
-  for (int i = 0; i < E; ++i) sums[wave][lane + 64 * i] = acc[i];
-  if (lane == 0) stats[wave][0] = m, stats[wave][1] = l;
+  top = wave_max(top);
+  if (lane == 0) wave_m[wave] = top;
   __syncthreads();
-  if ((int)threadIdx.x >= D) return;
-  m = a.o.sinks ? a.o.sinks[h] * 1.44269504088896340736f : -INFINITY;
-  for (int w = 0; w < 4; ++w) m = fmaxf(m, stats[w][0]);
-  const float base = m == -INFINITY ? 0.f : m;
-  float s = 0.f;
-  l = a.o.sinks ? __builtin_amdgcn_exp2f(a.o.sinks[h] * 1.44269504088896340736f - base) : 0.f;
-  for (int w = 0; w < 4; ++w) {
-    const float f = __builtin_amdgcn_exp2f(stats[w][0] - base);
-    s += sums[w][threadIdx.x] * f, l += stats[w][1] * f;
+  const float sink = a.o.sinks ? a.o.sinks[h] * 1.44269504088896340736f : -INFINITY;
+  float base = sink;
+  for (int w = 0; w < kJoin / 64; ++w) base = fmaxf(base, wave_m[w]);
+  if (base == -INFINITY) base = 0.f;
+#pragma unroll
+  for (int i = 0; i < (int)(kPartUnits / kJoin); ++i) {
+    const uint32_t p = tid + i * kJoin;
+    if (p >= pt.parts) break;
+    weight[p] = __builtin_amdgcn_exp2f(m[i] - base);
+    l += stat[2 * (unit0 + (uint64_t)p * units * 16) + 1] * weight[p];
   }
+  l = wave_sum(l);
+  if (lane == 0) wave_l[wave] = l;
+  __syncthreads();
+  f32x4 acc = {0, 0, 0, 0};
+  const float* src = a.part + unit0 * D + 4 * (tid % L);
+#pragma unroll 8
+  for (uint32_t p = tid / L; p < pt.parts; p += G)
+    acc += *reinterpret_cast<const f32x4*>(src + (uint64_t)p * units * 16 * D) * weight[p];
+  *reinterpret_cast<f32x4*>(&sums[4 * tid]) = acc;
+  __syncthreads();
+  if (tid >= D) return;
+  float s = 0.f;
+  l = __builtin_amdgcn_exp2f(sink - base);
+  for (int g = 0; g < G; ++g) s += sums[g * D + tid];
+  for (int x = 0; x < kJoin / 64; ++x) l += wave_l[x];
   const float v = l == 0.f ? 0.f : s / l;
-  uint16_t* dst = static_cast<uint16_t*>(a.out.p) + (uint64_t)pt.b * a.out.ts + (uint64_t)h * a.out.hs + threadIdx.x;
+  uint16_t* dst = static_cast<uint16_t*>(a.out.p) + (uint64_t)pt.b * a.out.ts + (uint64_t)h * a.out.hs + tid;
   *dst = (uint16_t)(a.out.dtype == MR_F16 ? pack_f16(v, 0.f) : pack_bf16(v, 0.f));
 }
 
-template <int FMT, int D>
-void decode(hipStream_t s, const DecodeArgs& a, dim3 g) {
-  hipLaunchKernelGGL((k_attn_decode<FMT, D>), g, dim3(64 * kWaves), 0, s, a);
-}
+using DecodeKernel = void (*)(DecodeArgs);
 template <int FMT>
-void decode_fmt(hipStream_t s, uint32_t D, const DecodeArgs& a, dim3 g) {
-  if (D == 64) decode<FMT, 64>(s, a, g);
-  if (D == 128) decode<FMT, 128>(s, a, g);
-  if (D == 256) decode<FMT, 256>(s, a, g);
+DecodeKernel pick(uint32_t D) {
+  return D == 64 ? k_attn_decode<FMT, 64> : D == 128 ? k_attn_decode<FMT, 128> : k_attn_decode<FMT, 256>;
 }
-
-constexpr uint32_t kPartUnits = 1024;  // parts times key heads and head tiles: four workgroups to a CU
 
 }  // namespace
 
@@ -410,31 +447,29 @@ uint64_t attn_decode_scratch_bytes() { return 2ull * kPartUnits * 16 * (256 + 2)
 
 hipError_t launch_attn_decode(const Launch& K, const KvPages& kv, uint32_t format, uint32_t D, const Heads& q, uint32_t B,
                               const int32_t* len, const int32_t* table, uint32_t max_pages, const AttnOpts& o,
-                              const Heads& out, uint32_t* err, float* scratch) {
-  DecodeArgs a{kv, q, out, len, table, max_pages, B, q.n / kv.n_heads, 0, 0, o, err, scratch};
+                              const Heads& out, uint32_t* err, float* scratch, int n_cu) {
+  DecodeArgs a{kv, q, out, len, table, max_pages, B, q.n / kv.n_heads, 0, 0, 0, o, err, scratch};
   a.head_tiles = (a.heads + 15) / 16;
   const uint32_t units = kv.n_heads * a.head_tiles;
-  // chunks a sequence can have: no more parts than they allow
+  const DecodeKernel kernel = format == MR_KV_F16 ? pick<MR_KV_F16>(D) : format == MR_KV_MXINT8 ? pick<MR_KV_MXINT8>(D) : pick<MR_KV_MXFP4>(D);
+  int per_cu = 0;
+  hipError_t e = hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kernel, 64 * kWaves, 0);
+  if (e != hipSuccess) return e;
+  a.room = std::max<uint32_t>(1, (uint32_t)(std::max(1, per_cu) * n_cu) / units);
   const uint64_t cap = (uint64_t)max_pages << (kv.page_shift - 6);
-  const uint64_t chunks = o.window ? std::min<uint64_t>(cap, (o.window + 62ull) / 64 + 1) : cap;
-  a.parts = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(kPartUnits / units, (uint64_t)B * ((chunks + kMinPart - 1) / kMinPart)));
-  const bool split = a.parts > 1 && chunks > kMinPart;
-  // a sequence's last part need not be full
-  const dim3 g(split ? a.parts + B : B, units);
+  const uint64_t chunks = o.window ? std::min<uint64_t>(cap, (o.window + 62ull) / 64 + 1) : cap;  // of a sequence at most
+  a.parts = chunks <= kMinPart ? 1 : std::max<uint32_t>(1, kPartUnits / units);
   {
     ProfScope ps(K, "attn_decode");
-    if (format == MR_KV_F16) decode_fmt<MR_KV_F16>(K.s, D, a, g);
-    if (format == MR_KV_MXINT8) decode_fmt<MR_KV_MXINT8>(K.s, D, a, g);
-    if (format == MR_KV_MXFP4) decode_fmt<MR_KV_MXFP4>(K.s, D, a, g);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess || !split) return e;
+    hipLaunchKernelGGL(kernel, dim3(a.parts > 1 ? a.parts + B : B, units), dim3(64 * kWaves), 0, K.s, a);
+    e = hipGetLastError();
+    if (e != hipSuccess || a.parts == 1) return e;
   }
   ProfScope ps(K, "attn_join");
-  // a split sequence has more than half of its parts full
-  const dim3 j(std::min(B, a.parts), q.n);
-  if (D == 64) hipLaunchKernelGGL((k_attn_join<64>), j, dim3(256), 0, K.s, a);
-  if (D == 128) hipLaunchKernelGGL((k_attn_join<128>), j, dim3(256), 0, K.s, a);
-  if (D == 256) hipLaunchKernelGGL((k_attn_join<256>), j, dim3(256), 0, K.s, a);
+  const dim3 j(std::min(B, a.parts), q.n), blk(kJoin);
+  if (D == 64) hipLaunchKernelGGL((k_attn_join<64>), j, blk, 0, K.s, a);
+  if (D == 128) hipLaunchKernelGGL((k_attn_join<128>), j, blk, 0, K.s, a);
+  if (D == 256) hipLaunchKernelGGL((k_attn_join<256>), j, blk, 0, K.s, a);
   return hipGetLastError();
 }
 
