@@ -148,7 +148,7 @@ int mr_attn_decode(mr_ctx* ctx, const mr_kv* kv, const mr_heads* q, uint32_t n_s
  * nothing). cu_q, cu_k: n_seqs + 1 offsets that do not decrease; offsets outside the rows are taken as
  * the nearest inside, decreasing ones as empty sequences, both with an error at mr_sync. Rows of `out`
  * in no sequence are left as they are. q, k, v and out: F16 or BF16, all the same; head_dim 64, 128 or
- * 256. opts NULL: defaults. */
+ * 256; token strides of k and v below 2^24 elements. opts NULL: defaults. */
 int mr_attn_prefill(mr_ctx* ctx, uint32_t head_dim, const mr_heads* q, uint32_t n_q, const mr_heads* k,
                     const mr_heads* v, uint32_t n_k, uint32_t n_seqs, const int32_t* cu_q, const int32_t* cu_k,
                     const mr_attn_opts* opts, const mr_heads* out);

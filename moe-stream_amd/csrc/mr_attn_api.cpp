@@ -345,6 +345,8 @@ int mr_attn_prefill(mr_ctx* c, uint32_t D, const mr_heads* q, uint32_t nq, const
   if ((rc = check_qo(c, hq, ho, hk.n)) || (rc = take_opts(c, opts, D, &o))) return rc;
   if (hk.dtype != hq.dtype || hv.dtype != hq.dtype)
     return fail(c, MR_E_UNSUPPORTED, "k and v must have the type of q");
+  if (hk.ts >= 1ull << 24 || hv.ts >= 1ull << 24)  // 64 rows within the 32-bit offsets of a buffer load
+    return fail(c, MR_E_INVAL, "k or v has a token stride of 2^24 elements or more");
   if (!cu_q || !cu_k || misaligned(cu_q, 4) || misaligned(cu_k, 4))
     return fail(c, MR_E_INVAL, "cu_q or cu_k is NULL or not 4-byte aligned");
   if (nq > 0x7FFFFFFFu || nk > 0x7FFFFFFFu || n_seqs >= 0x7FFFFFFFu) return fail(c, MR_E_INVAL, "2^31 rows or more");

@@ -18,6 +18,7 @@ typedef short i16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kRows = 128;  // query rows of a workgroup: 4 waves of 32
 constexpr int kKeys = 64;   // keys of a step
+constexpr float kSlack = 8.f;
 
 template <bool BF>
 __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
@@ -43,12 +44,14 @@ __device__ __forceinline__ int v_piece(int row, int c) {
   return D == 64 ? c ^ (((row >> 1) & 1) * 4) : c ^ ((row & 3) * 4);
 }
 
-// 16 bytes a lane from global memory straight to LDS, lane i's to dst + 16 i (dst: the same for all lanes).
-// Not the compiler's builtin: after that it waits for all of them before each LDS read that it cannot tell
-// apart, here for the next step's tile in the middle of this one. The caller waits (vmcnt) and synchronises.
-__device__ __forceinline__ void load_lds16(const void* src, const void* dst) {
-  const uint32_t to = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)dst);
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(src) : "memory", "m0");
+// 16 bytes a lane from base + offset (a lane's own) straight to LDS, lane i's to dst + 16 i (the same dst for all
+// lanes); zeros for lanes whose offset is `bytes` or more. Not the compiler's builtin: after that it waits for
+// all of them before each LDS read that it cannot tell apart, here for the next step's tile in the middle of
+// this one. The caller waits (vmcnt) and synchronises.
+__device__ __forceinline__ void load_lds16(uint64_t base, uint32_t bytes, uint32_t offset, uint32_t dst) {
+  const u32x4 rsrc = {(uint32_t)base, (uint32_t)(base >> 32), bytes, 0x00020000u};
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane(dst)), "v"(offset), "s"(rsrc)
+               : "memory", "m0");
 }
 
 struct PrefillArgs {
@@ -95,6 +98,7 @@ __device__ __forceinline__ bool find_tile(const PrefillArgs& a, int tile, bool r
     before += __shfl(sum, 63, kWave);
   }
   if (found < 0) return false;
+  found = __builtin_amdgcn_readfirstlane(found), found_before = __builtin_amdgcn_readfirstlane(found_before);
   p.q0 = in(a.cu_q[found], a.nq), p.q1 = in(a.cu_q[found + 1], a.nq);
   p.k0 = in(a.cu_k[found], a.nk), p.k1 = max(p.k0, in(a.cu_k[found + 1], a.nk));
   const int tiles = (p.q1 - p.q0 + kRows - 1) / kRows;
@@ -125,7 +129,9 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
   int first = pl.k0;
   if (a.o.window) first = (int)max((int64_t)first, (int64_t)pl.row + diff + 1 - (int64_t)a.o.window);
   const int see_last = row + diff;
-  const int64_t see_first = a.o.window ? max((int64_t)pl.k0, (int64_t)see_last + 1 - (int64_t)a.o.window) : pl.k0;
+  const int64_t w = a.o.window ? (int64_t)a.o.window : (int64_t)1 << 32;
+  const int see_first = (int)max((int64_t)pl.k0, (int64_t)see_last + 1 - w);
+  const int wave_first = (int)max((int64_t)pl.k0, (int64_t)pl.row + wave * 32 + 31 + diff + 1 - w);  // of its last row
 
   const float c = fmaxf(fabsf(a.o.scale) * 1.44269504088896340736f, 0x1p-126f);  // above zero: a masked score stays -inf
   u32x4 qf[D / 16];
@@ -138,18 +144,24 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
 
   const uint16_t* kp = static_cast<const uint16_t*>(a.k.p) + (uint64_t)hk * a.k.hs;
   const uint16_t* vp = static_cast<const uint16_t*>(a.v.p) + (uint64_t)hk * a.v.hs;
-  // Copies the 64 keys from k0 on into buffer b; rows behind the last key repeat it (they are masked).
-  auto fetch = [&](int k0, int b) {
-    uint16_t* kd = lds + b * 2 * kTile;
-    uint16_t* vd = kd + kTile;
+  // Copies the 64 keys from k0 on into buffer b, zeros for rows behind the last key. A wave's load is kStep / 4
+  // rows; the pieces' order within a row is the same every 16 rows.
+  constexpr int kLoads = kTile / 8 / 256, kStep = kKeys / kLoads, kOff = kStep < 16 ? 16 / kStep : 1;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint16_t*)lds;
+  uint32_t k_off[kOff], v_off;
+  {
+    const int r = (wave * 64 + lane) / P, cp = lane % P;
 #pragma unroll
-    for (int i = 0; i < kTile / 8 / 256; ++i) {
-      const int piece = (i * 4 + wave) * 64 + lane, r = piece / P, cp = piece % P;
-      const uint64_t key = (uint64_t)min(k0 + r, last);
-      const uint16_t* ks = kp + key * a.k.ts + 8 * k_piece<D>(r, cp);
-      const uint16_t* vs = vp + key * a.v.ts + 8 * v_piece<D>(r, cp);
-      load_lds16(ks, kd + (i * 4 + wave) * 512);
-      load_lds16(vs, vd + (i * 4 + wave) * 512);
+    for (int i = 0; i < kOff; ++i) k_off[i] = (uint32_t)(r * a.k.ts + 8 * k_piece<D>(r + i * kStep, cp)) * 2;
+    v_off = (uint32_t)(r * a.v.ts + 8 * v_piece<D>(r, cp)) * 2;
+  }
+  auto fetch = [&](int k0, int b) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int key = k0 + i * kStep, rows = min(last + 1 - key, kStep);
+      const uint32_t dst = lds0 + b * 4 * kTile + (i * 4 + wave) * 1024;
+      load_lds16((uint64_t)kp + (uint64_t)key * a.k.ts * 2, rows > 0 ? (uint32_t)((rows - 1) * a.k.ts + D) * 2 : 0, k_off[i % kOff], dst);
+      load_lds16((uint64_t)vp + (uint64_t)key * a.v.ts * 2, rows > 0 ? (uint32_t)((rows - 1) * a.v.ts + D) * 2 : 0, v_off, dst + 2 * kTile);
     }
   };
 
@@ -188,10 +200,8 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
         const u32x4 kf = *reinterpret_cast<const u32x4*>(kt + r * D + 8 * k_piece<D>(r, 2 * i + half));
         s[t] = mfma32<BF>(kf, qf[i], s[t]);
       }
-    // whether every row of the wave sees every key of the step
-    const bool whole = k0 + kKeys - 1 <= pl.row + wave * 32 + diff && k0 >= see_first;
-    const bool masked = !__all(whole);
-    if (masked) {
+    // not every row of the wave sees every key of the step
+    if (k0 + kKeys - 1 > pl.row + wave * 32 + diff || k0 < wave_first) {
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -204,9 +214,10 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
 #pragma unroll
     for (int i = 1; i < 32; ++i) top = fmaxf(top, s[i >> 4][i & 15]);
     top = max_xor32(top) * c;
-    const float m1 = fmaxf(m, top);
-    if (__any(m1 > m)) {
-      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m1);
+    // The base follows the maximum only when it has fallen kSlack behind: p is at most 2^kSlack, and the sums'
+    // rescaling is left out of nearly every step.
+    if (__any(top > m + kSlack)) {
+      const float m1 = fmaxf(m, top), f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m1);
       l *= f;
 #pragma unroll
       for (int t = 0; t < ND; ++t) acc[t] *= f;

@@ -215,6 +215,7 @@ def test_prefill_refusals(hctx):
             (dict(k=M.Heads(X, 3, M.F16), v=M.Heads(X, 3, M.F16)), M.MR_E_INVAL, "evenly"),
             (dict(cu_q=None), M.MR_E_INVAL, "cu_q"), (dict(cu_k=X + 2), M.MR_E_INVAL, "cu_k"),
             (dict(nq=1 << 31), M.MR_E_INVAL, "2^31"), (dict(scale=math.nan), M.MR_E_INVAL, "scale"),
+            (dict(k=M.Heads(X, 2, M.F16, token_stride=1 << 24)), M.MR_E_INVAL, "2^24"),
             (dict(k=M.Heads(X, 2, M.F16, token_stride=4)), M.MR_E_INVAL, "stride"), (dict(v=None), M.MR_E_INVAL, "v is NULL")):
         refused(status, text, call, **kw)
 
