@@ -107,10 +107,10 @@ __device__ __forceinline__ bool find_tile(const PrefillArgs& a, int tile, bool r
 }
 
 // One tile of rows and one head. p is 0 where a row does not see a key, but 0 * inf and 0 * NaN are NaN: a tile
-// that ends with such a sum returns false and is done over with `CAREFUL`, where values that are not finite
+// that ends with such a sum returns false and is done over with `careful`, where values that are not finite
 // are taken out of the steps that some row sees in part, and added at the end to the rows that see them.
-template <int D, bool BF, bool CAREFUL>
-__device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds, int unit) {
+template <int D, bool BF>
+__device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds, int unit, bool careful) {
   constexpr int P = D / 8, ND = D / 32;  // 16-byte pieces of a row; 32-wide tiles of a head
   constexpr int kTile = kKeys * D;       // elements of a key or value tile
   constexpr uint32_t kTop = BF ? 0x7F80u : 0x7C00u;  // the exponent of infinities and NaN
@@ -118,7 +118,7 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
 
   const int h = unit / a.n_tiles, hk = h / (int)(a.q.n / a.k.n);
   Place pl;
-  if (!find_tile(a, unit % a.n_tiles, unit == 0 && !CAREFUL, pl)) return true;
+  if (!find_tile(a, unit % a.n_tiles, unit == 0 && !careful, pl)) return true;
 
   // keys [first, last] of the tile's rows; a row r sees those up to r + diff, from r + diff - window + 1 on
   const int diff = pl.k1 - pl.q1;
@@ -155,13 +155,20 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
     for (int i = 0; i < kOff; ++i) k_off[i] = (uint32_t)(r * a.k.ts + 8 * k_piece<D>(r + i * kStep, cp)) * 2;
     v_off = (uint32_t)(r * a.v.ts + 8 * v_piece<D>(r, cp)) * 2;
   }
-  auto fetch = [&](int k0, int b) {
+  auto fetch_k = [&](int k0, int b) {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int key = k0 + i * kStep, rows = min(last + 1 - key, kStep);
-      const uint32_t dst = lds0 + b * 4 * kTile + (i * 4 + wave) * 1024;
-      load_lds16((uint64_t)kp + (uint64_t)key * a.k.ts * 2, rows > 0 ? (uint32_t)((rows - 1) * a.k.ts + D) * 2 : 0, k_off[i % kOff], dst);
-      load_lds16((uint64_t)vp + (uint64_t)key * a.v.ts * 2, rows > 0 ? (uint32_t)((rows - 1) * a.v.ts + D) * 2 : 0, v_off, dst + 2 * kTile);
+      load_lds16((uint64_t)kp + (uint64_t)key * a.k.ts * 2, rows > 0 ? (uint32_t)((rows - 1) * a.k.ts + D) * 2 : 0, k_off[i % kOff],
+                 lds0 + b * 4 * kTile + (i * 4 + wave) * 1024);
+    }
+  };
+  auto fetch_v = [&](int k0, int b) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int key = k0 + i * kStep, rows = min(last + 1 - key, kStep);
+      load_lds16((uint64_t)vp + (uint64_t)key * a.v.ts * 2, rows > 0 ? (uint32_t)((rows - 1) * a.v.ts + D) * 2 : 0, v_off,
+                 lds0 + b * 4 * kTile + 2 * kTile + (i * 4 + wave) * 1024);
     }
   };
 
@@ -178,44 +185,45 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
     l = half == 0 && m != -INFINITY ? 1.f : 0.f;  // the two halves of a row are added at the end
   }
 
-  if (first <= last) fetch(first, 0);
-  for (int k0 = first, b = 0; k0 <= last; k0 += kKeys, b ^= 1) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (k0 + kKeys <= last) fetch(k0 + kKeys, b ^ 1);
-    const uint16_t* kt = lds + b * 2 * kTile;
-    uint16_t* vt = lds + b * 2 * kTile + kTile;
-    if (CAREFUL && edge(k0)) {
-      for (int i = threadIdx.x; i < kTile; i += 256)
-        if ((vt[i] & kTop) == kTop) vt[i] = 0;
-      __syncthreads();
+  constexpr int NI = D / 16, NV = 4 * ND;
+  // Operand of the scores: 8 elements of key 32 t + n; of the values: V^T of 16 keys and 32 elements, where lane
+  // 16 g + i of a transposing read takes row (i >> 2), elements 4 (i & 3).. and gets column i of four rows.
+  // Pieces are exclusive-ored into place, and so are the parts' addresses from the first one's.
+  const int vr = 4 * half + ((lane & 15) >> 2), ve = (lane & 16) + 4 * (lane & 3);
+  uint32_t k_at = lds0 + 2 * (n * D + 8 * k_piece<D>(n, half));
+  uint32_t v_at = lds0 + 2 * (kTile + vr * D + 8 * v_piece<D>(vr, ve >> 3) + (ve & 7));
+  auto key_part = [&](int b, int t, int i) {
+    const uint32_t at = (k_at ^ (32 * i)) + b * 4 * kTile + t * 64 * D;
+    return *(const __attribute__((address_space(3))) u32x4*)(uintptr_t)at;
+  };
+  auto value_part = [&](int b, int q) {
+    const uint32_t at = (v_at ^ (64 * (q % ND))) + b * 4 * kTile + (q / ND) * 32 * D;
+    const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(uintptr_t)at));
+    const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(uintptr_t)(at + 16 * D)));
+    return u32x4{x.x, x.y, y.x, y.y};
+  };
+  auto mask = [&](int k0, f32x16& s0, f32x16& s1) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int key = k0 + 8 * (i >> 2) + 4 * half + (i & 3);
+      if (key > see_last || key < see_first) s0[i] = -INFINITY;
+      if (key + 32 > see_last || key + 32 < see_first) s1[i] = -INFINITY;
     }
-
-    f32x16 s[2] = {};
+  };
+  auto maximum = [&](const f32x16& s0, const f32x16& s1) {
+    float top = s0[0];
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        const int r = 32 * t + n;
-        const u32x4 kf = *reinterpret_cast<const u32x4*>(kt + r * D + 8 * k_piece<D>(r, 2 * i + half));
-        s[t] = mfma32<BF>(kf, qf[i], s[t]);
-      }
-    // not every row of the wave sees every key of the step
+    for (int i = 0; i < 16; ++i) top = fmaxf(fmaxf(top, s0[i]), s1[i]);
+    return top;
+  };
+  // Masks the scores of the keys from k0 on and moves the base m, with the sums, if their maximum has left it
+  // kSlack behind: p is at most 2^kSlack, and nearly no step rescales.
+  auto settle = [&](int k0, f32x16& s0, f32x16& s1, float top) {
     if (k0 + kKeys - 1 > pl.row + wave * 32 + diff || k0 < wave_first) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int key = k0 + 32 * t + 8 * (i >> 2) + 4 * half + (i & 3);
-          if (key > see_last || key < see_first) s[t][i] = -INFINITY;
-        }
+      mask(k0, s0, s1);
+      top = maximum(s0, s1);
     }
-    float top = s[0][0];
-#pragma unroll
-    for (int i = 1; i < 32; ++i) top = fmaxf(top, s[i >> 4][i & 15]);
     top = max_xor32(top) * c;
-    // The base follows the maximum only when it has fallen kSlack behind: p is at most 2^kSlack, and the sums'
-    // rescaling is left out of nearly every step.
     if (__any(top > m + kSlack)) {
       const float m1 = fmaxf(m, top), f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m1);
       l *= f;
@@ -223,35 +231,57 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
       for (int t = 0; t < ND; ++t) acc[t] *= f;
       m = m1;
     }
-    const float base = m == -INFINITY ? 0.f : m;
-    u32x4 pf[4];
-#pragma unroll
-    for (int i = 0; i < 32; i += 2) {
-      const float p0 = __builtin_amdgcn_exp2f(fmaf(s[i >> 4][i & 15], c, -base));
-      const float p1 = __builtin_amdgcn_exp2f(fmaf(s[i >> 4][(i & 15) + 1], c, -base));
-      l += p0 + p1;
-      pf[i >> 3][(i >> 1) & 3] = pack16<BF>(p0, p1);
-    }
-    // V^T: lane 16 g + i of a read takes row (i >> 2), elements 4 (i & 3).. and gets column i of four rows
-    auto values = [&](int t, int cc) {
-      u32x4 vf;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int r = 16 * cc + 8 * j + 4 * half + ((lane & 15) >> 2), e = 32 * t + (lane & 16) + 4 * (lane & 3);
-        const uint16_t* src = vt + r * D + 8 * v_piece<D>(r, e >> 3) + (e & 7);
-        const i16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)src);
-        const u32x2 w2 = __builtin_bit_cast(u32x2, w);
-        vf[2 * j] = w2.x, vf[2 * j + 1] = w2.y;
+  };
+  // Two of a step's 32 weights (pair i): rounded into the operand of the second product.
+  auto weigh = [&](const f32x16& s0, const f32x16& s1, int i, float base, u32x4 (&pf)[4]) {
+    const f32x16& s = i < 8 ? s0 : s1;
+    const float p0 = __builtin_amdgcn_exp2f(fmaf(s[2 * (i & 7)], c, -base));
+    const float p1 = __builtin_amdgcn_exp2f(fmaf(s[2 * (i & 7) + 1], c, -base));
+    l += p0 + p1;
+    pf[i >> 2][i & 3] = pack16<BF>(p0, p1);
+  };
+  if (first <= last) {
+    fetch_k(first, 0), fetch_v(first, 0);
+    for (int k0 = first, b = 0; k0 <= last; k0 += kKeys, b ^= 1) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      if (k0 + kKeys <= last) fetch_k(k0 + kKeys, b ^ 1), fetch_v(k0 + kKeys, b ^ 1);
+      if (careful && edge(k0)) {
+        uint16_t* vt = lds + b * 2 * kTile + kTile;
+        for (int i = threadIdx.x; i < kTile; i += 256)
+          if ((vt[i] & kTop) == kTop) vt[i] = 0;
+        __syncthreads();
       }
-      return vf;
-    };
+      f32x16 s0 = {}, s1 = {};
+      u32x4 pf[4], kf[2][2], vf[3];
+      kf[0][0] = key_part(b, 0, 0), kf[0][1] = key_part(b, 1, 0);
 #pragma unroll
-    for (int t = 0; t < ND; ++t)
+      for (int i = 0; i < NI; ++i) {
+        if (i + 1 < NI) kf[(i + 1) & 1][0] = key_part(b, 0, i + 1), kf[(i + 1) & 1][1] = key_part(b, 1, i + 1);
+        if (i >= NI - 2) vf[i - (NI - 2)] = value_part(b, i - (NI - 2));
+        s0 = mfma32<BF>(kf[i & 1][0], qf[i], s0);
+        s1 = mfma32<BF>(kf[i & 1][1], qf[i], s1);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      settle(k0, s0, s1, maximum(s0, s1));
+      const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
-      for (int cc = 0; cc < 4; ++cc) acc[t] = mfma32<BF>(values(t, cc), pf[cc], acc[t]);
+      for (int x = 0; x < 4; ++x) weigh(s0, s1, x, base, pf);
+#pragma unroll
+      for (int q = 0; q < NV; ++q) {
+        if (q + 2 < NV) vf[(q + 2) % 3] = value_part(b, q + 2);
+        acc[q % ND] = mfma32<BF>(vf[q % 3], pf[q / ND], acc[q % ND]);
+        // the next 16 keys' weights
+        if (q / ND < 3) {
+#pragma unroll
+          for (int x = 4 * (q / ND + 1) + q % ND * 4 / ND; x < 4 * (q / ND + 1) + (q % ND + 1) * 4 / ND; ++x) weigh(s0, s1, x, base, pf);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
   }
 
-  if (!CAREFUL) {
+  if (!careful) {
     bool odd = false;
 #pragma unroll
     for (int t = 0; t < ND; ++t)
@@ -272,7 +302,7 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
         *reinterpret_cast<u32x2*>(dst + 32 * t + 8 * (i >> 2) + 4 * half) = w;
       }
   }
-  if (CAREFUL) {
+  if (careful) {
     __syncthreads();  // the rows are written
     const int d = threadIdx.x % D;
     for (int k0 = first; k0 <= last; k0 += kKeys) {
@@ -293,16 +323,15 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
 }
 
 template <int D, bool BF>
-__global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void k_attn_prefill(PrefillArgs a) {
-  __shared__ __attribute__((aligned(16))) uint16_t lds[4 * kKeys * D];
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_prefill(PrefillArgs a) {
+  __shared__ __attribute__((aligned(1024))) uint16_t lds[4 * kKeys * D];  // rows at multiples of their length
   // Workgroups go to the 8 XCDs in turn. Each XCD gets a contiguous share of the (head, tile) pairs, so that
   // the query heads that share keys find them in one L2.
   const int units = a.n_tiles * (int)a.q.n, per = (units + 7) / 8;
-  int unit = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  const int unit = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
   if ((int)(blockIdx.x >> 3) >= per || unit >= units) return;
-  if (attend_tile<D, BF, false>(a, lds, unit)) return;
-  asm volatile("" : "+s"(unit));  // nothing of the first pass stays in registers for the second
-  attend_tile<D, BF, true>(a, lds, unit);
+  for (bool careful = false; !attend_tile<D, BF>(a, lds, unit, careful); careful = true) {
+  }
 }
 
 }  // namespace
