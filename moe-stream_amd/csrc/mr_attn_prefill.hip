@@ -191,14 +191,14 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
   // 16 g + i of a transposing read takes row (i >> 2), elements 4 (i & 3).. and gets column i of four rows.
   // Pieces are exclusive-ored into place, and so are the parts' addresses from the first one's.
   const int vr = 4 * half + ((lane & 15) >> 2), ve = (lane & 16) + 4 * (lane & 3);
-  uint32_t k_at = lds0 + 2 * (n * D + 8 * k_piece<D>(n, half));
-  uint32_t v_at = lds0 + 2 * (kTile + vr * D + 8 * v_piece<D>(vr, ve >> 3) + (ve & 7));
-  auto key_part = [&](int b, int t, int i) {
-    const uint32_t at = (k_at ^ (32 * i)) + b * 4 * kTile + t * 64 * D;
+  const uint32_t k_at = lds0 + 2 * (n * D + 8 * k_piece<D>(n, half));
+  const uint32_t v_at = lds0 + 2 * (kTile + vr * D + 8 * v_piece<D>(vr, ve >> 3) + (ve & 7));
+  auto key_part = [&](uint32_t k_at, int t, int i) {
+    const uint32_t at = (k_at ^ (32 * i)) + t * 64 * D;
     return *(const __attribute__((address_space(3))) u32x4*)(uintptr_t)at;
   };
-  auto value_part = [&](int b, int q) {
-    const uint32_t at = (v_at ^ (64 * (q % ND))) + b * 4 * kTile + (q / ND) * 32 * D;
+  auto value_part = [&](uint32_t v_at, int q) {
+    const uint32_t at = (v_at ^ (64 * (q % ND))) + (q / ND) * 32 * D;
     const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(uintptr_t)at));
     const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(uintptr_t)(at + 16 * D)));
     return u32x4{x.x, x.y, y.x, y.y};
@@ -208,7 +208,8 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
   auto settle = [&](int k0, f32x16& s0, f32x16& s1) {
     const int x = k0 + 4 * half;
     if (k0 + kKeys - 1 > pl.row + wave * 32 + diff) {
-      const int most = see_last - x;
+      int most = see_last - x;
+      asm volatile("" : "+v"(most));  // a branch: the compiler would do this in every step
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         s0[i] = 8 * (i >> 2) + (i & 3) > most ? -INFINITY : s0[i];
@@ -216,7 +217,8 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
       }
     }
     if (k0 < wave_first) {
-      const int least = see_first - x;
+      int least = see_first - x;
+      asm volatile("" : "+v"(least));
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         s0[i] = 8 * (i >> 2) + (i & 3) < least ? -INFINITY : s0[i];
@@ -257,16 +259,18 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
       }
       // keys behind all of the wave's rows, or in front of all their windows
       if (k0 > pl.row + wave * 32 + 31 + diff || k0 + kKeys <= wave_least) continue;
+      uint32_t kb = k_at + b * 4 * kTile, vb = v_at + b * 4 * kTile;
+      asm("" : "+v"(kb), "+v"(vb));  // the parts' addresses are worked out from here, not kept
       f32x16 s0 = {}, s1 = {};
       u32x4 pf[4], kf[2][2], vf[3];
-      kf[0][0] = key_part(b, 0, 0), kf[0][1] = key_part(b, 1, 0);
+      kf[0][0] = key_part(kb, 0, 0), kf[0][1] = key_part(kb, 1, 0);
       // Waves between their matrix instructions give way to those at them: the two of a SIMD then take turns
       // (8192 tokens, heads of 128: 675 -> 649 us).
       __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
-        if (i + 1 < NI) kf[(i + 1) & 1][0] = key_part(b, 0, i + 1), kf[(i + 1) & 1][1] = key_part(b, 1, i + 1);
-        if (i >= NI - 2) vf[i - (NI - 2)] = value_part(b, i - (NI - 2));
+        if (i + 1 < NI) kf[(i + 1) & 1][0] = key_part(kb, 0, i + 1), kf[(i + 1) & 1][1] = key_part(kb, 1, i + 1);
+        if (i >= NI - 2) vf[i - (NI - 2)] = value_part(vb, i - (NI - 2));
         s0 = mfma32<BF>(kf[i & 1][0], qf[i], s0);
         s1 = mfma32<BF>(kf[i & 1][1], qf[i], s1);
         __builtin_amdgcn_sched_barrier(0);
@@ -279,7 +283,7 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
       __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int q = 0; q < NV; ++q) {
-        if (q + 2 < NV) vf[(q + 2) % 3] = value_part(b, q + 2);
+        if (q + 2 < NV) vf[(q + 2) % 3] = value_part(vb, q + 2);
         acc[q % ND] = mfma32<BF>(vf[q % 3], pf[q / ND], acc[q % ND]);
         // the next 16 keys' weights
         if (q / ND < 3) {
