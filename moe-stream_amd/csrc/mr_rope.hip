@@ -21,52 +21,66 @@ struct RopeArgs {
 // with 8 of its elements as two quads: in the half layout elements 4u.. and rotary/2 + 4u.., so that a
 // lane holds both members of its pairs; adjacent quads in the interleaved layout and behind the rotated
 // part. The angle is reduced to a fraction of a turn in 64 bits (f32 would lose 2^-24 of a far position's
-// angle), the sine and cosine of that fraction are taken in f32, once per token and pair.
-__global__ __launch_bounds__(256) void k_qk_norm_rope(RopeArgs a, int L, int rows_per_wg) {
-  __shared__ float cs[256], sn[256];
-  const int t = blockIdx.x, half = a.rotary / 2;
+// angle), the sine and cosine of that fraction are taken in f32, once per token and pair, while the first R
+// heads of each lane group are on their way from memory. Memory bounds it: ROPE_FIGURES.
+template <int R>
+__global__ __launch_bounds__(256) void k_qk_norm_rope(RopeArgs a, int L) {
+  __shared__ __attribute__((aligned(16))) float cs[256], sn[256];
+  const int t = blockIdx.x, half = a.rotary / 2, per = 256 / L;
+  const int u = threadIdx.x & (L - 1);
+  const bool turn = u < a.rotary / 8, apart = turn && !a.interleaved;
+  const int e0 = apart ? 4 * u : 8 * u, e1 = apart ? half + 4 * u : 8 * u + 4;
+  const int row0 = blockIdx.y * per * R + threadIdx.x / L;
+  auto live = [&](int i) { return row0 + i * per < a.rows && u < a.D / 8; };
+  f32x4 x[R], y[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int row = row0 + i * per, q = row < (int)a.in[0].n;
+    if (!live(i)) continue;
+    const uint64_t o = q ? (uint64_t)t * a.in[0].ts + (uint64_t)row * a.in[0].hs
+                         : (uint64_t)t * a.in[1].ts + (uint64_t)(row - (int)a.in[0].n) * a.in[1].hs;
+    const void* p = q ? a.in[0].p : a.in[1].p;
+    x[i] = load4(p, a.in[0].dtype, o + e0);
+    y[i] = load4(p, a.in[0].dtype, o + e1);
+  }
   if ((int)threadIdx.x < half) {
-    const double x = (double)a.pos[t] * a.turns[threadIdx.x];
+    const double z = (double)a.pos[t] * a.turns[threadIdx.x];
     float s, c;
-    sincospif(2.f * (float)(x - rint(x)), &s, &c);
+    sincospif(2.f * (float)(z - rint(z)), &s, &c);
     cs[threadIdx.x] = c * a.mul, sn[threadIdx.x] = s * a.mul;
   }
   __syncthreads();
-  const int u = threadIdx.x & (L - 1), U = a.D / 8;
-  const int row0 = blockIdx.y * rows_per_wg, row1 = min(a.rows, row0 + rows_per_wg);
-  const bool turn = u < a.rotary / 8, apart = turn && !a.interleaved;
-  const int e0 = apart ? 4 * u : 8 * u, e1 = apart ? half + 4 * u : 8 * u + 4;
-  for (int base = row0; base < row1; base += 256 / L) {
-    const int row = base + threadIdx.x / L;
-    const bool live = row < row1 && u < U;
-    const int side = row >= (int)a.in[0].n, h = side ? row - a.in[0].n : row;
-    f32x4 x = {0, 0, 0, 0}, y = x;
-    if (live) {
-      const uint64_t o = (uint64_t)t * a.in[side].ts + (uint64_t)h * a.in[side].hs;
-      x = load4(a.in[side].p, a.in[side].dtype, o + e0);
-      y = load4(a.in[side].p, a.in[side].dtype, o + e1);
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int row = row0 + i * per, q = row < (int)a.in[0].n;
+    const float* w = q ? a.w[0] : a.w[1];
+    f32x4 v = x[i], z = y[i];
+    float s = v.x * v.x + v.y * v.y + v.z * v.z + v.w * v.w + z.x * z.x + z.y * z.y + z.z * z.z + z.w * z.w;
+    if (a.w[0] || a.w[1]) {
+      if (!live(i)) s = 0.f;
+      for (int o = L / 2; o >= 1; o >>= 1) s += __shfl_xor(s, o, kWave);
     }
-    const float* w = a.w[side];
-    float s = x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w + y.x * y.x + y.y * y.y + y.z * y.z + y.w * y.w;
-    for (int o = L / 2; o >= 1; o >>= 1) s += __shfl_xor(s, o, kWave);
-    if (!live) continue;
+    if (!live(i)) continue;
     if (w) {
       const float inv = 1.f / sqrtf(s / (float)a.D + a.eps);
-      const f32x4 wx = *reinterpret_cast<const f32x4*>(w + e0), wy = *reinterpret_cast<const f32x4*>(w + e1);
-      x = x * inv * wx, y = y * inv * wy;
+      v = v * inv * *reinterpret_cast<const f32x4*>(w + e0);
+      z = z * inv * *reinterpret_cast<const f32x4*>(w + e1);
     }
-    if (apart) {
+    if (turn) {
       const f32x4 c = *reinterpret_cast<const f32x4*>(cs + 4 * u), n = *reinterpret_cast<const f32x4*>(sn + 4 * u);
-      const f32x4 p = x * c - y * n, q = y * c + x * n;
-      x = p, y = q;
-    } else if (turn) {
-      const f32x4 c = *reinterpret_cast<const f32x4*>(cs + 4 * u), n = *reinterpret_cast<const f32x4*>(sn + 4 * u);
-      x = f32x4{x.x * c.x - x.y * n.x, x.y * c.x + x.x * n.x, x.z * c.y - x.w * n.y, x.w * c.y + x.z * n.y};
-      y = f32x4{y.x * c.z - y.y * n.z, y.y * c.z + y.x * n.z, y.z * c.w - y.w * n.w, y.w * c.w + y.z * n.w};
+      if (apart) {
+        const f32x4 b = v * c - z * n;
+        z = z * c + v * n, v = b;
+      } else {
+        v = f32x4{v.x * c.x - v.y * n.x, v.y * c.x + v.x * n.x, v.z * c.y - v.w * n.y, v.w * c.y + v.z * n.y};
+        z = f32x4{z.x * c.z - z.y * n.z, z.y * c.z + z.x * n.z, z.z * c.w - z.w * n.w, z.w * c.w + z.z * n.w};
+      }
     }
-    const uint64_t o = (uint64_t)t * a.out[side].ts + (uint64_t)h * a.out[side].hs;
-    store4(a.out[side].p, a.out[side].dtype, o + e0, x);
-    store4(a.out[side].p, a.out[side].dtype, o + e1, y);
+    const uint64_t o = q ? (uint64_t)t * a.out[0].ts + (uint64_t)row * a.out[0].hs
+                         : (uint64_t)t * a.out[1].ts + (uint64_t)(row - (int)a.in[0].n) * a.out[1].hs;
+    void* p = q ? a.out[0].p : a.out[1].p;
+    store4(p, a.out[0].dtype, o + e0, v);
+    store4(p, a.out[0].dtype, o + e1, z);
   }
 }
 
@@ -80,8 +94,15 @@ hipError_t launch_qk_norm_rope(const Launch& K, const mr_rope& r, const Heads& q
              r.d.layout == MR_ROPE_INTERLEAVED, (int)(q.n + k.n)};
   int L = 1;
   while (L < a.D / 8) L *= 2;
-  const int per = 256 / L;
-  hipLaunchKernelGGL(k_qk_norm_rope, dim3(T, (a.rows + per - 1) / per), dim3(256), 0, K.s, a, L, per);
+  // Up to four heads to a lane group, so that one workgroup's sines serve more of them, as long as that leaves
+  // each CU eight workgroups.
+  const int per = 256 / L, need = (a.rows + per - 1) / per;
+  const int R = (int)std::max<uint64_t>(1, std::min<uint64_t>(std::min(4, need), (uint64_t)T * need / 2048));
+  const dim3 g(T, (need + R - 1) / R);
+  if (R == 1) hipLaunchKernelGGL(k_qk_norm_rope<1>, g, dim3(256), 0, K.s, a, L);
+  if (R == 2) hipLaunchKernelGGL(k_qk_norm_rope<2>, g, dim3(256), 0, K.s, a, L);
+  if (R == 3) hipLaunchKernelGGL(k_qk_norm_rope<3>, g, dim3(256), 0, K.s, a, L);
+  if (R == 4) hipLaunchKernelGGL(k_qk_norm_rope<4>, g, dim3(256), 0, K.s, a, L);
   return hipGetLastError();
 }
 
