@@ -58,16 +58,4 @@ __device__ __forceinline__ float scale_value(uint32_t b) {
   return FMT == MR_KV_MXFP4 ? bits_f32(b << 23) : h2f(b << 8);
 }
 
-// Element d of token s of a chunk.
-template <int FMT, int D>
-__device__ __forceinline__ float kv_value(const uint8_t* chunk, bool key, int s, int d) {
-  using L = KvLayout<FMT, D>;
-  const uint8_t* p = chunk + (key ? L::k_off(s, d) : L::v_off(s, d));
-  if (FMT == MR_KV_F16) return h2f(*reinterpret_cast<const uint16_t*>(p));
-  const float sc = scale_value<FMT>(chunk[key ? L::ks_off(s, d >> 5) : L::vs_off(s, d >> 5)]);
-  if (FMT == MR_KV_MXINT8) return sc * (float)*reinterpret_cast<const int8_t*>(p);
-  const bool high = key ? d & 1 : d & 16;
-  return sc * fp4_value(high ? *p >> 4 : *p & 15u);
-}
-
 }  // namespace mr

@@ -43,106 +43,283 @@ __device__ __forceinline__ uint8_t* find(const KvPages& kv, int slot, uint32_t h
   return kv.at(page, head, ((uint32_t)slot & ((1u << kv.page_shift) - 1u)) >> 6);
 }
 
-constexpr int kWriteTokens = 64;  // tokens of a workgroup
+constexpr int kWindow = 64;  // tokens of a workgroup
 
-// blockIdx: 64 tokens, head, keys or values. D/8 lanes to a token; a lane has 8 elements as two quads:
-// adjacent ones for keys, 32 b + 4 w and 32 b + 16 + 4 w for values (the halves of a byte).
-template <int FMT, int D>
-__global__ __launch_bounds__(256) void k_kv_write(KvPages kv, Heads kin, Heads vin, int T, const int32_t* __restrict__ slots,
-                                                  uint32_t* err) {
+// Runs of tokens that fill a chunk. The values' bytes of a token lie 16 bytes apart in its chunk; where 64 tokens
+// in a row go to (come from) the 64 slots of a chunk in order, as most of a prompt's do, they are put together
+// in LDS and the chunk is moved whole (8191 tokens, 4 heads of 128, 8 bits: KV_FIGURES). The workgroup in whose
+// window of 64 tokens such a run begins does all of it; the tokens of no run are done one by one.
+struct Runs {
+  uint64_t start, single;  // bit i: token i of the window begins a run; is in none, and has a slot
+};
+// slots[i] is the slot of token i - 63 of the window, -1 outside the call. All threads call.
+__device__ __forceinline__ Runs find_runs(const KvPages& kv, const int32_t* __restrict__ slots, int T, int t0, int (&sl)[192],
+                                          uint64_t (&breaks)[3]) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  if (tid < 192) {
+    const int t = t0 - 63 + tid;
+    sl[tid] = tid < 191 && t >= 0 && t < T ? slots[t] : -1;
+  }
+  __syncthreads();
+  if (tid < 192) {
+    const bool b = tid == 191 || sl[tid] < 0 || (uint32_t)sl[tid + 1] != (uint32_t)sl[tid] + 1u;
+    const uint64_t m = __ballot(b);
+    if (lane == 0) breaks[tid >> 6] = m;
+  }
+  __syncthreads();
+  const int slot = sl[63 + lane], first = 63 + lane - (slot & 63);  // where this token's run would begin
+  bool in_run = false;
+  if (slot >= 0 && first >= 0 && ((uint32_t)slot >> kv.page_shift) < kv.n_pages) {
+    const int w = first >> 6, o = first & 63;
+    const uint64_t lo = breaks[w] >> o, hi = o && w < 2 ? breaks[w + 1] << (64 - o) : 0;
+    in_run = ((lo | hi) & 0x7FFFFFFFFFFFFFFFull) == 0;
+  }
+  Runs r;
+  r.start = __ballot(in_run && (slot & 63) == 0);
+  r.single = __ballot(!in_run && slot >= 0);
+  return r;
+}
+
+// Two quads of a token: 8 adjacent elements for keys, 32 b + 4 w and 32 b + 16 + 4 w for values (the two
+// nibbles of a byte).
+struct Quads {
+  int e0, e1;
+};
+__device__ __forceinline__ Quads quads(bool key, int u) {
+  const int e0 = key ? 8 * u : 32 * (u >> 2) + 4 * (u & 3);
+  return Quads{e0, key ? e0 + 4 : e0 + 16};
+}
+
+// Where the values' bytes lie in a chunk and in an image of its values: codes, then scales.
+template <int FMT, int D, bool IMAGE>
+struct Place {
   using L = KvLayout<FMT, D>;
-  constexpr int U = D / 8;
-  const bool key = blockIdx.z == 0;
-  const Heads in = key ? kin : vin;
-  const int u = threadIdx.x % U, h = blockIdx.y;
-  const int e0 = key ? 8 * u : 32 * (u >> 2) + 4 * (u & 3), e1 = key ? e0 + 4 : e0 + 16;
-  const int t1 = min(T, (int)(blockIdx.x + 1) * kWriteTokens);
-  for (int t = blockIdx.x * kWriteTokens + threadIdx.x / U; t < t1; t += 256 / U) {
-    int s = 0;
-    uint8_t* chunk = find(kv, slots[t], h, err, s);
-    if (!chunk) continue;  // the same for the U lanes of a token
-    const uint64_t o = (uint64_t)t * in.ts + (uint64_t)h * in.hs;
-    const f32x4 x = load4(in.p, in.dtype, o + e0), y = load4(in.p, in.dtype, o + e1);
-    float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-    float top = 0.f;
+  static __device__ __forceinline__ int v(int s, int d) { return L::v_off(s, d) - (IMAGE ? L::kV : 0); }
+  static __device__ __forceinline__ int vs(int s, int b) { return L::vs_off(s, b) - (IMAGE ? L::kVs - L::kCodes : 0); }
+};
+
+// Quantises 8 elements of token s and stores them in the chunk, or in an LDS image of its values. The 4 lanes of a
+// block call together.
+template <int FMT, int D, bool KEY, bool IMAGE = false>
+__device__ __forceinline__ void put(uint8_t* chunk, int s, int u, f32x4 x, f32x4 y) {
+  using L = KvLayout<FMT, D>;
+  using P = Place<FMT, D, IMAGE>;
+  const Quads e = quads(KEY, u);
+  float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+  float top = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = finite_or_inf(v[i]), top = fmaxf(top, fabsf(v[i]));
-    if (FMT == MR_KV_F16) {
+  for (int i = 0; i < 8; ++i) v[i] = finite_or_inf(v[i]), top = fmaxf(top, fabsf(v[i]));
+  if constexpr (FMT == MR_KV_F16) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = fminf(fmaxf(v[i], -65504.f), 65504.f);
-      if (key) {
-        *reinterpret_cast<u32x4*>(chunk + L::k_off(s, e0)) =
-            u32x4{pack_f16(v[0], v[1]), pack_f16(v[2], v[3]), pack_f16(v[4], v[5]), pack_f16(v[6], v[7])};
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          *reinterpret_cast<_Float16*>(chunk + L::v_off(s, (i < 4 ? e0 : e1 - 4) + i)) = (_Float16)v[i];
-      }
-      continue;
-    }
-    top = fmaxf(top, __shfl_xor(top, 1, kWave));
-    top = fmaxf(top, __shfl_xor(top, 2, kWave));
-    const int e = block_exp<FMT>(top);
-    const float inv = bits_f32((uint32_t)(127 - e) << 23);
-    uint32_t c[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = code<FMT>(v[i] * inv);
-    if ((u & 3) == 0) chunk[key ? L::ks_off(s, u >> 2) : L::vs_off(s, u >> 2)] = (uint8_t)scale_byte<FMT>(e);
-    if (key) {
-      if (FMT == MR_KV_MXFP4) {
-        uint32_t w = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w |= c[i] << (4 * i);
-        *reinterpret_cast<uint32_t*>(chunk + L::k_off(s, e0)) = w;
-      } else {
-        *reinterpret_cast<u32x2*>(chunk + L::k_off(s, e0)) =
-            u32x2{c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24};
-      }
+    for (int i = 0; i < 8; ++i) v[i] = fminf(fmaxf(v[i], -65504.f), 65504.f);
+    if constexpr (KEY) {
+      *reinterpret_cast<u32x4*>(chunk + L::k_off(s, e.e0)) =
+          u32x4{pack_f16(v[0], v[1]), pack_f16(v[2], v[3]), pack_f16(v[4], v[5]), pack_f16(v[6], v[7])};
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if (FMT == MR_KV_MXFP4) {
-          chunk[L::v_off(s, e0 + i)] = (uint8_t)(c[i] | c[i + 4] << 4);
+        *reinterpret_cast<_Float16*>(chunk + P::v(s, e.e0 + i)) = (_Float16)v[i];
+        *reinterpret_cast<_Float16*>(chunk + P::v(s, e.e1 + i)) = (_Float16)v[i + 4];
+      }
+    }
+  } else {
+    top = fmaxf(top, __shfl_xor(top, 1, kWave));
+    top = fmaxf(top, __shfl_xor(top, 2, kWave));
+    const int ex = block_exp<FMT>(top);
+    const float inv = bits_f32((uint32_t)(127 - ex) << 23);
+    uint32_t c[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = code<FMT>(v[i] * inv);
+    if ((u & 3) == 0) chunk[KEY ? L::ks_off(s, u >> 2) : P::vs(s, u >> 2)] = (uint8_t)scale_byte<FMT>(ex);
+    if constexpr (KEY && FMT == MR_KV_MXFP4) {
+      uint32_t w = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w |= c[i] << (4 * i);
+      *reinterpret_cast<uint32_t*>(chunk + L::k_off(s, e.e0)) = w;
+    } else if constexpr (KEY) {
+      *reinterpret_cast<u32x2*>(chunk + L::k_off(s, e.e0)) =
+          u32x2{c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24};
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (FMT == MR_KV_MXFP4) {
+          chunk[P::v(s, e.e0 + i)] = (uint8_t)(c[i] | c[i + 4] << 4);
         } else {
-          chunk[L::v_off(s, e0 + i)] = (uint8_t)c[i];
-          chunk[L::v_off(s, e1 + i)] = (uint8_t)c[i + 4];
+          chunk[P::v(s, e.e0 + i)] = (uint8_t)c[i];
+          chunk[P::v(s, e.e1 + i)] = (uint8_t)c[i + 4];
         }
       }
     }
   }
 }
 
+// The same elements back.
+template <int FMT, int D, bool KEY, bool IMAGE = false>
+__device__ __forceinline__ void get(const uint8_t* chunk, int s, int u, f32x4& x, f32x4& y) {
+  using L = KvLayout<FMT, D>;
+  using P = Place<FMT, D, IMAGE>;
+  const Quads e = quads(KEY, u);
+  float v[8];
+  if constexpr (FMT == MR_KV_F16) {
+    if constexpr (KEY) {
+      const u32x4 w = *reinterpret_cast<const u32x4*>(chunk + L::k_off(s, e.e0));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f32x2 p = unpack_f16(w[i]);
+        v[2 * i] = p.x, v[2 * i + 1] = p.y;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = (float)*reinterpret_cast<const _Float16*>(chunk + P::v(s, e.e0 + i));
+        v[i + 4] = (float)*reinterpret_cast<const _Float16*>(chunk + P::v(s, e.e1 + i));
+      }
+    }
+  } else {
+    const float sc = scale_value<FMT>(chunk[KEY ? L::ks_off(s, u >> 2) : P::vs(s, u >> 2)]);
+    if constexpr (KEY && FMT == MR_KV_MXFP4) {
+      const uint32_t w = *reinterpret_cast<const uint32_t*>(chunk + L::k_off(s, e.e0));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = sc * fp4_value(w >> (4 * i) & 15u);
+    } else if constexpr (KEY) {
+      const u32x2 w = *reinterpret_cast<const u32x2*>(chunk + L::k_off(s, e.e0));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = sc * (float)(int8_t)(w[i >> 2] >> (8 * (i & 3)));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (FMT == MR_KV_MXFP4) {
+          const uint32_t b = chunk[P::v(s, e.e0 + i)];
+          v[i] = sc * fp4_value(b & 15u), v[i + 4] = sc * fp4_value(b >> 4);
+        } else {
+          v[i] = sc * (float)(int8_t)chunk[P::v(s, e.e0 + i)], v[i + 4] = sc * (float)(int8_t)chunk[P::v(s, e.e1 + i)];
+        }
+      }
+    }
+  }
+  x = f32x4{v[0], v[1], v[2], v[3]}, y = f32x4{v[4], v[5], v[6], v[7]};
+}
+
+__device__ __forceinline__ uint64_t at(const Heads& h, int t, int head) { return (uint64_t)t * h.ts + (uint64_t)head * h.hs; }
+
+// Moves 16 bytes a thread; the scales lie behind the keys' scales in the chunk, behind the codes in the image.
+template <int FMT, int D, bool STORE>
+__device__ __forceinline__ void move_image(uint8_t* chunk, uint8_t* image) {
+  using L = KvLayout<FMT, D>;
+  for (int i = threadIdx.x * 16; i < L::kCodes + L::kScales; i += 256 * 16) {
+    u32x4* g = reinterpret_cast<u32x4*>(chunk + (i < L::kCodes ? L::kV + i : L::kVs + i - L::kCodes));
+    u32x4* l = reinterpret_cast<u32x4*>(image + i);
+    if (STORE) *g = *l;
+    else *l = *g;
+  }
+}
+
+// blockIdx: 64 tokens, head, keys or values. D / 8 lanes to a token.
+template <int FMT, int D>
+__global__ __launch_bounds__(256) void k_kv_write(KvPages kv, Heads kin, Heads vin, int T, const int32_t* __restrict__ slots,
+                                                  uint32_t* err) {
+  using L = KvLayout<FMT, D>;
+  constexpr int U = D / 8, N = 256 / U;  // lanes of a token, tokens at a time
+  const int u = threadIdx.x % U, i0 = threadIdx.x / U, h = blockIdx.y, t0 = blockIdx.x * kWindow;
+  if (blockIdx.z == 0) {
+    const Quads e = quads(true, u);
+#pragma unroll 4
+    for (int i = i0; i < kWindow; i += N) {
+      if (t0 + i >= T) break;
+      int s = 0;
+      uint8_t* chunk = find(kv, slots[t0 + i], h, err, s);
+      if (!chunk) continue;  // the same for the lanes of a token
+      const uint64_t o = at(kin, t0 + i, h);
+      put<FMT, D, true>(chunk, s, u, load4(kin.p, kin.dtype, o + e.e0), load4(kin.p, kin.dtype, o + e.e1));
+    }
+    return;
+  }
+  __shared__ int sl[192];
+  __shared__ uint64_t breaks[3];
+  __shared__ __attribute__((aligned(16))) uint8_t image[L::kCodes + L::kScales];
+  const Quads e = quads(false, u);
+  const Runs r = find_runs(kv, slots, T, t0, sl, breaks);
+  for (uint64_t todo = r.start; todo; todo &= todo - 1) {
+    const int b = __ffsll((unsigned long long)todo) - 1;
+#pragma unroll 4
+    for (int i = i0; i < 64; i += N) {
+      const uint64_t o = at(vin, t0 + b + i, h);
+      put<FMT, D, false, true>(image, i, u, load4(vin.p, vin.dtype, o + e.e0), load4(vin.p, vin.dtype, o + e.e1));
+    }
+    __syncthreads();
+    int s;
+    move_image<FMT, D, true>(find(kv, sl[63 + b], h, err, s), image);
+    __syncthreads();
+  }
+  for (int i = i0; i < kWindow; i += N) {
+    if (!(r.single >> i & 1)) continue;
+    int s = 0;
+    uint8_t* chunk = find(kv, sl[63 + i], h, err, s);
+    if (!chunk) continue;
+    const uint64_t o = at(vin, t0 + i, h);
+    put<FMT, D, false>(chunk, s, u, load4(vin.p, vin.dtype, o + e.e0), load4(vin.p, vin.dtype, o + e.e1));
+  }
+}
+
 template <int FMT, int D>
 __global__ __launch_bounds__(256) void k_kv_read(KvPages kv, int T, const int32_t* __restrict__ slots, Heads kout, Heads vout,
                                                  uint32_t* err) {
-  constexpr int U = D / 8;
-  const bool key = blockIdx.z == 0;
-  const Heads out = key ? kout : vout;
-  if (!out.p) return;
-  const int u = threadIdx.x % U, h = blockIdx.y;
-  const int e0 = key ? 8 * u : 32 * (u >> 2) + 4 * (u & 3), e1 = key ? e0 + 4 : e0 + 16;
-  const int t1 = min(T, (int)(blockIdx.x + 1) * kWriteTokens);
-  for (int t = blockIdx.x * kWriteTokens + threadIdx.x / U; t < t1; t += 256 / U) {
-    int s = 0;
-    const uint8_t* chunk = find(kv, slots[t], h, err, s);
-    f32x4 x = {0, 0, 0, 0}, y = x;
-    if (chunk) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[i] = kv_value<FMT, D>(chunk, key, s, e0 + i);
-        y[i] = kv_value<FMT, D>(chunk, key, s, e1 + i);
-      }
+  using L = KvLayout<FMT, D>;
+  constexpr int U = D / 8, N = 256 / U;
+  const int u = threadIdx.x % U, i0 = threadIdx.x / U, h = blockIdx.y, t0 = blockIdx.x * kWindow;
+  if (blockIdx.z == 0) {
+    if (!kout.p) return;
+    const Quads e = quads(true, u);
+#pragma unroll 4
+    for (int i = i0; i < kWindow; i += N) {
+      if (t0 + i >= T) break;
+      int s = 0;
+      const uint8_t* chunk = find(kv, slots[t0 + i], h, err, s);
+      f32x4 x = {0, 0, 0, 0}, y = x;
+      if (chunk) get<FMT, D, true>(chunk, s, u, x, y);
+      const uint64_t o = at(kout, t0 + i, h);
+      store4(kout.p, kout.dtype, o + e.e0, x), store4(kout.p, kout.dtype, o + e.e1, y);
     }
-    const uint64_t o = (uint64_t)t * out.ts + (uint64_t)h * out.hs;
-    store4(out.p, out.dtype, o + e0, x);
-    store4(out.p, out.dtype, o + e1, y);
+    return;
+  }
+  if (!vout.p) return;
+  __shared__ int sl[192];
+  __shared__ uint64_t breaks[3];
+  __shared__ __attribute__((aligned(16))) uint8_t image[L::kCodes + L::kScales];
+  const Quads e = quads(false, u);
+  const Runs r = find_runs(kv, slots, T, t0, sl, breaks);
+  for (uint64_t todo = r.start; todo; todo &= todo - 1) {
+    const int b = __ffsll((unsigned long long)todo) - 1;
+    int s;
+    move_image<FMT, D, false>(find(kv, sl[63 + b], h, err, s), image);
+    __syncthreads();
+#pragma unroll 4
+    for (int i = i0; i < 64; i += N) {
+      f32x4 x, y;
+      get<FMT, D, false, true>(image, i, u, x, y);
+      const uint64_t o = at(vout, t0 + b + i, h);
+      store4(vout.p, vout.dtype, o + e.e0, x), store4(vout.p, vout.dtype, o + e.e1, y);
+    }
+    __syncthreads();
+  }
+  // the others, and zeros for tokens without a slot
+  for (int i = i0; i < kWindow; i += N) {
+    if (t0 + i >= T) break;
+    const int slot = sl[63 + i];
+    if (slot >= 0 && !(r.single >> i & 1)) continue;
+    int s = 0;
+    const uint8_t* chunk = find(kv, slot, h, err, s);
+    f32x4 x = {0, 0, 0, 0}, y = x;
+    if (chunk) get<FMT, D, false>(chunk, s, u, x, y);
+    const uint64_t o = at(vout, t0 + i, h);
+    store4(vout.p, vout.dtype, o + e.e0, x), store4(vout.p, vout.dtype, o + e.e1, y);
   }
 }
 
 template <int FMT>
 hipError_t write_fmt(const Launch& K, const KvPages& kv, uint32_t D, const Heads& k, const Heads& v, uint32_t T,
                      const int32_t* slots, uint32_t* err) {
-  const dim3 g((T + kWriteTokens - 1) / kWriteTokens, kv.n_heads, 2);
+  const dim3 g((T + kWindow - 1) / kWindow, kv.n_heads, 2);
   if (D == 64) hipLaunchKernelGGL((k_kv_write<FMT, 64>), g, dim3(256), 0, K.s, kv, k, v, (int)T, slots, err);
   if (D == 128) hipLaunchKernelGGL((k_kv_write<FMT, 128>), g, dim3(256), 0, K.s, kv, k, v, (int)T, slots, err);
   if (D == 256) hipLaunchKernelGGL((k_kv_write<FMT, 256>), g, dim3(256), 0, K.s, kv, k, v, (int)T, slots, err);
@@ -152,7 +329,7 @@ hipError_t write_fmt(const Launch& K, const KvPages& kv, uint32_t D, const Heads
 template <int FMT>
 hipError_t read_fmt(const Launch& K, const KvPages& kv, uint32_t D, uint32_t T, const int32_t* slots, const Heads& k,
                     const Heads& v, uint32_t* err) {
-  const dim3 g((T + kWriteTokens - 1) / kWriteTokens, kv.n_heads, 2);
+  const dim3 g((T + kWindow - 1) / kWindow, kv.n_heads, 2);
   if (D == 64) hipLaunchKernelGGL((k_kv_read<FMT, 64>), g, dim3(256), 0, K.s, kv, (int)T, slots, k, v, err);
   if (D == 128) hipLaunchKernelGGL((k_kv_read<FMT, 128>), g, dim3(256), 0, K.s, kv, (int)T, slots, k, v, err);
   if (D == 256) hipLaunchKernelGGL((k_kv_read<FMT, 256>), g, dim3(256), 0, K.s, kv, (int)T, slots, k, v, err);
