@@ -90,74 +90,66 @@ __device__ __forceinline__ Quads quads(bool key, int u) {
   return Quads{e0, key ? e0 + 4 : e0 + 16};
 }
 
-// Where the values' bytes lie in a chunk and in an image of its values: codes, then scales.
-template <int FMT, int D, bool IMAGE>
-struct Place {
-  using L = KvLayout<FMT, D>;
-  static __device__ __forceinline__ int v(int s, int d) { return L::v_off(s, d) - (IMAGE ? L::kV : 0); }
-  static __device__ __forceinline__ int vs(int s, int b) { return L::vs_off(s, b) - (IMAGE ? L::kVs - L::kCodes : 0); }
-};
-
-// Quantises 8 elements of token s and stores them in the chunk, or in an LDS image of its values. The 4 lanes of a
-// block call together.
-template <int FMT, int D, bool KEY, bool IMAGE = false>
-__device__ __forceinline__ void put(uint8_t* chunk, int s, int u, f32x4 x, f32x4 y) {
-  using L = KvLayout<FMT, D>;
-  using P = Place<FMT, D, IMAGE>;
-  const Quads e = quads(KEY, u);
+// Codes of 8 elements (for F16 the f16 bits), and the block's exponent. The 4 lanes of a block call together.
+template <int FMT>
+__device__ __forceinline__ int quantise(f32x4 x, f32x4 y, uint32_t (&c)[8]) {
   float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
   float top = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = finite_or_inf(v[i]), top = fmaxf(top, fabsf(v[i]));
   if constexpr (FMT == MR_KV_F16) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = fminf(fmaxf(v[i], -65504.f), 65504.f);
-    if constexpr (KEY) {
-      *reinterpret_cast<u32x4*>(chunk + L::k_off(s, e.e0)) =
-          u32x4{pack_f16(v[0], v[1]), pack_f16(v[2], v[3]), pack_f16(v[4], v[5]), pack_f16(v[6], v[7])};
+    for (int i = 0; i < 8; ++i) c[i] = pack_f16(fminf(fmaxf(v[i], -65504.f), 65504.f), 0.f);
+    return 0;
+  }
+  top = fmaxf(top, __shfl_xor(top, 1, kWave));
+  top = fmaxf(top, __shfl_xor(top, 2, kWave));
+  const int ex = block_exp<FMT>(top);
+  const float inv = bits_f32((uint32_t)(127 - ex) << 23);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) c[i] = code<FMT>(v[i] * inv);
+  return ex;
+}
+
+// Quantises 8 elements of token s and stores them in the chunk. The 4 lanes of a block call together.
+template <int FMT, int D, bool KEY>
+__device__ __forceinline__ void put(uint8_t* chunk, int s, int u, f32x4 x, f32x4 y) {
+  using L = KvLayout<FMT, D>;
+  const Quads e = quads(KEY, u);
+  uint32_t c[8];
+  const int ex = quantise<FMT>(x, y, c);
+  if (FMT != MR_KV_F16 && (u & 3) == 0) chunk[KEY ? L::ks_off(s, u >> 2) : L::vs_off(s, u >> 2)] = (uint8_t)scale_byte<FMT>(ex);
+  if constexpr (KEY) {
+    uint8_t* p = chunk + L::k_off(s, e.e0);
+    if constexpr (FMT == MR_KV_F16) {
+      *reinterpret_cast<u32x4*>(p) = u32x4{c[0] | c[1] << 16, c[2] | c[3] << 16, c[4] | c[5] << 16, c[6] | c[7] << 16};
+    } else if constexpr (FMT == MR_KV_MXINT8) {
+      *reinterpret_cast<u32x2*>(p) = u32x2{c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24};
     } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        *reinterpret_cast<_Float16*>(chunk + P::v(s, e.e0 + i)) = (_Float16)v[i];
-        *reinterpret_cast<_Float16*>(chunk + P::v(s, e.e1 + i)) = (_Float16)v[i + 4];
-      }
-    }
-  } else {
-    top = fmaxf(top, __shfl_xor(top, 1, kWave));
-    top = fmaxf(top, __shfl_xor(top, 2, kWave));
-    const int ex = block_exp<FMT>(top);
-    const float inv = bits_f32((uint32_t)(127 - ex) << 23);
-    uint32_t c[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = code<FMT>(v[i] * inv);
-    if ((u & 3) == 0) chunk[KEY ? L::ks_off(s, u >> 2) : P::vs(s, u >> 2)] = (uint8_t)scale_byte<FMT>(ex);
-    if constexpr (KEY && FMT == MR_KV_MXFP4) {
       uint32_t w = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) w |= c[i] << (4 * i);
-      *reinterpret_cast<uint32_t*>(chunk + L::k_off(s, e.e0)) = w;
-    } else if constexpr (KEY) {
-      *reinterpret_cast<u32x2*>(chunk + L::k_off(s, e.e0)) =
-          u32x2{c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24};
-    } else {
+      *reinterpret_cast<uint32_t*>(p) = w;
+    }
+  } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (FMT == MR_KV_MXFP4) {
-          chunk[P::v(s, e.e0 + i)] = (uint8_t)(c[i] | c[i + 4] << 4);
-        } else {
-          chunk[P::v(s, e.e0 + i)] = (uint8_t)c[i];
-          chunk[P::v(s, e.e1 + i)] = (uint8_t)c[i + 4];
-        }
+    for (int i = 0; i < 4; ++i) {
+      uint8_t *lo = chunk + L::v_off(s, e.e0 + i), *hi = chunk + L::v_off(s, e.e1 + i);
+      if constexpr (FMT == MR_KV_MXFP4) {
+        *lo = (uint8_t)(c[i] | c[i + 4] << 4);
+      } else if constexpr (FMT == MR_KV_MXINT8) {
+        *lo = (uint8_t)c[i], *hi = (uint8_t)c[i + 4];
+      } else {
+        *reinterpret_cast<uint16_t*>(lo) = (uint16_t)c[i], *reinterpret_cast<uint16_t*>(hi) = (uint16_t)c[i + 4];
       }
     }
   }
 }
 
 // The same elements back.
-template <int FMT, int D, bool KEY, bool IMAGE = false>
+template <int FMT, int D, bool KEY>
 __device__ __forceinline__ void get(const uint8_t* chunk, int s, int u, f32x4& x, f32x4& y) {
   using L = KvLayout<FMT, D>;
-  using P = Place<FMT, D, IMAGE>;
   const Quads e = quads(KEY, u);
   float v[8];
   if constexpr (FMT == MR_KV_F16) {
@@ -171,12 +163,12 @@ __device__ __forceinline__ void get(const uint8_t* chunk, int s, int u, f32x4& x
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        v[i] = (float)*reinterpret_cast<const _Float16*>(chunk + P::v(s, e.e0 + i));
-        v[i + 4] = (float)*reinterpret_cast<const _Float16*>(chunk + P::v(s, e.e1 + i));
+        v[i] = (float)*reinterpret_cast<const _Float16*>(chunk + L::v_off(s, e.e0 + i));
+        v[i + 4] = (float)*reinterpret_cast<const _Float16*>(chunk + L::v_off(s, e.e1 + i));
       }
     }
   } else {
-    const float sc = scale_value<FMT>(chunk[KEY ? L::ks_off(s, u >> 2) : P::vs(s, u >> 2)]);
+    const float sc = scale_value<FMT>(chunk[KEY ? L::ks_off(s, u >> 2) : L::vs_off(s, u >> 2)]);
     if constexpr (KEY && FMT == MR_KV_MXFP4) {
       const uint32_t w = *reinterpret_cast<const uint32_t*>(chunk + L::k_off(s, e.e0));
 #pragma unroll
@@ -189,10 +181,10 @@ __device__ __forceinline__ void get(const uint8_t* chunk, int s, int u, f32x4& x
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if constexpr (FMT == MR_KV_MXFP4) {
-          const uint32_t b = chunk[P::v(s, e.e0 + i)];
+          const uint32_t b = chunk[L::v_off(s, e.e0 + i)];
           v[i] = sc * fp4_value(b & 15u), v[i + 4] = sc * fp4_value(b >> 4);
         } else {
-          v[i] = sc * (float)(int8_t)chunk[P::v(s, e.e0 + i)], v[i + 4] = sc * (float)(int8_t)chunk[P::v(s, e.e1 + i)];
+          v[i] = sc * (float)(int8_t)chunk[L::v_off(s, e.e0 + i)], v[i + 4] = sc * (float)(int8_t)chunk[L::v_off(s, e.e1 + i)];
         }
       }
     }
@@ -202,6 +194,78 @@ __device__ __forceinline__ void get(const uint8_t* chunk, int s, int u, f32x4& x
 
 __device__ __forceinline__ uint64_t at(const Heads& h, int t, int head) { return (uint64_t)t * h.ts + (uint64_t)head * h.hs; }
 
+// The values of tokens t .. t + 63 to an LDS image of a chunk's values (codes, then scales), and back. A thread has
+// 4 adjacent tokens: their codes of an element are adjacent too, a word (F16: two) of the image.
+template <int FMT, int D>
+__device__ __forceinline__ void put_run(uint8_t* image, const Heads& in, int t, int head) {
+  using L = KvLayout<FMT, D>;
+  constexpr int U = D / 8;
+  for (int i = threadIdx.x; i < U * 16; i += 256) {
+    const int u = i % U, s = 4 * (i / U);
+    const Quads e = quads(false, u);
+    f32x4 x[4], y[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint64_t o = at(in, t + s + j, head);
+      x[j] = load4(in.p, in.dtype, o + e.e0), y[j] = load4(in.p, in.dtype, o + e.e1);
+    }
+    uint32_t w[8] = {}, w2[8] = {}, sc = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t c[8];
+      const int ex = quantise<FMT>(x[j], y[j], c);
+      if (FMT != MR_KV_F16) sc |= scale_byte<FMT>(ex) << (8 * j);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (FMT == MR_KV_F16) (j < 2 ? w : w2)[k] |= c[k] << (16 * (j & 1));
+        else if (FMT == MR_KV_MXFP4) w[k & 3] |= c[k] << (8 * j + (k & 4));
+        else w[k] |= c[k] << (8 * j);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < (FMT == MR_KV_MXFP4 ? 4 : 8); ++k) {
+      uint8_t* p = image + L::v_off(s, (k < 4 ? e.e0 : e.e1 - 4) + k) - L::kV;
+      if (FMT == MR_KV_F16) *reinterpret_cast<u32x2*>(p) = u32x2{w[k], w2[k]};
+      else *reinterpret_cast<uint32_t*>(p) = w[k];
+    }
+    if (FMT != MR_KV_F16 && (u & 3) == 0) *reinterpret_cast<uint32_t*>(image + L::vs_off(s, u >> 2) - L::kVs + L::kCodes) = sc;
+  }
+}
+template <int FMT, int D>
+__device__ __forceinline__ void get_run(const uint8_t* image, const Heads& out, int t, int head) {
+  using L = KvLayout<FMT, D>;
+  constexpr int U = D / 8;
+  for (int i = threadIdx.x; i < U * 16; i += 256) {
+    const int u = i % U, s = 4 * (i / U);
+    const Quads e = quads(false, u);
+    uint32_t w[8] = {}, w2[8] = {}, sc = 0;
+#pragma unroll
+    for (int k = 0; k < (FMT == MR_KV_MXFP4 ? 4 : 8); ++k) {
+      const uint8_t* p = image + L::v_off(s, (k < 4 ? e.e0 : e.e1 - 4) + k) - L::kV;
+      if (FMT == MR_KV_F16) {
+        const u32x2 a = *reinterpret_cast<const u32x2*>(p);
+        w[k] = a.x, w2[k] = a.y;
+      } else {
+        w[k] = *reinterpret_cast<const uint32_t*>(p);
+      }
+    }
+    if (FMT != MR_KV_F16) sc = *reinterpret_cast<const uint32_t*>(image + L::vs_off(s, u >> 2) - L::kVs + L::kCodes);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float f = FMT == MR_KV_F16 ? 1.f : scale_value<FMT>(sc >> (8 * j) & 0xFFu);
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (FMT == MR_KV_F16) v[k] = h2f((j < 2 ? w : w2)[k] >> (16 * (j & 1)) & 0xFFFFu);
+        else if (FMT == MR_KV_MXFP4) v[k] = f * fp4_value(w[k & 3] >> (8 * j + (k & 4)) & 15u);
+        else v[k] = f * (float)(int8_t)(w[k] >> (8 * j));
+      }
+      const uint64_t o = at(out, t + s + j, head);
+      store4(out.p, out.dtype, o + e.e0, f32x4{v[0], v[1], v[2], v[3]});
+      store4(out.p, out.dtype, o + e.e1, f32x4{v[4], v[5], v[6], v[7]});
+    }
+  }
+}
 // Moves 16 bytes a thread; the scales lie behind the keys' scales in the chunk, behind the codes in the image.
 template <int FMT, int D, bool STORE>
 __device__ __forceinline__ void move_image(uint8_t* chunk, uint8_t* image) {
@@ -241,11 +305,7 @@ __global__ __launch_bounds__(256) void k_kv_write(KvPages kv, Heads kin, Heads v
   const Runs r = find_runs(kv, slots, T, t0, sl, breaks);
   for (uint64_t todo = r.start; todo; todo &= todo - 1) {
     const int b = __ffsll((unsigned long long)todo) - 1;
-#pragma unroll 4
-    for (int i = i0; i < 64; i += N) {
-      const uint64_t o = at(vin, t0 + b + i, h);
-      put<FMT, D, false, true>(image, i, u, load4(vin.p, vin.dtype, o + e.e0), load4(vin.p, vin.dtype, o + e.e1));
-    }
+    put_run<FMT, D>(image, vin, t0 + b, h);
     __syncthreads();
     int s;
     move_image<FMT, D, true>(find(kv, sl[63 + b], h, err, s), image);
@@ -293,13 +353,7 @@ __global__ __launch_bounds__(256) void k_kv_read(KvPages kv, int T, const int32_
     int s;
     move_image<FMT, D, false>(find(kv, sl[63 + b], h, err, s), image);
     __syncthreads();
-#pragma unroll 4
-    for (int i = i0; i < 64; i += N) {
-      f32x4 x, y;
-      get<FMT, D, false, true>(image, i, u, x, y);
-      const uint64_t o = at(vout, t0 + b + i, h);
-      store4(vout.p, vout.dtype, o + e.e0, x), store4(vout.p, vout.dtype, o + e.e1, y);
-    }
+    get_run<FMT, D>(image, vout, t0 + b, h);
     __syncthreads();
   }
   // the others, and zeros for tokens without a slot
