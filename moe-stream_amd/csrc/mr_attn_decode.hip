@@ -21,8 +21,7 @@ struct DecodeArgs {
   uint32_t max_pages, n_seqs;
   uint32_t heads;      // query heads of a key head
   uint32_t head_tiles; // tiles of 16 of them
-  uint32_t parts;      // full parts that all chunks are dealt out in at most; 1: a sequence a part
-  uint32_t room;       // parts that the CUs hold at once
+  uint32_t parts;      // parts that the CUs hold at once; 1: a sequence a part
   AttnOpts o;
   uint32_t* err;
   float* part;         // [slot][key head][head tile][16][D] sums, then [slot][..][16][2] maximum and sum
@@ -30,8 +29,16 @@ struct DecodeArgs {
 
 constexpr int kWaves = 4;
 constexpr uint32_t kPartUnits = 1024;  // most parts, times key heads and head tiles
-constexpr uint32_t kMinPart = kWaves;       // chunks of a part at least: one for each wave
-constexpr uint32_t kGoodPart = 4 * kWaves;  // chunks that make up for a part's beginning and end
+constexpr uint32_t kMinPart = kWaves;  // chunks of a part at least: one for each wave
+// Sequences that cannot have more chunks stay whole, which spares the second launch. One sequence of 1200 tokens whole
+// and in parts: 11.8 and 13.9 us (MXFP4, 4 heads of 128), 24.7 and 16.7 us (MXINT8, 2 heads of 256, where a chunk
+// takes a wave 4 us).
+__host__ __device__ inline uint32_t whole_chunks(uint32_t D) { return D == 256 ? 2 * kWaves : 5 * kWaves; }
+// Parts of all sequences at most. Those of split sequences, two or more of each, are then no more than `parts`.
+__host__ __device__ inline uint32_t part_limit(uint32_t parts, uint32_t n_seqs) {
+  const uint32_t some = n_seqs + parts / 2;
+  return parts > some ? parts : some;
+}
 
 // Which tokens of sequence b are seen, in chunks.
 struct Span {
@@ -59,9 +66,16 @@ struct Part {
   uint32_t b, part, parts, slot, size;
   Span sp;
 };
+// The sum over the wave in every lane, by the lane swaps and row moves of wave_sum_fast.
 __device__ __forceinline__ uint32_t wave_total(uint32_t v) {
-  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, kWave);
-  return v;
+  const auto a = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  v = a[0] + a[1];
+  const auto b = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = b[0] + b[1];
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xF, 0xF, false);  // row_ror:8
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xF, 0xF, false);  // row_ror:4
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, false);   // l ^ 2
+  return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, false);  // l ^ 1
 }
 __device__ __forceinline__ bool find_part(const DecodeArgs& a, uint32_t i, bool split_only, Part& r) {
   const uint32_t lane = threadIdx.x & 63;
@@ -72,11 +86,18 @@ __device__ __forceinline__ bool find_part(const DecodeArgs& a, uint32_t i, bool 
   }
   auto span = [&](uint32_t b) { return b < a.n_seqs ? span_of(a, b) : Span{}; };
   Span s = span(lane);
-  uint32_t all = s.chunks;
-  for (uint32_t b0 = 64; b0 < a.n_seqs; b0 += 64) all += span(b0 + lane).chunks;
-  all = wave_total(all);
-  // parts of kGoodPart chunks where that makes no fewer than the CUs hold at once, and no more than `parts`
-  r.size = max(max(kMinPart, (all + a.parts - 1) / a.parts), min(kGoodPart, (all + a.room - 1) / a.room));
+  // f(chunks) of every sequence, summed
+  auto sum_of = [&](auto f) {
+    uint32_t v = lane < a.n_seqs ? f((uint32_t)s.chunks) : 0;
+    for (uint32_t b0 = 64; b0 < a.n_seqs; b0 += 64)
+      if (b0 + lane < a.n_seqs) v += f((uint32_t)span_of(a, b0 + lane).chunks);
+    return wave_total(v);
+  };
+  // The smallest size, in steps of an eighth, at which the CUs hold all parts at once: a part more would run after
+  // the others, alone (32 sequences up to 24000: PART_FIGURES). Next to many sequences, the long ones are still split.
+  const uint32_t all = sum_of([](uint32_t c) { return c; }), most = part_limit(a.parts, a.n_seqs);
+  r.size = max(kMinPart, (all + a.parts - 1) / a.parts);
+  while (r.size < all && sum_of([&](uint32_t c) { return max(1u, (c + r.size - 1) / r.size); }) > most) r.size += (r.size + 7) / 8;
   uint32_t before = 0, slots = 0;
   for (uint32_t b0 = 0; b0 < a.n_seqs; b0 += 64) {
     if (b0) s = span(b0 + lane);
@@ -362,7 +383,7 @@ __global__ __launch_bounds__(64 * kWaves, (Tuning<FMT, D>::kPerSimd)) void k_att
     float* dst = a.part + unit * D;
 #pragma unroll
     for (int t = 0; t < NT; ++t) *reinterpret_cast<f32x4*>(dst + 16 * t + 4 * g) = acc[t];
-    float* st = a.part + (uint64_t)2 * a.parts * gridDim.y * 16 * D + unit * 2;
+    float* st = a.part + (uint64_t)a.parts * gridDim.y * 16 * D + unit * 2;
     if (g == 0) st[0] = m, st[1] = l;
     return;
   }
@@ -393,7 +414,7 @@ __global__ __launch_bounds__(kJoin) void k_attn_join(DecodeArgs a) {
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const uint32_t h = blockIdx.y, hk = h / a.heads, in = h % a.heads, units = a.kv.n_heads * a.head_tiles;
   const uint64_t unit0 = ((uint64_t)pt.slot * units + hk * a.head_tiles + in / 16) * 16 + in % 16;
-  const float* stat = a.part + (uint64_t)2 * a.parts * units * 16 * D;
+  const float* stat = a.part + (uint64_t)a.parts * units * 16 * D;
   float m[kPartUnits / kJoin], l = 0.f, top = -INFINITY;
 #pragma unroll
   for (int i = 0; i < (int)(kPartUnits / kJoin); ++i) {
@@ -436,32 +457,43 @@ __global__ __launch_bounds__(kJoin) void k_attn_join(DecodeArgs a) {
 }
 
 using DecodeKernel = void (*)(DecodeArgs);
+// The kernel of a format and width, and how many of its workgroups a CU holds.
+template <int FMT, int D>
+DecodeKernel pick(int& per_cu) {
+  static const int n = [] {
+    int v = 0;
+    return hipOccupancyMaxActiveBlocksPerMultiprocessor(&v, k_attn_decode<FMT, D>, 64 * kWaves, 0) == hipSuccess && v > 0 ? v : 1;
+  }();
+  per_cu = n;
+  return k_attn_decode<FMT, D>;
+}
 template <int FMT>
-DecodeKernel pick(uint32_t D) {
-  return D == 64 ? k_attn_decode<FMT, 64> : D == 128 ? k_attn_decode<FMT, 128> : k_attn_decode<FMT, 256>;
+DecodeKernel pick(uint32_t D, int& per_cu) {
+  return D == 64 ? pick<FMT, 64>(per_cu) : D == 128 ? pick<FMT, 128>(per_cu) : pick<FMT, 256>(per_cu);
 }
 
 }  // namespace
 
-uint64_t attn_decode_scratch_bytes() { return 2ull * kPartUnits * 16 * (256 + 2) * sizeof(float); }
+uint64_t attn_decode_scratch_bytes() { return (uint64_t)kPartUnits * 16 * (256 + 2) * sizeof(float); }
 
 hipError_t launch_attn_decode(const Launch& K, const KvPages& kv, uint32_t format, uint32_t D, const Heads& q, uint32_t B,
                               const int32_t* len, const int32_t* table, uint32_t max_pages, const AttnOpts& o,
                               const Heads& out, uint32_t* err, float* scratch, int n_cu) {
-  DecodeArgs a{kv, q, out, len, table, max_pages, B, q.n / kv.n_heads, 0, 0, 0, o, err, scratch};
+  DecodeArgs a{kv, q, out, len, table, max_pages, B, q.n / kv.n_heads, 0, 0, o, err, scratch};
   a.head_tiles = (a.heads + 15) / 16;
   const uint32_t units = kv.n_heads * a.head_tiles;
-  const DecodeKernel kernel = format == MR_KV_F16 ? pick<MR_KV_F16>(D) : format == MR_KV_MXINT8 ? pick<MR_KV_MXINT8>(D) : pick<MR_KV_MXFP4>(D);
-  int per_cu = 0;
-  hipError_t e = hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kernel, 64 * kWaves, 0);
-  if (e != hipSuccess) return e;
-  a.room = std::max<uint32_t>(1, (uint32_t)(std::max(1, per_cu) * n_cu) / units);
+  int per_cu = 1;
+  const DecodeKernel kernel = format == MR_KV_F16      ? pick<MR_KV_F16>(D, per_cu)
+                              : format == MR_KV_MXINT8 ? pick<MR_KV_MXINT8>(D, per_cu)
+                                                       : pick<MR_KV_MXFP4>(D, per_cu);
   const uint64_t cap = (uint64_t)max_pages << (kv.page_shift - 6);
   const uint64_t chunks = o.window ? std::min<uint64_t>(cap, (o.window + 62ull) / 64 + 1) : cap;  // of a sequence at most
-  a.parts = chunks <= kMinPart ? 1 : std::max<uint32_t>(1, kPartUnits / units);
+  const uint32_t room = std::min<uint32_t>(kPartUnits, per_cu * n_cu);
+  a.parts = chunks <= whole_chunks(D) ? 1 : std::max<uint32_t>(1, room / units);
+  hipError_t e;
   {
     ProfScope ps(K, "attn_decode");
-    hipLaunchKernelGGL(kernel, dim3(a.parts > 1 ? a.parts + B : B, units), dim3(64 * kWaves), 0, K.s, a);
+    hipLaunchKernelGGL(kernel, dim3(a.parts > 1 ? part_limit(a.parts, B) : B, units), dim3(64 * kWaves), 0, K.s, a);
     e = hipGetLastError();
     if (e != hipSuccess || a.parts == 1) return e;
   }
