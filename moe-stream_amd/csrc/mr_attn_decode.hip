@@ -103,12 +103,7 @@ __device__ __forceinline__ bool find_part(const DecodeArgs& a, uint32_t i, bool 
     if (b0) s = span(b0 + lane);
     const uint32_t n = b0 + lane < a.n_seqs ? max(1u, ((uint32_t)s.chunks + r.size - 1) / r.size) : 0;
     const uint32_t split = n > 1 ? n : 0, count = split_only ? split > 0 : n;
-    uint32_t sum = count, ssum = split;
-    if (a.n_seqs > 1)
-      for (int o = 1; o < 64; o *= 2) {
-        const uint32_t t = __shfl_up(sum, o, kWave), u = __shfl_up(ssum, o, kWave);
-        if ((int)lane >= o) sum += t, ssum += u;
-      }
+    const uint32_t sum = wave_prefix(count), ssum = wave_prefix(split);
     const uint64_t past = __ballot(before + sum > i);
     if (past) {
       const int l = __ffsll((unsigned long long)past) - 1;

@@ -46,6 +46,18 @@ __device__ __forceinline__ void store4(void* p, uint32_t dtype, uint64_t i, f32x
   *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p) + i) = w;
 }
 
+// The sum of lanes 0 .. l in lane l: shifts inside the rows of 16 lanes, then row ends broadcast to the rows after
+// them. All 64 lanes active.
+__device__ __forceinline__ uint32_t wave_prefix(uint32_t v) {
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, false);  // row_shr:1
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, false);
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, false);
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, false);
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false);  // row_bcast:15 to rows 1 and 3
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false);  // row_bcast:31 to rows 2 and 3
+  return v;
+}
+
 // Value of a doubled e2m1 code (0..15), halved on use: {0,1,2,3,4,6,8,12}.
 __device__ __forceinline__ float fp4_value(uint32_t c) {
   const uint32_t m = c & 7u;

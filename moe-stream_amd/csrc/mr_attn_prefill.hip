@@ -71,39 +71,31 @@ struct Place {
 __device__ __forceinline__ bool find_tile(const PrefillArgs& a, int tile, bool report, Place& p) {
   const int lane = threadIdx.x & 63;
   auto in = [](int x, int hi) { return min(max(x, 0), hi); };
-  int before = 0, found = -1, found_before = 0;
-  for (int s0 = 0; s0 < a.n_seqs; s0 += 64) {
+  int before = 0;
+  bool found = false;
+  for (int s0 = 0; s0 < a.n_seqs && (report || !found); s0 += 64) {
     const int s = s0 + lane;
-    int n = 0;
+    int x = 0, y = 0, kx = 0, ky = 0;
     bool bad = false;
     if (s < a.n_seqs) {
-      const int x = a.cu_q[s], y = a.cu_q[s + 1], kx = a.cu_k[s], ky = a.cu_k[s + 1];
+      x = a.cu_q[s], y = a.cu_q[s + 1], kx = a.cu_k[s], ky = a.cu_k[s + 1];
       bad = x < 0 || y < x || y > a.nq || kx < 0 || ky < kx || ky > a.nk;
-      n = max(0, in(y, a.nq) - in(x, a.nq));
-      n = (n + kRows - 1) / kRows;
+      x = in(x, a.nq), y = max(x, in(y, a.nq)), kx = in(kx, a.nk), ky = max(kx, in(ky, a.nk));
     }
     if (report && __any(bad) && lane == 0) atomicOr(a.err, kErrOffset);
-    int sum = n;
-    for (int o = 1; o < 64; o *= 2) {
-      const int t = __shfl_up(sum, o, kWave);
-      if (lane >= o) sum += t;
-    }
+    const int n = (y - x + kRows - 1) / kRows, sum = (int)wave_prefix((uint32_t)n);
     const uint64_t past = __ballot(before + sum > tile);
-    if (past && found < 0) {
+    if (past && !found) {
       const int l = __ffsll((unsigned long long)past) - 1;
-      found = s0 + l;
-      found_before = before + __shfl(sum - n, l, kWave);
-      if (!report) break;
+      p.q0 = __builtin_amdgcn_readlane(x, l), p.q1 = __builtin_amdgcn_readlane(y, l);
+      p.k0 = __builtin_amdgcn_readlane(kx, l), p.k1 = __builtin_amdgcn_readlane(ky, l);
+      // the longest rows first
+      p.row = p.q0 + (before + __builtin_amdgcn_readlane(sum, l) - 1 - tile) * kRows;
+      found = true;
     }
-    before += __shfl(sum, 63, kWave);
+    before += __builtin_amdgcn_readlane(sum, 63);
   }
-  if (found < 0) return false;
-  found = __builtin_amdgcn_readfirstlane(found), found_before = __builtin_amdgcn_readfirstlane(found_before);
-  p.q0 = in(a.cu_q[found], a.nq), p.q1 = in(a.cu_q[found + 1], a.nq);
-  p.k0 = in(a.cu_k[found], a.nk), p.k1 = max(p.k0, in(a.cu_k[found + 1], a.nk));
-  const int tiles = (p.q1 - p.q0 + kRows - 1) / kRows;
-  p.row = p.q0 + (tiles - 1 - (tile - found_before)) * kRows;  // the longest rows first
-  return true;
+  return found;
 }
 
 // One tile of rows and one head. p is 0 where a row does not see a key, but 0 * inf and 0 * NaN are NaN: a tile
