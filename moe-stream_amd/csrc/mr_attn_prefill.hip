@@ -68,8 +68,7 @@ struct Place {
   int q0, q1, k0, k1;  // the sequence's rows
   int row;             // the tile's first row
 };
-__device__ __forceinline__ bool find_tile(const PrefillArgs& a, int tile, bool report, Place& p) {
-  const int lane = threadIdx.x & 63;
+__device__ __forceinline__ bool find_tile(const PrefillArgs& a, int tile, bool report, int lane, Place& p) {
   auto in = [](int x, int hi) { return min(max(x, 0), hi); };
   int before = 0;
   bool found = false;
@@ -106,16 +105,17 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
   constexpr int P = D / 8, ND = D / 32;  // 16-byte pieces of a row; 32-wide tiles of a head
   constexpr int kTile = kKeys * D;       // elements of a key or value tile
   constexpr uint32_t kTop = BF ? 0x7F80u : 0x7C00u;  // the exponent of infinities and NaN
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 31, half = lane >> 5;
+  int thread = threadIdx.x;
+  asm volatile("" : "+v"(thread));  // nothing is kept in registers for the second time over
+  const int wave = __builtin_amdgcn_readfirstlane(thread >> 6), lane = thread & 63, n = lane & 31, half = lane >> 5;
 
   const int h = unit / a.n_tiles, hk = h / (int)(a.q.n / a.k.n);
   Place pl;
-  if (!find_tile(a, unit % a.n_tiles, unit == 0 && !careful, pl)) return true;
+  if (!find_tile(a, unit % a.n_tiles, unit == 0 && !careful, lane, pl)) return true;
 
   // keys [first, last] of the tile's rows; a row r sees those up to r + diff, from r + diff - window + 1 on
   const int diff = pl.k1 - pl.q1;
   const int row = pl.row + wave * 32 + n;  // this lane's query row
-  const bool live = row < pl.q1;
   const int last_row = min(pl.row + kRows, pl.q1) - 1;
   const int last = last_row + diff;  // < k1
   int first = pl.k0;
@@ -299,14 +299,17 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
 
   l = add_xor32(l);
   const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : NAN;
-  if (live) {
-    uint16_t* dst = static_cast<uint16_t*>(a.out.p) + (uint64_t)row * a.out.ts + (uint64_t)h * a.out.hs;
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));  // the row's address is worked out here, not kept through the steps
+  const int out_row = pl.row + wave * 32 + (tid & 31);
+  if (out_row < pl.q1) {
+    uint16_t* dst = static_cast<uint16_t*>(a.out.p) + (uint64_t)out_row * a.out.ts + (uint64_t)h * a.out.hs;
 #pragma unroll
     for (int t = 0; t < ND; ++t)
 #pragma unroll
       for (int i = 0; i < 16; i += 4) {
         const u32x2 w = {pack16<BF>(acc[t][i] * inv, acc[t][i + 1] * inv), pack16<BF>(acc[t][i + 2] * inv, acc[t][i + 3] * inv)};
-        *reinterpret_cast<u32x2*>(dst + 32 * t + 8 * (i >> 2) + 4 * half) = w;
+        *reinterpret_cast<u32x2*>(dst + 32 * t + 8 * (i >> 2) + 4 * (tid >> 5 & 1)) = w;
       }
   }
   if (careful) {
@@ -330,7 +333,7 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
 }
 
 template <int D, bool BF>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_prefill(PrefillArgs a) {
+__global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 4) void k_attn_prefill(PrefillArgs a) {
   __shared__ __attribute__((aligned(1024))) uint16_t lds[4 * kKeys * D];  // rows at multiples of their length
   // Workgroups go to the 8 XCDs in turn. Each XCD gets a contiguous share of the (head, tile) pairs, so that
   // the query heads that share keys find them in one L2.
