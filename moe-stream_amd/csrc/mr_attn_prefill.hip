@@ -237,54 +237,163 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
     l += p0 + p1;
     pf[i >> 2][i & 3] = pack16<BF>(p0, p1);
   };
-  if (first <= last) {
-    fetch_k(first, 0), fetch_v(first, 0);
-    for (int k0 = first, b = 0; k0 <= last; k0 += kKeys, b ^= 1) {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();
-      if (k0 + kKeys <= last) fetch_k(k0 + kKeys, b ^ 1), fetch_v(k0 + kKeys, b ^ 1);
-      if (careful && edge(k0)) {
-        uint16_t* vt = lds + b * 2 * kTile + kTile;
-        for (int i = threadIdx.x; i < kTile; i += 256)
-          if ((vt[i] & kTop) == kTop) vt[i] = 0;
+  // Takes the values that are not finite out of buffer b.
+  auto clean = [&](int b) {
+    uint16_t* vt = lds + b * 2 * kTile + kTile;
+    for (int i = threadIdx.x; i < kTile; i += 256)
+      if ((vt[i] & kTop) == kTop) vt[i] = 0;
+    __syncthreads();
+  };
+
+  if constexpr (D != 256) {
+    // Two waves or more to a SIMD: one's matrix instructions run beside another's exponentials.
+    if (first <= last) {
+      fetch_k(first, 0), fetch_v(first, 0);
+      for (int k0 = first, b = 0; k0 <= last; k0 += kKeys, b ^= 1) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
+        if (k0 + kKeys <= last) fetch_k(k0 + kKeys, b ^ 1), fetch_v(k0 + kKeys, b ^ 1);
+        if (careful && edge(k0)) clean(b);
+        // keys behind all of the wave's rows, or in front of all their windows
+        if (k0 > pl.row + wave * 32 + 31 + diff || k0 + kKeys <= wave_least) continue;
+        uint32_t kb = k_at + b * 4 * kTile, vb = v_at + b * 4 * kTile;
+        asm("" : "+v"(kb), "+v"(vb));  // the parts' addresses are worked out from here, not kept
+        f32x16 s0 = {}, s1 = {};
+        u32x4 pf[4], kf[2][2], vf[3];
+        kf[0][0] = key_part(kb, 0, 0), kf[0][1] = key_part(kb, 1, 0);
+        // Waves between their matrix instructions give way to those at them: the two of a SIMD then take turns
+        // (8192 tokens, heads of 128: 675 -> 649 us).
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          if (i + 1 < NI) kf[(i + 1) & 1][0] = key_part(kb, 0, i + 1), kf[(i + 1) & 1][1] = key_part(kb, 1, i + 1);
+          if (i >= NI - 2) vf[i - (NI - 2)] = value_part(vb, i - (NI - 2));
+          s0 = mfma32<BF>(kf[i & 1][0], qf[i], s0);
+          s1 = mfma32<BF>(kf[i & 1][1], qf[i], s1);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        __builtin_amdgcn_s_setprio(0);
+        settle(k0, s0, s1);
+        const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) weigh(s0, s1, x, base, pf);
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int q = 0; q < NV; ++q) {
+          if (q + 2 < NV) vf[(q + 2) % 3] = value_part(vb, q + 2);
+          acc[q % ND] = mfma32<BF>(vf[q % 3], pf[q / ND], acc[q % ND]);
+          // the next 16 keys' weights
+          if (q / ND < 3) {
+#pragma unroll
+            for (int x = 4 * (q / ND + 1) + q % ND * 4 / ND; x < 4 * (q / ND + 1) + (q % ND + 1) * 4 / ND; ++x) weigh(s0, s1, x, base, pf);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        __builtin_amdgcn_s_setprio(0);
       }
-      // keys behind all of the wave's rows, or in front of all their windows
-      if (k0 > pl.row + wave * 32 + 31 + diff || k0 + kKeys <= wave_least) continue;
-      uint32_t kb = k_at + b * 4 * kTile, vb = v_at + b * 4 * kTile;
+    }
+  } else {
+    // One wave to a SIMD: the scores run a step ahead of the values, so that a wave's matrix instructions have its own
+    // exponentials between them (8192 tokens, heads of 256: 742 -> 655 us; of 128, where two waves do the same
+    // for each other, 619 -> 647).
+    //
+    // Scores (p, q) of one step, their first and second 32 keys; the next ones go to x and, once p's weights are
+    // taken, to p.
+    auto step = [&](int k0, int b, f32x16& p, f32x16& q, f32x16& x) {
+      const float base = m == -INFINITY ? 0.f : m;
+      u32x4 pf[4], kf[3], vf[3];
+      uint32_t kb = k_at + (b ^ 1) * 4 * kTile, vb = v_at + b * 4 * kTile;
       asm("" : "+v"(kb), "+v"(vb));  // the parts' addresses are worked out from here, not kept
-      f32x16 s0 = {}, s1 = {};
-      u32x4 pf[4], kf[2][2], vf[3];
-      kf[0][0] = key_part(kb, 0, 0), kf[0][1] = key_part(kb, 1, 0);
-      // Waves between their matrix instructions give way to those at them: the two of a SIMD then take turns
-      // (8192 tokens, heads of 128: 675 -> 649 us).
+      kf[0] = key_part(kb, 0, 0), kf[1] = key_part(kb, 0, 1);
+      f32x16 n0 = {};
       __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
-        if (i + 1 < NI) kf[(i + 1) & 1][0] = key_part(kb, 0, i + 1), kf[(i + 1) & 1][1] = key_part(kb, 1, i + 1);
-        if (i >= NI - 2) vf[i - (NI - 2)] = value_part(vb, i - (NI - 2));
-        s0 = mfma32<BF>(kf[i & 1][0], qf[i], s0);
-        s1 = mfma32<BF>(kf[i & 1][1], qf[i], s1);
+        kf[(i + 2) % 3] = key_part(kb, (i + 2) / NI, (i + 2) % NI);
+        n0 = mfma32<BF>(kf[i % 3], qf[i], n0);
+#pragma unroll
+        for (int y = i * 8 / NI; y < (i + 1) * 8 / NI; ++y) weigh(p, p, y, base, pf);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      x = n0;
+      f32x16 n1 = {};
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        if (i + 2 < NI) kf[(NI + i + 2) % 3] = key_part(kb, 1, i + 2);
+        else vf[i + 2 - NI] = value_part(vb, i + 2 - NI);
+        n1 = mfma32<BF>(kf[(NI + i) % 3], qf[i], n1);
+#pragma unroll
+        for (int y = 8 + i * 8 / NI; y < 8 + (i + 1) * 8 / NI; ++y) weigh(q, q, y, base, pf);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      p = n1;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        if (i + 2 < NV) vf[(i + 2) % 3] = value_part(vb, i + 2);
+        acc[i % ND] = mfma32<BF>(vf[i % 3], pf[i / ND], acc[i % ND]);
         __builtin_amdgcn_sched_barrier(0);
       }
       __builtin_amdgcn_s_setprio(0);
-      settle(k0, s0, s1);
-      const float base = m == -INFINITY ? 0.f : m;
+      settle(k0 + kKeys, x, p);
+    };
+    // Between steps: the other buffer's tiles have come in, and this one's keys are no longer needed.
+    auto turn = [&](int k0, int b) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      if (k0 + kKeys <= last) fetch_v(k0 + kKeys, b ^ 1);
+      if (k0 + 2 * kKeys <= last) fetch_k(k0 + 2 * kKeys, b);
+      if (careful && edge(k0)) clean(b);
+    };
+    if (first <= last) {
+      fetch_k(first, 0), fetch_v(first, 0);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      if (first + kKeys <= last) fetch_k(first + kKeys, 1);
+      f32x16 s0 = {}, s1 = {}, s2 = {};
+      uint32_t kb = k_at;
+      asm("" : "+v"(kb));
 #pragma unroll
-      for (int x = 0; x < 4; ++x) weigh(s0, s1, x, base, pf);
-      __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-      for (int q = 0; q < NV; ++q) {
-        if (q + 2 < NV) vf[(q + 2) % 3] = value_part(vb, q + 2);
-        acc[q % ND] = mfma32<BF>(vf[q % 3], pf[q / ND], acc[q % ND]);
-        // the next 16 keys' weights
-        if (q / ND < 3) {
-#pragma unroll
-          for (int x = 4 * (q / ND + 1) + q % ND * 4 / ND; x < 4 * (q / ND + 1) + (q % ND + 1) * 4 / ND; ++x) weigh(s0, s1, x, base, pf);
+      for (int i = 0; i < NI; ++i) {
+        s0 = mfma32<BF>(key_part(kb, 0, i), qf[i], s0);
+        s1 = mfma32<BF>(key_part(kb, 1, i), qf[i], s1);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      settle(first, s0, s1);
+      int b = 0;
+      for (int k0 = first;;) {
+        turn(k0, b);
+        if (k0 + kKeys > last) break;
+        step(k0, b, s0, s1, s2);
+        k0 += kKeys, b ^= 1;
+        turn(k0, b);
+        if (k0 + kKeys > last) {
+          s1 = s0, s0 = s2;
+          break;
         }
-        __builtin_amdgcn_sched_barrier(0);
+        step(k0, b, s2, s0, s1);
+        k0 += kKeys, b ^= 1;
+        turn(k0, b);
+        if (k0 + kKeys > last) {
+          s0 = s1, s1 = s2;
+          break;
+        }
+        step(k0, b, s1, s2, s0);
+        k0 += kKeys, b ^= 1;
       }
-      __builtin_amdgcn_s_setprio(0);
+      const float base = m == -INFINITY ? 0.f : m;
+      u32x4 pf[4];
+      uint32_t vb = v_at + b * 4 * kTile;
+      asm("" : "+v"(vb));
+#pragma unroll
+      for (int cc = 0; cc < 4; ++cc) {
+#pragma unroll
+        for (int x = 4 * cc; x < 4 * cc + 4; ++x) weigh(s0, s1, x, base, pf);
+#pragma unroll
+        for (int t = 0; t < ND; ++t) {
+          acc[t] = mfma32<BF>(value_part(vb, cc * ND + t), pf[cc], acc[t]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
     }
   }
 
