@@ -337,8 +337,10 @@ __global__ __launch_bounds__(64 * kWaves, (Tuning<FMT, D>::kPerSimd)) void k_att
     for (int t = 0; t < 4; ++t) {
       float p[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) p[j] = __builtin_amdgcn_exp2f(fmaf(s[t][j], c, -base)), l += p[j];
-      pf[t >> 1][2 * (t & 1)] = pack_f16(p[0], p[1]), pf[t >> 1][2 * (t & 1) + 1] = pack_f16(p[2], p[3]);
+      for (int j = 0; j < 4; ++j) p[j] = __builtin_amdgcn_exp2f(fmaf(s[t][j], c, -base));
+      const uint32_t w0 = pack_f16(p[0], p[1]), w1 = pack_f16(p[2], p[3]);
+      pf[t >> 1][2 * (t & 1)] = w0, pf[t >> 1][2 * (t & 1) + 1] = w1;
+      l = add_f16(w1, add_f16(w0, l));
     }
 #pragma unroll
     for (int G = 0; G < 2; ++G)

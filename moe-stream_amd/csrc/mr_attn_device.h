@@ -28,6 +28,15 @@ __device__ __forceinline__ f32x2 unpack_f16(uint32_t w) {
 }
 __device__ __forceinline__ f32x2 unpack_bf16(uint32_t w) { return f32x2{bits_f32(w << 16), bits_f32(w & 0xFFFF0000u)}; }
 
+// s + the two f16 (bf16) of w: subnormal ones count too. The weights' sum is taken of the rounded weights, so that
+// what rounding one does to the sum of values it does to the divisor as well: a row on one key is exact.
+__device__ __forceinline__ float add_f16(uint32_t w, float s) {
+  return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), f16x2{(_Float16)1.f, (_Float16)1.f}, s, false);
+}
+__device__ __forceinline__ float add_bf16(uint32_t w, float s) {
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), bf16x2{(__bf16)1.f, (__bf16)1.f}, s, false);
+}
+
 // Four adjacent elements at element offset i of an array of type `dtype` (the same for all lanes).
 __device__ __forceinline__ f32x4 load4(const void* p, uint32_t dtype, uint64_t i) {
   if (dtype == MR_F32) return *reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + i);

@@ -234,8 +234,9 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
     const f32x16& s = i < 8 ? s0 : s1;
     const float p0 = __builtin_amdgcn_exp2f(fmaf(s[2 * (i & 7)], c, -base));
     const float p1 = __builtin_amdgcn_exp2f(fmaf(s[2 * (i & 7) + 1], c, -base));
-    l += p0 + p1;
-    pf[i >> 2][i & 3] = pack16<BF>(p0, p1);
+    const uint32_t w = pack16<BF>(p0, p1);
+    pf[i >> 2][i & 3] = w;
+    l = BF ? add_bf16(w, l) : add_f16(w, l);
   };
   // Takes the values that are not finite out of buffer b.
   auto clean = [&](int b) {

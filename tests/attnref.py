@@ -143,9 +143,10 @@ def attend(q, k, v, scale, first, last, sink=None):
 
 
 def attention_bound(y, size_v, size_s, n, D, out_type, p_half):
-    """How far a result may be off: the output's own rounding; p's (half a step p_half, and half of the
-    smallest f16 step, 2^-25, for each of n keys, whose weights sum to 1 or more before the division); and
-    the scores', D products summed in 32 bits and two more roundings before the exponential (whose own
-    error is a few steps of 32 bits), each an error of p relative to p, in sum and quotient."""
+    """How far a result may be off. The output's own rounding. The weights': each p is off by p_half of it at most (and
+    half of the smallest f16 step, 2^-25, for each of n keys, whose weights sum to 1 or more before the division), in
+    the sum of values and in the divisor alike, so the quotient by p_half (sum p |v| + |y| sum p) / sum p. The scores',
+    D products summed in 32 bits and two more roundings before the exponential (whose own error is a few steps of 32
+    bits), each an error of p relative to p, in sum and quotient."""
     ds = (D + 4) * 2.0 ** -24 * size_s + 8 * 2.0 ** -24
-    return HALF[out_type] * np.abs(y) * 1.01 + (p_half + 2 * ds + n ** 0.5 * 2.0 ** -23) * size_v + n * 2.0 ** -25 * np.max(size_v, initial=0) + 2.0 ** -25
+    return HALF[out_type] * np.abs(y) * 1.01 + p_half * np.abs(y) + (p_half + 2 * ds + n ** 0.5 * 2.0 ** -23) * size_v + n * 2.0 ** -25 * np.max(size_v, initial=0) + 2.0 ** -25
