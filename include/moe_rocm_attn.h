@@ -17,7 +17,12 @@
  *    graphs see their present values. An entry out of its range is never followed: the call
  *    leaves out what it names, as stated below, and the next mr_sync of the context returns
  *    MR_E_INVAL and says which kind of entry it was.
- *  - Zero tokens, rows or sequences: MR_OK, nothing is launched.
+ *  - Zero tokens, rows or sequences: MR_OK, nothing is launched. More than a launch can hold (2^24 tokens
+ *    of mr_qk_norm_rope, 2^24 tiles of 128 rows and a head of mr_attn_prefill): MR_E_INVAL.
+ *  - mr_attn_decode keeps partial results in scratch of the context, allocated with its first cache and of
+ *    one size for all calls: like all scratch of a context it serves one call at a time.
+ *  - Kernel names for mr_profile_read: "qk_norm_rope", "kv_write", "kv_read", "attn_decode", "attn_join",
+ *    "attn_prefill".
  */
 #ifndef MOE_ROCM_ATTN_H
 #define MOE_ROCM_ATTN_H
@@ -145,9 +150,9 @@ int mr_attn_decode(mr_ctx* ctx, const mr_kv* kv, const mr_heads* q, uint32_t n_s
 /* Packed prompts: sequence s has query rows cu_q[s] .. cu_q[s + 1] - 1 of the n_q rows of q and out, and
  * key/value rows cu_k[s] .. cu_k[s + 1] - 1 of the n_k rows of k and v; its queries are its last
  * positions (as many as keys: a whole prompt; fewer: the next part of one; more: the first ones see
- * nothing). cu_q, cu_k: n_seqs + 1 offsets that do not decrease; offsets outside the rows are taken as
- * the nearest inside, decreasing ones as empty sequences, both with an error at mr_sync. Rows of `out`
- * in no sequence are left as they are. q, k, v and out: F16 or BF16, all the same; head_dim 64, 128 or
+ * nothing). cu_q, cu_k: n_seqs + 1 offsets that do not decrease. Offsets outside the rows are taken as
+ * the nearest inside and decreasing ones as empty sequences, both with an error at mr_sync; rows that two
+ * sequences claim then hold either's result or none. Rows of `out` in no sequence are left as they are. q, k, v and out: F16 or BF16, all the same; head_dim 64, 128 or
  * 256; token strides of k and v below 2^24 elements. opts NULL: defaults. */
 int mr_attn_prefill(mr_ctx* ctx, uint32_t head_dim, const mr_heads* q, uint32_t n_q, const mr_heads* k,
                     const mr_heads* v, uint32_t n_k, uint32_t n_seqs, const int32_t* cu_q, const int32_t* cu_k,

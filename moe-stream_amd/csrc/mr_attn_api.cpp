@@ -44,6 +44,8 @@ bool capturing(mr_ctx* c) {
 
 bool misaligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; }
 
+constexpr uint32_t kMaxWork = 1u << 24;  // workgroups of 256 threads that a launch's 2^32 threads allow
+
 uint32_t elem_bytes(uint32_t dtype) { return dtype == MR_F32 ? 4 : 2; }
 
 // Checks rows of heads and fills in the default strides.
@@ -220,7 +222,7 @@ int mr_qk_norm_rope(mr_ctx* c, const mr_rope* r, const mr_heads* q, const mr_hea
   if (k_norm && !k) return fail(c, MR_E_INVAL, "k_norm without k");
   if ((rc = check_eps(c, eps))) return rc;
   if (!positions || misaligned(positions, 4)) return fail(c, MR_E_INVAL, "positions is NULL or not 4-byte aligned");
-  if (T > 0x7FFFFFFFu) return fail(c, MR_E_INVAL, "n_tokens %u is 2^31 or more", T);
+  if (T >= kMaxWork) return fail(c, MR_E_INVAL, "n_tokens %u is 2^24 or more", T);
   if (T == 0) return MR_OK;
   if ((rc = bind(c))) return rc;
   const hipError_t e = mr::launch_qk_norm_rope(c->launch(), *r, in[0], in[1], q_norm, k_norm, eps, positions, T, o[0], o[1]);
@@ -249,6 +251,7 @@ int mr_kv_create(mr_ctx* c, const mr_kv_desc* desc, mr_kv** out) {
       if (!c->attn_scratch) e = hipMalloc(&c->attn_scratch, mr::attn_decode_scratch_bytes());
       if (e == hipSuccess) e = hipMalloc(&kv->base, kv->bytes);
       if (e == hipSuccess) e = mr::launch_zero(mr::Launch{c->stream, nullptr}, kv->base, kv->bytes);
+      if (e == hipSuccess) e = hipStreamSynchronize(c->stream);  // the next call may be on another stream
       if (e != hipSuccess) rc = hip_fail(c, e, "cache pages");
     }
     if (rc) {
@@ -350,6 +353,8 @@ int mr_attn_prefill(mr_ctx* c, uint32_t D, const mr_heads* q, uint32_t nq, const
   if (!cu_q || !cu_k || misaligned(cu_q, 4) || misaligned(cu_k, 4))
     return fail(c, MR_E_INVAL, "cu_q or cu_k is NULL or not 4-byte aligned");
   if (nq > 0x7FFFFFFFu || nk > 0x7FFFFFFFu || n_seqs >= 0x7FFFFFFFu) return fail(c, MR_E_INVAL, "2^31 rows or more");
+  if (((uint64_t)nq / mr::kPrefillRows + n_seqs) * hq.n >= kMaxWork)
+    return fail(c, MR_E_INVAL, "%u rows of %u heads in %u sequences are 2^24 tiles or more", nq, hq.n, n_seqs);
   if (nq == 0 || n_seqs == 0) return MR_OK;
   if ((rc = bind(c))) return rc;
   c->attn_used = true;

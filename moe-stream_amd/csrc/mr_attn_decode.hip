@@ -34,6 +34,8 @@ constexpr uint32_t kMinPart = kWaves;  // chunks of a part at least: one for eac
 // and in parts: 11.8 and 13.9 us (MXFP4, 4 heads of 128), 24.7 and 16.7 us (MXINT8, 2 heads of 256, where a chunk
 // takes a wave 4 us).
 __host__ __device__ inline uint32_t whole_chunks(uint32_t D) { return D == 256 ? 2 * kWaves : 5 * kWaves; }
+// With more sequences none is split: each workgroup looks through their lengths to find its part.
+constexpr uint32_t kSplitSeqs = 1024;
 // Parts of all sequences at most. Those of split sequences, two or more of each, are then no more than `parts`.
 __host__ __device__ inline uint32_t part_limit(uint32_t parts, uint32_t n_seqs) {
   const uint32_t some = n_seqs + parts / 2;
@@ -486,7 +488,7 @@ hipError_t launch_attn_decode(const Launch& K, const KvPages& kv, uint32_t forma
   const uint64_t cap = (uint64_t)max_pages << (kv.page_shift - 6);
   const uint64_t chunks = o.window ? std::min<uint64_t>(cap, (o.window + 62ull) / 64 + 1) : cap;  // of a sequence at most
   const uint32_t room = std::min<uint32_t>(kPartUnits, per_cu * n_cu);
-  a.parts = chunks <= whole_chunks(D) ? 1 : std::max<uint32_t>(1, room / units);
+  a.parts = chunks <= whole_chunks(D) || B > kSplitSeqs ? 1 : std::max<uint32_t>(1, room / units);
   hipError_t e;
   {
     ProfScope ps(K, "attn_decode");

@@ -16,8 +16,11 @@ namespace {
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kRows = 128;  // query rows of a workgroup: 4 waves of 32
+constexpr int kRows = kPrefillRows;  // of a workgroup: 4 waves of 32
 constexpr int kKeys = 64;   // keys of a step
+// Up to so many sequences are looked through, 64 at a time, to find a tile's: each step costs about as much as one
+// of a search among more, which takes their log2.
+constexpr int kScan = 512;
 constexpr float kSlack = 8.f;
 
 template <bool BF>
@@ -62,32 +65,53 @@ struct PrefillArgs {
   uint32_t* err;
 };
 
-// The sequence and first row of row tile `tile`: sequences in turn, each in whole tiles. Offsets are
-// clamped into the rows; `report` also looks at all of them. Returns false behind the last tile.
+// The sequence and first row of row tile `tile`; false for a tile that there is not. Offsets are clamped into
+// the rows; `report` also looks at all of them.
 struct Place {
   int q0, q1, k0, k1;  // the sequence's rows
   int row;             // the tile's first row
 };
 __device__ __forceinline__ bool find_tile(const PrefillArgs& a, int tile, bool report, int lane, Place& p) {
-  auto in = [](int x, int hi) { return min(max(x, 0), hi); };
-  int before = 0;
+  struct Seq {
+    int q0, q1, k0, k1, tiles;
+    bool bad;
+  };
+  auto seq = [&](int s) {
+    auto in = [](int x, int hi) { return min(max(x, 0), hi); };
+    const int x = a.cu_q[s], y = a.cu_q[s + 1], kx = a.cu_k[s], ky = a.cu_k[s + 1];
+    Seq r{in(x, a.nq), in(y, a.nq), in(kx, a.nk), in(ky, a.nk), 0, x < 0 || y < x || y > a.nq || kx < 0 || ky < kx || ky > a.nk};
+    r.q1 = max(r.q0, r.q1), r.k1 = max(r.k0, r.k1), r.tiles = (r.q1 - r.q0 + kRows - 1) / kRows;
+    return r;
+  };
+  const bool search = a.n_seqs > kScan;
   bool found = false;
-  for (int s0 = 0; s0 < a.n_seqs && (report || !found); s0 += 64) {
-    const int s = s0 + lane;
-    int x = 0, y = 0, kx = 0, ky = 0;
-    bool bad = false;
-    if (s < a.n_seqs) {
-      x = a.cu_q[s], y = a.cu_q[s + 1], kx = a.cu_k[s], ky = a.cu_k[s + 1];
-      bad = x < 0 || y < x || y > a.nq || kx < 0 || ky < kx || ky > a.nk;
-      x = in(x, a.nq), y = max(x, in(y, a.nq)), kx = in(kx, a.nk), ky = max(kx, in(ky, a.nk));
+  if (search) {
+    // Sequence s has the tiles from cu_q[s] / kRows + s on: room for one that is not full, some left out.
+    int lo = 0, hi = a.n_seqs - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (min(max(a.cu_q[mid], 0), a.nq) / kRows + mid <= tile) lo = mid;
+      else hi = mid - 1;
     }
-    if (report && __any(bad) && lane == 0) atomicOr(a.err, kErrOffset);
-    const int n = (y - x + kRows - 1) / kRows, sum = (int)wave_prefix((uint32_t)n);
+    const Seq r = seq(lo);
+    const int i = tile - (r.q0 / kRows + lo);
+    found = i >= 0 && i < r.tiles;
+    p.q0 = __builtin_amdgcn_readfirstlane(r.q0), p.q1 = __builtin_amdgcn_readfirstlane(r.q1);
+    p.k0 = __builtin_amdgcn_readfirstlane(r.k0), p.k1 = __builtin_amdgcn_readfirstlane(r.k1);
+    p.row = __builtin_amdgcn_readfirstlane(r.q0 + (r.tiles - 1 - i) * kRows);
+    if (!report) return __builtin_amdgcn_readfirstlane(found);
+  }
+  int before = 0;
+  for (int s0 = 0; s0 < a.n_seqs && (report || !found); s0 += 64) {
+    const Seq r = s0 + lane < a.n_seqs ? seq(s0 + lane) : Seq{};
+    if (report && __any(r.bad) && lane == 0) atomicOr(a.err, kErrOffset);
+    if (search) continue;
+    const int sum = (int)wave_prefix((uint32_t)r.tiles);
     const uint64_t past = __ballot(before + sum > tile);
     if (past && !found) {
       const int l = __ffsll((unsigned long long)past) - 1;
-      p.q0 = __builtin_amdgcn_readlane(x, l), p.q1 = __builtin_amdgcn_readlane(y, l);
-      p.k0 = __builtin_amdgcn_readlane(kx, l), p.k1 = __builtin_amdgcn_readlane(ky, l);
+      p.q0 = __builtin_amdgcn_readlane(r.q0, l), p.q1 = __builtin_amdgcn_readlane(r.q1, l);
+      p.k0 = __builtin_amdgcn_readlane(r.k0, l), p.k1 = __builtin_amdgcn_readlane(r.k1, l);
       // the longest rows first
       p.row = p.q0 + (before + __builtin_amdgcn_readlane(sum, l) - 1 - tile) * kRows;
       found = true;
@@ -461,9 +485,8 @@ hipError_t launch_attn_prefill(const Launch& K, uint32_t D, const Heads& q, uint
                                const Heads& out, uint32_t* err) {
   ProfScope ps(K, "attn_prefill");
   // every sequence ends with at most one tile that is not full
-  const uint64_t tiles = std::min<uint64_t>((uint64_t)nq / kRows + n_seqs, nq);
-  const uint64_t units = tiles * q.n;
-  if (units > 0x7FFFFF00ull) return hipErrorInvalidConfiguration;
+  const uint64_t most = (uint64_t)nq / kRows + n_seqs, tiles = n_seqs > kScan ? most : std::min<uint64_t>(most, nq);
+  const uint64_t units = tiles * q.n;  // below 2^24, checked by the caller
   PrefillArgs a{q, k, v, out, (int)nq, (int)nk, (int)n_seqs, (int)tiles, cu_q, cu_k, o, err};
   const dim3 g((unsigned)((units + 7) / 8 * 8)), blk(256);
   const bool bf = q.dtype == MR_BF16;

@@ -130,7 +130,7 @@ def test_qk_norm_rope_refusals(hctx):
                      (dict(q=M.Heads(X, 4, 3)), "type"), (dict(q=M.Heads(X, 0)), "heads"), (dict(q=M.Heads(X, 1025)), "heads"),
                      (dict(q_out=M.Heads(X, 5)), "head counts"), (dict(pos=None), "positions"), (dict(pos=X + 2), "positions"),
                      (dict(eps=-1.0), "eps"), (dict(eps=math.nan), "eps"), (dict(q_norm=X + 4), "aligned"),
-                     (dict(k=None, k_out=None, k_norm=X), "k_norm"), (dict(n=1 << 31), "n_tokens"),
+                     (dict(k=None, k_out=None, k_norm=X), "k_norm"), (dict(n=1 << 24), "n_tokens"),
                      (dict(q=M.Heads(X, 4, token_stride=1 << 40)), "2^40")):
         refused(M.MR_E_INVAL, text, call, **kw)
     assert M.lib.mr_qk_norm_rope(None, r.h, None, None, None, None, 0.0, None, 0, None, None) == M.MR_E_INVAL
@@ -214,7 +214,7 @@ def test_prefill_refusals(hctx):
             (dict(v=M.Heads(X, 2, M.F32)), M.MR_E_UNSUPPORTED, "type of q"), (dict(v=M.Heads(X, 4, M.F16)), M.MR_E_INVAL, "heads"),
             (dict(k=M.Heads(X, 3, M.F16), v=M.Heads(X, 3, M.F16)), M.MR_E_INVAL, "evenly"),
             (dict(cu_q=None), M.MR_E_INVAL, "cu_q"), (dict(cu_k=X + 2), M.MR_E_INVAL, "cu_k"),
-            (dict(nq=1 << 31), M.MR_E_INVAL, "2^31"), (dict(scale=math.nan), M.MR_E_INVAL, "scale"),
+            (dict(nq=1 << 31), M.MR_E_INVAL, "2^31"), (dict(nq=1 << 28), M.MR_E_INVAL, "2^24"), (dict(scale=math.nan), M.MR_E_INVAL, "scale"),
             (dict(k=M.Heads(X, 2, M.F16, token_stride=1 << 24)), M.MR_E_INVAL, "2^24"),
             (dict(k=M.Heads(X, 2, M.F16, token_stride=4)), M.MR_E_INVAL, "stride"), (dict(v=None), M.MR_E_INVAL, "v is NULL")):
         refused(status, text, call, **kw)

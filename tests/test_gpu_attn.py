@@ -287,6 +287,21 @@ def test_decode_of_one_long_sequence(gpu_ctx, fmt, D, hk, group, n, window):
     dq.free(), out.free(), c.close()
 
 
+@pytest.mark.parametrize("n_seqs,long", [(65, 5000), (300, 9000), (1024, 3000), (1100, 2000)])
+def test_decode_of_many_sequences(gpu_ctx, n_seqs, long):
+    """Short sequences and some long ones among them, which are split or not."""
+    rng = np.random.default_rng(n_seqs)
+    lens = rng.integers(0, 70, n_seqs).tolist()
+    lens[1], lens[n_seqs // 2], lens[-1] = long, 1300, long // 2
+    c = Cached(gpu_ctx, M.KV_MXFP4, lens, 1, 64, 64, n_seqs)
+    q = R.rounded(rng.normal(size=(n_seqs, 3, 64)), M.F16)
+    dq, out = R.Rows(gpu_ctx, q, M.F16), R.Rows(gpu_ctx, None, M.F16, n_seqs, 3, 64)
+    c.kv.attend(dq.heads, n_seqs, c.d_len, c.d_table, c.max_pages, out.heads)
+    gpu_ctx.sync()
+    c.check(out.get(), q, M.F16, 3, 0.125)
+    dq.free(), out.free(), c.close()
+
+
 def test_decode_scores_of_any_size(gpu_ctx):
     """Scores far apart, a negative scale, queries near the types' ends: one key takes all the weight."""
     lens = [200, 700]
@@ -426,6 +441,14 @@ def test_prefill(gpu_ctx, D, hk, group, dtype, window, sink, past):
 @pytest.mark.parametrize("window", [0, 200])
 def test_prefill_long(gpu_ctx, D, window):
     prompts(gpu_ctx, D, 2, 4, M.BF16, [1000, 257, 3, 511], [1000, 257, 3, 2511], window, seed=D)
+
+
+@pytest.mark.parametrize("n_seqs", [65, 512, 513, 1500])
+def test_prefill_of_many_sequences(gpu_ctx, n_seqs):
+    rng = np.random.default_rng(n_seqs)
+    lens = rng.integers(0, 4, n_seqs)
+    lens[[3, n_seqs // 2, n_seqs - 1]] = 140, 257, 129
+    prompts(gpu_ctx, 64, 1, 2, M.BF16, lens, lens + rng.integers(0, 3, n_seqs), seed=n_seqs)
 
 
 @pytest.mark.parametrize("D", [64, 128, 256])
