@@ -42,6 +42,7 @@ struct Heads {
 //           32 G + 16 + 4 g + j - 4, for G = 0, 1 in turn; the elements are, in turn,
 //             MXFP4   blocks of 32: a byte for each j, element 32 b + m low, 32 b + 16 + m high
 //             others  tiles of 16: element 16 t + m for each j
+//   An MXINT8 code is stored with 128 added, the form that turns into f16 in the fewest instructions.
 //   key scales    [block][m][t], value scales [g][G][block][j]; a byte each, none for F16. The byte is
 //           e + 127 for MXFP4 (the scale operand of the conversion), the high byte of 2^e in f16 for
 //           MXINT8 (the factor of the packed f16 product).

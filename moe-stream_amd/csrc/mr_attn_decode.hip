@@ -135,9 +135,9 @@ __device__ __forceinline__ uint32_t fp4_pair(uint32_t w, uint32_t sc) {
 // Byte `sel` of w in the exponent field; the conversion takes no notice of the other bits.
 __device__ __forceinline__ uint32_t exp_bits(uint32_t w, int sel) { return sel == 3 ? w >> 1 : w << (23 - 8 * sel); }
 
-// Two bytes (signed, of a word with its sign bits flipped) as f16: 0x6400 | u is 1024 + u.
-__device__ __forceinline__ f16x2 int8_pair(uint32_t flipped, int pair) {
-  const uint32_t w = __builtin_amdgcn_perm(0x64646464u, flipped, pair ? 0x07030602u : 0x05010400u);
+// Two MXINT8 codes as f16: 0x6400 | u is 1024 + u.
+__device__ __forceinline__ f16x2 int8_pair(uint32_t codes, int pair) {
+  const uint32_t w = __builtin_amdgcn_perm(0x64646464u, codes, pair ? 0x07030602u : 0x05010400u);
   return __builtin_bit_cast(f16x2, w) - f16x2{(_Float16)1152.f, (_Float16)1152.f};
 }
 
@@ -182,7 +182,7 @@ struct Chunk {
       return u32x4{fp4_pair<0>(c, e), fp4_pair<1>(c, e), fp4_pair<2>(c, e), fp4_pair<3>(c, e)};
     } else {
       const int w = 2 * (t * (D / 32) + i);
-      const uint32_t c0 = k[w >> 2][w & 3] ^ 0x80808080u, c1 = k[w >> 2][(w & 3) + 1] ^ 0x80808080u;
+      const uint32_t c0 = k[w >> 2][w & 3], c1 = k[w >> 2][(w & 3) + 1];
       const uint32_t b = s >> (8 * t) & 0xFFu;
       const f16x2 e = __builtin_bit_cast(f16x2, b << 8 | b << 24);
       return u32x4{__builtin_bit_cast(uint32_t, int8_pair(c0, 0) * e), __builtin_bit_cast(uint32_t, int8_pair(c0, 1) * e),
@@ -217,7 +217,7 @@ struct Chunk {
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const int w = 2 * (G * (D / 16) + 2 * b + x);
-        const uint32_t c0 = v[w >> 2][w & 3] ^ 0x80808080u, c1 = v[w >> 2][(w & 3) + 1] ^ 0x80808080u;
+        const uint32_t c0 = v[w >> 2][w & 3], c1 = v[w >> 2][(w & 3) + 1];
         (x ? hi : lo) = u32x4{__builtin_bit_cast(uint32_t, int8_pair(c0, 0) * e[0]), __builtin_bit_cast(uint32_t, int8_pair(c0, 1) * e[1]),
                               __builtin_bit_cast(uint32_t, int8_pair(c1, 0) * e[2]), __builtin_bit_cast(uint32_t, int8_pair(c1, 1) * e[3])};
       }

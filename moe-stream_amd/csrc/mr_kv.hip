@@ -10,6 +10,9 @@ namespace {
 
 __device__ __forceinline__ float finite_or_inf(float x) { return x == x ? x : 0.f; }
 
+// Value of the MXINT8 code in the low byte of c; +0 for a slot that was never written (scale 0).
+__device__ __forceinline__ float int8_value(uint32_t c, float scale) { return fmaf((float)((int)(c & 0xFFu) - 128), scale, 0.f); }
+
 // The block exponent for the largest magnitude `top`.
 template <int FMT>
 __device__ __forceinline__ int block_exp(float top) {
@@ -25,7 +28,7 @@ __device__ __forceinline__ uint32_t scale_byte(int e) {
 }
 template <int FMT>
 __device__ __forceinline__ uint32_t code(float y) {
-  if (FMT == MR_KV_MXINT8) return (uint32_t)(int)rintf(fminf(fmaxf(y, -127.f), 127.f)) & 0xFFu;
+  if (FMT == MR_KV_MXINT8) return (uint32_t)((int)rintf(fminf(fmaxf(y, -127.f), 127.f)) + 128);
   const float a = fabsf(y);
   const uint32_t c = (uint32_t)(a > 0.25f) + (a >= 0.75f) + (a > 1.25f) + (a >= 1.75f) + (a > 2.5f) + (a >= 3.5f) + (a > 5.f);
   return y < 0.f && c ? c | 8u : c;
@@ -176,7 +179,7 @@ __device__ __forceinline__ void get(const uint8_t* chunk, int s, int u, f32x4& x
     } else if constexpr (KEY) {
       const u32x2 w = *reinterpret_cast<const u32x2*>(chunk + L::k_off(s, e.e0));
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = sc * (float)(int8_t)(w[i >> 2] >> (8 * (i & 3)));
+      for (int i = 0; i < 8; ++i) v[i] = int8_value(w[i >> 2] >> (8 * (i & 3)), sc);
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -184,7 +187,7 @@ __device__ __forceinline__ void get(const uint8_t* chunk, int s, int u, f32x4& x
           const uint32_t b = chunk[L::v_off(s, e.e0 + i)];
           v[i] = sc * fp4_value(b & 15u), v[i + 4] = sc * fp4_value(b >> 4);
         } else {
-          v[i] = sc * (float)(int8_t)chunk[L::v_off(s, e.e0 + i)], v[i + 4] = sc * (float)(int8_t)chunk[L::v_off(s, e.e1 + i)];
+          v[i] = int8_value(chunk[L::v_off(s, e.e0 + i)], sc), v[i + 4] = int8_value(chunk[L::v_off(s, e.e1 + i)], sc);
         }
       }
     }
@@ -258,7 +261,7 @@ __device__ __forceinline__ void get_run(const uint8_t* image, const Heads& out, 
       for (int k = 0; k < 8; ++k) {
         if (FMT == MR_KV_F16) v[k] = h2f((j < 2 ? w : w2)[k] >> (16 * (j & 1)) & 0xFFFFu);
         else if (FMT == MR_KV_MXFP4) v[k] = f * fp4_value(w[k & 3] >> (8 * j + (k & 4)) & 15u);
-        else v[k] = f * (float)(int8_t)(w[k] >> (8 * j));
+        else v[k] = int8_value(w[k] >> (8 * j), f);
       }
       const uint64_t o = at(out, t + s + j, head);
       store4(out.p, out.dtype, o + e.e0, f32x4{v[0], v[1], v[2], v[3]});
