@@ -6,6 +6,10 @@
 // codes into operands rounds nothing. Pages lie in the order in which the lanes read them (KvLayout): no LDS,
 // no barrier and no exchange of elements between lanes; a wave takes chunks of 64 tokens by itself.
 //
+// 32 sequences of 16000 tokens, 4 heads of 128: MXFP4 279 MB in 56 us, 5.0 TB/s, MXINT8 541 MB in 109 us, 5.0 TB/s, of
+// the 6 TB/s that reading alone reaches here; what is missing is the launch and the first and last chunks, about 8 us.
+// One short sequence is latency: 5.6 us.
+//
 // The sequences' chunks are dealt out to the workgroups in parts of one size, so that a long sequence next to
 // short ones is spread over many CUs; the parts of a sequence are joined by a second launch.
 #include "mr_attn_device.h"
@@ -96,7 +100,7 @@ __device__ __forceinline__ bool find_part(const DecodeArgs& a, uint32_t i, bool 
     return wave_total(v);
   };
   // The smallest size, in steps of an eighth, at which the CUs hold all parts at once: a part more would run after
-  // the others, alone (32 sequences up to 24000: PART_FIGURES). Next to many sequences, the long ones are still split.
+  // the others, alone (32 sequences up to 24000: 54 -> 49 us). Next to many sequences, the long ones are still split.
   const uint32_t all = sum_of([](uint32_t c) { return c; }), most = part_limit(a.parts, a.n_seqs);
   r.size = max(kMinPart, (all + a.parts - 1) / a.parts);
   while (r.size < all && sum_of([&](uint32_t c) { return max(1u, (c + r.size - 1) / r.size); }) > most) r.size += (r.size + 7) / 8;
@@ -226,7 +230,9 @@ struct Chunk {
 };
 
 // Waves of a SIMD, as many as the registers of a chunk and of the sums leave room for, and whether the next
-// chunk's keys are on their way while this one's values are used; both measured (DECODE_TABLE).
+// chunk's keys are on their way while this one's values are used. Measured: MXFP4, heads of 128, two waves and three:
+// 62 and 54 us (32 sequences up to 24000); MXINT8, of 256, one wave and ahead, two and not: 34.6 and 31.6 us (100001
+// tokens); F16, of 256, the same: 100 and 108 us (16 of 16000).
 template <int FMT, int D>
 struct Tuning {
   static constexpr int kPerSimd = D == 64 ? (FMT == 16 ? 3 : 4) : D == 128 ? (FMT == 4 ? 3 : 2) : FMT == 16 ? 1 : 2;
@@ -401,7 +407,7 @@ __global__ __launch_bounds__(64 * kWaves, (Tuning<FMT, D>::kPerSimd)) void k_att
 
 // Joins the parts of split sequence blockIdx.x for one query head: first all parts' weights, then the weighted
 // sums, D/4 lanes to a part and kJoin / (D/4) parts at a time, many loads in flight (a running maximum would
-// make each part wait for the one before: 36 us for 391 parts of 256, instead of JOIN_US).
+// make each part wait for the one before: 36 us for 391 parts of 256, instead of 7 us for 224).
 constexpr int kJoin = 256;
 template <int D>
 __global__ __launch_bounds__(kJoin) void k_attn_join(DecodeArgs a) {

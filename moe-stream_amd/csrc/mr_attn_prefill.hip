@@ -7,6 +7,14 @@
 // already where the second product wants its right operand, if that product counts its keys in the
 // order the first one left them in (16 c + 4 h + 0..3, then 16 c + 8 + 4 h + 0..3 for lane half h).
 // V^T in that order is what the transposing LDS read returns: four adjacent keys of one column.
+// p is rounded to the type of v for the second product, as the matrix instructions take it.
+//
+// Matrix instructions and the exponentials' vector instructions bound it in about equal parts (a step of 32 rows and 64
+// keys of 128: 1024 cycles of the one, 900 of the other), under the card's power limit: fewer cycles, as with the
+// pipelined form below, came at a lower clock. 8192 tokens: heads of 128 (32 on 4) 613 us, 897 TFLOP/s; of 64 (64 on 8)
+// 640 us, 859; of 256 (16 on 2) 645 us, 853; the library's products reach 1430 to 1490. With a window of 128, 64 heads
+// of 64, 61 us: 151 MB at 2.5 TB/s, the exponentials of steps that rows see in part; short prompts are latency, 6 us
+// for 61 tokens.
 #include "mr_attn_device.h"
 
 namespace mr {
@@ -287,7 +295,7 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
         u32x4 pf[4], kf[2][2], vf[3];
         kf[0][0] = key_part(kb, 0, 0), kf[0][1] = key_part(kb, 1, 0);
         // Waves between their matrix instructions give way to those at them: the two of a SIMD then take turns
-        // (8192 tokens, heads of 128: 675 -> 649 us).
+        // (8192 tokens, heads of 128: 675 -> 649 us, before the later steps).
         __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
