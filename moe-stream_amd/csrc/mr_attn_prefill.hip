@@ -431,12 +431,12 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
   }
 
   if (!careful) {
-    bool odd = false;
+    float most = 0.f;  // NaN if any sum is
 #pragma unroll
     for (int t = 0; t < ND; ++t)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) odd |= !(fabsf(acc[t][i]) < INFINITY);
-    if (__syncthreads_or(odd)) return false;
+      for (int i = 0; i < 16; ++i) most = __builtin_elementwise_maximum(most, fabsf(acc[t][i]));
+    if (__syncthreads_or(!(most < INFINITY))) return false;
   }
 
   l = add_xor32(l);
