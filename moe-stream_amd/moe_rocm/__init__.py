@@ -497,6 +497,42 @@ class GgufFile:
         L.norm_w, L.eps = nw.value, eps.value
         return L
 
+    def _meta(self, get, key: str, default):
+        try:
+            return get(key)
+        except MoeRocmError:
+            return default
+
+    def attention(self) -> dict:
+        """The attention shape the metadata gives: query and key heads, head width, rotated part of it, window (0: none)."""
+        a = self.meta_str("general.architecture")
+        heads = self.meta_u32(f"{a}.attention.head_count")
+        dim = self._meta(self.meta_u32, f"{a}.attention.key_length", 0) or self.meta_u32(f"{a}.embedding_length") // heads
+        return dict(n_heads=heads, n_kv_heads=self._meta(self.meta_u32, f"{a}.attention.head_count_kv", heads), head_dim=dim,
+                    rotary_dim=self._meta(self.meta_u32, f"{a}.rope.dimension_count", dim),
+                    window=self._meta(self.meta_u32, f"{a}.attention.sliding_window", 0))
+
+    def rope(self, ctx: "Context", layout: int = 0) -> "Rope":
+        """The model's rotary frequencies ({arch}.rope.*: freq_base, dimension_count, scaling.type linear or yarn with its
+        factor and original_context_length), for qk_norm_rope. layout: ROPE_HALF, the reference's, or ROPE_INTERLEAVED."""
+        a, shape = self.meta_str("general.architecture"), self.attention()
+        kind = self._meta(self.meta_str, f"{a}.rope.scaling.type", "none")
+        if kind not in ("none", "linear", "yarn"):
+            raise MoeRocmError(MR_E_UNSUPPORTED, f"rope scaling {kind!r}")
+        # GPT-OSS takes YaRN's bounds as they come, other models round them to whole pairs
+        scaling = {"none": ROPE_PLAIN, "linear": ROPE_LINEAR,
+                   "yarn": ROPE_YARN_EXACT if a.startswith(("gpt-oss", "gpt_oss")) else ROPE_YARN}[kind]
+        more = {} if kind == "none" else dict(
+            factor=self.meta_f32(f"{a}.rope.scaling.factor"),
+            orig_context=self._meta(self.meta_u32, f"{a}.rope.scaling.original_context_length", 0))
+        return Rope(ctx, shape["head_dim"], rotary_dim=shape["rotary_dim"], layout=layout, scaling=scaling,
+                    base=self._meta(self.meta_f32, f"{a}.rope.freq_base", 10000.0), **more)
+
+    def kv_cache(self, ctx: "Context", fmt: int, n_pages: int, page_size: int) -> "KvCache":
+        """One layer's cache of the model's key heads and width."""
+        shape = self.attention()
+        return KvCache(ctx, fmt, n_pages, page_size, shape["n_kv_heads"], shape["head_dim"])
+
 
 def topk(ctx: Context, logits, n_tokens: int, n_experts: int, top_k: int, flags: int, idx, w) -> None:
     ctx.check(_lib.mr_topk(ctx.h, _ptr(logits), n_tokens, n_experts, top_k, flags, _ptr(idx), _ptr(w)))

@@ -12,6 +12,7 @@ import moe_rocm as M
 from moe_rocm import attn as A
 
 import attnref as R
+import gguf_writer as G
 from test_rust_binding import _strip_c_comments, c_to_rust
 
 ROOT = Path(__file__).resolve().parent.parent
@@ -218,6 +219,35 @@ def test_prefill_refusals(hctx):
             (dict(k=M.Heads(X, 2, M.F16, token_stride=1 << 24)), M.MR_E_INVAL, "2^24"),
             (dict(k=M.Heads(X, 2, M.F16, token_stride=4)), M.MR_E_INVAL, "stride"), (dict(v=None), M.MR_E_INVAL, "v is NULL")):
         refused(status, text, call, **kw)
+
+
+def test_shapes_and_frequencies_from_a_model_file(hctx, tmp_path):
+    arch = [("general.architecture", G.STR, "gpt-oss"), ("gpt-oss.attention.head_count", G.U32, 64),
+            ("gpt-oss.attention.head_count_kv", G.U32, 8), ("gpt-oss.attention.key_length", G.U32, 64),
+            ("gpt-oss.attention.sliding_window", G.U32, 128), ("gpt-oss.rope.freq_base", G.F32, 150000.0)]
+    yarn = [("gpt-oss.rope.scaling.type", G.STR, "yarn"), ("gpt-oss.rope.scaling.factor", G.F32, 32.0),
+            ("gpt-oss.rope.scaling.original_context_length", G.U32, 4096)]
+    G.write(tmp_path / "a.gguf", arch + yarn, [])
+    with M.GgufFile(tmp_path / "a.gguf") as g:
+        assert g.attention() == dict(n_heads=64, n_kv_heads=8, head_dim=64, rotary_dim=64, window=128)
+        r, kv = g.rope(hctx), g.kv_cache(hctx, M.KV_MXFP4, 4, 64)
+        f, mul = r.frequencies()
+        rf, rmul = R.rope_freqs(64, 150000.0, "yarn_exact", 32.0, 4096)
+        assert np.allclose(f, rf, rtol=1e-13, atol=0) and abs(mul - rmul) <= 2.0 ** -24 * rmul
+        assert (kv.desc.n_heads, kv.desc.head_dim) == (8, 64)
+        r.close(), kv.close()
+    # defaults: width from the embedding, as many key heads as heads, no scaling; part of a head rotated
+    G.write(tmp_path / "b.gguf", [("general.architecture", G.STR, "x"), ("x.attention.head_count", G.U32, 4),
+                                  ("x.embedding_length", G.U32, 512), ("x.rope.dimension_count", G.U32, 32)], [])
+    with M.GgufFile(tmp_path / "b.gguf") as g:
+        assert g.attention() == dict(n_heads=4, n_kv_heads=4, head_dim=128, rotary_dim=32, window=0)
+        r = g.rope(hctx, M.ROPE_INTERLEAVED)
+        f, mul = r.frequencies()
+        assert np.allclose(f, R.rope_freqs(32, 10000.0)[0], rtol=1e-13, atol=0) and mul == 1.0
+        r.close()
+    G.write(tmp_path / "c.gguf", arch + [("gpt-oss.rope.scaling.type", G.STR, "su")], [])
+    with M.GgufFile(tmp_path / "c.gguf") as g:
+        refused(M.MR_E_UNSUPPORTED, "su", g.rope, hctx)
 
 
 # The plain forms the GPU tests compare with, at values worked out by hand.
