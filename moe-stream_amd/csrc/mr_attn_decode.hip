@@ -494,7 +494,9 @@ hipError_t launch_attn_decode(const Launch& K, const KvPages& kv, uint32_t forma
   const uint64_t cap = (uint64_t)max_pages << (kv.page_shift - 6);
   const uint64_t chunks = o.window ? std::min<uint64_t>(cap, (o.window + 62ull) / 64 + 1) : cap;  // of a sequence at most
   const uint32_t room = std::min<uint32_t>(kPartUnits, per_cu * n_cu);
-  a.parts = chunks <= whole_chunks(D) || B > kSplitSeqs ? 1 : std::max<uint32_t>(1, room / units);
+  // the parts are counted in 32 bits
+  const bool whole = chunks <= whole_chunks(D) || B > kSplitSeqs || B * chunks >= 1ull << 31;
+  a.parts = whole ? 1 : std::max<uint32_t>(1, room / units);
   hipError_t e;
   {
     ProfScope ps(K, "attn_decode");

@@ -602,6 +602,44 @@ def test_prompt_then_decode(gpu_ctx, fmt, graph):
     kv.close(), rope.close()
 
 
+def test_two_graphs_on_one_workspace(gpu_ctx):
+    """Graphs of split calls of two caches, replayed in turn with eager calls between: each replay is the eager
+    result to the bit, and sees the lengths of its time."""
+    caches = [Cached(gpu_ctx, M.KV_MXFP4, [5000, 700], 2, 128, 256, 1), Cached(gpu_ctx, M.KV_F16, [3000], 1, 64, 64, 2)]
+    rng = np.random.default_rng(5)
+    rows, graphs = [], []
+    for c in caches:
+        B, H, D = len(c.lens), 4 * c.kv.desc.n_heads, c.kv.desc.head_dim
+        rows.append([R.Rows(gpu_ctx, rng.normal(size=(B, H, D)), M.F16)] + [R.Rows(gpu_ctx, None, M.F16, B, H, D) for _ in range(2)])
+
+    def call(i, out):
+        c = caches[i]
+        c.kv.attend(rows[i][0].heads, len(c.lens), c.d_len, c.d_table, c.max_pages, rows[i][out].heads)
+
+    for i in range(2):
+        gpu_ctx.graph_begin()
+        call(i, 1)
+        graphs.append(gpu_ctx.graph_end())
+    for cut in (0, 100, 2500):
+        for c in caches:
+            c.d_len.upload(np.maximum(np.array(c.lens, np.int32) - cut, 0).astype(np.int32))
+        for _ in range(2):
+            for i in (0, 1):
+                graphs[i].launch()
+                call(1 - i, 2)
+                call(i, 2)
+            gpu_ctx.sync()
+            for q, replayed, eager in rows:
+                assert (replayed.all() == eager.all()).all()
+    for g in graphs:
+        g.close()
+    for c in caches:
+        c.close()
+    for r in rows:
+        for b in r:
+            b.free()
+
+
 def test_two_contexts_and_a_callers_stream(gpu_ctx):
     """Two contexts at once, one of them on a stream of the caller's, each with its own cache and workspace."""
     lens = [3000, 700]
