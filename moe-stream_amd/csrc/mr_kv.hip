@@ -2,7 +2,7 @@
 //
 // A block of 32 elements is stored as codes * 2^e. e comes from the bits of the largest magnitude and
 // x * 2^-e is exact, so the codes are the nearest ones, with no rounding before the last. Memory bounds large calls
-// (100001 tokens of 2 heads of 256, f32 to 8 bits: 516 MB in 128 us, 4.0 TB/s), latency small ones: 5 us.
+// (100001 tokens of 2 heads of 256, f32 to 8 bits: 516 MB in 126 us, 4.1 TB/s), latency small ones: 5 us.
 #include "mr_attn_device.h"
 
 namespace mr {
@@ -51,12 +51,17 @@ constexpr int kWindow = 64;  // tokens of a workgroup
 
 // Runs of tokens that fill a chunk. The values' bytes of a token lie 16 bytes apart in its chunk; where 64 tokens
 // in a row go to (come from) the 64 slots of a chunk in order, as most of a prompt's do, they are put together
-// in LDS and the chunk is moved whole (8191 tokens, 4 heads of 128, 8 bits: written in 16.3 us one by one, in 14.0 so,
-// read in 22.9 and 13.8; 100001 tokens, 2 heads of 256: written in 232 and 128 us). The workgroup in whose
-// window of 64 tokens such a run begins does all of it; the tokens of no run are done one by one.
+// in LDS and the chunk is moved whole (8192 tokens, 4 heads of 128, 8 bits: 8.4 us written, 8.0 read; 100001 tokens,
+// 2 heads of 256: written in 232 us one by one, in 126 so). The workgroup in whose
+// window of 64 tokens such a run begins does all of it. Of the others, kPiece tokens or more in a row in a chunk (a
+// prompt's first and last) go four at a time to words of the chunk: 8191 tokens were written in 12.4 us and read in 12.9 with
+// the last 63 one by one, each byte an access of its own in one workgroup, and are in 10.7 and 8.9. The rest go one by one.
 struct Runs {
-  uint64_t start, single;  // bit i: token i of the window begins a run; is in none, and has a slot
+  // bit i: token i of the window begins a run; begins a piece; ends a row of tokens in a chunk; is in none, and has a slot
+  uint64_t start, piece, end, single;
 };
+constexpr int kPiece = 8;
+__device__ __forceinline__ int piece_length(uint64_t end, int b) { return __ffsll((unsigned long long)(end >> b)); }
 // slots[i] is the slot of token i - 63 of the window, -1 outside the call. All threads call.
 __device__ __forceinline__ Runs find_runs(const KvPages& kv, const int32_t* __restrict__ slots, int T, int t0, int (&sl)[192],
                                           uint64_t (&breaks)[3]) {
@@ -81,7 +86,16 @@ __device__ __forceinline__ Runs find_runs(const KvPages& kv, const int32_t* __re
   }
   Runs r;
   r.start = __ballot(in_run && (slot & 63) == 0);
-  r.single = __ballot(!in_run && slot >= 0);
+  const uint64_t rest = __ballot(!in_run && slot >= 0);
+  r.end = __ballot(lane == 63 || (breaks[(63 + lane) >> 6] >> ((63 + lane) & 63) & 1) || (slot & 63) == 63);
+  // a piece: begins behind an end, is long enough, and lies in the cache
+  const bool first_in = (lane == 0 || (r.end >> (lane - 1) & 1)) && (rest >> lane & 1);
+  r.piece = __ballot(first_in && ((uint32_t)slot >> kv.page_shift) < kv.n_pages && piece_length(r.end, lane) >= kPiece);
+  r.single = rest;
+  for (uint64_t todo = r.piece; todo; todo &= todo - 1) {
+    const int b = __ffsll((unsigned long long)todo) - 1;
+    r.single &= ~((~0ull >> (64 - piece_length(r.end, b))) << b);
+  }
   return r;
 }
 
@@ -199,19 +213,21 @@ __device__ __forceinline__ void get(const uint8_t* chunk, int s, int u, f32x4& x
 
 __device__ __forceinline__ uint64_t at(const Heads& h, int t, int head) { return (uint64_t)t * h.ts + (uint64_t)head * h.hs; }
 
-// The values of tokens t .. t + 63 to an LDS image of a chunk's values (codes, then scales), and back. A thread has
-// 4 adjacent tokens: their codes of an element are adjacent too, a word (F16: two) of the image.
+// The values of tokens t + lo .. t + hi - 1 to slots lo .. hi - 1 of an LDS image of a chunk's values (codes, then
+// scales); other slots get something. A thread has 4 adjacent slots: their codes of an element are adjacent too, a
+// word (F16: two) of the image.
 template <int FMT, int D>
-__device__ __forceinline__ void put_run(uint8_t* image, const Heads& in, int t, int head) {
+__device__ __forceinline__ void put_run(uint8_t* image, const Heads& in, int t, int head, int lo, int hi) {
   using L = KvLayout<FMT, D>;
   constexpr int U = D / 8;
   for (int i = threadIdx.x; i < U * 16; i += 256) {
     const int u = i % U, s = 4 * (i / U);
+    if (s + 4 <= lo || s >= hi) continue;  // the same for the lanes of a token
     const Quads e = quads(false, u);
     f32x4 x[4], y[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const uint64_t o = at(in, t + s + j, head);
+      const uint64_t o = at(in, t + min(max(s + j, lo), hi - 1), head);
       x[j] = load4(in.p, in.dtype, o + e.e0), y[j] = load4(in.p, in.dtype, o + e.e1);
     }
     uint32_t w[8] = {}, w2[8] = {}, sc = 0;
@@ -236,17 +252,47 @@ __device__ __forceinline__ void put_run(uint8_t* image, const Heads& in, int t, 
     if (FMT != MR_KV_F16 && (u & 3) == 0) *reinterpret_cast<uint32_t*>(image + L::vs_off(s, u >> 2) - L::kVs + L::kCodes) = sc;
   }
 }
+// Slots lo .. hi - 1 of the image to the chunk, by 4 adjacent slots; the ends, which share those bytes with tokens
+// that others may be writing, one by one.
 template <int FMT, int D>
-__device__ __forceinline__ void get_run(const uint8_t* image, const Heads& out, int t, int head) {
+__device__ __forceinline__ void store_piece(uint8_t* chunk, const uint8_t* image, int lo, int hi) {
+  using L = KvLayout<FMT, D>;
+  constexpr int E = FMT == MR_KV_F16 ? 2 : 1;  // bytes of a token's code
+  for (int i = threadIdx.x * 4 * E; i < L::kCodes + L::kScales; i += 256 * 4 * E) {
+    // v_off and vs_off the other way round: j, and the slot's bits 5 and 2 to 3
+    const bool codes = i < L::kCodes;
+    const int n = codes ? ((i >> 10) * 16 + (i & 15)) / E : i - L::kCodes, q = (n >> 3) / (codes && FMT != MR_KV_MXFP4 ? D / 16 : D / 32);
+    const int s = 4 * (n & 4) + (codes ? 32 * q + 4 * (i >> 8 & 3) : 32 * (q & 1) + 4 * (q >> 1));
+    if (s + 4 <= lo || s >= hi) continue;
+    uint8_t* g = chunk + (codes ? L::kV + i : L::kVs + i - L::kCodes);
+    const uint8_t* l = image + i;
+    if (s >= lo && s + 4 <= hi) {
+      if (FMT == MR_KV_F16) *reinterpret_cast<u32x2*>(g) = *reinterpret_cast<const u32x2*>(l);
+      else *reinterpret_cast<uint32_t*>(g) = *reinterpret_cast<const uint32_t*>(l);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (s + j < lo || s + j >= hi) continue;
+        if (FMT == MR_KV_F16) reinterpret_cast<uint16_t*>(g)[j] = reinterpret_cast<const uint16_t*>(l)[j];
+        else g[j] = l[j];
+      }
+    }
+  }
+}
+// And back: all 64 tokens, or tokens t + lo .. t + hi - 1, of the image or of the chunk itself.
+template <int FMT, int D, bool WHOLE>
+__device__ __forceinline__ void get_run(const uint8_t* codes, const uint8_t* scales, const Heads& out, int t, int head, int lo = 0,
+                                        int hi = 64) {
   using L = KvLayout<FMT, D>;
   constexpr int U = D / 8;
   for (int i = threadIdx.x; i < U * 16; i += 256) {
     const int u = i % U, s = 4 * (i / U);
+    if (!WHOLE && (s + 4 <= lo || s >= hi)) continue;
     const Quads e = quads(false, u);
     uint32_t w[8] = {}, w2[8] = {}, sc = 0;
 #pragma unroll
     for (int k = 0; k < (FMT == MR_KV_MXFP4 ? 4 : 8); ++k) {
-      const uint8_t* p = image + L::v_off(s, (k < 4 ? e.e0 : e.e1 - 4) + k) - L::kV;
+      const uint8_t* p = codes + L::v_off(s, (k < 4 ? e.e0 : e.e1 - 4) + k) - L::kV;
       if (FMT == MR_KV_F16) {
         const u32x2 a = *reinterpret_cast<const u32x2*>(p);
         w[k] = a.x, w2[k] = a.y;
@@ -254,9 +300,10 @@ __device__ __forceinline__ void get_run(const uint8_t* image, const Heads& out, 
         w[k] = *reinterpret_cast<const uint32_t*>(p);
       }
     }
-    if (FMT != MR_KV_F16) sc = *reinterpret_cast<const uint32_t*>(image + L::vs_off(s, u >> 2) - L::kVs + L::kCodes);
+    if (FMT != MR_KV_F16) sc = *reinterpret_cast<const uint32_t*>(scales + L::vs_off(s, u >> 2) - L::kVs);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
+      if (!WHOLE && (s + j < lo || s + j >= hi)) continue;
       const float f = FMT == MR_KV_F16 ? 1.f : scale_value<FMT>(sc >> (8 * j) & 0xFFu);
       float v[8];
 #pragma unroll
@@ -308,12 +355,16 @@ __global__ __launch_bounds__(256) void k_kv_write(KvPages kv, Heads kin, Heads v
   __shared__ __attribute__((aligned(16))) uint8_t image[L::kCodes + L::kScales];
   const Quads e = quads(false, u);
   const Runs r = find_runs(kv, slots, T, t0, sl, breaks);
-  for (uint64_t todo = r.start; todo; todo &= todo - 1) {
+  for (uint64_t todo = r.start | r.piece; todo; todo &= todo - 1) {
     const int b = __ffsll((unsigned long long)todo) - 1;
-    put_run<FMT, D>(image, vin, t0 + b, h);
+    const bool whole = r.start >> b & 1;
+    int lo;
+    uint8_t* chunk = find(kv, sl[63 + b], h, err, lo);
+    const int hi = whole ? 64 : lo + piece_length(r.end, b);
+    put_run<FMT, D>(image, vin, t0 + b - lo, h, lo, hi);
     __syncthreads();
-    int s;
-    move_image<FMT, D, true>(find(kv, sl[63 + b], h, err, s), image);
+    if (whole) move_image<FMT, D, true>(chunk, image);
+    else store_piece<FMT, D>(chunk, image, lo, hi);
     __syncthreads();
   }
   for (int i = i0; i < kWindow; i += N) {
@@ -358,8 +409,14 @@ __global__ __launch_bounds__(256) void k_kv_read(KvPages kv, int T, const int32_
     int s;
     move_image<FMT, D, false>(find(kv, sl[63 + b], h, err, s), image);
     __syncthreads();
-    get_run<FMT, D>(image, vout, t0 + b, h);
+    get_run<FMT, D, true>(image, image + L::kCodes, vout, t0 + b, h);
     __syncthreads();
+  }
+  for (uint64_t todo = r.piece; todo; todo &= todo - 1) {
+    const int b = __ffsll((unsigned long long)todo) - 1;
+    int lo;
+    const uint8_t* chunk = find(kv, sl[63 + b], h, err, lo);
+    get_run<FMT, D, false>(chunk + L::kV, chunk + L::kVs, vout, t0 + b - lo, h, lo, lo + piece_length(r.end, b));
   }
   // the others, and zeros for tokens without a slot
   for (int i = i0; i < kWindow; i += N) {

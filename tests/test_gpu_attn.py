@@ -172,6 +172,45 @@ def test_write_of_a_run_of_tokens(gpu_ctx, T, start):
         kv.close()
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_rows_of_every_length_written_and_read(gpu_ctx, fmt, D):
+    """Rows of adjacent slots, of every length and place in a chunk, with gaps and negative slots between them; read
+    in the same order, in rows cut elsewhere, and slot by slot."""
+    rng = np.random.default_rng(D)
+    fmt, H, page, pages = FORMATS[fmt], 2, 128, 24
+    kv = M.KvCache(gpu_ctx, fmt, pages, page, H, D)
+    rows = []
+    for chunk in rng.permutation(pages * page // 64):
+        a, b = sorted(rng.choice(65, 2, replace=False))
+        rows.append(64 * chunk + np.arange(a, b))
+        if chunk % 5 == 0:
+            rows.append(np.array([-1]))
+    slots = np.concatenate(rows).astype(np.int32)
+    T = len(slots)
+    x, y = (R.rounded(_values(rng, (T, H, D)), M.BF16) for _ in range(2))
+    dk, dv, ds = R.Rows(gpu_ctx, x, M.BF16), R.Rows(gpu_ctx, y, M.BF16), R.i32(gpu_ctx, slots)
+    kv.write(dk.heads, dv.heads, T, ds)
+    live = slots >= 0
+    held = [np.zeros((pages * page, H, D)) for _ in range(2)]
+    for h, a in zip(held, (x, y)):
+        h[slots[live]] = R.stored(a[live], fmt)
+    for order in (slots, np.arange(pages * page)[5:-9], rng.permutation(pages * page)):
+        n = len(order)
+        ko, vo = (R.Rows(gpu_ctx, None, M.F32, n, H, D, pad=1) for _ in range(2))
+        do = R.i32(gpu_ctx, order.astype(np.int32))
+        kv.read(n, do, ko.heads, vo.heads)
+        gpu_ctx.sync()
+        for got, h in ((ko.get(), held[0]), (vo.get(), held[1])):
+            want = np.where((order >= 0)[:, None, None], h[np.maximum(order, 0)], 0.0)
+            assert (got == want).all()
+        for b in (ko, vo, do):
+            b.free()
+    for b in (dk, dv, ds):
+        b.free()
+    kv.close()
+
+
 def test_slots_out_of_range_are_left_out_and_reported(gpu_ctx):
     H, D, page = 2, 64, 64
     kv = M.KvCache(gpu_ctx, M.KV_MXFP4, 2, page, H, D)
