@@ -11,10 +11,12 @@
 //
 // Matrix instructions and the exponentials' vector instructions bound it in about equal parts (a step of 32 rows and 64
 // keys of 128: 1024 cycles of the one, 900 of the other), under the card's power limit: fewer cycles, as with the
-// pipelined form below, came at a lower clock. 8192 tokens: heads of 128 (32 on 4) 613 us, 897 TFLOP/s; of 64 (64 on 8)
-// 640 us, 859; of 256 (16 on 2) 645 us, 853; the library's products reach 1430 to 1490. With a window of 128, 64 heads
+// pipelined form below, came at a lower clock. 8192 tokens, the card warm: heads of 128 (32 on 4) 520 us, 1057
+// TFLOP/s; of 64 (64 on 8) 573 us, 959; of 256 (16 on 2) 584 us, 941; the library's products reach 1430 to 1490. With a window of 128, 64 heads
 // of 64, 61 us: 151 MB at 2.5 TB/s, the exponentials of steps that rows see in part; short prompts are latency, 6 us
 // for 61 tokens.
+#include <numeric>
+
 #include "mr_attn_device.h"
 
 namespace mr {
@@ -67,7 +69,7 @@ __device__ __forceinline__ void load_lds16(uint64_t base, uint32_t bytes, uint32
 
 struct PrefillArgs {
   Heads q, k, v, out;
-  int nq, nk, n_seqs, n_tiles;
+  int nq, nk, n_seqs, n_tiles, together;  // together: heads whose tiles take turns
   const int32_t *cu_q, *cu_k;
   AttnOpts o;
   uint32_t* err;
@@ -141,9 +143,10 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
   asm volatile("" : "+v"(thread));  // nothing is kept in registers for the second time over
   const int wave = __builtin_amdgcn_readfirstlane(thread >> 6), lane = thread & 63, n = lane & 31, half = lane >> 5;
 
-  const int h = unit / a.n_tiles, hk = h / (int)(a.q.n / a.k.n);
+  const int set = unit / (a.n_tiles * a.together), in_set = unit % (a.n_tiles * a.together);
+  const int h = set * a.together + in_set % a.together, hk = h / (int)(a.q.n / a.k.n);
   Place pl;
-  if (!find_tile(a, unit % a.n_tiles, unit == 0 && !careful, lane, pl)) return true;
+  if (!find_tile(a, in_set / a.together, unit == 0 && !careful, lane, pl)) return true;
 
   // keys [first, last] of the tile's rows; a row r sees those up to r + diff, from r + diff - window + 1 on
   const int diff = pl.k1 - pl.q1;
@@ -479,11 +482,11 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
 template <int D, bool BF>
 __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 4) void k_attn_prefill(PrefillArgs a) {
   __shared__ __attribute__((aligned(1024))) uint16_t lds[4 * kKeys * D];  // rows at multiples of their length
-  // Workgroups go to the 8 XCDs in turn. Each XCD gets a contiguous share of the (head, tile) pairs, so that
-  // the query heads that share keys find them in one L2.
+  // Workgroups go to the 8 XCDs in turn. Each XCD gets an eighth of the heads, so that the query heads that share
+  // keys find them in one L2; heads that are not a multiple of 8 are spread over all.
   const int units = a.n_tiles * (int)a.q.n, per = (units + 7) / 8;
-  const int unit = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  if ((int)(blockIdx.x >> 3) >= per || unit >= units) return;
+  const int unit = a.q.n % 8 ? (int)blockIdx.x : (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if (unit >= units) return;
   for (bool careful = false; !attend_tile<D, BF>(a, lds, unit, careful); careful = true) {
   }
 }
@@ -497,7 +500,12 @@ hipError_t launch_attn_prefill(const Launch& K, uint32_t D, const Heads& q, uint
   // every sequence ends with at most one tile that is not full
   const uint64_t most = (uint64_t)nq / kRows + n_seqs, tiles = n_seqs > kScan ? most : std::min<uint64_t>(most, nq);
   const uint64_t units = tiles * q.n;  // below 2^24, checked by the caller
-  PrefillArgs a{q, k, v, out, (int)nq, (int)nk, (int)n_seqs, (int)tiles, cu_q, cu_k, o, err};
+  // Workgroups start in the order of their units, the longest rows first: with that for all of an XCD's heads at once the
+  // last to start are short (4096 tokens, 32 heads of 128 on 4: 177 us head by head, 142 so; on 32: 179 and 144; 28 on
+  // 4, over all XCDs: 170 and 130). More than 16 heads that share no keys lose more by it in the L2s than they gain
+  // (256 heads on 256, 32 of them to an XCD: 349 and 362).
+  const int per_xcd = (int)q.n / 8, together = q.n % 8 ? (int)q.n : per_xcd <= 16 ? per_xcd : (int)std::gcd(per_xcd, 16);
+  PrefillArgs a{q, k, v, out, (int)nq, (int)nk, (int)n_seqs, (int)tiles, together, cu_q, cu_k, o, err};
   const dim3 g((unsigned)((units + 7) / 8 * 8)), blk(256);
   const bool bf = q.dtype == MR_BF16;
   if (D == 64) hipLaunchKernelGGL((bf ? k_attn_prefill<64, true> : k_attn_prefill<64, false>), g, blk, 0, K.s, a);
