@@ -89,7 +89,7 @@ struct AttnOpts {
   const float* sinks;
 };
 
-constexpr int kPrefillRows = 128;  // query rows of a prefill tile
+constexpr int kPrefillRows = 128;  // query rows of a prefill tile, times the heads side by side
 
 hipError_t launch_qk_norm_rope(const Launch& K, const mr_rope& r, const Heads& q, const Heads& k, const float* qn,
                                const float* kn, float eps, const int32_t* pos, uint32_t T, const Heads& qo,

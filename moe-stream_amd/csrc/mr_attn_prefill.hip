@@ -13,7 +13,7 @@
 // keys of 128: 1024 cycles of the one, 900 of the other), under the card's power limit: fewer cycles, as with the
 // pipelined form below, came at a lower clock. 8192 tokens, the card warm: heads of 128 (32 on 4) 520 us, 1057
 // TFLOP/s; of 64 (64 on 8) 573 us, 959; of 256 (16 on 2) 584 us, 941; the library's products reach 1430 to 1490. With a window of 128, 64 heads
-// of 64, 61 us: 151 MB at 2.5 TB/s, the exponentials of steps that rows see in part; short prompts are latency, 6 us
+// of 64, 58 us: 151 MB at 2.6 TB/s, the exponentials of steps that rows see in part; short prompts are latency, 6 us
 // for 61 tokens.
 #include <numeric>
 
@@ -26,7 +26,6 @@ namespace {
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kRows = kPrefillRows;  // of a workgroup: 4 waves of 32
 constexpr int kKeys = 64;   // keys of a step
 // Up to so many sequences are looked through, 64 at a time, to find a tile's: each step costs about as much as one
 // of a search among more, which takes their log2.
@@ -67,9 +66,23 @@ __device__ __forceinline__ void load_lds16(uint64_t base, uint32_t bytes, uint32
                : "memory", "m0");
 }
 
+// Division of x < 2^24 by 1 <= d < 2^24: with 2^b <= d < 2^(b + 1), x ceil(2^(39 + b) / d) has 64 bits, and over
+// 2^(39 + b) it is above x / d by less than x / 2^(39 + b) < 1 / d.
+struct Divisor {
+  uint64_t mul;
+  uint32_t d, shift;
+  explicit Divisor(uint32_t d) : d(d), shift(70 - __builtin_clz(d)) { mul = ((1ull << shift) + d - 1) / d; }
+  __device__ __forceinline__ uint32_t of(uint32_t x) const { return (uint32_t)((x * mul) >> shift); }
+};
+
 struct PrefillArgs {
   Heads q, k, v, out;
-  int nq, nk, n_seqs, n_tiles, together;  // together: heads whose tiles take turns
+  int nq, nk, n_seqs, n_tiles;
+  int share;        // log2 of the heads side by side: 2, 1, 0, with tiles of 32, 64, 128 rows
+  Divisor together;  // head sets (of 1 << share heads) whose tiles take turns
+  Divisor turn;      // their tiles
+  Divisor group;     // query heads that share a key head
+  __device__ __forceinline__ int rows() const { return kPrefillRows >> share; }
   const int32_t *cu_q, *cu_k;
   AttnOpts o;
   uint32_t* err;
@@ -86,29 +99,30 @@ __device__ __forceinline__ bool find_tile(const PrefillArgs& a, int tile, bool r
     int q0, q1, k0, k1, tiles;
     bool bad;
   };
+  const int row_bits = 7 - a.share;
   auto seq = [&](int s) {
     auto in = [](int x, int hi) { return min(max(x, 0), hi); };
     const int x = a.cu_q[s], y = a.cu_q[s + 1], kx = a.cu_k[s], ky = a.cu_k[s + 1];
     Seq r{in(x, a.nq), in(y, a.nq), in(kx, a.nk), in(ky, a.nk), 0, x < 0 || y < x || y > a.nq || kx < 0 || ky < kx || ky > a.nk};
-    r.q1 = max(r.q0, r.q1), r.k1 = max(r.k0, r.k1), r.tiles = (r.q1 - r.q0 + kRows - 1) / kRows;
+    r.q1 = max(r.q0, r.q1), r.k1 = max(r.k0, r.k1), r.tiles = (r.q1 - r.q0 + a.rows() - 1) >> row_bits;
     return r;
   };
   const bool search = a.n_seqs > kScan;
   bool found = false;
   if (search) {
-    // Sequence s has the tiles from cu_q[s] / kRows + s on: room for one that is not full, some left out.
+    // Sequence s has the tiles from cu_q[s] / rows + s on: room for one that is not full, some left out.
     int lo = 0, hi = a.n_seqs - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if (min(max(a.cu_q[mid], 0), a.nq) / kRows + mid <= tile) lo = mid;
+      if ((min(max(a.cu_q[mid], 0), a.nq) >> row_bits) + mid <= tile) lo = mid;
       else hi = mid - 1;
     }
     const Seq r = seq(lo);
-    const int i = tile - (r.q0 / kRows + lo);
+    const int i = tile - ((r.q0 >> row_bits) + lo);
     found = i >= 0 && i < r.tiles;
     p.q0 = __builtin_amdgcn_readfirstlane(r.q0), p.q1 = __builtin_amdgcn_readfirstlane(r.q1);
     p.k0 = __builtin_amdgcn_readfirstlane(r.k0), p.k1 = __builtin_amdgcn_readfirstlane(r.k1);
-    p.row = __builtin_amdgcn_readfirstlane(r.q0 + (r.tiles - 1 - i) * kRows);
+    p.row = __builtin_amdgcn_readfirstlane(r.q0 + (r.tiles - 1 - i) * a.rows());
     if (!report) return __builtin_amdgcn_readfirstlane(found);
   }
   int before = 0;
@@ -123,7 +137,7 @@ __device__ __forceinline__ bool find_tile(const PrefillArgs& a, int tile, bool r
       p.q0 = __builtin_amdgcn_readlane(r.q0, l), p.q1 = __builtin_amdgcn_readlane(r.q1, l);
       p.k0 = __builtin_amdgcn_readlane(r.k0, l), p.k1 = __builtin_amdgcn_readlane(r.k1, l);
       // the longest rows first
-      p.row = p.q0 + (before + __builtin_amdgcn_readlane(sum, l) - 1 - tile) * kRows;
+      p.row = p.q0 + (before + __builtin_amdgcn_readlane(sum, l) - 1 - tile) * a.rows();
       found = true;
     }
     before += __builtin_amdgcn_readlane(sum, 63);
@@ -143,23 +157,24 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
   asm volatile("" : "+v"(thread));  // nothing is kept in registers for the second time over
   const int wave = __builtin_amdgcn_readfirstlane(thread >> 6), lane = thread & 63, n = lane & 31, half = lane >> 5;
 
-  const int set = unit / (a.n_tiles * a.together), in_set = unit % (a.n_tiles * a.together);
-  const int h = set * a.together + in_set % a.together, hk = h / (int)(a.q.n / a.k.n);
+  const uint32_t set = a.turn.of(unit), in_set = unit - set * a.turn.d, tile = a.together.of(in_set);
+  const int h0 = (int)(set * a.together.d + in_set - tile * a.together.d) << a.share, h = h0 + (wave & ((1 << a.share) - 1));
+  const int hk = (int)a.group.of(h0), wave_row = (wave >> a.share) * 32;
   Place pl;
-  if (!find_tile(a, in_set / a.together, unit == 0 && !careful, lane, pl)) return true;
+  if (!find_tile(a, (int)tile, unit == 0 && !careful, lane, pl)) return true;
 
   // keys [first, last] of the tile's rows; a row r sees those up to r + diff, from r + diff - window + 1 on
   const int diff = pl.k1 - pl.q1;
-  const int row = pl.row + wave * 32 + n;  // this lane's query row
-  const int last_row = min(pl.row + kRows, pl.q1) - 1;
+  const int row = pl.row + wave_row + n;  // this lane's query row
+  const int last_row = min(pl.row + a.rows(), pl.q1) - 1;
   const int last = last_row + diff;  // < k1
   int first = pl.k0;
   if (a.o.window) first = (int)max((int64_t)first, (int64_t)pl.row + diff + 1 - (int64_t)a.o.window);
   const int see_last = row + diff;
   const int64_t w = a.o.window ? (int64_t)a.o.window : (int64_t)1 << 32;
   const int see_first = (int)max((int64_t)pl.k0, (int64_t)see_last + 1 - w);
-  const int wave_least = (int)max((int64_t)pl.k0, (int64_t)pl.row + wave * 32 + diff + 1 - w);  // first key of its first row
-  const int wave_first = (int)max((int64_t)pl.k0, (int64_t)pl.row + wave * 32 + 31 + diff + 1 - w);  // of its last row
+  const int wave_least = (int)max((int64_t)pl.k0, (int64_t)pl.row + wave_row + diff + 1 - w);  // first key of its first row
+  const int wave_first = (int)max((int64_t)pl.k0, (int64_t)pl.row + wave_row + 31 + diff + 1 - w);  // of its last row
 
   const float c = fmaxf(fabsf(a.o.scale) * 1.44269504088896340736f, 0x1p-126f);  // above zero: a masked score stays -inf
   u32x4 qf[D / 16];
@@ -234,7 +249,7 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
   // kSlack behind: p is at most 2^kSlack, and nearly no step rescales.
   auto settle = [&](int k0, f32x16& s0, f32x16& s1) {
     const int x = k0 + 4 * half;
-    if (k0 + kKeys - 1 > pl.row + wave * 32 + diff) {
+    if (k0 + kKeys - 1 > pl.row + wave_row + diff) {
       int most = see_last - x;
       asm volatile("" : "+v"(most));  // a branch: the compiler would do this in every step
 #pragma unroll
@@ -291,7 +306,7 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
         if (k0 + kKeys <= last) fetch_k(k0 + kKeys, b ^ 1), fetch_v(k0 + kKeys, b ^ 1);
         if (careful && edge(k0)) clean(b);
         // keys behind all of the wave's rows, or in front of all their windows
-        if (k0 > pl.row + wave * 32 + 31 + diff || k0 + kKeys <= wave_least) continue;
+        if (k0 > pl.row + wave_row + 31 + diff || k0 + kKeys <= wave_least) continue;
         uint32_t kb = k_at + b * 4 * kTile, vb = v_at + b * 4 * kTile;
         asm("" : "+v"(kb), "+v"(vb));  // the parts' addresses are worked out from here, not kept
         f32x16 s0 = {}, s1 = {};
@@ -448,7 +463,7 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
   const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : NAN;
   int tid = threadIdx.x;
   asm volatile("" : "+v"(tid));  // the row's address is worked out here, not kept through the steps
-  const int out_row = pl.row + wave * 32 + (tid & 31);
+  const int out_row = pl.row + wave_row + (tid & 31);
   if (out_row < pl.q1) {
     uint16_t* dst = static_cast<uint16_t*>(a.out.p) + (uint64_t)out_row * a.out.ts + (uint64_t)h * a.out.hs;
 #pragma unroll
@@ -467,9 +482,10 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
       for (int key = k0; key < min(k0 + kKeys, last + 1); ++key) {
         const uint16_t x = vp[(uint64_t)key * a.v.ts + d];
         if ((x & kTop) != kTop) continue;
-        for (int r = pl.row + threadIdx.x / D; r <= last_row; r += 256 / D) {
+        for (int i = threadIdx.x / D; i < (last_row + 1 - pl.row) << a.share; i += 256 / D) {
+          const int r = pl.row + (i >> a.share), head = h0 + (i & ((1 << a.share) - 1));
           if (key > r + diff || (a.o.window && key <= (int64_t)r + diff - (int64_t)a.o.window)) continue;
-          uint16_t* dst = static_cast<uint16_t*>(a.out.p) + (uint64_t)r * a.out.ts + (uint64_t)h * a.out.hs + d;
+          uint16_t* dst = static_cast<uint16_t*>(a.out.p) + (uint64_t)r * a.out.ts + (uint64_t)head * a.out.hs + d;
           const float y = BF ? bits_f32((uint32_t)*dst << 16) + bits_f32((uint32_t)x << 16) : h2f(*dst) + h2f(x);
           *dst = (uint16_t)pack16<BF>(y, 0.f);
         }
@@ -482,10 +498,10 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
 template <int D, bool BF>
 __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 4) void k_attn_prefill(PrefillArgs a) {
   __shared__ __attribute__((aligned(1024))) uint16_t lds[4 * kKeys * D];  // rows at multiples of their length
-  // Workgroups go to the 8 XCDs in turn. Each XCD gets an eighth of the heads, so that the query heads that share
-  // keys find them in one L2; heads that are not a multiple of 8 are spread over all.
-  const int units = a.n_tiles * (int)a.q.n, per = (units + 7) / 8;
-  const int unit = a.q.n % 8 ? (int)blockIdx.x : (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  // Workgroups go to the 8 XCDs in turn. Each XCD gets an eighth of the head sets, so that the query heads that share
+  // keys find them in one L2; sets that are not a multiple of 8 are spread over all.
+  const int sets = (int)a.q.n >> a.share, units = a.n_tiles * sets;
+  const int unit = sets % 8 ? (int)blockIdx.x : (blockIdx.x & 7) * (units / 8) + (blockIdx.x >> 3);
   if (unit >= units) return;
   for (bool careful = false; !attend_tile<D, BF>(a, lds, unit, careful); careful = true) {
   }
@@ -497,15 +513,22 @@ hipError_t launch_attn_prefill(const Launch& K, uint32_t D, const Heads& q, uint
                                uint32_t nk, uint32_t n_seqs, const int32_t* cu_q, const int32_t* cu_k, const AttnOpts& o,
                                const Heads& out, uint32_t* err) {
   ProfScope ps(K, "attn_prefill");
+  // A tile is of 4, 2 or 1 heads that share their keys and of 32, 64 or 128 rows. With the 4 waves at the same rows all take
+  // all of the tile's steps: with a window of 128 they are 3, not 4 of which each wave needs 3 (8192 tokens, 64 heads
+  // of 64: 63.2 us by 128 rows, 58.4 by 32 and 4 heads; 2000 earlier tokens, 16 heads of 256: 229 and 221; 20 prompts
+  // of 17 tokens: 10.7 and 7.6; but one of 61 tokens 5.8 and 6.5, in half as many workgroups).
+  const uint32_t group = q.n / k.n, share = group % 4 == 0 ? 2 : group % 2 == 0 ? 1 : 0, rows = kPrefillRows >> share;
   // every sequence ends with at most one tile that is not full
-  const uint64_t most = (uint64_t)nq / kRows + n_seqs, tiles = n_seqs > kScan ? most : std::min<uint64_t>(most, nq);
-  const uint64_t units = tiles * q.n;  // below 2^24, checked by the caller
+  const uint64_t most = (uint64_t)nq / rows + n_seqs, tiles = n_seqs > kScan ? most : std::min<uint64_t>(most, nq);
+  const uint32_t sets = q.n >> share, per_xcd = sets / 8;
+  const uint64_t units = tiles * sets;  // below 2^24, checked by the caller
   // Workgroups start in the order of their units, the longest rows first: with that for all of an XCD's heads at once the
   // last to start are short (4096 tokens, 32 heads of 128 on 4: 177 us head by head, 142 so; on 32: 179 and 144; 28 on
   // 4, over all XCDs: 170 and 130). More than 16 heads that share no keys lose more by it in the L2s than they gain
   // (256 heads on 256, 32 of them to an XCD: 349 and 362).
-  const int per_xcd = (int)q.n / 8, together = q.n % 8 ? (int)q.n : per_xcd <= 16 ? per_xcd : (int)std::gcd(per_xcd, 16);
-  PrefillArgs a{q, k, v, out, (int)nq, (int)nk, (int)n_seqs, (int)tiles, together, cu_q, cu_k, o, err};
+  const uint32_t together = sets % 8 ? sets : per_xcd <= 16 ? per_xcd : std::gcd(per_xcd, 16u);
+  PrefillArgs a{q, k, v, out, (int)nq, (int)nk, (int)n_seqs, (int)tiles, (int)share, Divisor(together),
+                Divisor(together * (uint32_t)tiles), Divisor(group), cu_q, cu_k, o, err};
   const dim3 g((unsigned)((units + 7) / 8 * 8)), blk(256);
   const bool bf = q.dtype == MR_BF16;
   if (D == 64) hipLaunchKernelGGL((bf ? k_attn_prefill<64, true> : k_attn_prefill<64, false>), g, blk, 0, K.s, a);

@@ -540,6 +540,44 @@ def test_prefill_infinities_and_nan_where_rows_do_not_look(gpu_ctx, D, dtype):
         b.free()
 
 
+@pytest.mark.parametrize("hk,group", [(8, 4), (4, 8), (2, 8), (3, 4), (8, 2), (5, 2), (3, 6), (16, 1), (17, 1), (136, 1), (5, 5), (40, 8)])
+def test_prefill_heads_in_every_arrangement(gpu_ctx, hk, group):
+    """Heads that share keys by 1, 2 and 4, in numbers that are a multiple of 8 and not."""
+    lens = [5, 0, 70, 33] if hk * group < 100 else [0, 34, 2]
+    prompts(gpu_ctx, 64, hk, group, M.BF16, lens, [n + 40 for n in lens], 50, seed=hk)
+    prompts(gpu_ctx, 64, hk, group, M.F16, lens, lens, seed=group)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("group", [2, 4])
+def test_prefill_infinities_and_nan_with_shared_keys(gpu_ctx, D, group):
+    """All heads of a group: rows that see an infinite value have it, rows that do not are as without it."""
+    n, window, hk = 150, 50, 2
+    rng = np.random.default_rng(D)
+    q, k, v = (R.rounded(rng.normal(size=(n, h, D)), M.BF16) for h in (hk * group, hk, hk))
+    clean = v.copy()
+    v[20, 0, 5], v[70, 1, 1], v[90, 0, 7] = np.inf, -np.inf, np.nan
+    dq, dk, dv, out = (R.Rows(gpu_ctx, a, M.BF16, n, h, D) for a, h in ((q, hk * group), (k, hk), (v, hk), (None, hk * group)))
+    cu = R.i32(gpu_ctx, [0, n])
+    M.attn_prefill(gpu_ctx, D, dq.heads, dk.heads, dv.heads, n, n, 1, cu, cu, out.heads, window=window)
+    gpu_ctx.sync()
+    got = out.get()
+    for r in range(n):
+        for h in range(hk * group):
+            first, g = max(0, r - window + 1), h // group
+            y, av, ss, cnt = R.attend(q[r, h], k[:, g], clean[:, g], D ** -0.5, first, r)
+            y = y.copy()
+            for at, head, d, x in ((20, 0, 5, np.inf), (70, 1, 1, -np.inf), (90, 0, 7, np.nan)):
+                if g == head and first <= at <= r:
+                    y[d] = x
+            fine = np.isfinite(y)
+            tol = R.attention_bound(np.where(fine, y, 0), av, ss, cnt, D, M.BF16, R.HALF[M.BF16])
+            assert np.array_equal(got[r, h][~fine], y[~fine], equal_nan=True), (r, h)
+            assert (np.abs(got[r, h] - y)[fine] <= tol[fine]).all(), (r, h)
+    for b in (dq, dk, dv, out, cu):
+        b.free()
+
+
 @pytest.mark.parametrize("cu_q,cu_k", [([0, 40, 999], [0, 40, 90]), ([0, 50, 30], [0, 50, 90]), ([-9, 40, 90], [0, 40, 90]),
                                        ([0, 40, 90], [0, 40, 2 ** 31 - 1]), ([0, 40, 90], [0, 60, 50]),
                                        ([0, 40, 90], [-2 ** 31, 40, 90])])
