@@ -120,7 +120,8 @@ void mr_kv_destroy(mr_kv* kv);
 uint64_t mr_kv_bytes(const mr_kv_desc* desc);
 /* Quantises token t of k and v (n_heads heads each, any types) into slot slots[t]. A negative slot
  * leaves the token out; so does one past the last page, with an error at mr_sync. The slots of a call
- * differ from each other: a slot named twice holds some mixture of the tokens. */
+ * differ from each other: a slot named twice holds some mixture of the tokens. n_tokens of a call, here
+ * and below: up to 2^30 - 64. */
 int mr_kv_write(mr_ctx* ctx, mr_kv* kv, const mr_heads* k, const mr_heads* v, uint32_t n_tokens,
                 const int32_t* slots);
 /* The values of slot slots[t] to token t of k and v (any types; either may be NULL): zeros for a

@@ -45,6 +45,7 @@ bool capturing(mr_ctx* c) {
 bool misaligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; }
 
 constexpr uint32_t kMaxWork = 1u << 24;  // workgroups of 256 threads that a launch's 2^32 threads allow
+constexpr uint32_t kMaxTokens = (kMaxWork - 1) * 64;  // of a cache write or read, 64 to a workgroup
 
 uint32_t elem_bytes(uint32_t dtype) { return dtype == MR_F32 ? 4 : 2; }
 
@@ -282,7 +283,7 @@ int mr_kv_write(mr_ctx* c, mr_kv* kv, const mr_heads* k, const mr_heads* v, uint
   if (hk.n != kv->d.n_heads || hv.n != kv->d.n_heads)
     return fail(c, MR_E_INVAL, "k has %u heads, v %u, the cache %u", hk.n, hv.n, kv->d.n_heads);
   if (!slots || misaligned(slots, 4)) return fail(c, MR_E_INVAL, "slots is NULL or not 4-byte aligned");
-  if (T > 0x7FFFFFFFu) return fail(c, MR_E_INVAL, "n_tokens %u is 2^31 or more", T);
+  if (T > kMaxTokens) return fail(c, MR_E_INVAL, "n_tokens %u is above 2^30 - 64", T);
   if (T == 0) return MR_OK;
   if ((rc = bind(c))) return rc;
   c->attn_used = true;
@@ -301,7 +302,7 @@ int mr_kv_read(mr_ctx* c, const mr_kv* kv, uint32_t T, const int32_t* slots, con
   if ((k && hk.n != kv->d.n_heads) || (v && hv.n != kv->d.n_heads))
     return fail(c, MR_E_INVAL, "k or v has another head count than the cache's %u", kv->d.n_heads);
   if (!slots || misaligned(slots, 4)) return fail(c, MR_E_INVAL, "slots is NULL or not 4-byte aligned");
-  if (T > 0x7FFFFFFFu) return fail(c, MR_E_INVAL, "n_tokens %u is 2^31 or more", T);
+  if (T > kMaxTokens) return fail(c, MR_E_INVAL, "n_tokens %u is above 2^30 - 64", T);
   if (T == 0) return MR_OK;
   if ((rc = bind(c))) return rc;
   c->attn_used = true;

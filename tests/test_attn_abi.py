@@ -160,6 +160,16 @@ def test_cache_bytes():
     assert M.KvCache.nbytes(M.KV_F16, 1, 1024, 8, 64) == 1024 * 8 * 2 * 128
 
 
+def test_tokens_of_a_write_fit_a_launch(hctx):
+    kv = M.KvCache(hctx, M.KV_MXFP4, 4, 64, 2, 64)
+    h, most = M.Heads(X, 2, M.F16), 2 ** 30 - 64
+    refused(M.MR_E_NODEV, "host-only", kv.write, h, h, most, X)
+    refused(M.MR_E_NODEV, "host-only", kv.read, most, X, h, h)
+    refused(M.MR_E_INVAL, "n_tokens", kv.write, h, h, most + 1, X)
+    refused(M.MR_E_INVAL, "n_tokens", kv.read, most + 1, X, h, h)
+    kv.close()
+
+
 def test_write_and_read_refusals(hctx):
     kv = M.KvCache(hctx, M.KV_MXFP4, 4, 64, 2, 64)
     h = M.Heads(X, 2, M.F16)
