@@ -198,21 +198,22 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
     for (int i = 0; i < kOff; ++i) k_off[i] = (uint32_t)(r * a.k.ts + 8 * k_piece<D>(r + i * kStep, cp)) * 2;
     v_off = (uint32_t)(r * a.v.ts + 8 * v_piece<D>(r, cp)) * 2;
   }
+  // One base and bound for a tile, with the rows in the lanes' offsets: worked out for each load it was 90 scalar instructions
+  // a step (8192 tokens, heads of 128 504 -> 496 us, of 256 577 -> 541).
+  const uint32_t k_step = (uint32_t)(kStep * a.k.ts) * 2, v_step = (uint32_t)(kStep * a.v.ts) * 2;
   auto fetch_k = [&](int k0, int b) {
+    const uint64_t base = (uint64_t)kp + (uint64_t)k0 * a.k.ts * 2;
+    const uint32_t bytes = (uint32_t)(min(last - k0, kKeys - 1) * a.k.ts + D) * 2;
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int key = k0 + i * kStep, rows = min(last + 1 - key, kStep);
-      load_lds16((uint64_t)kp + (uint64_t)key * a.k.ts * 2, rows > 0 ? (uint32_t)((rows - 1) * a.k.ts + D) * 2 : 0, k_off[i % kOff],
-                 lds0 + b * 4 * kTile + (i * 4 + wave) * 1024);
-    }
+    for (int i = 0; i < kLoads; ++i)
+      load_lds16(base, bytes, k_off[i % kOff] + i * k_step, lds0 + b * 4 * kTile + (i * 4 + wave) * 1024);
   };
   auto fetch_v = [&](int k0, int b) {
+    const uint64_t base = (uint64_t)vp + (uint64_t)k0 * a.v.ts * 2;
+    const uint32_t bytes = (uint32_t)(min(last - k0, kKeys - 1) * a.v.ts + D) * 2;
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int key = k0 + i * kStep, rows = min(last + 1 - key, kStep);
-      load_lds16((uint64_t)vp + (uint64_t)key * a.v.ts * 2, rows > 0 ? (uint32_t)((rows - 1) * a.v.ts + D) * 2 : 0, v_off,
-                 lds0 + b * 4 * kTile + 2 * kTile + (i * 4 + wave) * 1024);
-    }
+    for (int i = 0; i < kLoads; ++i)
+      load_lds16(base, bytes, v_off + i * v_step, lds0 + b * 4 * kTile + 2 * kTile + (i * 4 + wave) * 1024);
   };
 
   // whether some row of the workgroup does not see some key of the step
