@@ -75,6 +75,12 @@ struct Divisor {
   __device__ __forceinline__ uint32_t of(uint32_t x) const { return (uint32_t)((x * mul) >> shift); }
 };
 
+// x where bit `at` of `seen` is set, else -infinity.
+__device__ __forceinline__ float seen_or_least(float x, uint32_t seen, int at) {
+  const uint32_t keep = (uint32_t)__builtin_amdgcn_sbfe((int)seen, (uint32_t)at, 1u);
+  return bits_f32((keep & __float_as_uint(x)) | (~keep & 0xFF800000u));
+}
+
 struct PrefillArgs {
   Heads q, k, v, out;
   int nq, nk, n_seqs, n_tiles;
@@ -249,28 +255,23 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
   // Masks the scores of the keys from k0 on and moves the base m, with the sums, if their maximum has left it
   // kSlack behind: p is at most 2^kSlack, and nearly no step rescales.
   auto settle = [&](int k0, f32x16& s0, f32x16& s1) {
-    const int x = k0 + 4 * half;
-    if (k0 + kKeys - 1 > pl.row + wave_row + diff) {
-      int most = see_last - x;
+    if (k0 + kKeys - 1 > pl.row + wave_row + diff || k0 < wave_first) {
+      // Bit i: the row sees the i-th key from its half's first on. A bit and a select a score; a comparison and a select for
+      // each end have waits between them (8192 tokens, heads of 128, with the maxima below: 496 -> 492 us).
+      int most = see_last - k0 - 4 * half, least = see_first - k0 - 4 * half;
       asm volatile("" : "+v"(most));  // a branch: the compiler would do this in every step
+      const uint64_t seen = (most < 0 ? 0 : ~0ull >> (63 - min(most, 63))) & (least > 63 ? 0 : ~0ull << max(least, 0));
+      const uint32_t seen0 = (uint32_t)seen, seen1 = (uint32_t)(seen >> 32);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        s0[i] = 8 * (i >> 2) + (i & 3) > most ? -INFINITY : s0[i];
-        s1[i] = 8 * (i >> 2) + (i & 3) + 32 > most ? -INFINITY : s1[i];
-      }
-    }
-    if (k0 < wave_first) {
-      int least = see_first - x;
-      asm volatile("" : "+v"(least));
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s0[i] = 8 * (i >> 2) + (i & 3) < least ? -INFINITY : s0[i];
-        s1[i] = 8 * (i >> 2) + (i & 3) + 32 < least ? -INFINITY : s1[i];
+        const int at = 8 * (i >> 2) + (i & 3);
+        s0[i] = seen_or_least(s0[i], seen0, at);
+        s1[i] = seen_or_least(s1[i], seen1, at);
       }
     }
     float top = s0[0];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) top = fmaxf(fmaxf(top, s0[i]), s1[i]);
+    for (int i = 0; i < 16; ++i) top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, s0[i]), s1[i]);
     top = max_xor32(top) * c;
     if (__any(top > m + kSlack)) {
       const float m1 = fmaxf(m, top), f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m1);
