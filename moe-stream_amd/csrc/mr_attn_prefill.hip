@@ -497,13 +497,25 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
   return true;
 }
 
+// Waves of a SIMD, and so workgroups of a CU.
+template <int D>
+constexpr int kLayers = D == 256 ? 1 : D == 128 ? 2 : 4;
+
 template <int D, bool BF>
-__global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 4) void k_attn_prefill(PrefillArgs a) {
+__global__ __launch_bounds__(256, kLayers<D>) void k_attn_prefill(PrefillArgs a) {
   __shared__ __attribute__((aligned(1024))) uint16_t lds[4 * kKeys * D];  // rows at multiples of their length
   // Workgroups go to the 8 XCDs in turn. Each XCD gets an eighth of the head sets, so that the query heads that share
   // keys find them in one L2; sets that are not a multiple of 8 are spread over all.
   const int sets = (int)a.q.n >> a.share, units = a.n_tiles * sets;
-  const int unit = sets % 8 ? (int)blockIdx.x : (blockIdx.x & 7) * (units / 8) + (blockIdx.x >> 3);
+  // An XCD's 32 CUs hold so many workgroups each at once, the first 32 one each, and so on: every second of these layers goes
+  // the other way round, so that a CU's tiles are long and short ones (2048 tokens, 32 heads of 128: 50.7 us without,
+  // 46.2 so; 4096, 12 heads: 83.4 and 75.7; 64 heads of 64: 158.5 and 153.8; three prompts behind 2000 tokens, heads
+  // of 128: 185 and 188).
+  const int per = (units + 7) / 8, xcd = blockIdx.x & 7;
+  int at = blockIdx.x >> 3;
+  const int layer = at / 32;
+  if (layer < kLayers<D> && (layer & 1)) at = 32 * layer + min(32, per - 32 * layer) - 1 - at % 32;
+  const int unit = sets % 8 ? at * 8 + xcd : xcd * per + at;
   if (unit >= units) return;
   for (bool careful = false; !attend_tile<D, BF>(a, lds, unit, careful); careful = true) {
   }
