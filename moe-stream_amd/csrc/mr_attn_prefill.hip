@@ -11,9 +11,9 @@
 //
 // Matrix instructions and the exponentials' vector instructions bound it in about equal parts (a step of 32 rows and 64
 // keys of 128: 1024 cycles of the one, 900 of the other), under the card's power limit: fewer cycles, as with the
-// pipelined form below, came at a lower clock. 8192 tokens, the card warm: heads of 128 (32 on 4) 520 us, 1057
-// TFLOP/s; of 64 (64 on 8) 573 us, 959; of 256 (16 on 2) 584 us, 941; the library's products reach 1430 to 1490. With a window of 128, 64 heads
-// of 64, 58 us: 151 MB at 2.6 TB/s, the exponentials of steps that rows see in part; short prompts are latency, 6 us
+// pipelined form below, came at a lower clock. 8192 tokens, the card warm: heads of 128 (32 on 4) 507 us, 1084
+// TFLOP/s; of 64 (64 on 8) 569 us, 966; of 256 (16 on 2) 546 us, 1007; the library's products reach 1430 to 1490. With a window of 128, 64 heads
+// of 64, 56 us: 151 MB at 2.7 TB/s, the exponentials of steps that rows see in part; short prompts are latency, 6 us
 // for 61 tokens.
 #include <numeric>
 
