@@ -11,7 +11,7 @@
 //
 // Matrix instructions and the exponentials' vector instructions bound it in about equal parts (a step of 32 rows and 64
 // keys of 128: 1024 cycles of the one, 900 of the other), under the card's power limit: fewer cycles, as with the
-// pipelined form below, came at a lower clock. 8192 tokens, the card warm: heads of 128 (32 on 4) 507 us, 1084
+// pipelined form below, came at a lower clock. 8192 tokens, the card warm: heads of 128 (32 on 4) 505 us, 1089
 // TFLOP/s; of 64 (64 on 8) 569 us, 966; of 256 (16 on 2) 546 us, 1007; the library's products reach 1430 to 1490. With a window of 128, 64 heads
 // of 64, 56 us: 151 MB at 2.7 TB/s, the exponentials of steps that rows see in part; short prompts are latency, 6 us
 // for 61 tokens.
@@ -312,17 +312,24 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
         uint32_t kb = k_at + b * 4 * kTile, vb = v_at + b * 4 * kTile;
         asm("" : "+v"(kb), "+v"(vb));  // the parts' addresses are worked out from here, not kept
         f32x16 s0 = {}, s1 = {};
-        u32x4 pf[4], kf[2][2], vf[3];
-        kf[0][0] = key_part(kb, 0, 0), kf[0][1] = key_part(kb, 1, 0);
+        // Key operands are read so many pairs of products ahead: for heads of 128 one 512 us, two 505; for heads of 64 the second
+        // pair has no registers left.
+        constexpr int kAhead = D == 128 ? 2 : 1;
+        u32x4 pf[4], kf[kAhead + 1][2], vf[3];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) kf[i][0] = key_part(kb, 0, i), kf[i][1] = key_part(kb, 1, i);
         // Waves between their matrix instructions give way to those at them: the two of a SIMD then take turns
         // (8192 tokens, heads of 128: 675 -> 649 us, before the later steps).
         __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-          if (i + 1 < NI) kf[(i + 1) & 1][0] = key_part(kb, 0, i + 1), kf[(i + 1) & 1][1] = key_part(kb, 1, i + 1);
+          if (i + kAhead < NI) {
+            kf[(i + kAhead) % (kAhead + 1)][0] = key_part(kb, 0, i + kAhead);
+            kf[(i + kAhead) % (kAhead + 1)][1] = key_part(kb, 1, i + kAhead);
+          }
           if (i >= NI - 2) vf[i - (NI - 2)] = value_part(vb, i - (NI - 2));
-          s0 = mfma32<BF>(kf[i & 1][0], qf[i], s0);
-          s1 = mfma32<BF>(kf[i & 1][1], qf[i], s1);
+          s0 = mfma32<BF>(kf[i % (kAhead + 1)][0], qf[i], s0);
+          s1 = mfma32<BF>(kf[i % (kAhead + 1)][1], qf[i], s1);
           __builtin_amdgcn_sched_barrier(0);
         }
         __builtin_amdgcn_s_setprio(0);
