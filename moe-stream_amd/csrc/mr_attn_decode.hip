@@ -32,6 +32,7 @@ struct DecodeArgs {
 };
 
 constexpr int kWaves = 4;
+constexpr float kLargest = 0x1.fffffep127f;
 constexpr uint32_t kPartUnits = 1024;  // most parts, times key heads and head tiles
 constexpr uint32_t kMinPart = kWaves;  // chunks of a part at least: one for each wave
 // Sequences that cannot have more chunks stay whole, which spares the second launch. One sequence of 1200 tokens whole
@@ -277,10 +278,12 @@ __global__ __launch_bounds__(64 * kWaves, (Tuning<FMT, D>::kPerSimd)) void k_att
       for (int j = 0; j < 8; ++j) y[j] = ldexpf(x[2 * i + (j >> 2)][j & 3], -e) * sign;
       qf[i] = u32x4{pack_f16(y[0], y[1]), pack_f16(y[2], y[3]), pack_f16(y[4], y[5]), pack_f16(y[6], y[7])};
     }
-    // above zero: a masked score times c stays -inf
-    c = fmaxf(ldexpf(fabsf(a.o.scale) * 1.44269504088896340736f, e), 0x1p-126f);
+    // above zero and finite: a masked score times c stays -inf, a score of zero zero
+    c = fminf(fmaxf(ldexpf(fabsf(a.o.scale) * 1.44269504088896340736f, e), 0x1p-126f), kLargest);
   }
 
+  // m: the largest score so far. A weight is 2^((s - m) c), the difference first: s c - m c would be off by the
+  // rounding of m c, which for scores of 2^28 and more is more than the range of the weights' 16 bits.
   f32x4 acc[NT] = {};
   float m = -INFINITY, l = 0.f;
   const int begin = sp.c0 + (int)(pt.part * pt.size), end = sp.c0 + (int)min((uint32_t)sp.chunks, (pt.part + 1) * pt.size);
@@ -330,10 +333,10 @@ __global__ __launch_bounds__(64 * kWaves, (Tuning<FMT, D>::kPerSimd)) void k_att
     float top = s[0][0];
 #pragma unroll
     for (int t = 0; t < 16; ++t) top = fmaxf(top, s[t >> 2][t & 3]);
-    top = max_xor16(max_xor32(top)) * c;
+    top = max_xor16(max_xor32(top));
     const float m1 = fmaxf(m, top);
     if (__any(m1 > m)) {
-      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m1);
+      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - m1) * c);
       l *= f;
 #pragma unroll
       for (int t = 0; t < NT; ++t) acc[t] *= f;
@@ -345,7 +348,7 @@ __global__ __launch_bounds__(64 * kWaves, (Tuning<FMT, D>::kPerSimd)) void k_att
     for (int t = 0; t < 4; ++t) {
       float p[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) p[j] = __builtin_amdgcn_exp2f(fmaf(s[t][j], c, -base));
+      for (int j = 0; j < 4; ++j) p[j] = __builtin_amdgcn_exp2f((s[t][j] - base) * c);
       const uint32_t w0 = pack_f16(p[0], p[1]), w1 = pack_f16(p[2], p[3]);
       pf[t >> 1][2 * (t & 1)] = w0, pf[t >> 1][2 * (t & 1) + 1] = w1;
       l = add_f16(w1, add_f16(w0, l));
@@ -373,8 +376,8 @@ __global__ __launch_bounds__(64 * kWaves, (Tuning<FMT, D>::kPerSimd)) void k_att
     __syncthreads();
     if (wave < w) {
       const float m2 = stats[wave][n][0], l2 = stats[wave][n][1], m1 = fmaxf(m, m2);
-      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m1);
-      const float f2 = m2 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m2 - m1);
+      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - m1) * c);
+      const float f2 = m2 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m2 - m1) * c);
 #pragma unroll
       for (int t = 0; t < NT; ++t)
         acc[t] = acc[t] * f + *reinterpret_cast<const f32x4*>(&sums[wave][n * D + 16 * t + 4 * g]) * f2;
@@ -383,6 +386,8 @@ __global__ __launch_bounds__(64 * kWaves, (Tuning<FMT, D>::kPerSimd)) void k_att
     __syncthreads();
   }
   if (wave > 0 || (uint32_t)n >= heads) return;
+  // What the weights are relative to, for sinks and other parts; its rounding is one of the score.
+  if (m > -INFINITY) m = fminf(fmaxf(m * c, -kLargest), kLargest);
   if (pt.parts > 1) {
     const uint64_t unit = ((uint64_t)(pt.slot + pt.part) * gridDim.y + blockIdx.y) * 16 + n;
     float* dst = a.part + unit * D;

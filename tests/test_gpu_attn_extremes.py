@@ -1,0 +1,114 @@
+"""The attention-side operators on the GPU where sums run out of bits: scores of any finite size, weights far below
+the largest, sinks at the ends of their range; parts of a split sequence with sinks and with missing pages; and which
+keys each row of a long sequence sees, counted."""
+import numpy as np
+import pytest
+
+import moe_rocm as M
+
+import attnref as R
+from test_gpu_attn import FORMATS, TYPES
+
+pytestmark = pytest.mark.gpu
+
+
+def decode(ctx, kv, q, dtype, lens, table, **kw):
+    """One call over the cache `kv`: q [n_seqs, heads, D]."""
+    H, D = q.shape[1:]
+    dq, out = R.Rows(ctx, q, dtype), R.Rows(ctx, None, dtype, len(lens), H, D)
+    dl, dt = R.i32(ctx, lens), R.i32(ctx, table)
+    sinks = kw.pop("sinks", None)
+    ds = None if sinks is None else ctx.to_device(np.asarray(sinks, np.float32))
+    kv.attend(dq.heads, len(lens), dl, dt, table.shape[1], out.heads, sinks=ds, **kw)
+    try:
+        ctx.sync()
+        return out.get()
+    finally:
+        for b in (dq, out, dl, dt, ds):
+            if b is not None:
+                b.free()
+
+
+def filled(ctx, fmt, seqs, page=64):
+    """A cache with the sequences (k, v) [n, heads, D] on pages one after the other -> (cache, table)."""
+    H, D = seqs[0][0].shape[1:]
+    counts = [max(1, -(-len(k) // page)) for k, _ in seqs]
+    kv = M.KvCache(ctx, fmt, sum(counts), page, H, D)
+    table = np.zeros((len(seqs), max(counts)), np.int32)
+    at = 0
+    for i, ((k, v), c) in enumerate(zip(seqs, counts)):
+        table[i, :c] = at + np.arange(c)
+        if len(k):
+            dk, dv = R.Rows(ctx, k, M.F32), R.Rows(ctx, v, M.F32)
+            ds = R.i32(ctx, at * page + np.arange(len(k)))
+            kv.write(dk.heads, dv.heads, len(k), ds)
+            ctx.sync()
+            dk.free(), dv.free(), ds.free()
+        at += c
+    return kv, table
+
+
+# ---- scores of any finite size ---------------------------------------------------------------------
+def check_one_of(got, q, k, v, scale, dtype):
+    """A row whose scores are so large that 32 bits hold them to whole powers of e or worse. On one key it is the key's
+    value. With the largest score clear of the others by more than the scores' own error (D products summed in 32 bits
+    and three more roundings: (D + 4) 2^-24 of the sum of magnitudes, at either key) and 40 (e^-40 for each of 700 others at
+    most: nothing, in 16 bits of output), it is that key's value too. Else weights are whatever the error makes them,
+    but they are weights: the row lies between the least and the largest value, give or take the output's rounding and the
+    weights' (each off by half a step of 16 bits of weight, in sum and divisor)."""
+    q, k = q.astype(np.float64), k.astype(np.float64)
+    s = k @ q * scale
+    err = (len(q) + 4) * 2.0 ** -24 * (np.abs(k) @ np.abs(q)) * abs(scale)
+    top = int(s.argmax())
+    clear = all(s[top] - s[j] > err[top] + err[j] + 40 for j in range(len(s)) if j != top)
+    if clear:
+        assert (got == R.rounded(v[top], dtype)).all(), (len(s), got[:4], v[top][:4])
+    else:
+        room = (2 * R.HALF[dtype] + 2.0 ** -10) * np.abs(v).max()
+        assert (got >= v.min(0) - room).all() and (got <= v.max(0) + room).all(), (len(s), got[:4])
+    return clear
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("dtype,q_size,k_size,scale", [("f16", 8000, 8000, 0.0), ("f16", 60000, 60000, 0.0), ("bf16", 20000, 3e4, -0.3),
+                                                       ("bf16", 1e6, 100.0, 1.0), ("f16", 500, 500, 1e6), ("bf16", 1e30, 6e4, 1e-24),
+                                                       ("f16", 6e4, 6e4, 1e25)])
+def test_decode_scores_beyond_the_bits_of_the_base(gpu_ctx, fmt, D, dtype, q_size, k_size, scale):
+    dtype, fmt = TYPES[dtype], FORMATS[fmt]
+    rng = np.random.default_rng(D)
+    lens, hk, group = [1] * 12 + [2, 3, 5, 70, 700], 2, 3
+    seqs = [((rng.uniform(-1, 1, (n, hk, D)) * k_size).astype(np.float32), rng.normal(size=(n, hk, D)).astype(np.float32)) for n in lens]
+    kv, table = filled(gpu_ctx, fmt, seqs)
+    q = R.rounded(rng.uniform(-1, 1, (len(lens), hk * group, D)) * q_size, dtype)
+    got = decode(gpu_ctx, kv, q, dtype, lens, table, scale=scale)
+    n_clear = 0
+    for i, (k, v) in enumerate(seqs):
+        k, v = R.stored(k, fmt), R.stored(v, fmt)
+        for h in range(hk * group):
+            n_clear += check_one_of(got[i, h], q[i, h], k[:, h // group], v[:, h // group], scale or D ** -0.5, dtype)
+    assert n_clear >= 12 * hk * group
+    kv.close()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("D", [64, 256])
+def test_decode_of_a_split_sequence_with_large_scores(gpu_ctx, fmt, D):
+    """The parts' bases differ by less than their own last bits: the key that takes all weight lies in any part."""
+    fmt = FORMATS[fmt]
+    rng = np.random.default_rng(D)
+    n = 9000
+    k, v = (rng.uniform(-1, 1, (n, 1, D)) * 2.0).astype(np.float32), rng.normal(size=(n, 1, D)).astype(np.float32)
+    at = np.array([0, 4000, 8999, 77])
+    q = np.zeros((1, 4, D), np.float32)
+    for h, a in enumerate(at):  # a key that lies along the query, larger than all others
+        k[a, 0] = np.sign(rng.normal(size=D)) * 64
+        q[0, h] = np.sign(k[a, 0]) * 16384
+    kv, table = filled(gpu_ctx, fmt, [(k, v)], page=256)
+    ks, vs = R.stored(k, fmt), R.stored(v, fmt)
+    for scale in (1.0, 1e4):
+        got = decode(gpu_ctx, kv, q, M.F16, [n], table, scale=scale)
+        for h in range(4):
+            assert check_one_of(got[0, h], q[0, h], ks[:, 0], vs[:, 0], scale, M.F16)
+            assert int((ks[:, 0] @ q[0, h]).argmax()) == at[h]
+    kv.close()
