@@ -112,3 +112,50 @@ def test_decode_of_a_split_sequence_with_large_scores(gpu_ctx, fmt, D):
             assert check_one_of(got[0, h], q[0, h], ks[:, 0], vs[:, 0], scale, M.F16)
             assert int((ks[:, 0] @ q[0, h]).argmax()) == at[h]
     kv.close()
+
+
+# ---- weights far below the largest -----------------------------------------------------------------
+def fine_bound(y, size_v, size_s, n, D, out_type, p_half, least):
+    """How far a result may be off. The output's own rounding (and half of the smallest step of f16). Each weight is off
+    by p_half of itself or by `least` of the largest weight, in the sum of values and in the divisor; its score, D products
+    summed in 32 bits and four more roundings, by `ds`, each an error of p relative to p; the sums' own by n roundings."""
+    ds = (D + 6) * 2.0 ** -24 * size_s + 8 * 2.0 ** -24
+    return (R.HALF[out_type] * np.abs(y) + (p_half + 2 * ds + n * 2.0 ** -24) * (size_v + np.abs(y))
+            + least * n * (np.abs(y) + 1.0) * 4 + 2.0 ** -25)
+
+
+def tail(rng, n, H, D, lead, scale_q):
+    """n keys with scores of about 0 (spread 0.3) against q = scale_q * ones, and values about 1 (spread 0.3); with
+    `lead`, the first one's score is that and its value zero."""
+    k = (rng.normal(size=(n, H, D)) * 0.3 / scale_q).astype(np.float32)  # scores sum over D, times D^-1/2
+    v = (1 + 0.3 * rng.normal(size=(n, H, D))).astype(np.float32)
+    if lead is not None:
+        k[0], v[0] = lead * D ** -0.5 / scale_q, 0.0
+    return k, v
+
+
+def far_below(q, k, v, scale, sink):
+    """The row by 64 bits -> (row, sum p |v|, largest sum of magnitudes of a score's terms, keys)."""
+    return R.attend(q, k, v, scale, 0, len(k) - 1, sink)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("n,lead,sink", [(24000, 16.0, None), (24000, 18.0, None), (1000, 18.0, None), (24000, None, 18.0), (1000, 15.0, 17.0)])
+def test_decode_of_a_long_tail_far_below_the_largest(gpu_ctx, fmt, D, dtype, n, lead, sink):
+    """One key (a first token, say) or a sink takes nearly all weight and has no value: the rest is the result."""
+    dtype, fmt = TYPES[dtype], FORMATS[fmt]
+    rng = np.random.default_rng(D)
+    k, v = tail(rng, n, 1, D, lead, 1.0)
+    kv, table = filled(gpu_ctx, fmt, [(k, v)], page=256)
+    k, v = R.stored(k, fmt)[:, 0], R.stored(v, fmt)[:, 0]
+    q = np.ones((1, 2, D), np.float32)
+    got = decode(gpu_ctx, kv, q, dtype, [n], table, sinks=None if sink is None else [sink, sink])
+    for h in range(2):
+        y, av, ss, cnt = far_below(q[0, h], k, v, D ** -0.5, sink)
+        # weights in f16, the largest of them 2^14: half of the smallest step is 2^-39 of it
+        tol = fine_bound(y, av, ss, cnt, D, dtype, 2.0 ** -11, 2.0 ** -39)
+        assert (np.abs(got[0, h] - y) <= tol).all(), float((np.abs(got[0, h] - y) / tol).max())
+        assert (tol <= 0.05 * np.abs(y) + 2.0 ** -25).all()  # the bound sees a lost tail
+    kv.close()
