@@ -230,10 +230,8 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
 #pragma unroll
   for (int t = 0; t < ND; ++t) acc[t] = f32x16{};
   float m = -INFINITY, l = 0.f;
-  if (a.o.sinks) {
-    m = a.o.sinks[h] * 1.44269504088896340736f;
-    l = half == 0 && m != -INFINITY ? 1.f : 0.f;  // the two halves of a row are added at the end
-  }
+  // A sink joins at the end: as the first maximum, one far above the scores left their weights no bits in f16.
+  const float sink = a.o.sinks ? a.o.sinks[h] * 1.44269504088896340736f : -INFINITY;
 
   constexpr int NI = D / 16, NV = 4 * ND;
   // Operand of the scores: 8 elements of key 32 t + n; of the values: V^T of 16 keys and 32 elements, where lane
@@ -469,7 +467,13 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
   }
 
   l = add_xor32(l);
-  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : NAN;
+  float own = 1.f;
+  if (sink != -INFINITY) {
+    const float m1 = fmaxf(m, sink);
+    own = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m1);
+    l = l * own + __builtin_amdgcn_exp2f(sink - m1);  // NaN for a sink that is infinite or NaN
+  }
+  const float inv = l > 0.f ? own / l : l == 0.f ? 0.f : NAN;
   int tid = threadIdx.x;
   asm volatile("" : "+v"(tid));  // the row's address is worked out here, not kept through the steps
   const int out_row = pl.row + wave_row + (tid & 31);

@@ -29,6 +29,22 @@ def decode(ctx, kv, q, dtype, lens, table, **kw):
                 b.free()
 
 
+def prompt(ctx, q, k, v, dtype, cu_q, cu_k, **kw):
+    D = q.shape[2]
+    dq, dk, dv = (R.Rows(ctx, x, dtype) for x in (q, k, v))
+    out = R.Rows(ctx, None, dtype, *q.shape)
+    dcq, dck = R.i32(ctx, cu_q), R.i32(ctx, cu_k)
+    sinks = kw.pop("sinks", None)
+    ds = None if sinks is None else ctx.to_device(np.asarray(sinks, np.float32))
+    M.attn_prefill(ctx, D, dq.heads, dk.heads, dv.heads, len(q), len(k), len(cu_q) - 1, dcq, dck, out.heads, sinks=ds, **kw)
+    ctx.sync()
+    y = out.get()
+    for b in (dq, dk, dv, out, dcq, dck, ds):
+        if b is not None:
+            b.free()
+    return y
+
+
 def filled(ctx, fmt, seqs, page=64):
     """A cache with the sequences (k, v) [n, heads, D] on pages one after the other -> (cache, table)."""
     H, D = seqs[0][0].shape[1:]
@@ -158,4 +174,41 @@ def test_decode_of_a_long_tail_far_below_the_largest(gpu_ctx, fmt, D, dtype, n, 
         tol = fine_bound(y, av, ss, cnt, D, dtype, 2.0 ** -11, 2.0 ** -39)
         assert (np.abs(got[0, h] - y) <= tol).all(), float((np.abs(got[0, h] - y) / tol).max())
         assert (tol <= 0.05 * np.abs(y) + 2.0 ** -25).all()  # the bound sees a lost tail
+    kv.close()
+
+
+# ---- sinks ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_sinks_at_the_ends_of_their_range(gpu_ctx, D):
+    """-inf is no sink, 3e38 or any that is far above the scores leaves nothing, inf and NaN have no result: the same
+    over the cache, whole and split, and over a prompt."""
+    rng = np.random.default_rng(D)
+    sinks = np.array([-np.inf, np.inf, np.nan, 200.0, -1e30, 1e38], np.float32)
+    H = len(sinks)
+    for n in (3, 90, 5000):
+        k, v = rng.normal(size=(n, 1, D)).astype(np.float32), rng.normal(size=(n, 1, D)).astype(np.float32)
+        q = R.rounded(rng.normal(size=(1, H, D)), M.F16)
+        kv, table = filled(gpu_ctx, M.KV_F16, [(k, v)])
+        k, v = R.stored(k, M.KV_F16), R.stored(v, M.KV_F16)
+        got = [decode(gpu_ctx, kv, q, M.F16, [n], table, sinks=sinks)[0], prompt(gpu_ctx, q, k, v, M.F16, [0, 1], [0, n], sinks=sinks)[0],
+               prompt(gpu_ctx, q, k, v, M.BF16, [0, 1], [0, n], sinks=sinks)[0]]
+        for g, dtype in zip(got, (M.F16, M.F16, M.BF16)):
+            assert np.isnan(g[1:3]).all() and (g[[3, 5]] == 0).all(), (n, g[1:, :2])
+            for h in (0, 4):
+                x, kk, vv = (R.rounded(a, dtype) for a in (q[0, h], k[:, 0], v[:, 0]))
+                y, av, ss, cnt = R.attend(x, kk, vv, D ** -0.5, 0, n - 1)
+                assert (np.abs(g[h] - y) <= R.attention_bound(y, av, ss, cnt, D, dtype, R.HALF[dtype])).all()
+        kv.close()
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_sinks_of_rows_that_see_nothing(gpu_ctx, D):
+    """With no key a sink that has a weight takes it all: zeros; one that is not a number or infinite has no result."""
+    sinks = [0.5, -np.inf, np.inf, np.nan]
+    q, k = np.ones((3, 4, D), np.float32), np.ones((1, 1, D), np.float32)
+    got = prompt(gpu_ctx, q, k, k, M.F16, [0, 3], [0, 1], sinks=sinks)
+    assert (got[:2, :2] == 0).all() and np.isnan(got[:2, 2:]).all()
+    kv, table = filled(gpu_ctx, M.KV_F16, [(k, k)])
+    got = decode(gpu_ctx, kv, q[:1], M.F16, [0], table, sinks=sinks)
+    assert (got[0, :2] == 0).all() and np.isnan(got[0, 2:]).all()
     kv.close()
