@@ -1,7 +1,7 @@
 // mr_attn_prefill.hip -- causal attention over packed prompts.
 //
 // One pass over the keys with the running maximum m and sum l of each row's softmax:
-//   S = K Q^T (keys down, rows across), p = 2^(S c - m), O = 2^(m_old - m) O + V^T p,  c = scale log2 e.
+//   S = K Q^T (keys down, rows across), p = 2^((S - m) c), O = 2^((m_old - m) c) O + V^T p,  c = scale log2 e.
 // Both products are 32x32x16 matrix instructions. With the keys down, a lane holds the scores of one
 // row, 16 of each 32 keys, so that maximum, sum and p need one exchange between two lanes; and p is
 // already where the second product wants its right operand, if that product counts its keys in the
@@ -31,6 +31,8 @@ constexpr int kKeys = 64;   // keys of a step
 // of a search among more, which takes their log2.
 constexpr int kScan = 512;
 constexpr float kSlack = 8.f;
+constexpr float kFar = 0x1p22f;  // a base's last bit is half a power of two from here on, its rounding a quarter
+constexpr float kLargest = 0x1.fffffep127f;
 
 template <bool BF>
 __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
@@ -154,6 +156,10 @@ __device__ __forceinline__ bool find_tile(const PrefillArgs& a, int tile, bool r
 // One tile of rows and one head. p is 0 where a row does not see a key, but 0 * inf and 0 * NaN are NaN: a tile
 // that ends with such a sum returns false and is done over with `careful`, where values that are not finite
 // are taken out of the steps that some row sees in part, and added at the end to the rows that see them.
+//
+// p is 2^((S - m) c). For heads of 64 and 128 it is worked out as 2^(S c - base), base = m c, an instruction less: the
+// base's rounding is then the same factor on all of a row's weights. Where a base is so large (kFar) that this factor could
+// leave the range of 16 bits, the tile is done over `careful` too, with the differences taken first.
 template <int D, bool BF>
 __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds, int unit, bool careful) {
   constexpr int P = D / 8, ND = D / 32;  // 16-byte pieces of a row; 32-wide tiles of a head
@@ -182,7 +188,8 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
   const int wave_least = (int)max((int64_t)pl.k0, (int64_t)pl.row + wave_row + diff + 1 - w);  // first key of its first row
   const int wave_first = (int)max((int64_t)pl.k0, (int64_t)pl.row + wave_row + 31 + diff + 1 - w);  // of its last row
 
-  const float c = fmaxf(fabsf(a.o.scale) * 1.44269504088896340736f, 0x1p-126f);  // above zero: a masked score stays -inf
+  // above zero and finite: a masked score times c stays -inf, a score of zero zero
+  const float c = fminf(fmaxf(fabsf(a.o.scale) * 1.44269504088896340736f, 0x1p-126f), kLargest);
   u32x4 qf[D / 16];
   {
     const uint16_t* qp = static_cast<const uint16_t*>(a.q.p) + (uint64_t)min(row, pl.q1 - 1) * a.q.ts + (uint64_t)h * a.q.hs;
@@ -229,7 +236,11 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
   f32x16 acc[ND];
 #pragma unroll
   for (int t = 0; t < ND; ++t) acc[t] = f32x16{};
+  constexpr bool kDiff = D == 256;  // the differences always: they run beside the matrix instructions
   float m = -INFINITY, l = 0.f;
+  const float c_base = careful ? 0.f : c;
+  // finite where no key has been seen (-inf, or 0 * -inf): a masked score stays -inf
+  auto base_of = [&] { return fmaxf(kDiff ? m : m * c_base, -kLargest); };
   // A sink joins at the end: as the first maximum, one far above the scores left their weights no bits in f16.
   const float sink = a.o.sinks ? a.o.sinks[h] * 1.44269504088896340736f : -INFINITY;
 
@@ -270,20 +281,26 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
     float top = s0[0];
 #pragma unroll
     for (int i = 0; i < 16; ++i) top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, s0[i]), s1[i]);
-    top = max_xor32(top) * c;
-    if (__any(top > m + kSlack)) {
-      const float m1 = fmaxf(m, top), f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m1);
+    top = max_xor32(top);
+    if (__any((top - m) * c > kSlack)) {
+      const float m1 = fmaxf(m, top), f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - m1) * c);
       l *= f;
 #pragma unroll
       for (int t = 0; t < ND; ++t) acc[t] *= f;
       m = m1;
     }
+    if (!kDiff && careful) {
+      const float first = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s0[i] -= first, s1[i] -= first;
+    }
   };
   // Two of a step's 32 weights (pair i): rounded into the operand of the second product.
   auto weigh = [&](const f32x16& s0, const f32x16& s1, int i, float base, u32x4 (&pf)[4]) {
     const f32x16& s = i < 8 ? s0 : s1;
-    const float p0 = __builtin_amdgcn_exp2f(fmaf(s[2 * (i & 7)], c, -base));
-    const float p1 = __builtin_amdgcn_exp2f(fmaf(s[2 * (i & 7) + 1], c, -base));
+    const float x0 = s[2 * (i & 7)], x1 = s[2 * (i & 7) + 1];
+    const float p0 = __builtin_amdgcn_exp2f(kDiff ? (x0 - base) * c : fmaf(x0, c, -base));
+    const float p1 = __builtin_amdgcn_exp2f(kDiff ? (x1 - base) * c : fmaf(x1, c, -base));
     const uint32_t w = pack16<BF>(p0, p1);
     pf[i >> 2][i & 3] = w;
     l = BF ? add_bf16(w, l) : add_f16(w, l);
@@ -332,7 +349,7 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
         }
         __builtin_amdgcn_s_setprio(0);
         settle(k0, s0, s1);
-        const float base = m == -INFINITY ? 0.f : m;
+        const float base = base_of();
 #pragma unroll
         for (int x = 0; x < 4; ++x) weigh(s0, s1, x, base, pf);
         __builtin_amdgcn_s_setprio(1);
@@ -359,7 +376,7 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
     // taken, to p.
     constexpr int kAhead = 3;  // products between an operand's read and its use: 2 618 us, 3 604, 4 and 5 no better
     auto step = [&](int k0, int b, f32x16& p, f32x16& q, f32x16& x) {
-      const float base = m == -INFINITY ? 0.f : m;
+      const float base = base_of();
       u32x4 pf[4], kf[kAhead + 1], vf[kAhead + 1];
       uint32_t kb = k_at + (b ^ 1) * 4 * kTile, vb = v_at + b * 4 * kTile;
       asm("" : "+v"(kb), "+v"(vb));  // the parts' addresses are worked out from here, not kept
@@ -440,7 +457,7 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
         step(k0, b, s1, s2, s0);
         k0 += kKeys, b ^= 1;
       }
-      const float base = m == -INFINITY ? 0.f : m;
+      const float base = base_of();
       u32x4 pf[4];
       uint32_t vb = v_at + b * 4 * kTile;
       asm("" : "+v"(vb));
@@ -463,14 +480,15 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
     for (int t = 0; t < ND; ++t)
 #pragma unroll
       for (int i = 0; i < 16; ++i) most = __builtin_elementwise_maximum(most, fabsf(acc[t][i]));
-    if (__syncthreads_or(!(most < INFINITY))) return false;
+    const bool far = !kDiff && m != -INFINITY && !(fabsf(m) * c < kFar);
+    if (__syncthreads_or(far || !(most < INFINITY))) return false;
   }
 
   l = add_xor32(l);
   float own = 1.f;
   if (sink != -INFINITY) {
-    const float m1 = fmaxf(m, sink);
-    own = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m1);
+    const float top = m == -INFINITY ? m : fminf(fmaxf(m * c, -kLargest), kLargest), m1 = fmaxf(top, sink);
+    own = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - m1);
     l = l * own + __builtin_amdgcn_exp2f(sink - m1);  // NaN for a sink that is infinite or NaN
   }
   const float inv = l > 0.f ? own / l : l == 0.f ? 0.f : NAN;

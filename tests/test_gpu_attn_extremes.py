@@ -130,6 +130,30 @@ def test_decode_of_a_split_sequence_with_large_scores(gpu_ctx, fmt, D):
     kv.close()
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("dtype,q_size,k_size,scale", [("f16", 8000, 8000, 0.0), ("f16", 60000, 60000, 0.0), ("bf16", 1e4, 1e5, -0.3),
+                                                       ("bf16", 1e9, 1e7, 0.0), ("f16", 500, 500, 1e6), ("bf16", 1e25, 1e6, 1e-20),
+                                                       ("f16", 6e4, 6e4, 1e25)])
+@pytest.mark.parametrize("window", [0, 1, 30])
+def test_prefill_scores_beyond_the_bits_of_the_base(gpu_ctx, D, dtype, q_size, k_size, scale, window):
+    dtype = TYPES[dtype]
+    rng = np.random.default_rng(D + window)
+    lens, hk, group = [1, 1, 1, 2, 3, 40, 150], 1, 2
+    cu = np.concatenate([[0], np.cumsum(lens)])
+    q = R.rounded(rng.uniform(-1, 1, (cu[-1], hk * group, D)) * q_size, dtype)
+    k = R.rounded(rng.uniform(-1, 1, (cu[-1], hk, D)) * k_size, dtype)
+    v = R.rounded(rng.normal(size=(cu[-1], hk, D)), dtype)
+    got = prompt(gpu_ctx, q, k, v, dtype, cu, cu, scale=scale, window=window)
+    n_clear = 0
+    for a, b in zip(cu[:-1], cu[1:]):
+        for r in range(a, b):
+            first = max(a, r - window + 1) if window else a
+            for h in range(hk * group):
+                n_clear += check_one_of(got[r, h], q[r, h], k[first:r + 1, h // group], v[first:r + 1, h // group],
+                                        scale or D ** -0.5, dtype)
+    assert n_clear >= len(lens) * hk * group
+
+
 # ---- weights far below the largest -----------------------------------------------------------------
 def fine_bound(y, size_v, size_s, n, D, out_type, p_half, least):
     """How far a result may be off. The output's own rounding (and half of the smallest step of f16). Each weight is off
