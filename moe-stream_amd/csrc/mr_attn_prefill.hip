@@ -31,6 +31,11 @@ constexpr int kKeys = 64;   // keys of a step
 // of a search among more, which takes their log2.
 constexpr int kScan = 512;
 constexpr float kSlack = 8.f;
+// f16 weights are 2^kLift times as large: up to 2^15 with kSlack. Ones down to 2^-21 of the largest keep all of
+// f16's bits, and what is lost of smaller ones is 2^-32 of it at most; not lifted, 20,000 keys 18 below a first one that has no
+// value were lost. bf16 has the range of 32 bits.
+template <bool BF>
+constexpr float kLift = BF ? 0.f : 7.f;
 constexpr float kFar = 0x1p22f;  // a base's last bit is half a power of two from here on, its rounding a quarter
 constexpr float kLargest = 0x1.fffffep127f;
 
@@ -157,7 +162,7 @@ __device__ __forceinline__ bool find_tile(const PrefillArgs& a, int tile, bool r
 // that ends with such a sum returns false and is done over with `careful`, where values that are not finite
 // are taken out of the steps that some row sees in part, and added at the end to the rows that see them.
 //
-// p is 2^((S - m) c). For heads of 64 and 128 it is worked out as 2^(S c - base), base = m c, an instruction less: the
+// p is 2^((S - m) c + kLift). For heads of 64 and 128 it is worked out as 2^(S c - base), base = m c - kLift, an instruction less: the
 // base's rounding is then the same factor on all of a row's weights. Where a base is so large (kFar) that this factor could
 // leave the range of 16 bits, the tile is done over `careful` too, with the differences taken first.
 template <int D, bool BF>
@@ -240,7 +245,7 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
   float m = -INFINITY, l = 0.f;
   const float c_base = careful ? 0.f : c;
   // finite where no key has been seen (-inf, or 0 * -inf): a masked score stays -inf
-  auto base_of = [&] { return fmaxf(kDiff ? m : m * c_base, -kLargest); };
+  auto base_of = [&] { return fmaxf(kDiff ? m : fmaf(m, c_base, -kLift<BF>), -kLargest); };
   // A sink joins at the end: as the first maximum, one far above the scores left their weights no bits in f16.
   const float sink = a.o.sinks ? a.o.sinks[h] * 1.44269504088896340736f : -INFINITY;
 
@@ -299,8 +304,8 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
   auto weigh = [&](const f32x16& s0, const f32x16& s1, int i, float base, u32x4 (&pf)[4]) {
     const f32x16& s = i < 8 ? s0 : s1;
     const float x0 = s[2 * (i & 7)], x1 = s[2 * (i & 7) + 1];
-    const float p0 = __builtin_amdgcn_exp2f(kDiff ? (x0 - base) * c : fmaf(x0, c, -base));
-    const float p1 = __builtin_amdgcn_exp2f(kDiff ? (x1 - base) * c : fmaf(x1, c, -base));
+    const float p0 = __builtin_amdgcn_exp2f(kDiff ? fmaf(x0 - base, c, kLift<BF>) : fmaf(x0, c, -base));
+    const float p1 = __builtin_amdgcn_exp2f(kDiff ? fmaf(x1 - base, c, kLift<BF>) : fmaf(x1, c, -base));
     const uint32_t w = pack16<BF>(p0, p1);
     pf[i >> 2][i & 3] = w;
     l = BF ? add_bf16(w, l) : add_f16(w, l);
@@ -487,7 +492,7 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
   l = add_xor32(l);
   float own = 1.f;
   if (sink != -INFINITY) {
-    const float top = m == -INFINITY ? m : fminf(fmaxf(m * c, -kLargest), kLargest), m1 = fmaxf(top, sink);
+    const float top = m == -INFINITY ? m : fminf(fmaxf(m * c, -kLargest), kLargest) - kLift<BF>, m1 = fmaxf(top, sink);
     own = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - m1);
     l = l * own + __builtin_amdgcn_exp2f(sink - m1);  // NaN for a sink that is infinite or NaN
   }

@@ -201,6 +201,25 @@ def test_decode_of_a_long_tail_far_below_the_largest(gpu_ctx, fmt, D, dtype, n, 
     kv.close()
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("n,lead,sink", [(20000, 16.0, None), (20000, 18.0, None), (300, None, 16.0), (20000, None, 18.0), (20000, 12.0, 17.0)])
+def test_prefill_of_a_long_tail_far_below_the_largest(gpu_ctx, D, dtype, n, lead, sink):
+    dtype = TYPES[dtype]
+    rng = np.random.default_rng(D)
+    k, v = (R.rounded(x, dtype) for x in tail(rng, n, 1, D, lead, 1.0))
+    q = np.ones((40, 2, D), np.float32)
+    got = prompt(gpu_ctx, q, k, v, dtype, [0, 40], [0, n], sinks=None if sink is None else [sink, sink])
+    for r in (0, 1, 31, 32, 39):
+        for h in range(2):
+            seen = n - 40 + r + 1
+            y, av, ss, cnt = far_below(q[r, h], k[:seen, 0], v[:seen, 0], D ** -0.5, sink)
+            # f16: the largest weight is 2^7 or more, half of the smallest step 2^-25; bf16: the range of 32 bits
+            tol = fine_bound(y, av, ss, cnt, D, dtype, R.HALF[dtype], 2.0 ** -32 if dtype == M.F16 else 0.0)
+            assert (np.abs(got[r, h] - y) <= tol).all(), (r, float((np.abs(got[r, h] - y) / tol).max()))
+            assert (tol <= 0.15 * np.abs(y) + 2.0 ** -25).all()
+
+
 # ---- sinks ---------------------------------------------------------------------------------------
 @pytest.mark.parametrize("D", [64, 128, 256])
 def test_sinks_at_the_ends_of_their_range(gpu_ctx, D):
