@@ -498,40 +498,113 @@ class GgufFile:
         return L
 
     def _meta(self, get, key: str, default):
+        """The value of `key`, the default where the file has no such key; one of another type is an error."""
         try:
             return get(key)
-        except MoeRocmError:
+        except MoeRocmError as e:
+            if "key not found" not in e.message:
+                raise
             return default
 
-    def attention(self) -> dict:
-        """The attention shape the metadata gives: query and key heads, head width, rotated part of it, window (0: none)."""
-        a = self.meta_str("general.architecture")
-        heads = self.meta_u32(f"{a}.attention.head_count")
-        dim = self._meta(self.meta_u32, f"{a}.attention.key_length", 0) or self.meta_u32(f"{a}.embedding_length") // heads
-        return dict(n_heads=heads, n_kv_heads=self._meta(self.meta_u32, f"{a}.attention.head_count_kv", heads), head_dim=dim,
-                    rotary_dim=self._meta(self.meta_u32, f"{a}.rope.dimension_count", dim),
-                    window=self._meta(self.meta_u32, f"{a}.attention.sliding_window", 0))
+    def _per_layer(self, key: str, default: int, layer: int | None) -> int:
+        """A number for all layers, or `layer`'s of an array with one for each."""
+        try:
+            return self._meta(self.meta_u32, key, default)
+        except MoeRocmError:
+            each = self.meta_u32_array(key)
+        if layer is not None and layer >= len(each):
+            raise MoeRocmError(MR_E_INVAL, f"layer {layer}: {key} has {len(each)} entries")
+        if layer is None and len(set(each)) != 1:
+            raise MoeRocmError(MR_E_INVAL, f"{key} differs from layer to layer: a layer has to be named")
+        return each[layer or 0]
 
-    def rope(self, ctx: "Context", layout: int = 0) -> "Rope":
+    def attention(self, layer: int | None = None) -> dict:
+        """The attention shape the metadata gives: query and key heads, head width, rotated part of it, window (0: none).
+        With `layer`, that layer's, where the file has a number for each. A window that a file gives once is that of the
+        layers that have one: with `layer`, GPT-OSS's even ones have it and its odd ones do not; of other models' layers all do."""
+        if layer is not None and layer < 0:
+            raise MoeRocmError(MR_E_INVAL, f"layer {layer} is negative")
+        a = self.meta_str("general.architecture")
+        heads, dim = self._heads(a, layer), self._head_dim(a, layer)
+        if self._meta(self.meta_u32, f"{a}.attention.value_length", dim) != dim:
+            raise MoeRocmError(MR_E_UNSUPPORTED, "values of another width than keys")
+        window = self._per_layer(f"{a}.attention.sliding_window", 0, layer)
+        if layer is not None and window and not self._is_array(f"{a}.attention.sliding_window"):
+            if self._has(f"{a}.attention.sliding_window_pattern"):
+                raise MoeRocmError(MR_E_UNSUPPORTED, f"{a}.attention.sliding_window_pattern")
+            if _is_gpt_oss(a) and layer % 2:
+                window = 0
+        return dict(n_heads=heads, n_kv_heads=self._per_layer(f"{a}.attention.head_count_kv", heads, layer), head_dim=dim,
+                    rotary_dim=self._meta(self.meta_u32, f"{a}.rope.dimension_count", dim), window=window)
+
+    def _heads(self, arch: str, layer: int | None) -> int:
+        heads = self._per_layer(f"{arch}.attention.head_count", 0, layer)
+        if not heads:
+            raise MoeRocmError(MR_E_INVAL, f"{arch}.attention.head_count is missing or 0")
+        return heads
+
+    def _head_dim(self, arch: str, layer: int | None = None) -> int:
+        return (self._meta(self.meta_u32, f"{arch}.attention.key_length", 0)
+                or self.meta_u32(f"{arch}.embedding_length") // self._heads(arch, layer))
+
+    def _is_array(self, key: str) -> bool:
+        try:
+            self.meta_u32_array(key)
+        except MoeRocmError:
+            return False
+        return True
+
+    def _has(self, key: str) -> bool:
+        try:
+            self.meta_u32(key)
+        except MoeRocmError as e:
+            return "key not found" not in e.message
+        return True
+
+    def rope(self, ctx: "Context", layout: int = 0, *, attn_factor: float = 0.0) -> "Rope":
         """The model's rotary frequencies ({arch}.rope.*: freq_base, dimension_count, scaling.type linear or yarn with its
-        factor and original_context_length), for qk_norm_rope. layout: ROPE_HALF, the reference's, or ROPE_INTERLEAVED."""
-        a, shape = self.meta_str("general.architecture"), self.attention()
+        factor, original_context_length, yarn_beta_fast, yarn_beta_slow and attn_factor), for qk_norm_rope. layout: ROPE_HALF,
+        the reference's, or ROPE_INTERLEAVED. A file with other rules for the rotation is refused, and so is one with an
+        attn_factor beside YaRN, which files mean in two ways (in the place of YaRN's own, and times it), unless
+        `attn_factor` says what the factor on cosine and sine is in all."""
+        a = self.meta_str("general.architecture")
+        dim = self._head_dim(a)
         kind = self._meta(self.meta_str, f"{a}.rope.scaling.type", "none")
         if kind not in ("none", "linear", "yarn"):
             raise MoeRocmError(MR_E_UNSUPPORTED, f"rope scaling {kind!r}")
+        for key, usual in (("scale_linear", 1.0), ("dimension_sections", None), ("freq_base_swa", None),
+                           ("scaling.yarn_ext_factor", 1.0), ("scaling.yarn_log_multiplier", 0.0)):
+            key = f"{a}.rope.{key}"
+            if self._has(key) and (usual is None or self.meta_f32(key) != usual):
+                raise MoeRocmError(MR_E_UNSUPPORTED, key)
+        if "rope_freqs.weight" in self.tensor_names():
+            raise MoeRocmError(MR_E_UNSUPPORTED, "rope_freqs.weight: a factor for each frequency")
+        scaling = f"{a}.rope.scaling"
+        for key in (f"{scaling}.attn_factor", f"{scaling}.yarn_attn_factor"):
+            if kind == "yarn" and not attn_factor and self._has(key):
+                raise MoeRocmError(MR_E_UNSUPPORTED, f"{key} beside YaRN: attn_factor has to be given")
+        if not attn_factor:
+            attn_factor = self._meta(self.meta_f32, f"{scaling}.attn_factor", 0.0)
+        more = {}
+        if kind != "none":
+            more = dict(factor=self.meta_f32(f"{scaling}.factor"),
+                        orig_context=self._meta(self.meta_u32, f"{scaling}.original_context_length", 0))
+        if kind == "yarn":
+            more.update(beta_fast=self._meta(self.meta_f32, f"{scaling}.yarn_beta_fast", 0.0),
+                        beta_slow=self._meta(self.meta_f32, f"{scaling}.yarn_beta_slow", 0.0))
         # GPT-OSS takes YaRN's bounds as they come, other models round them to whole pairs
-        scaling = {"none": ROPE_PLAIN, "linear": ROPE_LINEAR,
-                   "yarn": ROPE_YARN_EXACT if a.startswith(("gpt-oss", "gpt_oss")) else ROPE_YARN}[kind]
-        more = {} if kind == "none" else dict(
-            factor=self.meta_f32(f"{a}.rope.scaling.factor"),
-            orig_context=self._meta(self.meta_u32, f"{a}.rope.scaling.original_context_length", 0))
-        return Rope(ctx, shape["head_dim"], rotary_dim=shape["rotary_dim"], layout=layout, scaling=scaling,
-                    base=self._meta(self.meta_f32, f"{a}.rope.freq_base", 10000.0), **more)
+        code = {"none": ROPE_PLAIN, "linear": ROPE_LINEAR, "yarn": ROPE_YARN_EXACT if _is_gpt_oss(a) else ROPE_YARN}[kind]
+        return Rope(ctx, dim, rotary_dim=self._meta(self.meta_u32, f"{a}.rope.dimension_count", dim), layout=layout,
+                    scaling=code, base=self._meta(self.meta_f32, f"{a}.rope.freq_base", 10000.0), attn_factor=attn_factor, **more)
 
-    def kv_cache(self, ctx: "Context", fmt: int, n_pages: int, page_size: int) -> "KvCache":
-        """One layer's cache of the model's key heads and width."""
-        shape = self.attention()
+    def kv_cache(self, ctx: "Context", fmt: int, n_pages: int, page_size: int, layer: int | None = None) -> "KvCache":
+        """One layer's cache of the model's key heads and width; `layer` where they differ from layer to layer."""
+        shape = self.attention(layer)
         return KvCache(ctx, fmt, n_pages, page_size, shape["n_kv_heads"], shape["head_dim"])
+
+
+def _is_gpt_oss(arch: str) -> bool:
+    return arch.startswith(("gpt-oss", "gpt_oss"))
 
 
 def topk(ctx: Context, logits, n_tokens: int, n_experts: int, top_k: int, flags: int, idx, w) -> None:
