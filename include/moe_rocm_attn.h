@@ -17,8 +17,9 @@
  *    graphs see their present values. An entry out of its range is never followed: the call
  *    leaves out what it names, as stated below, and the next mr_sync of the context returns
  *    MR_E_INVAL and says which kind of entry it was.
- *  - Zero tokens, rows or sequences: MR_OK, nothing is launched. More than a launch can hold (2^24 tokens
- *    of mr_qk_norm_rope, 2^24 tiles of 128 rows and a head of mr_attn_prefill): MR_E_INVAL.
+ *  - Zero tokens, rows or sequences: MR_OK, nothing is launched. More than a launch can hold
+ *    (2^24 tokens or more of mr_qk_norm_rope, more than 2^24 - 8 tiles of 128 rows and a head, one of them
+ *    for each sequence's last rows, of mr_attn_prefill): MR_E_INVAL.
  *  - mr_attn_decode keeps partial results in scratch of the context, allocated with its first cache and of
  *    one size for all calls: like all scratch of a context it serves one call at a time.
  *  - Kernel names for mr_profile_read: "qk_norm_rope", "kv_write", "kv_read", "attn_decode", "attn_join",

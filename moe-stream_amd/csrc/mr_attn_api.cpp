@@ -354,8 +354,8 @@ int mr_attn_prefill(mr_ctx* c, uint32_t D, const mr_heads* q, uint32_t nq, const
   if (!cu_q || !cu_k || misaligned(cu_q, 4) || misaligned(cu_k, 4))
     return fail(c, MR_E_INVAL, "cu_q or cu_k is NULL or not 4-byte aligned");
   if (nq > 0x7FFFFFFFu || nk > 0x7FFFFFFFu || n_seqs >= 0x7FFFFFFFu) return fail(c, MR_E_INVAL, "2^31 rows or more");
-  if (((uint64_t)nq / mr::kPrefillRows + n_seqs + 1) * hq.n >= kMaxWork)
-    return fail(c, MR_E_INVAL, "%u rows of %u heads in %u sequences are 2^24 tiles or more", nq, hq.n, n_seqs);
+  if (((uint64_t)nq / mr::kPrefillRows + n_seqs + 1) * hq.n > kMaxWork - 8)  // the launch takes eights of them
+    return fail(c, MR_E_INVAL, "%u rows of %u heads in %u sequences are more than 2^24 - 8 tiles", nq, hq.n, n_seqs);
   if (nq == 0 || n_seqs == 0) return MR_OK;
   if ((rc = bind(c))) return rc;
   c->attn_used = true;
