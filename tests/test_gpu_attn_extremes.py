@@ -7,7 +7,7 @@ import pytest
 import moe_rocm as M
 
 import attnref as R
-from test_gpu_attn import FORMATS, TYPES
+from test_gpu_attn import FORMATS, TYPES, Cached, sync_error
 
 pytestmark = pytest.mark.gpu
 
@@ -255,3 +255,120 @@ def test_sinks_of_rows_that_see_nothing(gpu_ctx, D):
     got = decode(gpu_ctx, kv, q[:1], M.F16, [0], table, sinks=sinks)
     assert (got[0, :2] == 0).all() and np.isnan(got[0, 2:]).all()
     kv.close()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("D,hk,group", [(64, 8, 8), (128, 4, 8), (256, 2, 8), (64, 1, 20), (128, 2, 3)])
+@pytest.mark.parametrize("window", [0, 4097])
+def test_decode_of_split_sequences_with_sinks(gpu_ctx, fmt, D, hk, group, window):
+    lens = [9000, 0, 1500, 20, 5011]
+    c = Cached(gpu_ctx, FORMATS[fmt], lens, hk, D, 256, D + group)
+    rng = np.random.default_rng(4)
+    H = hk * group
+    q = R.rounded(rng.normal(size=(len(lens), H, D)), M.BF16)
+    sinks = rng.normal(size=H).astype(np.float32) * 3
+    sinks[0], sinks[-1], sinks[H // 2] = -np.inf, 40.0, 8.0
+    got = decode(gpu_ctx, c.kv, q, M.BF16, lens, c.table, window=window, sinks=sinks)
+    c.check(got, q, M.BF16, group, D ** -0.5, window, sinks)
+    c.close()
+
+
+@pytest.mark.parametrize("sink", [False, True])
+@pytest.mark.parametrize("D,hk,group", [(64, 2, 4), (256, 1, 3)])
+def test_decode_of_split_sequences_with_pages_missing(gpu_ctx, D, hk, group, sink):
+    """Pages out of range in places, in a row longer than any part, and all of them; lengths out of range."""
+    lens = [20000, 6000, 3000]
+    c = Cached(gpu_ctx, M.KV_MXINT8, lens, hk, D, 64, 3)
+    rng = np.random.default_rng(4)
+    H = hk * group
+    q = R.rounded(rng.normal(size=(3, H, D)), M.F16)
+    sinks = rng.normal(size=H).astype(np.float32) if sink else None
+    table = c.table.copy()
+    there = [np.ones(n, bool) for n in lens]
+    for page in [0, 7, *range(20, 290)]:
+        table[0, page] = -1
+        there[0][64 * page:64 * page + 64] = False
+    table[1, :] = int(c.kv.desc.n_pages)
+    there[1][:] = False
+    dq, out, dl, dt = R.Rows(gpu_ctx, q, M.F16), R.Rows(gpu_ctx, None, M.F16, 3, H, D), R.i32(gpu_ctx, lens), R.i32(gpu_ctx, table)
+    ds = gpu_ctx.to_device(sinks) if sink else None
+    c.kv.attend(dq.heads, 3, dl, dt, table.shape[1], out.heads, sinks=ds)
+    sync_error(gpu_ctx, "block_table")
+    got = out.get()
+    assert (got[1] == 0).all()
+    c.check(got, q, M.F16, group, D ** -0.5, 0, sinks, there)
+    # a length beyond the table's: its pages behind the sequence's are out of range; one below zero: none
+    dl.upload(np.array([2 ** 31 - 1, -3, 3000], np.int32)), dt.upload(c.table)
+    c.kv.attend(dq.heads, 3, dl, dt, table.shape[1], out.heads, sinks=ds)
+    sync_error(gpu_ctx, "seq_len block_table")
+    got = out.get()
+    assert (got[1] == 0).all() and np.isfinite(got).all()
+    c.lens, c.k, c.v = [3000], c.k[2:], c.v[2:]
+    c.check(got[2:], q[2:], M.F16, group, D ** -0.5, 0, sinks)
+    for b in (dq, out, dl, dt, ds):
+        if b is not None:
+            b.free()
+    c.close()
+
+
+# ---- which keys a row sees, counted ----------------------------------------------------------------
+def counted(n, H, D):
+    """Values that count: key j has a one in column j % D."""
+    v = np.zeros((n, H, D), np.float32)
+    v[np.arange(n), :, np.arange(n) % D] = 1.0
+    return v
+
+
+def shares(first, last, D):
+    """Of keys first..last (arrays), the part in each column."""
+    d = np.arange(D)
+    upto = lambda x: np.maximum(0, (x[:, None] - d) // D + 1)  # noqa: E731  keys 0..x in the column
+    n = upto(last) - upto(first - 1)
+    return n / np.maximum(last - first + 1, 1)[:, None]
+
+
+@pytest.mark.parametrize("D,hk,group,dtype", [(128, 4, 8, "bf16"), (64, 8, 8, "bf16"), (256, 2, 8, "f16"), (128, 3, 1, "f16"),
+                                              (64, 2, 6, "f16"), (256, 9, 2, "bf16")])
+@pytest.mark.parametrize("lens,past,window", [([8192], 0, 0), ([8192], 0, 128), ([5000, 1, 2100], 700, 0), ([3001, 777, 4100], 64, 1000)])
+def test_prefill_sees_every_key_of_a_long_prompt_once(gpu_ctx, D, hk, group, dtype, lens, past, window):
+    """Scores of zero: a row is the mean of the values it sees, whose columns count them. A key too many or too few is a
+    part in 128 of a column or more at 8192 keys and D = 64. All weights are one power of two, so that only the quotient (2 steps
+    of 32 bits) and the output are rounded."""
+    dtype = TYPES[dtype]
+    cu_q = np.concatenate([[0], np.cumsum(lens)])
+    cu_k = np.concatenate([[0], np.cumsum([n + past for n in lens])])
+    H = hk * group
+    rng = np.random.default_rng(0)
+    q = np.zeros((cu_q[-1], H, D), np.float32)
+    k = R.rounded(rng.normal(size=(cu_k[-1], hk, D)), dtype)
+    v = np.concatenate([counted(n + past, hk, D) for n in lens])
+    got = prompt(gpu_ctx, q, k, v, dtype, cu_q, cu_k, window=window)
+    for s, n in enumerate(lens):
+        last = past + np.arange(n)
+        first = np.maximum(0, last - window + 1) if window else np.zeros(n, int)
+        y = shares(first, last, D)[:, None]
+        d = np.abs(got[cu_q[s]:cu_q[s + 1]] - y)
+        assert (d <= (R.HALF[dtype] + 2.0 ** -22) * y + (2.0 ** -25 if dtype == M.F16 else 0)).all(), (s, np.argwhere(d.max(-1) == d.max())[0])
+
+
+def check_decode_counted(ctx, fmt, D, hk, group, lens, window):
+    rng = np.random.default_rng(1)
+    seqs = [(rng.normal(size=(n, hk, D)).astype(np.float32), counted(n, hk, D)) for n in lens]
+    kv, table = filled(ctx, fmt, seqs, page=128)
+    got = decode(ctx, kv, np.zeros((len(lens), hk * group, D), np.float32), M.F16, lens, table, window=window)
+    last = np.array(lens) - 1
+    first = np.maximum(0, last - window + 1) if window else np.zeros(len(lens), int)
+    y = shares(first, last, D)[:, None]
+    assert (np.abs(got - y) <= (2.0 ** -11 + 2.0 ** -21) * y + 2.0 ** -25).all()
+    kv.close()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("D,hk,group", [(64, 8, 8), (128, 4, 8), (256, 2, 8), (128, 1, 33)])
+@pytest.mark.parametrize("lens,window", [([24000, 0, 1, 700, 9000], 0), ([24000, 64, 8193], 5000), ([1] * 30 + [7000], 0)])
+def test_decode_sees_every_key_once(gpu_ctx, fmt, D, hk, group, lens, window):
+    check_decode_counted(gpu_ctx, FORMATS[fmt], D, hk, group, lens, window)
+
+
+def test_decode_of_more_sequences_than_are_split_sees_every_key_once(gpu_ctx):
+    check_decode_counted(gpu_ctx, M.KV_MXFP4, 64, 1, 4, [300] * 1030 + [5000], 0)
