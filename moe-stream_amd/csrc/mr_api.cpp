@@ -330,14 +330,14 @@ int mr_ctx_create(int device, mr_ctx** out) {
   if (e == hipSuccess) e = hipDeviceGetAttribute(&c->n_cu, hipDeviceAttributeMultiprocessorCount, device);
   if (e == hipSuccess && hipDeviceGetAttribute(&c->wall_khz, hipDeviceAttributeWallClockRate, device) != hipSuccess)
     c->wall_khz = 100000;  // the documented 100 MHz when the runtime does not report it
-  if (e == hipSuccess) e = hipMalloc(&c->attn_err, 256);
+  if (e == hipSuccess) e = hipHostMalloc(&c->attn_err_host, mr::kAttnErrWords * 4, hipHostMallocMapped | hipHostMallocCoherent);
   if (e == hipSuccess) {
-    const uint32_t zero = 0;
-    e = hipMemcpy(c->attn_err, &zero, 4, hipMemcpyHostToDevice);
+    memset(c->attn_err_host, 0, mr::kAttnErrWords * 4);
+    e = hipHostGetDevicePointer(reinterpret_cast<void**>(&c->attn_err), c->attn_err_host, 0);
   }
   if (e != hipSuccess) {
     int rc = hip_fail(nullptr, e, "context setup");
-    if (c->attn_err) (void)hipFree(c->attn_err);
+    if (c->attn_err_host) (void)hipHostFree(c->attn_err_host);
     if (c->stream) (void)hipStreamDestroy(c->stream);
     delete c;
     return rc;
@@ -358,7 +358,7 @@ void mr_ctx_destroy(mr_ctx* c) {
     if (c->stream) (void)hipStreamSynchronize(c->stream);
     if (c->scratch.base) (void)hipFree(c->scratch.base);
     for (void* r : c->retired) (void)hipFree(r);
-    if (c->attn_err) (void)hipFree(c->attn_err);
+    if (c->attn_err_host) (void)hipHostFree(c->attn_err_host);
     if (c->attn_scratch) (void)hipFree(c->attn_scratch);
     if (c->ev0) (void)hipEventDestroy(c->ev0);
     if (c->ev1) (void)hipEventDestroy(c->ev1);
@@ -434,19 +434,18 @@ int mr_sync(mr_ctx* c) {
     if (ran_out)
       return set_err(c, MR_E_LAUNCH, "fused decode kernel: a cross-workgroup wait ran out (results of that launch are invalid)");
   }
-  if (c->attn_used) {
-    uint32_t bits = 0;
-    e = hipMemcpy(&bits, c->attn_err, 4, hipMemcpyDeviceToHost);
-    if (e != hipSuccess) return hip_fail(c, e, "read attention error word");
-    if (bits) {
-      const uint32_t zero = 0;
-      e = hipMemcpy(c->attn_err, &zero, 4, hipMemcpyHostToDevice);
-      if (e != hipSuccess) return hip_fail(c, e, "reset attention error word");
-      return set_err(c, MR_E_INVAL, "attention: an entry was out of range in%s%s%s%s (what it names was left out)",
-                     bits & 1u ? " slots" : "", bits & 2u ? " seq_len" : "", bits & 4u ? " block_table" : "",
-                     bits & 8u ? " cu_q or cu_k" : "");
-    }
+  static const char* const kKinds[mr::kAttnErrWords] = {" slots", " seq_len", " block_table", " cu_q or cu_k"};
+  const char* kinds[mr::kAttnErrWords];
+  bool any = false;
+  for (int i = 0; i < mr::kAttnErrWords; ++i) {
+    volatile uint32_t* word = c->attn_err_host + i;
+    kinds[i] = *word ? kKinds[i] : "";
+    any |= *word != 0;
+    *word = 0;
   }
+  if (any)
+    return set_err(c, MR_E_INVAL, "attention: an entry was out of range in%s%s%s%s (what it names was left out)", kinds[0],
+                   kinds[1], kinds[2], kinds[3]);
   return MR_OK;
 }
 

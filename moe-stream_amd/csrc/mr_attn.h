@@ -23,8 +23,9 @@ struct mr_kv {
 
 namespace mr {
 
-// Bits of the context's attention error word: what kind of device index was out of range.
-constexpr uint32_t kErrSlot = 1, kErrLength = 2, kErrPage = 4, kErrOffset = 8;
+// Of the context's attention error words: which kind of device index was out of range.
+constexpr uint32_t kErrSlot = 0, kErrLength = 1, kErrPage = 2, kErrOffset = 3;
+static_assert(kErrOffset + 1 == kAttnErrWords, "a word for each kind");
 
 // mr_heads with its defaults filled in.
 struct Heads {

@@ -286,7 +286,6 @@ int mr_kv_write(mr_ctx* c, mr_kv* kv, const mr_heads* k, const mr_heads* v, uint
   if (T > kMaxTokens) return fail(c, MR_E_INVAL, "n_tokens %u is above 2^30 - 64", T);
   if (T == 0) return MR_OK;
   if ((rc = bind(c))) return rc;
-  c->attn_used = true;
   const hipError_t e = mr::launch_kv_write(c->launch(), pages(kv), kv->d.format, kv->d.head_dim, hk, hv, T, slots, c->attn_err);
   return e == hipSuccess ? MR_OK : hip_fail(c, e, "kv_write launch");
 }
@@ -305,7 +304,6 @@ int mr_kv_read(mr_ctx* c, const mr_kv* kv, uint32_t T, const int32_t* slots, con
   if (T > kMaxTokens) return fail(c, MR_E_INVAL, "n_tokens %u is above 2^30 - 64", T);
   if (T == 0) return MR_OK;
   if ((rc = bind(c))) return rc;
-  c->attn_used = true;
   const hipError_t e = mr::launch_kv_read(c->launch(), pages(kv), kv->d.format, kv->d.head_dim, T, slots, hk, hv, c->attn_err);
   return e == hipSuccess ? MR_OK : hip_fail(c, e, "kv_read launch");
 }
@@ -328,7 +326,6 @@ int mr_attn_decode(mr_ctx* c, const mr_kv* kv, const mr_heads* q, uint32_t B, co
   if (B > 65535) return fail(c, MR_E_INVAL, "n_seqs %u is above 65535", B);
   if (B == 0) return MR_OK;
   if ((rc = bind(c))) return rc;
-  c->attn_used = true;
   const hipError_t e = mr::launch_attn_decode(c->launch(), pages(kv), kv->d.format, D, hq, B, seq_len, block_table,
                                               max_pages, o, ho, c->attn_err, c->attn_scratch, c->n_cu);
   return e == hipSuccess ? MR_OK : hip_fail(c, e, "attn_decode launch");
@@ -358,7 +355,6 @@ int mr_attn_prefill(mr_ctx* c, uint32_t D, const mr_heads* q, uint32_t nq, const
     return fail(c, MR_E_INVAL, "%u rows of %u heads in %u sequences are more than 2^24 - 8 tiles", nq, hq.n, n_seqs);
   if (nq == 0 || n_seqs == 0) return MR_OK;
   if ((rc = bind(c))) return rc;
-  c->attn_used = true;
   const hipError_t e = mr::launch_attn_prefill(c->launch(), D, hq, nq, hk, hv, nk, n_seqs, cu_q, cu_k, o, ho, c->attn_err);
   return e == hipSuccess ? MR_OK : hip_fail(c, e, "attn_prefill launch");
 }

@@ -254,7 +254,7 @@ __global__ __launch_bounds__(64 * kWaves, (Tuning<FMT, D>::kPerSimd)) void k_att
   Part pt;
   if (!find_part(a, blockIdx.x, false, pt)) return;
   const Span sp = pt.sp;
-  if (threadIdx.x == 0 && blockIdx.y == 0 && pt.part == 0 && sp.bad) atomicOr(a.err, kErrLength);
+  if (threadIdx.x == 0 && blockIdx.y == 0 && pt.part == 0 && sp.bad) note_error(a.err, kErrLength);
   const uint32_t hk = blockIdx.y / a.head_tiles, h0 = 16 * (blockIdx.y % a.head_tiles);  // first query head within the group
   const uint32_t heads = min(16u, a.heads - h0);
   const uint32_t hq = hk * a.heads + h0 + min((uint32_t)n, heads - 1);  // this lane's query head (the last one repeated)
@@ -297,7 +297,7 @@ __global__ __launch_bounds__(64 * kWaves, (Tuning<FMT, D>::kPerSimd)) void k_att
     if (chunk >= end) return -1;
     const int p = a.table[(uint64_t)pt.b * a.max_pages + (uint32_t)(chunk >> (a.kv.page_shift - 6))];
     if (p >= 0 && (uint32_t)p < a.kv.n_pages) return p;
-    atomicOr(a.err, kErrPage);
+    note_error(a.err, kErrPage);
     return -1;
   };
   auto address = [&](int page, int chunk) { return a.kv.at(page < 0 ? 0 : page, hk, chunk & (cpp - 1)); };

@@ -55,6 +55,11 @@ __device__ __forceinline__ void store4(void* p, uint32_t dtype, uint64_t i, f32x
   *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p) + i) = w;
 }
 
+// Sets the error word of a kind; it is the host's memory.
+__device__ __forceinline__ void note_error(uint32_t* err, uint32_t kind) {
+  __hip_atomic_store(err + kind, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+}
+
 // The sum of lanes 0 .. l in lane l: shifts inside the rows of 16 lanes, then row ends broadcast to the rows after
 // them. All 64 lanes active.
 __device__ __forceinline__ uint32_t wave_prefix(uint32_t v) {

@@ -141,7 +141,7 @@ __device__ __forceinline__ bool find_tile(const PrefillArgs& a, int tile, bool r
   int before = 0;
   for (int s0 = 0; s0 < a.n_seqs && (report || !found); s0 += 64) {
     const Seq r = s0 + lane < a.n_seqs ? seq(s0 + lane) : Seq{};
-    if (report && __any(r.bad) && lane == 0) atomicOr(a.err, kErrOffset);
+    if (report && __any(r.bad) && lane == 0) note_error(a.err, kErrOffset);
     if (search) continue;
     const int sum = (int)wave_prefix((uint32_t)r.tiles);
     const uint64_t past = __ballot(before + sum > tile);

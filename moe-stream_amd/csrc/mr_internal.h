@@ -16,6 +16,7 @@ namespace mr {
 constexpr uint32_t kMaxTopK = 16;        // softmax_topk_kernel limit (fused_ops.metal:150)
 constexpr uint32_t kMaxExperts = 512;    // same limit (fused_ops.metal:158)
 constexpr uint32_t kMaxHidden = 16384;   // LDS-staged activation limit of the VALU kernels
+constexpr int kAttnErrWords = 4;         // kinds of device index entries (mr_attn.h)
 // Size of the static scratch array of mr_moe_forward_batched_noalloc (one per GPU).
 constexpr uint64_t kStaticScratchBytes = MR_STATIC_SCRATCH_BYTES;
 
@@ -107,10 +108,10 @@ struct mr_ctx {
   // mr_ctx_create; nullptr with static_err set when the lookup failed.
   void* static_scratch = nullptr;
   hipError_t static_err = hipSuccess;
-  // Error word of the attention-side calls (moe_rocm_attn.h), allocated with the context; read by
-  // mr_sync once such a call was made.
+  // Error words of the attention-side calls (moe_rocm_attn.h), one for each kind of entry, allocated with the
+  // context in pinned host memory: mr_sync reads them without a copy. attn_err: their device address.
+  uint32_t* attn_err_host = nullptr;
   uint32_t* attn_err = nullptr;
-  bool attn_used = false;
   // Partial results of mr_attn_decode, of one size for all calls; allocated with the first cache.
   float* attn_scratch = nullptr;
   hipEvent_t ev0 = nullptr, ev1 = nullptr;

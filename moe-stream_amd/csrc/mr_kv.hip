@@ -35,12 +35,12 @@ __device__ __forceinline__ uint32_t code(float y) {
   return y < 0.f && c ? c | 8u : c;
 }
 
-// Token s of the chunk that slot `slot` lies in; nullptr (and the error bit) for a slot out of range.
+// Token s of the chunk that slot `slot` lies in; nullptr (and the error word) for a slot out of range.
 __device__ __forceinline__ uint8_t* find(const KvPages& kv, int slot, uint32_t head, uint32_t* err, int& s) {
   const uint32_t page = (uint32_t)slot >> kv.page_shift;
   if (slot < 0) return nullptr;
   if (page >= kv.n_pages) {
-    atomicOr(err, kErrSlot);
+    note_error(err, kErrSlot);
     return nullptr;
   }
   s = slot & 63;
