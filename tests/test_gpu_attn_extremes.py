@@ -372,3 +372,28 @@ def test_decode_sees_every_key_once(gpu_ctx, fmt, D, hk, group, lens, window):
 
 def test_decode_of_more_sequences_than_are_split_sees_every_key_once(gpu_ctx):
     check_decode_counted(gpu_ctx, M.KV_MXFP4, 64, 1, 4, [300] * 1030 + [5000], 0)
+
+
+# ---- offsets of many sequences -----------------------------------------------------------------------
+@pytest.mark.parametrize("n_seqs", [513, 1500])
+@pytest.mark.parametrize("at,value", [(0, -1), (1, 2 ** 31 - 1), (448, -7), (512, 0), (-1, 10 ** 6)])
+def test_offsets_out_of_range_among_many_sequences(gpu_ctx, n_seqs, at, value):
+    """One key offset out of range, or below the one before, anywhere: reported, and the sequences that do not have it are as
+    they are without."""
+    rng = np.random.default_rng(n_seqs)
+    lens = rng.integers(1, 4, n_seqs)
+    cu = np.concatenate([[0], np.cumsum(lens)])
+    bad = cu.copy()
+    bad[at] = value
+    D, T = 64, int(cu[-1])
+    q, k, v = (R.rounded(rng.normal(size=(T, 1, D)), M.F16) for _ in range(3))
+    want = prompt(gpu_ctx, q, k, v, M.F16, cu, cu)
+    rows = [R.Rows(gpu_ctx, x, M.F16) for x in (q, k, v)] + [R.Rows(gpu_ctx, None, M.F16, T, 1, D), R.i32(gpu_ctx, cu), R.i32(gpu_ctx, bad)]
+    dq, dk, dv, out, dcq, dck = rows
+    M.attn_prefill(gpu_ctx, D, dq.heads, dk.heads, dv.heads, T, T, n_seqs, dcq, dck, out.heads)
+    sync_error(gpu_ctx, "cu_q or cu_k")
+    got, at = out.get(), at % (n_seqs + 1)
+    first, last = cu[max(at - 1, 0)], cu[min(at + 1, n_seqs)]
+    assert (got[:first] == want[:first]).all() and (got[last:] == want[last:]).all()
+    for b in rows:
+        b.free()
