@@ -84,8 +84,9 @@ void mr_rope_destroy(mr_rope* rope);
 const double* mr_rope_frequencies(const mr_rope* rope, uint32_t* n, float* attn_factor);
 
 /* For each token t and head: x = in (RMSNorm over head_dim with weight w and eps where w is given:
- * x = in / sqrt(mean(in^2) + eps) * w), then the pairs of x turn by positions[t] * f_i. Angles are
- * reduced in 64 bits: any int32 position. q_norm, k_norm: f32 [head_dim] or NULL (no norm);
+ * x = in / sqrt(mean(in^2) + eps) * w, the squares summed in 32 bits, which magnitudes beyond 1e18 leave), then
+ * the pairs of x turn by positions[t] * f_i. Angles are reduced in 64 bits: any int32 position. q_norm, k_norm:
+ * f32 [head_dim] or NULL (no norm);
  * 0 <= eps <= 1. k and k_out: both NULL for queries alone. Types of inputs and outputs are free,
  * q's and k's alike; q_out may be q (k_out k) with the same type and strides. */
 int mr_qk_norm_rope(mr_ctx* ctx, const mr_rope* rope, const mr_heads* q, const mr_heads* k, const float* q_norm,
@@ -133,8 +134,15 @@ int mr_kv_read(mr_ctx* ctx, const mr_kv* kv, uint32_t n_tokens, const int32_t* s
 /* ---- attention (SDPA with shared heads, sinks and windows, attention.rs:178-271) -- */
 /* Query head h reads key/value head h / (query heads / key heads). A position sees the keys at its own
  * and at earlier positions, with window > 0 the last `window` of them, its own among them.
- * out = sum_j p_j v_j, p = softmax(scale * q.k); a sink is one more score of the softmax with no value.
- * A row that sees no key is zero. */
+ * out = sum_j p_j v_j, p = softmax(scale * q.k); a sink is one more score of the softmax with no value (-infinity:
+ * none; +infinity or NaN: the head's rows are NaN). A row that sees no key is zero.
+ *
+ * Numerics. Scores, maxima and sums are 32-bit floats; scores of any size that 32 bits hold are right to their
+ * own rounding. Weights are rounded to 16 bits for the product with the values, and the divisor is the sum of the
+ * rounded ones. Over the cache they are f16: 11 bits down to 2^-28 of the largest, and what lies below 2^-39 of it
+ * is dropped. Over prompts they have the inputs' type: f16, 11 bits down to 2^-21 and nothing below 2^-32, or bf16,
+ * 8 bits and the range of 32. mr_attn_decode takes a query head as f16 times a power of two: all its bits down to
+ * 2^-30 of its largest element. The same call gives the same bits. */
 typedef struct mr_attn_opts {
   float scale;        /* 0: 1 / sqrt(head_dim) */
   uint32_t window;    /* 0: all earlier positions */
@@ -145,7 +153,14 @@ typedef struct mr_attn_opts {
  * or BF16, both the same; sequence b has seq_len[b] tokens in the cache, its own among them (0: the
  * row is zero), token i in slot block_table[b * max_pages + i / page_size] * page_size + i % page_size.
  * A length below 0 or beyond max_pages * page_size is taken as the nearest that is not, a page out of
- * range as tokens that are not there; both give an error at mr_sync. opts NULL: defaults. */
+ * range as tokens that are not there; both give an error at mr_sync. opts NULL: defaults.
+ *
+ * Long sequences are spread over the CUs in calls of up to 1024 sequences whose tables hold less than 2^37
+ * tokens in all (n_seqs * max_pages * page_size). In others a sequence is one workgroup's for each key head:
+ * 100,001 tokens among 1023 and among 1024 others of one token take 0.23 and 0.48 ms (MXFP4, 4 heads of 128), 0.17
+ * and 1.2 ms (MXINT8, 2 of 256). Whether a call is split is decided by what the table holds, not by the lengths:
+ * for 1280 tokens or less (heads of 256: 512), or a window of 1217 (449) or less, there is one launch and not
+ * two (8 sequences of 250 tokens: 7.5 and 10.4 us). */
 int mr_attn_decode(mr_ctx* ctx, const mr_kv* kv, const mr_heads* q, uint32_t n_seqs, const int32_t* seq_len,
                    const int32_t* block_table, uint32_t max_pages, const mr_attn_opts* opts, const mr_heads* out);
 
@@ -154,8 +169,10 @@ int mr_attn_decode(mr_ctx* ctx, const mr_kv* kv, const mr_heads* q, uint32_t n_s
  * positions (as many as keys: a whole prompt; fewer: the next part of one; more: the first ones see
  * nothing). cu_q, cu_k: n_seqs + 1 offsets that do not decrease. Offsets outside the rows are taken as
  * the nearest inside and decreasing ones as empty sequences, both with an error at mr_sync; rows that two
- * sequences claim then hold either's result or none. Rows of `out` in no sequence are left as they are. q, k, v and out: F16 or BF16, all the same; head_dim 64, 128 or
- * 256; token strides of k and v below 2^24 elements. opts NULL: defaults. */
+ * sequences claim then hold either's result or none. Rows of `out` in no sequence are left as they are.
+ * Keys and values that are not finite reach the rows that see them and no others: an element of a row that sees a value of
+ * infinity or NaN is one of the two. q, k, v and out: F16 or BF16, all the same; head_dim 64, 128 or 256; token strides
+ * of k and v below 2^24 elements. opts NULL: defaults. */
 int mr_attn_prefill(mr_ctx* ctx, uint32_t head_dim, const mr_heads* q, uint32_t n_q, const mr_heads* k,
                     const mr_heads* v, uint32_t n_k, uint32_t n_seqs, const int32_t* cu_q, const int32_t* cu_k,
                     const mr_attn_opts* opts, const mr_heads* out);

@@ -6,9 +6,12 @@
 // codes into operands rounds nothing. Pages lie in the order in which the lanes read them (KvLayout): no LDS,
 // no barrier and no exchange of elements between lanes; a wave takes chunks of 64 tokens by itself.
 //
-// 32 sequences of 16000 tokens, 4 heads of 128: MXFP4 279 MB in 56 us, 5.0 TB/s, MXINT8 541 MB in 109 us, 5.0 TB/s, of
-// the 6 TB/s that reading alone reaches here; what is missing is the launch and the first and last chunks, about 8 us.
+// 32 sequences of 16000 tokens, 4 heads of 128: MXFP4 279 MB in 54 us, 5.2 TB/s, MXINT8 541 MB in 105 us, 5.2 TB/s; 16
+// of 16000, 2 heads of 256, F16: 524 MB in 101 us, 5.2 TB/s; of the 6 TB/s that reading alone reaches here; what is missing
+// is the launch and the first and last chunks, about 8 us.
 // One short sequence is latency: 5.6 us.
+//
+// Weights are rounded to f16 for the second product, the largest of them 2^14 (kLift), and their sum is that of the rounded ones.
 //
 // The sequences' chunks are dealt out to the workgroups in parts of one size, so that a long sequence next to
 // short ones is spread over many CUs; the parts of a sequence are joined by a second launch.

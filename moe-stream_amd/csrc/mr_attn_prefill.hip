@@ -9,12 +9,13 @@
 // V^T in that order is what the transposing LDS read returns: four adjacent keys of one column.
 // p is rounded to the type of v for the second product, as the matrix instructions take it.
 //
-// Matrix instructions and the exponentials' vector instructions bound it in about equal parts (a step of 32 rows and 64
-// keys of 128: 1024 cycles of the one, 900 of the other), under the card's power limit: fewer cycles, as with the
-// pipelined form below, came at a lower clock. 8192 tokens, the card warm: heads of 128 (32 on 4) 505 us, 1089
-// TFLOP/s; of 64 (64 on 8) 569 us, 966; of 256 (16 on 2) 546 us, 1007; the library's products reach 1430 to 1490. With a window of 128, 64 heads
-// of 64, 56 us: 151 MB at 2.7 TB/s, the exponentials of steps that rows see in part; short prompts are latency, 6 us
-// for 61 tokens.
+// Heads of 128: matrix instructions and the exponentials' vector instructions bound it in about equal parts (55% and 46%
+// of the cycles), under the card's power limit (1.75 GHz): fewer cycles, as with the pipelined form below, came at a lower
+// clock. Of 64: the vector instructions (50% and 73%). Of 256: one wave to a SIMD, whose instructions wait for each other (40% and
+// 27%, 2.1 GHz). 8192 tokens, the card warm: heads of 128 (32 on 4) 497 to 515 us by card, 1067 to 1106 TFLOP/s; of 64 (64 on 8) 567
+// to 580 us, 948 to 970; of 256 (16 on 2) 555 to 560 us, 982 to 991; the library's products reach 1430 to 1490. With a window of
+// 128, 64 heads of 64, 57 us: 151 MB at 2.6 TB/s, the exponentials of steps that rows see in part; short prompts are
+// latency, 6 us for 61 tokens.
 #include <numeric>
 
 #include "mr_attn_device.h"
@@ -266,8 +267,8 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
     const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(uintptr_t)(at + 16 * D)));
     return u32x4{x.x, x.y, y.x, y.y};
   };
-  // Masks the scores of the keys from k0 on and moves the base m, with the sums, if their maximum has left it
-  // kSlack behind: p is at most 2^kSlack, and nearly no step rescales.
+  // Masks the scores of the keys from k0 on and moves the maximum m, with the sums, if theirs has left it
+  // kSlack behind: p is at most 2^(kSlack + kLift), and nearly no step rescales.
   auto settle = [&](int k0, f32x16& s0, f32x16& s1) {
     if (k0 + kKeys - 1 > pl.row + wave_row + diff || k0 < wave_first) {
       // Bit i: the row sees the i-th key from its half's first on. A bit and a select a score; a comparison and a select for

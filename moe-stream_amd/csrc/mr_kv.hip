@@ -51,7 +51,7 @@ constexpr int kWindow = 64;  // tokens of a workgroup
 
 // Runs of tokens that fill a chunk. The values' bytes of a token lie 16 bytes apart in its chunk; where 64 tokens
 // in a row go to (come from) the 64 slots of a chunk in order, as most of a prompt's do, they are put together
-// in LDS and the chunk is moved whole (8192 tokens, 4 heads of 128, 8 bits: 8.4 us written, 8.0 read; 100001 tokens,
+// in LDS and the chunk is moved whole (8192 tokens, 4 heads of 128, 8 bits, the same again: 8.3 us written, 8.0 read; 100001 tokens,
 // 2 heads of 256: written in 232 us one by one, in 126 so). The workgroup in whose
 // window of 64 tokens such a run begins does all of it. Of the others, kPiece tokens or more in a row in a chunk (a
 // prompt's first and last) go four at a time to words of the chunk: 8191 tokens were written in 12.4 us and read in 12.9 with

@@ -23,7 +23,7 @@ struct RopeArgs {
 // part. The angle is reduced to a fraction of a turn in 64 bits (f32 would lose 2^-24 of a far position's
 // angle), the sine and cosine of that fraction are taken in f32, once per token and pair, while the first R
 // heads of each lane group are on their way from memory. Memory bounds it: 4096 tokens of 36 heads of 128, f32 to
-// bf16 with norms, 29.6 us, 113 MB at 3.8 TB/s (a large copy: 4.9); one token of 72 heads of 64: 3.0 us.
+// bf16 with norms, 28.6 us, 113 MB at 4.0 TB/s (a large copy: 4.9); one token of 72 heads of 64: 2.9 us.
 template <int R>
 __global__ __launch_bounds__(256) void k_qk_norm_rope(RopeArgs a, int L) {
   __shared__ __attribute__((aligned(16))) float cs[256], sn[256];
