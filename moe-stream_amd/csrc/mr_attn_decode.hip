@@ -405,7 +405,7 @@ __global__ __launch_bounds__(64 * kWaves, (Tuning<FMT, D>::kPerSimd)) void k_att
     return;
   }
   if (a.o.sinks) {
-    const float sink = a.o.sinks[hq] * 1.44269504088896340736f, m1 = fmaxf(m, sink);
+    const float sink = sink_of(a.o.sinks, hq), m1 = fmaxf(m, sink);
     const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m1);
     l = l * f + (sink == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sink - m1));
 #pragma unroll
@@ -442,7 +442,7 @@ __global__ __launch_bounds__(kJoin) void k_attn_join(DecodeArgs a) {
   top = wave_max(top);
   if (lane == 0) wave_m[wave] = top;
   __syncthreads();
-  const float sink = a.o.sinks ? a.o.sinks[h] * 1.44269504088896340736f : -INFINITY;
+  const float sink = sink_of(a.o.sinks, h);
   float base = sink;
   for (int w = 0; w < kJoin / 64; ++w) base = fmaxf(base, wave_m[w]);
   if (base == -INFINITY) base = 0.f;

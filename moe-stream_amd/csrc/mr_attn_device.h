@@ -55,6 +55,12 @@ __device__ __forceinline__ void store4(void* p, uint32_t dtype, uint64_t i, f32x
   *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p) + i) = w;
 }
 
+// A head's sink in powers of two; a finite one stays finite. No sinks: -infinity.
+__device__ __forceinline__ float sink_of(const float* sinks, uint32_t h) {
+  const float s = sinks ? sinks[h] : -INFINITY;
+  return (s > 0x1p127f && s < INFINITY ? 0x1p127f : s) * 1.44269504088896340736f;
+}
+
 // Sets the error word of a kind; it is the host's memory.
 __device__ __forceinline__ void note_error(uint32_t* err, uint32_t kind) {
   __hip_atomic_store(err + kind, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);

@@ -248,7 +248,7 @@ __device__ __forceinline__ bool attend_tile(const PrefillArgs& a, uint16_t* lds,
   // finite where no key has been seen (-inf, or 0 * -inf): a masked score stays -inf
   auto base_of = [&] { return fmaxf(kDiff ? m : fmaf(m, c_base, -kLift<BF>), -kLargest); };
   // A sink joins at the end: as the first maximum, one far above the scores left their weights no bits in f16.
-  const float sink = a.o.sinks ? a.o.sinks[h] * 1.44269504088896340736f : -INFINITY;
+  const float sink = sink_of(a.o.sinks, h);
 
   constexpr int NI = D / 16, NV = 4 * ND;
   // Operand of the scores: 8 elements of key 32 t + n; of the values: V^T of 16 keys and 32 elements, where lane

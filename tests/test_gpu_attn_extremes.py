@@ -397,3 +397,19 @@ def test_offsets_out_of_range_among_many_sequences(gpu_ctx, n_seqs, at, value):
     assert (got[:first] == want[:first]).all() and (got[last:] == want[last:]).all()
     for b in rows:
         b.free()
+
+
+# ---- sinks whose powers of two leave 32 bits ---------------------------------------------------------
+@pytest.mark.parametrize("n", [3, 5000])
+def test_finite_sinks_near_the_largest_number(gpu_ctx, n):
+    """Finite sinks up to the largest have a result: nothing is left beside one, nothing is taken by a least one."""
+    D, sinks = 64, np.array([3e38, np.finfo(np.float32).max, -3e38, np.finfo(np.float32).min], np.float32)
+    rng = np.random.default_rng(n)
+    q, k, v = (R.rounded(rng.normal(size=s), M.F16) for s in ((1, 4, D), (n, 1, D), (n, 1, D)))
+    kv, table = filled(gpu_ctx, M.KV_F16, [(k, v)])
+    for got in (decode(gpu_ctx, kv, q, M.F16, [n], table, sinks=sinks), prompt(gpu_ctx, q, k, v, M.F16, [0, 1], [0, n], sinks=sinks)):
+        assert (got[0, :2] == 0).all()
+        for h in (2, 3):
+            y, av, ss, cnt = R.attend(q[0, h], k[:, 0], v[:, 0], D ** -0.5, 0, n - 1)
+            assert (np.abs(got[0, h] - y) <= R.attention_bound(y, av, ss, cnt, D, M.F16, 2.0 ** -11)).all()
+    kv.close()
