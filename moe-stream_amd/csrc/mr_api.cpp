@@ -360,6 +360,7 @@ void mr_ctx_destroy(mr_ctx* c) {
     for (void* r : c->retired) (void)hipFree(r);
     if (c->attn_err_host) (void)hipHostFree(c->attn_err_host);
     if (c->attn_scratch) (void)hipFree(c->attn_scratch);
+    if (c->delta_scratch) (void)hipFree(c->delta_scratch);
     if (c->ev0) (void)hipEventDestroy(c->ev0);
     if (c->ev1) (void)hipEventDestroy(c->ev1);
     for (hipEvent_t ev : c->prof.pool) (void)hipEventDestroy(ev);
@@ -434,7 +435,8 @@ int mr_sync(mr_ctx* c) {
     if (ran_out)
       return set_err(c, MR_E_LAUNCH, "fused decode kernel: a cross-workgroup wait ran out (results of that launch are invalid)");
   }
-  static const char* const kKinds[mr::kAttnErrWords] = {" slots", " seq_len", " block_table", " cu_q or cu_k"};
+  static const char* const kKinds[mr::kAttnErrWords] = {" slots", " seq_len", " block_table", " cu_q or cu_k", " cu",
+                                                        " source or target"};
   const char* kinds[mr::kAttnErrWords];
   bool any = false;
   for (int i = 0; i < mr::kAttnErrWords; ++i) {
@@ -444,8 +446,8 @@ int mr_sync(mr_ctx* c) {
     *word = 0;
   }
   if (any)
-    return set_err(c, MR_E_INVAL, "attention: an entry was out of range in%s%s%s%s (what it names was left out)", kinds[0],
-                   kinds[1], kinds[2], kinds[3]);
+    return set_err(c, MR_E_INVAL, "attention: an entry was out of range in%s%s%s%s%s%s (what it names was left out)", kinds[0],
+                   kinds[1], kinds[2], kinds[3], kinds[4], kinds[5]);
   return MR_OK;
 }
 

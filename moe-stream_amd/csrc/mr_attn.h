@@ -24,8 +24,8 @@ struct mr_kv {
 namespace mr {
 
 // Of the context's attention error words: which kind of device index was out of range.
-constexpr uint32_t kErrSlot = 0, kErrLength = 1, kErrPage = 2, kErrOffset = 3;
-static_assert(kErrOffset + 1 == kAttnErrWords, "a word for each kind");
+constexpr uint32_t kErrSlot = 0, kErrLength = 1, kErrPage = 2, kErrOffset = 3, kErrPacked = 4, kErrState = 5;
+static_assert(kErrState + 1 == kAttnErrWords, "a word for each kind");
 
 // mr_heads with its defaults filled in.
 struct Heads {

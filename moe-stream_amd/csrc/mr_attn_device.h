@@ -61,6 +61,15 @@ __device__ __forceinline__ float sink_of(const float* sinks, uint32_t h) {
   return (s > 0x1p127f && s < INFINITY ? 0x1p127f : s) * 1.44269504088896340736f;
 }
 
+// Division of x < 2^24 by 1 <= d < 2^24: with 2^b <= d < 2^(b + 1), x ceil(2^(39 + b) / d) has 64 bits, and over
+// 2^(39 + b) it is above x / d by less than x / 2^(39 + b) < 1 / d.
+struct Divisor {
+  uint64_t mul;
+  uint32_t d, shift;
+  explicit Divisor(uint32_t d) : d(d), shift(70 - __builtin_clz(d)) { mul = ((1ull << shift) + d - 1) / d; }
+  __device__ __forceinline__ uint32_t of(uint32_t x) const { return (uint32_t)((x * mul) >> shift); }
+};
+
 // Sets the error word of a kind; it is the host's memory.
 __device__ __forceinline__ void note_error(uint32_t* err, uint32_t kind) {
   __hip_atomic_store(err + kind, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);

@@ -1,0 +1,423 @@
+// mr_attn_extend.hip -- attention of the new tokens of many sequences over the paged cache.
+//
+// One pass over the keys with each row's running maximum and sum, as in mr_attn_decode.hip. A sequence's rows are its
+// new tokens times the query heads that share a key head, token by token; a tile is some of them in a row, whatever
+// the number of heads.
+#include "mr_kv_operand.h"
+#include "mr_state_device.h"
+
+namespace mr {
+
+namespace {
+
+constexpr int kWaves = 4;
+constexpr uint32_t kSplitSeqs = 1024;      // with more sequences none is split: each workgroup looks through them all
+constexpr uint32_t kScratchRows = 65536;   // rows of partial results
+constexpr uint32_t kMinPart = kWaves;      // chunks of a part at least
+
+struct ExtendArgs {
+  KvPages kv;
+  Heads q, out;
+  const int32_t *cu, *len, *table;
+  uint32_t max_pages, n_seqs;
+  int nq;
+  Divisor group;       // query heads of a key head
+  int bits;            // log2 of a tile's rows
+  uint32_t parts;      // parts that the CUs hold at once; 1: none is split
+  AttnOpts o;
+  uint32_t* err;
+  float* part;         // [slot][key head][row][D] sums, then [slot][..][row][2] maximum and sum
+};
+
+// A sequence's rows and keys, in chunks.
+struct Span {
+  int q0, n, len;       // first row (token) of the call, new tokens, cached tokens
+  int c0, chunks;       // chunks that some row sees
+  uint32_t tiles;
+};
+__device__ __forceinline__ int first_seen(const ExtendArgs& a, int pos) {
+  return a.o.window && pos >= 0 && (uint32_t)pos >= a.o.window ? pos - (int)a.o.window + 1 : 0;
+}
+__device__ __forceinline__ Span span_of(const ExtendArgs& a, uint32_t b) {
+  Span s;
+  int q1;
+  rows_of(a.cu, a.nq, b, s.q0, q1);
+  s.n = q1 - s.q0;
+  const int64_t cap = (int64_t)a.max_pages << a.kv.page_shift;
+  s.len = (int)min(max((int64_t)a.len[b], (int64_t)0), cap);
+  s.c0 = first_seen(a, s.len - s.n) >> 6;
+  s.chunks = s.n && s.len ? ((s.len - 1) >> 6) + 1 - s.c0 : 0;
+  s.tiles = ((uint32_t)s.n * a.group.d + (1u << a.bits) - 1) >> a.bits;
+  return s;
+}
+
+// Unit `i`: a tile of a sequence and a part of its keys. split_only: tile i of the sequences of several parts, whose
+// part is then 0. slot: parts of split sequences in front of the tile's.
+struct Unit {
+  uint32_t b, tile, part, parts, slot;
+  Span sp;
+};
+__device__ __forceinline__ bool find_unit(const ExtendArgs& a, uint32_t i, bool split_only, Unit& r) {
+  const uint32_t lane = threadIdx.x & 63;
+  if (a.parts == 1) {
+    if (split_only) return false;
+    r.b = find_seq(a.cu, a.n_seqs, a.nq, a.group.d, a.bits, i);
+    r.sp = span_of(a, r.b);
+    const int64_t tile = (int64_t)i - first_tile(a.cu, a.nq, r.b, a.group.d, a.bits);
+    r.tile = (uint32_t)tile, r.part = 0, r.parts = 1, r.slot = 0;
+    return tile >= 0 && tile < (int64_t)r.sp.tiles;
+  }
+  Span s = lane < a.n_seqs ? span_of(a, lane) : Span{};
+  // f(tiles, chunks) of every sequence, summed
+  auto sum_of = [&](auto f) {
+    uint32_t v = lane < a.n_seqs ? f(s.tiles, (uint32_t)s.chunks) : 0;
+    for (uint32_t b0 = 64; b0 < a.n_seqs; b0 += 64)
+      if (b0 + lane < a.n_seqs) {
+        const Span x = span_of(a, b0 + lane);
+        v += f(x.tiles, (uint32_t)x.chunks);
+      }
+    return wave_total(v);
+  };
+  // The smallest size, in steps of an eighth, at which the CUs hold all parts at once.
+  const uint32_t all = sum_of([](uint32_t t, uint32_t c) { return t * c; }), tiles = sum_of([](uint32_t t, uint32_t) { return t; });
+  const uint32_t most = max(a.parts, tiles + a.parts / 2);
+  uint32_t size = max(kMinPart, (all + a.parts - 1) / a.parts);
+  while (size < all && sum_of([&](uint32_t t, uint32_t c) { return t * max(1u, (c + size - 1) / size); }) > most) size += (size + 7) / 8;
+  uint32_t before = 0, slots = 0;
+  for (uint32_t b0 = 0; b0 < a.n_seqs; b0 += 64) {
+    if (b0) s = b0 + lane < a.n_seqs ? span_of(a, b0 + lane) : Span{};
+    const uint32_t parts = max(1u, ((uint32_t)s.chunks + size - 1) / size), n = s.tiles * parts;
+    const uint32_t split = parts > 1 ? n : 0, count = split_only ? (parts > 1 ? s.tiles : 0) : n;
+    const uint32_t sum = wave_prefix(count), ssum = wave_prefix(split);
+    const uint64_t past = __ballot(before + sum > i);
+    if (past) {
+      const int l = __ffsll((unsigned long long)past) - 1;
+      r.b = b0 + l;
+      r.parts = __builtin_amdgcn_readlane(parts, l);
+      const uint32_t in = i - before - __builtin_amdgcn_readlane(sum - count, l);
+      r.tile = split_only ? in : in / r.parts;
+      r.part = split_only ? 0 : in - r.tile * r.parts;
+      r.slot = slots + __builtin_amdgcn_readlane(ssum - split, l) + r.tile * r.parts;
+      r.sp = Span{__builtin_amdgcn_readlane(s.q0, l), __builtin_amdgcn_readlane(s.n, l), __builtin_amdgcn_readlane(s.len, l),
+                  __builtin_amdgcn_readlane(s.c0, l), __builtin_amdgcn_readlane(s.chunks, l),
+                  (uint32_t)__builtin_amdgcn_readlane(s.tiles, l)};
+      return true;
+    }
+    before += __builtin_amdgcn_readlane(sum, 63);
+    slots += __builtin_amdgcn_readlane(ssum, 63);
+  }
+  return false;
+}
+
+// What a tile's rows see of the part's keys.
+struct Reach {
+  int r0, rows;          // first row and rows
+  int pos0, pos1;        // positions of the first and last row
+  int begin, end;        // chunks
+};
+__device__ __forceinline__ Reach reach_of(const ExtendArgs& a, const Unit& u) {
+  Reach t;
+  t.r0 = (int)(u.tile << a.bits);
+  t.rows = min(1 << a.bits, (int)((uint32_t)u.sp.n * a.group.d) - t.r0);
+  const int ahead = u.sp.len - u.sp.n;
+  t.pos0 = ahead + (int)a.group.of(t.r0), t.pos1 = ahead + (int)a.group.of(t.r0 + t.rows - 1);
+  const int c0 = first_seen(a, t.pos0) >> 6, chunks = t.pos1 < 0 ? 0 : (t.pos1 >> 6) + 1 - c0;
+  const int size = (chunks + (int)u.parts - 1) / (int)u.parts;
+  t.begin = c0 + min((int)u.part * size, chunks), t.end = c0 + min(((int)u.part + 1) * size, chunks);
+  return t;
+}
+
+template <int NT, int FMT, int D>
+constexpr int kPerSimd = NT * D >= 256 ? 1 : 2;
+
+// A tile of NT times 16 rows, the columns of the matrix products S = K Q^T and O = V^T P. A wave takes chunks of 64 tokens by
+// itself, operands straight from the pages.
+template <int NT, int FMT, int D>
+__global__ __launch_bounds__(64 * kWaves, (kPerSimd<NT, FMT, D>)) void k_attn_extend(ExtendArgs a) {
+  constexpr int ND = D / 16;
+  __shared__ __attribute__((aligned(16))) float sums[kWaves / 2][16 * D];
+  __shared__ float stats[kWaves / 2][16][2];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const uint32_t hk = blockIdx.y;
+  if (blockIdx.x == 0 && hk == 0) {
+    check_offsets(a.cu, a.n_seqs, a.nq, a.err, kErrOffset);
+    for (uint32_t s = threadIdx.x; s < a.n_seqs; s += blockDim.x)
+      if (a.len[s] < 0 || (int64_t)a.len[s] > (int64_t)a.max_pages << a.kv.page_shift) note_error(a.err, kErrLength);
+  }
+  Unit u;
+  if (!find_unit(a, blockIdx.x, false, u)) return;
+  const Reach t = reach_of(a, u);
+
+  // This lane's row of each 16: its place in q and out, and which keys it sees. The query as f16 times a power of
+  // two, its largest element in [2^14, 2^15): exact for f16, for bf16 all but what lies 2^-30 below the largest.
+  u32x4 qf[NT][D / 32];
+  float c[NT];
+  int pos[NT];
+  auto place = [&](int j, uint64_t& row, uint32_t& head) {
+    const uint32_t r = (uint32_t)(t.r0 + min(16 * j + n, t.rows - 1)), i = a.group.of(r);
+    row = (uint64_t)(u.sp.q0 + (int)i), head = hk * a.group.d + (r - i * a.group.d);
+    return u.sp.len - u.sp.n + (int)i;
+  };
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    uint64_t row;
+    uint32_t head;
+    pos[j] = place(j, row, head);
+    const uint64_t o = row * a.q.ts + (uint64_t)head * a.q.hs + g * (D / 4);
+    f32x4 x[D / 16];
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      x[i] = load4(a.q.p, a.q.dtype, o + 4 * i);
+      top = fmaxf(fmaxf(fmaxf(top, fabsf(x[i].x)), fmaxf(fabsf(x[i].y), fabsf(x[i].z))), fabsf(x[i].w));
+    }
+    top = max_xor16(max_xor32(top));
+    const int e = top > 0.f ? ilogbf(fminf(top, 3.0e38f)) - 14 : 0;
+    const float sign = a.o.scale < 0.f ? -1.f : 1.f;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      float y[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) y[k] = ldexpf(x[2 * i + (k >> 2)][k & 3], -e) * sign;
+      qf[j][i] = u32x4{pack_f16(y[0], y[1]), pack_f16(y[2], y[3]), pack_f16(y[4], y[5]), pack_f16(y[6], y[7])};
+    }
+    // above zero and finite: a masked score times c stays -inf, a score of zero zero
+    c[j] = fminf(fmaxf(ldexpf(fabsf(a.o.scale) * 1.44269504088896340736f, e), 0x1p-126f), kLargest);
+  }
+
+  f32x4 acc[NT][ND] = {};
+  float m[NT], l[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) m[j] = -INFINITY, l[j] = 0.f;
+  const int cpp = 1 << (a.kv.page_shift - 6);
+  auto page_of = [&](int chunk) -> int {
+    if (chunk >= t.end) return -1;
+    const int p = a.table[(uint64_t)u.b * a.max_pages + (uint32_t)(chunk >> (a.kv.page_shift - 6))];
+    if (p >= 0 && (uint32_t)p < a.kv.n_pages) return p;
+    note_error(a.err, kErrPage);
+    return -1;
+  };
+  Chunk<FMT, D> ch;
+  int pages = -1;
+  for (int i = 0, cidx = t.begin + wave; cidx < t.end; ++i, cidx += kWaves) {
+    if ((i & 63) == 0) pages = page_of(cidx + kWaves * lane);
+    const int page = __builtin_amdgcn_readlane(pages, i & 63);
+    const bool there = page >= 0;
+    const uint8_t* chunk = a.kv.at(there ? page : 0, hk, cidx & (cpp - 1));
+    ch.load_k(chunk, lane);
+    ch.load_v(chunk, lane, 0), ch.load_v(chunk, lane, 1);
+    f32x4 s[NT][4] = {};
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        const u32x4 k = ch.key(x, i);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) s[j][x] = mfma16(k, qf[j][i], s[j][x]);
+      }
+    const int k0 = cidx << 6;
+    // some row does not see some key
+    const bool edge = !there || k0 + 63 > t.pos0 || k0 < first_seen(a, t.pos1);
+    u32x4 pf[NT][2];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      if (edge) {
+        const int from = first_seen(a, pos[j]);
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const int key = k0 + 16 * x + 4 * g + y;
+            if (!there || key < from || key > pos[j]) s[j][x][y] = -INFINITY;
+          }
+      }
+      float top = s[j][0][0];
+#pragma unroll
+      for (int x = 0; x < 16; ++x) top = fmaxf(top, s[j][x >> 2][x & 3]);
+      top = max_xor16(max_xor32(top));
+      const float m1 = fmaxf(m[j], top);
+      if (__any(m1 > m[j])) {
+        const float f = m[j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m[j] - m1) * c[j]);
+        l[j] *= f;
+#pragma unroll
+        for (int x = 0; x < ND; ++x) acc[j][x] *= f;
+        m[j] = m1;
+      }
+      const float base = m[j] == -INFINITY ? 0.f : m[j];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        float p[4];
+#pragma unroll
+        for (int y = 0; y < 4; ++y) p[y] = __builtin_amdgcn_exp2f(fmaf(s[j][x][y] - base, c[j], kLift));
+        const uint32_t w0 = pack_f16(p[0], p[1]), w1 = pack_f16(p[2], p[3]);
+        pf[j][x >> 1][2 * (x & 1)] = w0, pf[j][x >> 1][2 * (x & 1) + 1] = w1;
+        l[j] = add_f16(w1, add_f16(w0, l[j]));
+      }
+    }
+#pragma unroll
+    for (int G = 0; G < 2; ++G)
+#pragma unroll
+      for (int b = 0; b < D / 32; ++b) {
+        u32x4 lo, hi;
+        ch.value(G, b, lo, hi);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          acc[j][2 * b] = mfma16(lo, pf[j][G], acc[j][2 * b]);
+          acc[j][2 * b + 1] = mfma16(hi, pf[j][G], acc[j][2 * b + 1]);
+        }
+      }
+  }
+
+  // The waves' results are joined in pairs, 16 rows after the other: (0, 2) and (1, 3), then (0, 1).
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    l[j] = add_xor16(add_xor32(l[j]));
+#pragma unroll
+    for (int w = kWaves / 2; w >= 1; w /= 2) {
+      if (wave >= w && wave < 2 * w) {
+#pragma unroll
+        for (int x = 0; x < ND; ++x) *reinterpret_cast<f32x4*>(&sums[wave - w][n * D + 16 * x + 4 * g]) = acc[j][x];
+        if (g == 0) stats[wave - w][n][0] = m[j], stats[wave - w][n][1] = l[j];
+      }
+      __syncthreads();
+      if (wave < w) {
+        const float m2 = stats[wave][n][0], l2 = stats[wave][n][1], m1 = fmaxf(m[j], m2);
+        const float f = m[j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m[j] - m1) * c[j]);
+        const float f2 = m2 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m2 - m1) * c[j]);
+#pragma unroll
+        for (int x = 0; x < ND; ++x)
+          acc[j][x] = acc[j][x] * f + *reinterpret_cast<const f32x4*>(&sums[wave][n * D + 16 * x + 4 * g]) * f2;
+        l[j] = l[j] * f + l2 * f2, m[j] = m1;
+      }
+      __syncthreads();
+    }
+  }
+  if (wave > 0) return;
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    if (16 * j + n >= t.rows) continue;
+    // What the weights are relative to, for sinks and other parts; its rounding is one of the score.
+    if (m[j] > -INFINITY) m[j] = fminf(fmaxf(m[j] * c[j], -kLargest), kLargest) - kLift;
+    if (u.parts > 1) {
+      const uint64_t unit = (((uint64_t)(u.slot + u.part) * a.kv.n_heads + hk) << a.bits) + 16 * j + n;
+      float* dst = a.part + unit * D;
+#pragma unroll
+      for (int x = 0; x < ND; ++x) *reinterpret_cast<f32x4*>(dst + 16 * x + 4 * g) = acc[j][x];
+      float* st = a.part + (uint64_t)kScratchRows * D + unit * 2;
+      if (g == 0) st[0] = m[j], st[1] = l[j];
+      continue;
+    }
+    uint64_t row;
+    uint32_t head;
+    place(j, row, head);
+    float f = 1.f;
+    const float sink = sink_of(a.o.sinks, head);
+    if (a.o.sinks) {
+      const float m1 = fmaxf(m[j], sink);
+      f = m[j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[j] - m1);
+      l[j] = l[j] * f + (sink == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sink - m1));
+    }
+    const float inv = l[j] == 0.f ? 0.f : 1.f / l[j];
+#pragma unroll
+    for (int x = 0; x < ND; ++x)
+      store4(a.out.p, a.out.dtype, row * a.out.ts + (uint64_t)head * a.out.hs + 16 * x + 4 * g, acc[j][x] * f * inv);
+  }
+}
+
+// Joins the parts of split tile blockIdx.x, a wave for each row: first all parts' weights, then the weighted sums.
+template <int D>
+__global__ __launch_bounds__(64 * kWaves) void k_extend_join(ExtendArgs a) {
+  constexpr int L = D / 4, G = 64 / L;  // lanes of a row, parts at a time
+  Unit u;
+  if (!find_unit(a, blockIdx.x, true, u)) return;
+  const Reach t = reach_of(a, u);
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const uint32_t hk = blockIdx.y;
+  const uint64_t apart = (uint64_t)a.kv.n_heads << a.bits;  // rows from a part to the next
+  for (int x = blockIdx.z * kWaves + wave; x < t.rows; x += gridDim.z * kWaves) {
+    const uint32_t r = (uint32_t)(t.r0 + x), i = a.group.of(r), head = hk * a.group.d + (r - i * a.group.d);
+    const uint64_t unit0 = (((uint64_t)u.slot * a.kv.n_heads + hk) << a.bits) + x;
+    const float* stat = a.part + (uint64_t)kScratchRows * D + 2 * unit0;
+    const float sink = sink_of(a.o.sinks, head);
+    float top = sink;
+    for (uint32_t p = lane; p < u.parts; p += 64) top = fmaxf(top, stat[2 * p * apart]);
+    float base = wave_max(top);
+    if (base == -INFINITY) base = 0.f;
+    float l = 0.f;
+    for (uint32_t p = lane; p < u.parts; p += 64) l += stat[2 * p * apart + 1] * __builtin_amdgcn_exp2f(stat[2 * p * apart] - base);
+    l = wave_sum_fast(l) + __builtin_amdgcn_exp2f(sink - base);
+    f32x4 acc = {};
+    const float* src = a.part + unit0 * D + 4 * (lane % L);
+#pragma unroll 4
+    for (uint32_t p = lane / L; p < u.parts; p += G)
+      acc += *reinterpret_cast<const f32x4*>(src + p * apart * D) * __builtin_amdgcn_exp2f(stat[2 * p * apart] - base);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (G >= 2) acc[j] = add_xor32(acc[j]);
+      if (G >= 4) acc[j] = add_xor16(acc[j]);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (lane < L)
+      store4(a.out.p, a.out.dtype, (uint64_t)(u.sp.q0 + (int)i) * a.out.ts + (uint64_t)head * a.out.hs + 4 * lane, acc * inv);
+  }
+}
+
+using ExtendKernel = void (*)(ExtendArgs);
+template <int NT, int FMT, int D>
+ExtendKernel pick(int& per_cu) {
+  static const int n = [] {
+    int v = 0;
+    return hipOccupancyMaxActiveBlocksPerMultiprocessor(&v, k_attn_extend<NT, FMT, D>, 64 * kWaves, 0) == hipSuccess && v > 0 ? v : 1;
+  }();
+  per_cu = n;
+  return k_attn_extend<NT, FMT, D>;
+}
+template <int FMT, int D>
+ExtendKernel pick(int& bits, int& per_cu) {
+  if (bits == 4) return pick<1, FMT, D>(per_cu);
+  if (bits == 5 || D == 256) return bits = 5, pick<2, FMT, D>(per_cu);
+  return pick<4, FMT, D == 256 ? 128 : D>(per_cu);
+}
+template <int FMT>
+ExtendKernel pick(uint32_t D, int& bits, int& per_cu) {
+  return D == 64 ? pick<FMT, 64>(bits, per_cu) : D == 128 ? pick<FMT, 128>(bits, per_cu) : pick<FMT, 256>(bits, per_cu);
+}
+
+}  // namespace
+
+uint64_t attn_extend_scratch_bytes() { return (uint64_t)kScratchRows * (256 + 2) * sizeof(float); }
+
+hipError_t launch_attn_extend(const Launch& K, const KvPages& kv, uint32_t format, uint32_t D, const Heads& q, uint32_t nq,
+                              uint32_t n_seqs, const int32_t* cu, const int32_t* len, const int32_t* table,
+                              uint32_t max_pages, const AttnOpts& o, const Heads& out, uint32_t* err, float* scratch,
+                              int n_cu) {
+  const uint32_t group = q.n / kv.n_heads;
+  const uint64_t rows = (uint64_t)nq * group;
+  int bits = rows <= 16ull * n_seqs ? 4 : rows <= 32ull * n_seqs ? 5 : 6, per_cu = 1;
+  const ExtendKernel kernel = format == MR_KV_F16      ? pick<MR_KV_F16>(D, bits, per_cu)
+                              : format == MR_KV_MXINT8 ? pick<MR_KV_MXINT8>(D, bits, per_cu)
+                                                       : pick<MR_KV_MXFP4>(D, bits, per_cu);
+  ExtendArgs a{kv, q, out, cu, len, table, max_pages, n_seqs, (int)nq, Divisor(group), bits, 0, o, err, scratch};
+  const uint64_t cap = (uint64_t)max_pages << (kv.page_shift - 6);
+  const uint64_t tiles = (rows >> bits) + n_seqs;  // at most
+  const uint32_t room = std::min<uint32_t>(kScratchRows >> bits, per_cu * n_cu);
+  // the chunks of all tiles are counted in 32 bits
+  const bool whole = cap <= 2 * kWaves || n_seqs > kSplitSeqs || tiles * cap >= 1ull << 31;
+  a.parts = whole ? 1 : std::max<uint32_t>(1, room / kv.n_heads);
+  hipError_t e;
+  {
+    ProfScope ps(K, "attn_extend");
+    const uint64_t units = a.parts > 1 ? std::max<uint64_t>(a.parts, tiles + a.parts / 2) : tiles;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)units, kv.n_heads), dim3(64 * kWaves), 0, K.s, a);
+    e = hipGetLastError();
+    if (e != hipSuccess || a.parts == 1) return e;
+  }
+  ProfScope ps(K, "extend_join");
+  const dim3 j((unsigned)std::min<uint64_t>(tiles, a.parts / 2 + 1), kv.n_heads, 4), blk(64 * kWaves);
+  if (D == 64) hipLaunchKernelGGL((k_extend_join<64>), j, blk, 0, K.s, a);
+  if (D == 128) hipLaunchKernelGGL((k_extend_join<128>), j, blk, 0, K.s, a);
+  if (D == 256) hipLaunchKernelGGL((k_extend_join<256>), j, blk, 0, K.s, a);
+  return hipGetLastError();
+}
+
+}  // namespace mr

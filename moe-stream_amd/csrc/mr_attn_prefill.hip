@@ -74,15 +74,6 @@ __device__ __forceinline__ void load_lds16(uint64_t base, uint32_t bytes, uint32
                : "memory", "m0");
 }
 
-// Division of x < 2^24 by 1 <= d < 2^24: with 2^b <= d < 2^(b + 1), x ceil(2^(39 + b) / d) has 64 bits, and over
-// 2^(39 + b) it is above x / d by less than x / 2^(39 + b) < 1 / d.
-struct Divisor {
-  uint64_t mul;
-  uint32_t d, shift;
-  explicit Divisor(uint32_t d) : d(d), shift(70 - __builtin_clz(d)) { mul = ((1ull << shift) + d - 1) / d; }
-  __device__ __forceinline__ uint32_t of(uint32_t x) const { return (uint32_t)((x * mul) >> shift); }
-};
-
 // x where bit `at` of `seen` is set, else -infinity.
 __device__ __forceinline__ float seen_or_least(float x, uint32_t seen, int at) {
   const uint32_t keep = (uint32_t)__builtin_amdgcn_sbfe((int)seen, (uint32_t)at, 1u);

@@ -16,7 +16,7 @@ namespace mr {
 constexpr uint32_t kMaxTopK = 16;        // softmax_topk_kernel limit (fused_ops.metal:150)
 constexpr uint32_t kMaxExperts = 512;    // same limit (fused_ops.metal:158)
 constexpr uint32_t kMaxHidden = 16384;   // LDS-staged activation limit of the VALU kernels
-constexpr int kAttnErrWords = 4;         // kinds of device index entries (mr_attn.h)
+constexpr int kAttnErrWords = 6;         // kinds of device index entries (mr_attn.h)
 // Size of the static scratch array of mr_moe_forward_batched_noalloc (one per GPU).
 constexpr uint64_t kStaticScratchBytes = MR_STATIC_SCRATCH_BYTES;
 
@@ -112,8 +112,10 @@ struct mr_ctx {
   // context in pinned host memory: mr_sync reads them without a copy. attn_err: their device address.
   uint32_t* attn_err_host = nullptr;
   uint32_t* attn_err = nullptr;
-  // Partial results of mr_attn_decode, of one size for all calls; allocated with the first cache.
+  // Partial results of mr_attn_decode and mr_attn_extend, of one size for all calls; allocated with the first cache.
   float* attn_scratch = nullptr;
+  // Workspace of mr_delta_rule, of one size for all calls; allocated with the first mr_delta.
+  void* delta_scratch = nullptr;
   hipEvent_t ev0 = nullptr, ev1 = nullptr;
   bool capturing = false;
   mr::Prof prof;

@@ -622,3 +622,4 @@ def exported_symbols() -> list[str]:
 from .attn import (BF16, F16, F32, KV_F16, KV_MXFP4, KV_MXINT8, ROPE_HALF, ROPE_INTERLEAVED,  # noqa: E402,F401
                    ROPE_LINEAR, ROPE_PLAIN, ROPE_YARN, ROPE_YARN_EXACT, Heads, KvCache, Rope, attn_prefill,
                    qk_norm_rope)
+from .state import DeltaRule, Rows, causal_conv  # noqa: E402,F401

@@ -128,6 +128,13 @@ class KvCache:
         self.ctx.check(_lib.mr_attn_decode(self.ctx.h, self.h, _heads(q), n_seqs, _ptr(seq_len), _ptr(block_table),
                                            max_pages, C.byref(o), _heads(out)))
 
+    def extend(self, q: Heads, n_q: int, n_seqs: int, cu_q, seq_len, block_table, max_pages: int, out: Heads, *,
+               scale: float = 0.0, window: int = 0, sinks=None) -> None:
+        """mr_attn_extend: the packed new tokens of each sequence over its cached tokens, themselves among them."""
+        o = _opts(scale, window, sinks)
+        self.ctx.check(_lib.mr_attn_extend(self.ctx.h, self.h, _heads(q), n_q, n_seqs, _ptr(cu_q), _ptr(seq_len),
+                                           _ptr(block_table), max_pages, C.byref(o), _heads(out)))
+
     def close(self) -> None:
         if self.h:
             _lib.mr_kv_destroy(self.h)

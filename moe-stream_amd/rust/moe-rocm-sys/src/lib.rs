@@ -12,6 +12,8 @@ use core::ffi::{c_char, c_int, c_void};
 
 /// include/moe_rocm_attn.h
 pub mod attn;
+/// include/moe_rocm_state.h
+pub mod state;
 
 // ---- status codes
 pub const MR_OK: c_int = 0;

@@ -1,0 +1,344 @@
+"""The operators over kept states on the GPU against plain 64-bit forms (attnref.py, stateref.py), at the lengths, strides, masks
+and index entries where they can go wrong. Tolerances are derived where they stand."""
+import numpy as np
+import pytest
+
+import moe_rocm as M
+
+import attnref as R
+import stateref as S
+from test_gpu_attn import FORMATS, TYPES, sync_error
+
+pytestmark = pytest.mark.gpu
+
+
+def offsets(counts, start=0):
+    return np.concatenate([[start], start + np.cumsum(counts)]).astype(np.int32)
+
+
+# ---- attention of new tokens over the cache ------------------------------------------------------
+class Cached:
+    """A cache with sequences of the given lengths in pages in any order, and what it holds of them."""
+
+    def __init__(self, ctx, fmt, page, hk, D, lens, rng, scale=1.0):
+        self.counts = [(n + page - 1) // page for n in lens]
+        n_pages = sum(self.counts) + 2
+        self.kv = M.KvCache(ctx, fmt, n_pages, page, hk, D)
+        order = rng.permutation(n_pages).astype(np.int32)
+        self.table = np.full((len(lens), max(1, max(self.counts, default=1))), -1, np.int32)  # unused entries: no page
+        self.k, self.v, at = [], [], 0
+        for i, n in enumerate(lens):
+            self.table[i, :self.counts[i]] = order[at:at + self.counts[i]]
+            at += self.counts[i]
+            k, v = rng.normal(size=(n, hk, D)).astype(np.float32) * scale, rng.normal(size=(n, hk, D)).astype(np.float32)
+            self.k.append(R.stored(k, fmt)), self.v.append(R.stored(v, fmt))
+            if n == 0:
+                continue
+            t = np.arange(n)
+            bk, bv = R.Rows(ctx, k, M.F32), R.Rows(ctx, v, M.F32)
+            slots = R.i32(ctx, self.table[i][t // page] * page + t % page)
+            self.kv.write(bk.heads, bv.heads, n, slots)
+            ctx.sync()
+            for b in (bk, bv, slots):
+                b.free()
+
+
+def extend_ref(q, cache, new, lens, scale, window, sinks, out_type, there=None):
+    """-> (rows, bound); weights are f16 (half a step of 2^-11), see attnref.attention_bound."""
+    T, hq, D = q.shape
+    y, tol = np.zeros(q.shape), np.zeros(q.shape)
+    at = 0
+    for s, n in enumerate(new):
+        hk = cache.k[s].shape[1]
+        for i in range(n):
+            pos = lens[s] - n + i
+            for h in range(hq):
+                first = max(0, pos - window + 1) if window else 0
+                k, v = cache.k[s][:, h // (hq // hk)], cache.v[s][:, h // (hq // hk)]
+                keep = np.arange(len(k))
+                if there is not None:
+                    keep = keep[there[s][:len(k)]]
+                sel = keep[(keep >= first) & (keep <= pos)]
+                a, size_v, size_s, seen = R.attend(q[at + i, h], k[sel], v[sel], scale, 0, len(sel) - 1,
+                                                   None if sinks is None else sinks[h])
+                y[at + i, h] = a
+                tol[at + i, h] = R.attention_bound(a, size_v, size_s, max(seen, 1), D, out_type, 2.0 ** -11)
+        at += n
+    return y, tol
+
+
+CASES = [
+    # D, key heads, heads of each, page, new tokens, lengths, window, sinks
+    (64, 2, 8, 64, [1], [1], 0, False),
+    (64, 1, 1, 64, [1, 1, 1], [1, 64, 65], 0, True),
+    (64, 2, 3, 128, [3, 0, 5, 1], [3, 10, 200, 0], 0, True),
+    (64, 2, 8, 64, [4, 1, 2], [700, 129, 2], 128, True),
+    (128, 2, 8, 64, [5, 2, 1, 7], [300, 2, 127, 193], 0, False),
+    (128, 1, 5, 256, [13, 1], [13, 1000], 100, False),
+    (128, 1, 16, 64, [9], [777], 0, True),
+    (256, 2, 4, 64, [3, 4], [70, 400], 0, True),
+    (256, 1, 8, 128, [1, 17], [600, 17], 33, False),
+    (64, 1, 64, 64, [2, 1], [90, 3], 0, False),
+    (128, 3, 1, 64, [40, 2], [150, 64], 0, True),
+    (64, 1, 4, 64, [5], [3], 0, True),            # more new tokens than cached ones: the first rows see nothing
+    (64, 2, 8, 64, [70, 1], [170, 500], 0, True),
+    (128, 1, 8, 64, [90], [91], 64, False),
+    (256, 1, 8, 64, [33, 1], [40, 200], 0, False),
+    (64, 1, 2, 64, [130], [1300], 1, False),      # only itself
+    (128, 1, 4, 64, [200, 3], [264, 320], 200, True),
+]
+
+
+@pytest.mark.parametrize("D,hk,group,page,new,lens,window,sinks", CASES)
+@pytest.mark.parametrize("fmt,kind", [("mxfp4", "bf16"), ("mxint8", "f16"), ("f16", "bf16")])
+def test_extend(gpu_ctx, D, hk, group, page, new, lens, window, sinks, fmt, kind):
+    rng = np.random.default_rng(D + sum(new) + sum(lens))
+    kind = TYPES[kind]
+    cache = Cached(gpu_ctx, FORMATS[fmt], page, hk, D, lens, rng)
+    T, hq = sum(new), hk * group
+    before, after = 2, 3  # rows in no sequence
+    q = R.rounded(rng.normal(size=(before + T + after, hq, D)), kind)
+    sk = rng.normal(size=hq).astype(np.float32) if sinks else None
+    bq, out = R.Rows(gpu_ctx, q, kind, pad=1, first=1), R.Rows(gpu_ctx, None, kind, before + T + after, hq, D, pad=2, first=1)
+    dev = [R.i32(gpu_ctx, a) for a in (offsets(new, before), lens, cache.table)]
+    ds = gpu_ctx.to_device(sk) if sinks else None
+    for _ in range(2):
+        cache.kv.extend(bq.heads, before + T + after, len(new), dev[0], dev[1], dev[2], cache.table.shape[1], out.heads,
+                        window=window, sinks=ds)
+        gpu_ctx.sync()
+        got = out.get()
+        y, tol = extend_ref(q[before:before + T], cache, new, lens, D ** -0.5, window, sk, kind)
+        assert (np.abs(got[before:before + T] - y) <= tol).all(), float((np.abs(got[before:before + T] - y) / tol).max())
+        mark = R.from_bits(np.array([out.mark]), kind)[0]
+        assert (got[:before] == mark).all() and (got[before + T:] == mark).all()
+    for b in (bq, out, *dev):
+        b.free()
+    if ds is not None:
+        ds.free()
+    cache.kv.close()
+
+
+def test_extend_of_single_tokens_is_decode(gpu_ctx):
+    rng = np.random.default_rng(3)
+    lens = [1, 0, 700, 1300, 64]
+    cache = Cached(gpu_ctx, M.KV_MXFP4, 64, 2, 128, lens, rng)
+    q = R.rounded(rng.normal(size=(5, 16, 128)), M.BF16)
+    bq, o1, o2 = R.Rows(gpu_ctx, q, M.BF16), R.Rows(gpu_ctx, None, M.BF16, 5, 16, 128), R.Rows(gpu_ctx, None, M.BF16, 5, 16, 128)
+    cu, dl, dt = (R.i32(gpu_ctx, a) for a in (offsets([1] * 5), lens, cache.table))
+    cache.kv.attend(bq.heads, 5, dl, dt, cache.table.shape[1], o1.heads)
+    cache.kv.extend(bq.heads, 5, 5, cu, dl, dt, cache.table.shape[1], o2.heads)
+    gpu_ctx.sync()
+    # the same sums in other orders: a step of the outputs' type at most
+    a, b = o1.get(), o2.get()
+    assert (np.abs(a - b) <= 2 * 2.0 ** -8 * np.abs(a) + 1e-6).all()
+    for x in (bq, o1, o2, cu, dl, dt):
+        x.free()
+    cache.kv.close()
+
+
+def test_extend_entries_out_of_range(gpu_ctx):
+    rng = np.random.default_rng(5)
+    lens, new = [200, 130], [4, 2]
+    cache = Cached(gpu_ctx, M.KV_MXINT8, 64, 1, 64, lens, rng)
+    q = R.rounded(rng.normal(size=(6, 4, 64)), M.BF16)
+    bq, out = R.Rows(gpu_ctx, q, M.BF16), R.Rows(gpu_ctx, None, M.BF16, 6, 4, 64)
+    mp = cache.table.shape[1]
+
+    def run(cu, ln, table):
+        dev = [R.i32(gpu_ctx, a) for a in (cu, ln, table)]
+        cache.kv.extend(bq.heads, 6, 2, *dev, mp, out.heads)
+        return dev
+
+    # a page that is not there: its tokens are left out
+    table = cache.table.copy()
+    table[0, 1] = 10 ** 6
+    dev = run(offsets(new), lens, table)
+    sync_error(gpu_ctx, "block_table")
+    there = [np.ones(200, bool), np.ones(130, bool)]
+    there[0][64:128] = False
+    y, tol = extend_ref(q, cache, new, lens, 0.125, 0, None, M.BF16, there)
+    assert (np.abs(out.get() - y) <= tol).all()
+    # a length beyond the table is the table's: the queries stand at its end, pages there are missing
+    dev += run(offsets(new), [10 ** 9, 130], cache.table)
+    sync_error(gpu_ctx, "seq_len")
+    # offsets out of range and out of order
+    for cu in ([0, 4, 9], [-3, 4, 6], [5, 2, 6]):
+        dev += run(np.array(cu, np.int32), lens, cache.table)
+        sync_error(gpu_ctx, "cu_q")
+    for b in (bq, out, *dev):
+        b.free()
+    cache.kv.close()
+
+
+# ---- causal convolution --------------------------------------------------------------------------
+@pytest.mark.parametrize("C_,new", [(8, [1]), (64, [1, 1, 1, 1, 1]), (520, [2, 0, 5, 1, 33]), (2056, [16, 17, 15, 4, 3]),
+                                    (4104, [100, 1]), (64, [0, 0, 3])])
+@pytest.mark.parametrize("taps,silu,bias,src,dst", [(4, True, False, "bf16", "bf16"), (4, False, True, "f32", "f32"),
+                                                    (3, True, True, "f16", "f32"), (2, True, False, "f32", "f16")])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_conv(gpu_ctx, C_, new, taps, silu, bias, src, dst, in_place):
+    rng = np.random.default_rng(C_ + taps)
+    src, dst, n = TYPES[src], TYPES[dst], len(new)
+    T, before, after, P = sum(new), 1, 2, taps - 1
+    x = R.rounded(rng.normal(size=(before + T + after, 1, C_)) * 2, src)
+    w = (rng.normal(size=(C_, taps)) / 2).astype(np.float32)
+    b = rng.normal(size=C_).astype(np.float32) if bias else None
+    states = rng.normal(size=(2 * n + 1, P, C_)).astype(np.float32)
+    source = rng.permutation(n).astype(np.int32)
+    source[n // 2] = -1
+    target = source.copy() if in_place else (np.arange(n) + n).astype(np.int32)
+    if not in_place:
+        target[n - 1] = -1
+    bx, out = R.Rows(gpu_ctx, x, src, pad=1), R.Rows(gpu_ctx, None, dst, before + T + after, 1, C_, pad=2)
+    dw, db, dst_states = gpu_ctx.to_device(w), gpu_ctx.to_device(b) if bias else None, gpu_ctx.to_device(states)
+    dev = [R.i32(gpu_ctx, a) for a in (offsets(new, before), source, target)]
+    M.causal_conv(gpu_ctx, M.Rows(bx.buf, C_, src, bx.width), dw, taps, before + T + after, n, dev[0],
+                  M.Rows(out.buf, C_, dst, out.width), bias=db, silu=silu, states=dst_states, n_slots=2 * n + 1,
+                  source=dev[1], target=dev[2])
+    gpu_ctx.sync()
+    got, kept = out.get()[:, 0], dst_states.download(np.float32).reshape(states.shape)
+    want, at = states.astype(np.float64).copy(), before
+    for s, m in enumerate(new):
+        old = states[source[s]] if source[s] >= 0 else np.zeros((P, C_))
+        y, off, last = S.conv(x[at:at + m, 0], w, b, silu, old)
+        tol = off + R.HALF[dst] * np.abs(y) * 1.01 * (dst != M.F32) + 2.0 ** -25 * (dst == M.F16)
+        assert (np.abs(got[at:at + m] - y) <= tol).all(), (s, float((np.abs(got[at:at + m] - y) / tol).max()))
+        if target[s] >= 0:
+            want[target[s]] = last
+        at += m
+    assert (kept == want).all()  # inputs, as they are
+    mark = R.from_bits(np.array([out.mark]), dst)[0]
+    assert (got[:before] == mark).all() and (got[before + T:] == mark).all()
+    for a in (bx, out, dw, dst_states, *dev):
+        a.free()
+    if bias:
+        db.free()
+
+
+# ---- gated delta rule ----------------------------------------------------------------------------
+class Delta:
+    """Inputs of a call, its device copies, and a run of it."""
+
+    def __init__(self, ctx, kh, vh, dk, dv, new, kind, raw, rng, states=None, strong=False):
+        self.ctx, self.kh, self.vh, self.dk, self.dv, self.new, self.kind, self.raw = ctx, kh, vh, dk, dv, new, kind, raw
+        T = self.T = sum(new) + 3
+        self.q, self.k = (R.rounded(rng.normal(size=(T, kh, dk)), kind) for _ in range(2))
+        self.v = R.rounded(rng.normal(size=(T, vh, dv)) * 2, kind)
+        self.a, self.b = (rng.normal(size=(T, vh + 2)).astype(np.float32) for _ in range(2))
+        self.a_log = rng.uniform(-1, 2, vh).astype(np.float32) if raw else None
+        self.dt_bias = rng.uniform(-4, 0, vh).astype(np.float32) if raw else None
+        self.eps = 1e-6 if raw else 0.0
+        if not raw:
+            self.a = -np.abs(self.a) * np.float32(20.0 if strong else 0.3)
+            self.b = (1 / (1 + np.exp(-self.b))).astype(np.float32)
+            self.q, self.k = (R.rounded(x / np.sqrt((x * x).sum(-1, keepdims=True)), kind) for x in (self.q, self.k))
+        n = len(new)
+        self.states = (rng.normal(size=(2 * n + 1, vh, dk, dv)) if states is None else states).astype(np.float32)
+        self.source = rng.permutation(n).astype(np.int32)
+        self.target = (np.arange(n) + n).astype(np.int32)
+
+    def run(self, in_place=False, start=1, cu=None, error=None):
+        c, n = self.ctx, len(self.new)
+        if in_place:
+            self.target = self.source.copy()
+        self.start = start
+        rows = [R.Rows(c, self.q, self.kind, pad=self.kh + self.vh, first=0), R.Rows(c, self.k, self.kind, pad=1, first=1),
+                R.Rows(c, self.v, self.kind), R.Rows(c, None, self.kind, self.T, self.vh, self.dv, pad=1, first=1)]
+        flat = [c.to_device(x) for x in (self.a, self.b, self.states)]
+        gate = [c.to_device(x) for x in (self.a_log, self.dt_bias)] if self.raw else [None, None]
+        dev = [R.i32(c, x) for x in (offsets(self.new, start) if cu is None else cu, self.source, self.target)]
+        rule = M.DeltaRule(c, self.kh, self.vh, self.dk, self.dv, unit_eps=self.eps, gate_stride=self.vh + 2, a_log=gate[0],
+                           dt_bias=gate[1])
+        rule.forward(rows[0].heads, rows[1].heads, rows[2].heads, flat[0], flat[1], self.T, n, dev[0], rows[3].heads,
+                     states=flat[2], n_slots=len(self.states), source=dev[1], target=dev[2])
+        if error:
+            sync_error(c, error)
+        else:
+            c.sync()
+        self.mark = R.from_bits(np.array([rows[3].mark]), self.kind)[0]
+        self.out, self.kept = rows[3].get(), flat[2].download(np.float32).reshape(self.states.shape)
+        rule.close()
+        for x in (*rows, *flat, *dev):
+            x.free()
+        for x in gate:
+            if x is not None:
+                x.free()
+
+    def check(self):
+        g, beta, g_off, b_off = S.gates(self.a[:, :self.vh], self.b[:, :self.vh], self.a_log, self.dt_bias)
+        want, bound, at = self.states.astype(np.float64), np.zeros(self.states.shape), self.start
+        half = R.HALF[self.kind]
+        for s, n in enumerate(self.new):
+            for h in range(self.vh):
+                hk = h // (self.vh // self.kh)
+                old = self.states[self.source[s], h] if self.source[s] >= 0 else np.zeros((self.dk, self.dv))
+                i = slice(at, at + n)
+                y, off, last, e = S.delta(self.q[i, hk], self.k[i, hk], self.v[i, h], g[i, h], beta[i, h], old, self.dk ** -0.5,
+                                          self.eps, g_off[i, h], b_off[i, h])
+                tol = off * (1 + half) + half * np.abs(y) * 1.01 + 2.0 ** -25 * (self.kind == M.F16)
+                d = np.abs(self.out[i, h] - y)
+                assert (d <= tol).all(), (s, h, n, float((d / tol).max()))
+                if self.target[s] >= 0:
+                    want[self.target[s], h], bound[self.target[s], h] = last, e + 1e-37
+            at += n
+        d = np.abs(self.kept - want)
+        assert (d <= bound).all(), float((d / np.maximum(bound, 1e-37)).max())
+        assert (self.out[:self.start] == self.mark).all() and (self.out[at:] == self.mark).all()
+        return float((d / np.maximum(bound, 1e-37)).max())
+
+
+LENGTHS = [[1], [1, 1, 1], [2, 0, 5, 1], [9, 17, 8], [64, 1, 65, 63], [130, 3], [128, 127], [200]]
+
+
+@pytest.mark.parametrize("new", LENGTHS)
+@pytest.mark.parametrize("kh,vh,dk,dv", [(1, 1, 128, 128), (2, 4, 128, 128), (1, 3, 64, 128), (2, 2, 128, 64), (1, 2, 64, 64)])
+@pytest.mark.parametrize("kind,raw", [("bf16", True), ("f16", False)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_delta(gpu_ctx, new, kh, vh, dk, dv, kind, raw, in_place):
+    rng = np.random.default_rng(sum(new) + 7 * dk + dv)
+    c = Delta(gpu_ctx, kh, vh, dk, dv, new, TYPES[kind], raw, rng)
+    c.source[len(new) // 2] = -1  # starts from zeros
+    c.run(in_place)
+    if not in_place and len(new) > 1:
+        assert (c.kept[:len(new)] == c.states[:len(new)]).all()  # the states before stay
+    c.check()
+
+
+@pytest.mark.parametrize("new", [[1, 3], [150, 70]])
+def test_delta_decays_of_any_size(gpu_ctx, new):
+    rng = np.random.default_rng(8)
+    c = Delta(gpu_ctx, 1, 2, 128, 128, new, M.BF16, False, rng, strong=True)
+    c.a[::5] = -np.inf  # forgets all
+    c.a[1::7] = -1000.0
+    c.a[2::9] = 0.0
+    c.b[3::11] = 0.0
+    c.b[4::11] = 1.0
+    c.run()
+    c.check()
+
+
+def test_delta_of_no_state(gpu_ctx):
+    """Without slots sequences start from zeros and nothing is kept."""
+    rng = np.random.default_rng(9)
+    c = Delta(gpu_ctx, 1, 1, 64, 64, [5, 100], M.F16, False, rng)
+    rows = [R.Rows(gpu_ctx, x, M.F16) for x in (c.q, c.k, c.v)] + [R.Rows(gpu_ctx, None, M.F16, c.T, 1, 64)]
+    a, b, cu = gpu_ctx.to_device(c.a), gpu_ctx.to_device(c.b), R.i32(gpu_ctx, offsets(c.new, 1))
+    rule = M.DeltaRule(gpu_ctx, 1, 1, 64, 64, gate_stride=3)
+    rule.forward(rows[0].heads, rows[1].heads, rows[2].heads, a, b, c.T, 2, cu, rows[3].heads)
+    gpu_ctx.sync()
+    c.out, c.kept, c.start, c.mark = rows[3].get(), c.states, 1, -7.5
+    c.source[:], c.target[:] = -1, -1
+    c.check()
+    rule.close()
+    for x in (*rows, a, b, cu):
+        x.free()
+
+
+def test_delta_slots_out_of_range(gpu_ctx):
+    rng = np.random.default_rng(10)
+    for new in ([2, 3], [90, 70]):
+        c = Delta(gpu_ctx, 1, 1, 64, 64, new, M.BF16, False, rng)
+        c.source[0], c.target[1] = 5, 10 ** 9  # 5 slots
+        c.run(error="source or target")
+        c.source[0], c.target[1] = -1, -1
+        c.check()
