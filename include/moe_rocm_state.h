@@ -65,7 +65,7 @@ int mr_causal_conv(mr_ctx* ctx, const mr_rows* x, const float* w, uint32_t taps,
 /* ---- gated delta rule (deltanet.rs:330-543) ------------------------------------------- */
 typedef struct mr_delta_desc {
   uint32_t n_key_heads;   /* heads of q and k */
-  uint32_t n_value_heads; /* a multiple; value head h goes with key head h / (value heads / key heads); up to 1024 */
+  uint32_t n_value_heads; /* a multiple; value head h goes with key head h / (value heads / key heads); up to 256 */
   uint32_t key_dim;       /* 64 or 128 */
   uint32_t value_dim;     /* 64 or 128 */
   float scale;            /* 0: 1 / sqrt(key_dim) */

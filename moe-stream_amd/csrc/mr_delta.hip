@@ -28,7 +28,7 @@ __device__ __forceinline__ void gates(const DeltaArgs& a, uint64_t t, uint32_t h
 // A state's rows lie across the lanes, four columns each; a thread has every G-th row. S'^T k and S'^T q are taken
 // together, as out = scale (S'^T q + (k . q) correction): one exchange between the lanes for each token.
 template <int DK, int DV, bool BF>
-__global__ __launch_bounds__(256) void k_delta_step(DeltaArgs a) {
+__global__ __launch_bounds__(256) void k_delta_step(DeltaArgs a, int most) {
   constexpr int L = DV / 4, G = 256 / L, N = DK / G, E = DK / 64;
   constexpr int kT = 8;  // tokens staged at once
   constexpr uint32_t kType = BF ? MR_BF16 : MR_F16;
@@ -41,7 +41,7 @@ __global__ __launch_bounds__(256) void k_delta_step(DeltaArgs a) {
   rows_of(sq.cu, sq.n_rows, s, q0, q1);
   const int n = q1 - q0;
   const int source = slot_of(sq, sq.source, s), target = slot_of(sq, sq.target, s);
-  if (n == 0 && (target < 0 || target == source)) return;
+  if (n > most || (n == 0 && (target < 0 || target == source))) return;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = tid / L, col = 4 * (tid % L);
 
   f32x4 S[N] = {};
@@ -111,27 +111,497 @@ __global__ __launch_bounds__(256) void k_delta_step(DeltaArgs a) {
   }
 }
 
+// ---- many tokens: chunks of 64 -------------------------------------------------------------
+// With G_i the sum of the chunk's log decays up to token i, S the state before it, and
+//   A_ij = beta_i k_i.k_j e^(G_i - G_j) for j < i,  T = (I + A)^-1,
+// the corrections of the chunk's tokens are V' = T beta (V - e^G K S), and
+//   out = scale (e^G Q S + P V'), P_ij = q_i.k_j e^(G_i - G_j) for j <= i;   S' = e^(G_63) S + (e^(G_63 - G) K)^T V'.
+// T and P do not need the state: k_delta_prepare works them out for all chunks at once; k_delta_chunks then goes
+// through a sequence's chunks, a workgroup for 16 columns of a head's state.
+//
+// States are held to 32 bits: S, T, V - K S and V' enter the 16-bit matrix instructions as sums of three bf16 parts (8 bits each),
+// in as many products as reach 2^-24; P, and S and V' for the outputs alone, as two. k and q are exact: themselves in bf16, or,
+// for f16, two bf16 parts.
+constexpr int kChunk = 64;
+
+typedef u32x4 Operand;  // 8 numbers of 16 bits of a lane: lane (m, g), row (or column) m, the 8 at 8 g of 32
+
+__device__ __forceinline__ f32x4 mfma_bf16(Operand a, Operand b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma_f16(Operand a, Operand b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// Four numbers as N sums of bf16 parts, the largest first.
+template <int N>
+__device__ __forceinline__ void split(f32x4 x, u32x2 (&part)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    part[i] = u32x2{pack_bf16(x.x, x.y), pack_bf16(x.z, x.w)};
+    if (i + 1 < N) {
+      const f32x2 a = unpack_bf16(part[i].x), b = unpack_bf16(part[i].y);
+      x -= f32x4{a.x, a.y, b.x, b.y};
+    }
+  }
+}
+
+// What k_delta_prepare leaves, in the order of the lanes that read it: operands of 1 KB.
+// A chunk's tokens 32 s + 4 g + r and 32 s + 16 + 4 g + r (r = 0..3) are, in turn, the 8 numbers of lane group g in step s of a sum
+// over tokens: what the lanes of a product's result hold of two tiles of 16.
+// The state's row 16 t + 4 g + r is the key's element 32 (t / 2) + 8 g + 4 (t % 2) + r: so the sums over a key's elements
+// read 8 adjacent ones.
+template <int DK, int NP>
+struct DeltaImage {
+  static constexpr int kT = 0;                // [tile and step][3 parts]: T beta
+  static constexpr int kP = 18 * 1024;        // [tile and step][2 parts]: scale P
+  static constexpr int kVec = 30 * 1024;      // f32: [64] of K S, [64] of Q S, [64] of V', [0] of S
+  static constexpr int kValue = 31 * 1024;    // bytes of a value head's chunk
+  static constexpr int kK = 0;                // [tile of tokens][step][NP]
+  static constexpr int kQ = DK / 8 * NP * 1024;
+  static constexpr int kKT = 2 * kQ;          // [tile of the state's rows][step][NP]
+  static constexpr int kKey = 3 * kQ;         // bytes of a key head's chunk
+  // Tile w of T and P needs the steps 0 .. w / 2.
+  static __device__ __forceinline__ int lower(int w, int s) { return w < 2 ? w : 2 * (w - 1) + s; }
+};
+
+struct ChunkArgs {
+  DeltaArgs a;
+  uint8_t *values, *keys;  // images [chunk][value head], [chunk][key head]
+  float* carry;            // [2][value head][state]: of the sequences that go on in the next launch
+  uint32_t first, last;    // chunks of this launch, by their numbers
+  int least;               // sequences of fewer tokens are not this path's
+};
+
+// Chunk number `at`: its sequence, and which of the sequence's chunks.
+__device__ __forceinline__ bool find_chunk(const ChunkArgs& c, uint32_t at, int& row, int& n) {
+  const Sequences& q = c.a.s;
+  const uint32_t s = find_seq(q.cu, q.n_seqs, q.n_rows, 1, 6, at);
+  int q0, q1;
+  rows_of(q.cu, q.n_rows, s, q0, q1);
+  const int64_t i = (int64_t)at - first_tile(q.cu, q.n_rows, s, 1, 6);
+  if (i < 0 || i * kChunk >= q1 - q0 || q1 - q0 < c.least) return false;
+  row = q0 + (int)i * kChunk, n = min(kChunk, q1 - row);
+  return true;
+}
+
+template <int DK, bool BF>
+__global__ __launch_bounds__(256) void k_delta_prepare(ChunkArgs c) {
+  constexpr int NP = BF ? 1 : 2, NS = DK / 32, kPad = 68;
+  using I = DeltaImage<DK, NP>;
+  __shared__ __attribute__((aligned(16))) float B[kChunk][kPad], W[kChunk][kPad];  // A^T and T^T
+  __shared__ __attribute__((aligned(16))) uint16_t kst[kChunk][DK + 8];
+  __shared__ float hi[kChunk], lo[kChunk], beta[kChunk], unit_k[kChunk], unit_q[kChunk];
+  __shared__ int bad[kChunk];
+  const DeltaArgs& a = c.a;
+  const uint32_t h = blockIdx.x, group = a.d.value_heads / a.d.key_heads, hk = h / group;
+  int row, n;
+  if (!find_chunk(c, c.first + blockIdx.y, row, n)) return;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+  uint8_t* image = c.values + ((uint64_t)blockIdx.y * a.d.value_heads + h) * I::kValue;
+  uint8_t* key_image = c.keys + ((uint64_t)blockIdx.y * a.d.key_heads + hk) * I::kKey;
+
+  // rows of keys and queries as operands, zeros behind the last
+  auto rows16 = [&](const Heads& x, int t, int s) {
+    const int i = 16 * t + m;
+    if (i >= n) return Operand{0, 0, 0, 0};
+    return *reinterpret_cast<const Operand*>(static_cast<const uint16_t*>(x.p) + (uint64_t)(row + i) * x.ts + (uint64_t)hk * x.hs + 32 * s + 8 * g);
+  };
+  auto squares = [&](const Operand (&x)[NS]) {
+    float v = 0.f;
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const f32x2 y = BF ? unpack_bf16(x[s][e]) : unpack_f16(x[s][e]);
+        v = fmaf(y.x, y.x, v), v = fmaf(y.y, y.y, v);
+      }
+    return add_xor16(add_xor32(v));
+  };
+  auto dot = [](Operand x, Operand y, f32x4 z) { return BF ? mfma_bf16(x, y, z) : mfma_f16(x, y, z); };
+  Operand kw[NS], qw[NS];
+#pragma unroll
+  for (int s = 0; s < NS; ++s) kw[s] = rows16(a.k, wave, s), qw[s] = rows16(a.q, wave, s);
+  {
+    const float kk = squares(kw), qq = squares(qw);
+    if (g == 0) {
+      unit_k[16 * wave + m] = a.d.unit_eps > 0.f ? 1.f / sqrtf(kk + a.d.unit_eps) : 1.f;
+      unit_q[16 * wave + m] = a.d.scale * (a.d.unit_eps > 0.f ? 1.f / sqrtf(qq + a.d.unit_eps) : 1.f);
+      bad[16 * wave + m] = !(kk < INFINITY);
+    }
+    if (h % group == 0) {
+#pragma unroll
+      for (int s = 0; s < NS; ++s) *reinterpret_cast<Operand*>(&kst[16 * wave + m][32 * s + 8 * g]) = kw[s];
+    }
+  }
+  __syncthreads();
+  if (wave == 0) {
+    // Sums of the decays in powers of two and 64 bits, kept as two numbers of 32: what two sums differ by is what counts. A token whose
+    // key, decay or beta is not finite counts as none here, and as NaN for all that comes after it.
+    float lg = 0.f, b = 0.f;
+    if (lane < n) gates(a, (uint64_t)(row + lane), h, lg, b);
+    const bool wrong = bad[lane] || !(lg < INFINITY) || !(fabsf(b) < INFINITY);
+    if (wrong) lg = 0.f, b = 0.f;
+    double sum = fmax((double)lg, -1e4) * 1.4426950408889634;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const double x = __shfl_up(sum, o, 64);
+      if (lane >= o) sum += x;
+    }
+    hi[lane] = (float)sum, lo[lane] = (float)(sum - (double)(float)sum), beta[lane] = b, bad[lane] = wrong;
+    const double end = __shfl(sum, 63, 64);
+    const float rise = __builtin_amdgcn_exp2f((float)sum), fall = __builtin_amdgcn_exp2f((float)(end - sum));
+    float* vec = reinterpret_cast<float*>(image + I::kVec);
+    vec[lane] = wrong ? NAN : rise * unit_k[lane];
+    vec[64 + lane] = rise * unit_q[lane];
+    vec[128 + lane] = fall * unit_k[lane];
+    if (lane == 0) vec[192] = __builtin_amdgcn_exp2f((float)end);
+  }
+  __syncthreads();
+  // Tiles of A^T and P^T: rows are the earlier tokens j, this wave's 16 tokens i the columns.
+  const int i = 16 * wave + m;
+  f32x4 pt[4] = {};
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    if (t > wave) break;
+    f32x4 kk = {}, qk = {};
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      const Operand k = t == wave ? kw[s] : rows16(a.k, t, s);
+      kk = dot(k, kw[s], kk), qk = dot(k, qw[s], qk);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int j = 16 * t + 4 * g + r;
+      const float decay = __builtin_amdgcn_exp2f((hi[i] - hi[j]) + (lo[i] - lo[j]));
+      const bool none = bad[i] || bad[j];
+      B[j][i] = j < i && !none ? kk[r] * unit_k[j] * unit_k[i] * beta[i] * decay : 0.f;
+      pt[t][r] = j <= i && !bad[j] ? qk[r] * unit_k[j] * unit_q[i] * decay : 0.f;
+    }
+  }
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    if (s > wave / 2) break;
+    u32x2 x[2], y[2];
+    split(pt[2 * s], x), split(pt[2 * s + 1], y);
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+      *reinterpret_cast<Operand*>(image + I::kP + (I::lower(wave, s) * 2 + p) * 1024 + lane * 16) = Operand{x[p].x, x[p].y, y[p].x, y[p].y};
+  }
+  __syncthreads();
+  // W = T^T = (I + B)^-1, B strictly upper: blocks of 16 on the diagonal column by column, from the last row up; then
+  // W_ji = -W_jj sum_(k = j + 1 .. i) B_jk W_ki, a diagonal of blocks after the other, in products of 32 bits.
+  {
+    float w[16];
+#pragma unroll
+    for (int r = 15; r >= 0; --r) {
+      float v = r == m ? 1.f : 0.f;
+#pragma unroll
+      for (int k = r + 1; k < 16; ++k) v = fmaf(-B[16 * wave + r][16 * wave + k], w[k], v);
+      w[r] = v;
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      if (g == r >> 2) W[16 * wave + r][i] = w[r];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int d = 1; d < 4; ++d) {
+    const int j = wave, e = wave + d;
+    if (e < 4) {
+      f32x4 y = {}, z = {};
+      for (int k = j + 1; k <= e; ++k) {
+        const f32x4 b = *reinterpret_cast<const f32x4*>(&B[16 * j + m][16 * k + 4 * g]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) y = __builtin_amdgcn_mfma_f32_16x16x4f32(b[r], W[16 * k + 4 * g + r][16 * e + m], y, 0, 0, 0);
+      }
+      const f32x4 b = *reinterpret_cast<const f32x4*>(&W[16 * j + m][16 * j + 4 * g]);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) z = __builtin_amdgcn_mfma_f32_16x16x4f32(b[r], y[r], z, 0, 0, 0);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) W[16 * j + 4 * g + r][16 * e + m] = -z[r];
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    if (s > wave / 2) break;
+    u32x2 part[2][3];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      f32x4 v = {};
+      if (2 * s + x <= wave) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int j = 32 * s + 16 * x + 4 * g + r;
+          v[r] = W[j][i] * beta[j];
+        }
+      }
+      split(v, part[x]);
+    }
+#pragma unroll
+    for (int p = 0; p < 3; ++p)
+      *reinterpret_cast<Operand*>(image + I::kT + (I::lower(wave, s) * 3 + p) * 1024 + lane * 16) =
+          Operand{part[0][p].x, part[0][p].y, part[1][p].x, part[1][p].y};
+  }
+  if (h % group) return;
+  // A key head's operands: f16 numbers as two bf16 ones.
+  auto put = [&](uint8_t* to, Operand x) {
+    if constexpr (BF) {
+      *reinterpret_cast<Operand*>(to + lane * 16) = x;
+    } else {
+      u32x2 part[2][2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const f32x2 y = unpack_f16(x[2 * e]), z = unpack_f16(x[2 * e + 1]);
+        split(f32x4{y.x, y.y, z.x, z.y}, part[e]);
+      }
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+        *reinterpret_cast<Operand*>(to + p * 1024 + lane * 16) = Operand{part[0][p].x, part[0][p].y, part[1][p].x, part[1][p].y};
+    }
+  };
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    put(key_image + I::kK + (wave * NS + s) * NP * 1024, kw[s]);
+    put(key_image + I::kQ + (wave * NS + s) * NP * 1024, qw[s]);
+  }
+  for (int t = wave; t < DK / 16; t += 4) {
+    const int e = 32 * (t >> 1) + 8 * (m >> 2) + 4 * (t & 1) + (m & 3);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      Operand x;
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const int j = 32 * s + 16 * (y >> 1) + 4 * g + 2 * (y & 1);
+        x[y] = (uint32_t)kst[j][e] | (uint32_t)kst[j + 1][e] << 16;
+      }
+      put(key_image + I::kKT + (t * 2 + s) * NP * 1024, x);
+    }
+  }
+}
+
+// A sequence's chunks for 16 columns of a head's state. Wave w has the tokens 16 w .. of a chunk, and of the state its tiles of 16
+// rows from w * (DK / 64) on. The state, V - K S and V' go round through LDS as operands.
+template <int DK, int NP, bool BF>
+__global__ __launch_bounds__(256) void k_delta_chunks(ChunkArgs c, uint32_t slices, int parity) {
+  constexpr int NS = DK / 32, NT = DK / 64;
+  constexpr uint32_t kType = BF ? MR_BF16 : MR_F16;
+  using I = DeltaImage<DK, NP>;
+  __shared__ __attribute__((aligned(16))) uint8_t state[NS][3][1024], rest[2][3][1024], fresh[2][2][1024], faded[2][3][1024];
+  __shared__ __attribute__((aligned(16))) int first_bad[16][4];
+  const DeltaArgs& a = c.a;
+  const Sequences& q = a.s;
+  const uint32_t h = blockIdx.x / slices, slice = blockIdx.x % slices, s = blockIdx.y;
+  const uint32_t hk = h / (a.d.value_heads / a.d.key_heads), DV = a.d.value_dim;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+  int q0, q1;
+  rows_of(q.cu, q.n_rows, s, q0, q1);
+  const int n = q1 - q0;
+  if (c.least == 0 && blockIdx.x == 0 && s == 0) check_offsets(q.cu, q.n_seqs, q.n_rows, q.err, kErrPacked);  // else k_delta_step has
+  if (n < c.least) return;
+  const uint32_t start = first_tile(q.cu, q.n_rows, s, 1, 6), count = (n + kChunk - 1) / kChunk;
+  const uint32_t end = start + max(count, 1u);  // a sequence without tokens takes part in one launch
+  if (end <= c.first || start >= c.last) return;
+  const int source = slot_of(q, q.source, s), target = slot_of(q, q.target, s);
+  const uint32_t col = 16 * slice + m;
+  // this lane's numbers of a state: rows 4 g + r of each of the wave's tiles, one column
+  auto at = [&](float* base, int t, int r) {
+    const int x = wave * NT + t;
+    return base + (uint64_t)(32 * (x >> 1) + 8 * g + 4 * (x & 1) + r) * DV + col;
+  };
+  const uint64_t state_size = (uint64_t)DK * DV;
+  float* carried = c.carry + ((uint64_t)(parity ^ 1) * a.d.value_heads + h) * state_size;
+  float* carry = c.carry + ((uint64_t)parity * a.d.value_heads + h) * state_size;
+  f32x4 S[NT] = {};
+  {
+    float* from = start < c.first ? carried : source >= 0 ? q.states + ((uint64_t)source * a.d.value_heads + h) * state_size : nullptr;
+    if (from)
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) S[t][r] = *at(from, t, r);
+  }
+  // The state's tiles 2 s and 2 s + 1 are step s of the sums over a key's elements.
+  auto publish = [&] {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      u32x2 part[3];
+      split(S[t], part);
+      const int x = wave * NT + t;
+#pragma unroll
+      for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x2*>(&state[x >> 1][p][lane * 16 + 8 * (x & 1)]) = part[p];
+    }
+  };
+  publish();
+  __syncthreads();
+  auto operand = [&](const uint8_t* p) { return *reinterpret_cast<const Operand*>(p + lane * 16); };
+  for (uint32_t at_chunk = max(start, c.first); at_chunk < min(start + count, c.last); ++at_chunk) {
+    const uint8_t* image = c.values + ((uint64_t)(at_chunk - c.first) * a.d.value_heads + h) * I::kValue;
+    const uint8_t* key_image = c.keys + ((uint64_t)(at_chunk - c.first) * a.d.key_heads + hk) * I::kKey;
+    const float* vec = reinterpret_cast<const float*>(image + I::kVec);
+    const int row = q0 + (int)(at_chunk - start) * kChunk, left = min(kChunk, q1 - row), t0 = 16 * wave + 4 * g;
+    // K S and Q S of this wave's tokens
+    f32x4 ks = {}, qs = {};
+#pragma unroll
+    for (int x = 0; x < NS; ++x) {
+      Operand S3[3];
+#pragma unroll
+      for (int p = 0; p < 3; ++p) S3[p] = operand(state[x][p]);
+#pragma unroll
+      for (int p = NP - 1; p >= 0; --p) {
+        const Operand k = operand(key_image + I::kK + ((wave * NS + x) * NP + p) * 1024);
+        const Operand y = operand(key_image + I::kQ + ((wave * NS + x) * NP + p) * 1024);
+#pragma unroll
+        for (int z = 2 - p; z >= 0; --z) ks = mfma_bf16(k, S3[z], ks);
+#pragma unroll
+        for (int z = 1 - p; z >= 0; --z) qs = mfma_bf16(y, S3[z], qs);
+      }
+    }
+    const f32x4 of_k = *reinterpret_cast<const f32x4*>(vec + t0), of_q = *reinterpret_cast<const f32x4*>(vec + 64 + t0),
+                of_v = *reinterpret_cast<const f32x4*>(vec + 128 + t0);
+    f32x4 R;
+    int bad = kChunk;
+#pragma unroll
+    for (int r = 3; r >= 0; --r) {
+      float v = 0.f;
+      if (t0 + r < left) {
+        const uint16_t x = static_cast<const uint16_t*>(a.v.p)[(uint64_t)(row + t0 + r) * a.v.ts + (uint64_t)h * a.v.hs + col];
+        v = BF ? bits_f32((uint32_t)x << 16) : h2f(x);
+      }
+      R[r] = fmaf(-of_k[r], ks[r], v);
+      // zeros take no part in the sums over tokens, but 0 times NaN would: the column's rows from here on are NaN at the end
+      if (!(fabsf(R[r]) < INFINITY)) bad = t0 + r, R[r] = 0.f;
+    }
+    bad = min(bad, __shfl_xor(bad, 16, 64));
+    bad = min(bad, __shfl_xor(bad, 32, 64));
+    if (g == 0) first_bad[m][wave] = bad;
+    const int half = lane * 16 + 8 * (wave & 1);  // the tile's half of its step
+    {
+      u32x2 part[3];
+      split(R, part);
+#pragma unroll
+      for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x2*>(&rest[wave >> 1][p][half]) = part[p];
+    }
+    __syncthreads();
+    const i32x4 bads = *reinterpret_cast<const i32x4*>(first_bad[m]);
+    const int first = min(min(bads.x, bads.y), min(bads.z, bads.w));
+    f32x4 V = {};
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      if (x > wave / 2) break;
+      Operand T[3], y[3];
+#pragma unroll
+      for (int p = 0; p < 3; ++p) T[p] = operand(image + I::kT + (I::lower(wave, x) * 3 + p) * 1024), y[p] = operand(rest[x][p]);
+#pragma unroll
+      for (int p = 2; p >= 0; --p)
+#pragma unroll
+        for (int z = 2 - p; z >= 0; --z) V = mfma_bf16(T[p], y[z], V);
+    }
+    {
+      u32x2 part[2], faint[3];
+      split(V, part), split(V * of_v, faint);
+#pragma unroll
+      for (int p = 0; p < 2; ++p) *reinterpret_cast<u32x2*>(&fresh[wave >> 1][p][half]) = part[p];
+#pragma unroll
+      for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x2*>(&faded[wave >> 1][p][half]) = faint[p];
+    }
+    __syncthreads();
+    f32x4 o = qs * of_q;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      if (x > wave / 2) break;
+      const Operand p0 = operand(image + I::kP + I::lower(wave, x) * 2048), p1 = operand(image + I::kP + I::lower(wave, x) * 2048 + 1024);
+      const Operand v0 = operand(fresh[x][0]), v1 = operand(fresh[x][1]);
+      o = mfma_bf16(p1, v0, o), o = mfma_bf16(p0, v1, o), o = mfma_bf16(p0, v0, o);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      if (t0 + r >= left) continue;
+      const float v = t0 + r >= first ? NAN : o[r];
+      static_cast<uint16_t*>(a.out.p)[(uint64_t)(row + t0 + r) * a.out.ts + (uint64_t)h * a.out.hs + col] =
+          (uint16_t)(kType == MR_BF16 ? pack_bf16(v, 0.f) : pack_f16(v, 0.f));
+    }
+    const float fade = first < kChunk ? NAN : vec[192];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      S[t] *= fade;
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int p = NP - 1; p >= 0; --p) {
+          const Operand k = operand(key_image + I::kKT + (((wave * NT + t) * 2 + x) * NP + p) * 1024);
+#pragma unroll
+          for (int z = 2 - p; z >= 0; --z) S[t] = mfma_bf16(k, operand(faded[x][z]), S[t]);
+        }
+    }
+    publish();
+    __syncthreads();
+  }
+  float* to = end > c.last ? carry : target >= 0 ? q.states + ((uint64_t)target * a.d.value_heads + h) * state_size : nullptr;
+  if (!to || (n == 0 && target == source)) return;
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) *at(to, t, r) = S[t][r];
+}
+
 template <int DK, int DV>
-void launch(const Launch& K, bool bf, const DeltaArgs& a) {
+void launch_step(const Launch& K, bool bf, const DeltaArgs& a, int most) {
   const dim3 g(a.d.value_heads, a.s.n_seqs), b(256);
-  hipLaunchKernelGGL((bf ? k_delta_step<DK, DV, true> : k_delta_step<DK, DV, false>), g, b, 0, K.s, a);
+  hipLaunchKernelGGL((bf ? k_delta_step<DK, DV, true> : k_delta_step<DK, DV, false>), g, b, 0, K.s, a, most);
+}
+
+// Sequences of up to so many tokens go through k_delta_step.
+constexpr int kStepTokens = 32;
+constexpr uint64_t kScratch = 256ull << 20;
+
+template <int DK, bool BF>
+hipError_t launch_chunks(const Launch& K, const DeltaArgs& a, int least, uint8_t* scratch) {
+  using I = DeltaImage<DK, BF ? 1 : 2>;
+  const uint32_t vh = a.d.value_heads, kh = a.d.key_heads, dv = a.d.value_dim;
+  const uint64_t carry = 2ull * vh * DK * dv * sizeof(float), chunk = (uint64_t)vh * I::kValue + (uint64_t)kh * I::kKey;
+  const uint32_t all = ((uint32_t)a.s.n_rows >> 6) + a.s.n_seqs, room = (uint32_t)std::min<uint64_t>((kScratch - carry) / chunk, 65535);
+  ChunkArgs c{a, nullptr, nullptr, reinterpret_cast<float*>(scratch), 0, 0, least};
+  int parity = 0;
+  for (c.first = 0; c.first < all; c.first = c.last, parity ^= 1) {
+    c.last = std::min(all, c.first + room);
+    c.values = scratch + carry;
+    c.keys = c.values + (uint64_t)(c.last - c.first) * vh * I::kValue;
+    {
+      ProfScope ps(K, "delta_prepare");
+      hipLaunchKernelGGL((k_delta_prepare<DK, BF>), dim3(vh, c.last - c.first), dim3(256), 0, K.s, c);
+    }
+    ProfScope ps(K, "delta_chunks");
+    hipLaunchKernelGGL((k_delta_chunks<DK, BF ? 1 : 2, BF>), dim3(vh * (dv / 16), a.s.n_seqs), dim3(256), 0, K.s, c, dv / 16, parity);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 }  // namespace
 
-uint64_t delta_scratch_bytes() { return 256; }
+uint64_t delta_scratch_bytes() { return kScratch; }
 
 hipError_t launch_delta_rule(const Launch& K, const DeltaShape& d, const Heads& q, const Heads& k, const Heads& v,
                              const float* decay, const float* beta, const Sequences& s, const Heads& out, void* scratch) {
-  (void)scratch;
   const DeltaArgs a{d, q, k, v, out, decay, beta, s};
   const bool bf = q.dtype == MR_BF16;
-  ProfScope ps(K, "delta_step");
-  if (d.key_dim == 64 && d.value_dim == 64) launch<64, 64>(K, bf, a);
-  if (d.key_dim == 64 && d.value_dim == 128) launch<64, 128>(K, bf, a);
-  if (d.key_dim == 128 && d.value_dim == 64) launch<128, 64>(K, bf, a);
-  if (d.key_dim == 128 && d.value_dim == 128) launch<128, 128>(K, bf, a);
-  return hipGetLastError();
+  const bool chunks = s.n_rows > kStepTokens, steps = !chunks || s.n_seqs > 1;  // one sequence takes one path
+  if (steps) {
+    ProfScope ps(K, "delta_step");
+    if (d.key_dim == 64 && d.value_dim == 64) launch_step<64, 64>(K, bf, a, kStepTokens);
+    if (d.key_dim == 64 && d.value_dim == 128) launch_step<64, 128>(K, bf, a, kStepTokens);
+    if (d.key_dim == 128 && d.value_dim == 64) launch_step<128, 64>(K, bf, a, kStepTokens);
+    if (d.key_dim == 128 && d.value_dim == 128) launch_step<128, 128>(K, bf, a, kStepTokens);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || !chunks) return e;
+  }
+  const int least = steps ? kStepTokens + 1 : 0;
+  uint8_t* w = static_cast<uint8_t*>(scratch);
+  if (d.key_dim == 64) return bf ? launch_chunks<64, true>(K, a, least, w) : launch_chunks<64, false>(K, a, least, w);
+  return bf ? launch_chunks<128, true>(K, a, least, w) : launch_chunks<128, false>(K, a, least, w);
 }
 
 }  // namespace mr

@@ -91,8 +91,8 @@ int mr_delta_create(mr_ctx* c, const mr_delta_desc* desc, mr_delta** out) {
   *out = nullptr;
   if (!desc) return fail(c, MR_E_INVAL, "delta description is NULL");
   mr_delta_desc d = *desc;
-  if (d.n_key_heads == 0 || d.n_value_heads == 0 || d.n_value_heads > 1024 || d.n_value_heads % d.n_key_heads)
-    return fail(c, MR_E_INVAL, "%u value heads do not share %u key heads evenly, or are not 1..1024", d.n_value_heads, d.n_key_heads);
+  if (d.n_key_heads == 0 || d.n_value_heads == 0 || d.n_value_heads > 256 || d.n_value_heads % d.n_key_heads)
+    return fail(c, MR_E_INVAL, "%u value heads do not share %u key heads evenly, or are not 1..256", d.n_value_heads, d.n_key_heads);
   if ((d.key_dim != 64 && d.key_dim != 128) || (d.value_dim != 64 && d.value_dim != 128))
     return fail(c, MR_E_UNSUPPORTED, "key_dim %u or value_dim %u is not 64 or 128", d.key_dim, d.value_dim);
   if (!std::isfinite(d.scale)) return fail(c, MR_E_INVAL, "scale is not finite");

@@ -342,3 +342,68 @@ def test_delta_slots_out_of_range(gpu_ctx):
         c.run(error="source or target")
         c.source[0], c.target[1] = -1, -1
         c.check()
+
+
+@pytest.mark.parametrize("what", ["value", "key", "beta", "decay", "query"])
+@pytest.mark.parametrize("at", [0, 20, 63, 64, 100])
+def test_delta_what_is_not_finite_reaches_no_earlier_token(gpu_ctx, what, at):
+    """A value that is not finite reaches its column from its token on, a key, decay or beta all columns, a query its row."""
+    rng = np.random.default_rng(at)
+    n, dv = 140, 64
+    c = Delta(gpu_ctx, 1, 2, 64, dv, [n], M.BF16, False, rng)
+    row = at + 1
+    clean = c.v.copy(), c.k.copy(), c.b.copy(), c.a.copy(), c.q.copy()
+    if what == "value":
+        c.v[row, 1, 5] = np.inf
+    if what == "key":
+        c.k[row, 0, 3] = np.nan
+    if what == "beta":
+        c.b[row, 1] = np.nan
+    if what == "decay":
+        c.a[row, 1] = np.inf
+    if what == "query":
+        c.q[row, 0, 9] = np.nan
+    c.run()
+    out, kept, target = c.out, c.kept, c.target
+    c.v, c.k, c.b, c.a, c.q = clean
+    c.run()
+    c.check()
+    hit = np.zeros(out.shape, bool)
+    if what == "value":
+        hit[row:n + 1, 1, 5] = True
+    if what == "key":
+        hit[row:n + 1] = True
+    if what in ("beta", "decay"):
+        hit[row:n + 1, 1] = True
+    if what == "query":
+        hit[row] = True
+    assert not np.isfinite(out[hit]).any()
+    assert (out[~hit] == c.out[~hit]).all()
+    assert not np.isfinite(kept[target[0]][hit[n].nonzero()[0][:1]]).all() if what in ("key", "beta", "decay") else True
+    if what == "query":
+        assert (kept == c.kept).all()
+    if what == "value":
+        assert not np.isfinite(kept[target[0], 1, :, 5]).any()
+        mask = np.ones((2, 64, dv), bool)
+        mask[1, :, 5] = False
+        assert (kept[target[0]][mask] == c.kept[target[0]][mask]).all()
+
+
+def test_delta_of_more_chunks_than_the_workspace_holds(gpu_ctx):
+    """256 heads of 128 leave room for about ten chunks at once: two sequences cross from one launch to the next."""
+    rng = np.random.default_rng(11)
+    new = [40, 1000, 3, 700, 65]
+    c = Delta(gpu_ctx, 256, 256, 128, 128, new, M.BF16, False, rng, states=np.zeros((11, 256, 128, 128)))
+    c.source[:] = -1
+    c.run()
+    heads = [0, 100, 255]
+    g, beta, g_off, b_off = S.gates(c.a[:, :256], c.b[:, :256], None, None)
+    at = 1
+    for s, n in enumerate(new):
+        for h in heads:
+            i = slice(at, at + n)
+            y, off, last, e = S.delta(c.q[i, h], c.k[i, h], c.v[i, h], g[i, h], beta[i, h], np.zeros((128, 128)), 128 ** -0.5, 0.0,
+                                      g_off[i, h], b_off[i, h])
+            assert (np.abs(c.out[i, h] - y) <= off * 1.01 + 2.0 ** -8 * np.abs(y)).all(), (s, h)
+            assert (np.abs(c.kept[c.target[s], h] - last) <= e + 1e-37).all(), (s, h)
+        at += n

@@ -114,7 +114,7 @@ def test_conv_refusals(hctx):  # noqa: F811
 
 @pytest.mark.parametrize("kw,status,text", [
     (dict(n_key_heads=0), M.MR_E_INVAL, "heads"), (dict(n_value_heads=0), M.MR_E_INVAL, "heads"),
-    (dict(n_value_heads=3), M.MR_E_INVAL, "evenly"), (dict(n_value_heads=1026), M.MR_E_INVAL, "1..1024"),
+    (dict(n_value_heads=3), M.MR_E_INVAL, "evenly"), (dict(n_value_heads=258), M.MR_E_INVAL, "1..256"),
     (dict(key_dim=96), M.MR_E_UNSUPPORTED, "key_dim"), (dict(value_dim=256), M.MR_E_UNSUPPORTED, "value_dim"),
     (dict(scale=math.nan), M.MR_E_INVAL, "scale"), (dict(unit_eps=-1.0), M.MR_E_INVAL, "unit_eps"),
     (dict(unit_eps=math.nan), M.MR_E_INVAL, "unit_eps"), (dict(gate_stride=3), M.MR_E_INVAL, "gate_stride"),
