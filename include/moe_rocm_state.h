@@ -84,7 +84,7 @@ void mr_delta_destroy(mr_delta* delta);
 /* For each value head, a state S [key_dim, value_dim] (f32, a slot is [n_value_heads, key_dim, value_dim]) and token t
  * with its key k, query q, value v, g = decay (a log: 0 or less, -infinity among them) and beta:
  *   S' = exp(g) S, S = S' + beta k (v - S'^T k)^T, out = scale S^T q.
- * q, k, v and out: F16 or BF16, all the same; decay, beta: f32 [tokens, value heads] with gate_stride. States, sums,
+ * q, k, v and out: F16 or BF16, all the same, token strides below 2^24 elements; decay, beta: f32 [tokens, value heads] with gate_stride. States, sums,
  * and all that the next state comes from are held to 32 bits or the like: products of more than a few tokens run on
  * 16-bit matrix instructions in three parts of 8 bits a number. out is rounded once. Decays above 0 (growth) are taken
  * as they are. n_tokens: up to 2^24 - 1; n_seqs: up to 65535. */

@@ -139,6 +139,7 @@ __device__ __forceinline__ void split(f32x4 x, u32x2 (&part)[N]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     part[i] = u32x2{pack_bf16(x.x, x.y), pack_bf16(x.z, x.w)};
+    asm("" : "+v"(part[i]));  // taken apart again below, not rounded anew
     if (i + 1 < N) {
       const f32x2 a = unpack_bf16(part[i].x), b = unpack_bf16(part[i].y);
       x -= f32x4{a.x, a.y, b.x, b.y};
@@ -384,15 +385,17 @@ __global__ __launch_bounds__(256) void k_delta_prepare(ChunkArgs c) {
 // A sequence's chunks for 16 columns of a head's state. Wave w has the tokens 16 w .. of a chunk, and of the state its tiles of 16
 // rows from w * (DK / 64) on. The state, V - K S and V' go round through LDS as operands.
 template <int DK, int NP, bool BF>
-__global__ __launch_bounds__(256) void k_delta_chunks(ChunkArgs c, uint32_t slices, int parity) {
+__global__ __launch_bounds__(256, 2) void k_delta_chunks(ChunkArgs c, uint32_t slices, int parity) {
   constexpr int NS = DK / 32, NT = DK / 64;
   constexpr uint32_t kType = BF ? MR_BF16 : MR_F16;
   using I = DeltaImage<DK, NP>;
   __shared__ __attribute__((aligned(16))) uint8_t state[NS][3][1024], rest[2][3][1024], fresh[2][2][1024], faded[2][3][1024];
-  __shared__ __attribute__((aligned(16))) int first_bad[16][4];
+  __shared__ __attribute__((aligned(16))) int first_bad[4][16], any_bad[4];
   const DeltaArgs& a = c.a;
   const Sequences& q = a.s;
-  const uint32_t h = blockIdx.x / slices, slice = blockIdx.x % slices, s = blockIdx.y;
+  // Workgroups go to the 8 XCDs in turn: the slices of a head, which read the same operands, to one of them.
+  const uint32_t unit = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3), h = unit / slices, slice = unit % slices, s = blockIdx.y;
+  if (h >= c.a.d.value_heads) return;
   const uint32_t hk = h / (a.d.value_heads / a.d.key_heads), DV = a.d.value_dim;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
   int q0, q1;
@@ -434,48 +437,100 @@ __global__ __launch_bounds__(256) void k_delta_chunks(ChunkArgs c, uint32_t slic
     }
   };
   publish();
-  __syncthreads();
   auto operand = [&](const uint8_t* p) { return *reinterpret_cast<const Operand*>(p + lane * 16); };
-  for (uint32_t at_chunk = max(start, c.first); at_chunk < min(start + count, c.last); ++at_chunk) {
-    const uint8_t* image = c.values + ((uint64_t)(at_chunk - c.first) * a.d.value_heads + h) * I::kValue;
-    const uint8_t* key_image = c.keys + ((uint64_t)(at_chunk - c.first) * a.d.key_heads + hk) * I::kKey;
-    const float* vec = reinterpret_cast<const float*>(image + I::kVec);
-    const int row = q0 + (int)(at_chunk - start) * kChunk, left = min(kChunk, q1 - row), t0 = 16 * wave + 4 * g;
-    // K S and Q S of this wave's tokens
-    f32x4 ks = {}, qs = {};
+  // The operands of a chunk are on their way while the chunk before is worked on: each part is asked for as soon as its
+  // registers have been read.
+  const uint32_t begin = max(start, c.first), stop = min(start + count, c.last);
+  const uint64_t value_step = (uint64_t)a.d.value_heads * I::kValue, key_step = (uint64_t)a.d.key_heads * I::kKey;
+  const uint8_t* image = c.values + (uint64_t)(begin - c.first) * value_step + (uint64_t)h * I::kValue;
+  const uint8_t* key_image = c.keys + (uint64_t)(begin - c.first) * key_step + (uint64_t)hk * I::kKey;
+  const int t0 = 16 * wave + 4 * g;
+  Operand K[NS][NP], Q[NS][NP], T[2][3], P[2][2], KT[NT][2][NP];
+  f32x4 of_k, of_q, of_v;
+  float fade;
+  uint16_t vals[4];
+  auto load_keys = [&] {
+#pragma unroll
+    for (int x = 0; x < NS; ++x)
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        K[x][p] = operand(key_image + I::kK + ((wave * NS + x) * NP + p) * 1024);
+        Q[x][p] = operand(key_image + I::kQ + ((wave * NS + x) * NP + p) * 1024);
+      }
+  };
+  const int t_ld = (int)a.v.ts * 2, o_ld = (int)a.out.ts * 2;  // bytes from a token to the next
+  auto load_rest = [&](int row) {
+    const float* vec = reinterpret_cast<const float*>(image + I::kVec) + t0;
+    of_k = *reinterpret_cast<const f32x4*>(vec), of_q = *reinterpret_cast<const f32x4*>(vec + 64);
+    of_v = *reinterpret_cast<const f32x4*>(vec + 128);
+    const uint8_t* v = static_cast<const uint8_t*>(a.v.p) + ((uint64_t)row * a.v.ts + (uint64_t)h * a.v.hs + 16 * slice) * 2;
+    const int last = q1 - 1 - row;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) vals[r] = *reinterpret_cast<const uint16_t*>(v + (uint32_t)(min(t0 + r, last) * t_ld + 2 * m));
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int p = 0; p < 3; ++p) T[x][p] = operand(image + I::kT + (I::lower(wave, min(x, wave / 2)) * 3 + p) * 1024);
+  };
+  auto load_mix = [&] {
+    fade = reinterpret_cast<const float*>(image + I::kVec)[192];
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int p = 0; p < 2; ++p) P[x][p] = operand(image + I::kP + (I::lower(wave, min(x, wave / 2)) * 2 + p) * 1024);
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int p = 0; p < NP; ++p) KT[t][x][p] = operand(key_image + I::kKT + (((wave * NT + t) * 2 + x) * NP + p) * 1024);
+  };
+  int row = q0 + (int)(begin - start) * kChunk;
+  if (begin < stop) load_keys(), load_rest(row), load_mix();
+  __syncthreads();
+  for (uint32_t chunk = begin; chunk < stop; ++chunk, row += kChunk) {
+    const int left = min(kChunk, q1 - row);
+    // The last chunk loads itself again: a wait for one load must know how many others there are behind it.
+    const bool more = chunk + 1 < stop;
+    const uint64_t value_next = more ? value_step : 0, key_next = more ? key_step : 0;
+    // K S and Q S of this wave's tokens; sums of products of like size, so that they do not wait for each other
+    f32x4 ks[3] = {}, qs[2] = {};
 #pragma unroll
     for (int x = 0; x < NS; ++x) {
       Operand S3[3];
 #pragma unroll
       for (int p = 0; p < 3; ++p) S3[p] = operand(state[x][p]);
 #pragma unroll
-      for (int p = NP - 1; p >= 0; --p) {
-        const Operand k = operand(key_image + I::kK + ((wave * NS + x) * NP + p) * 1024);
-        const Operand y = operand(key_image + I::kQ + ((wave * NS + x) * NP + p) * 1024);
+      for (int p = 0; p < NP; ++p) {
 #pragma unroll
-        for (int z = 2 - p; z >= 0; --z) ks = mfma_bf16(k, S3[z], ks);
+        for (int z = 0; z + p < 3; ++z) ks[z + p] = mfma_bf16(K[x][p], S3[z], ks[z + p]);
 #pragma unroll
-        for (int z = 1 - p; z >= 0; --z) qs = mfma_bf16(y, S3[z], qs);
+        for (int z = 0; z + p < 2; ++z) qs[z + p] = mfma_bf16(Q[x][p], S3[z], qs[z + p]);
       }
     }
-    const f32x4 of_k = *reinterpret_cast<const f32x4*>(vec + t0), of_q = *reinterpret_cast<const f32x4*>(vec + 64 + t0),
-                of_v = *reinterpret_cast<const f32x4*>(vec + 128 + t0);
-    f32x4 R;
-    int bad = kChunk;
+    key_image += key_next;
+    load_keys();
+    f32x4 R = (ks[2] + ks[1]) + ks[0], o = (qs[1] + qs[0]) * of_q;
+    bool wrong = false;
 #pragma unroll
-    for (int r = 3; r >= 0; --r) {
-      float v = 0.f;
-      if (t0 + r < left) {
-        const uint16_t x = static_cast<const uint16_t*>(a.v.p)[(uint64_t)(row + t0 + r) * a.v.ts + (uint64_t)h * a.v.hs + col];
-        v = BF ? bits_f32((uint32_t)x << 16) : h2f(x);
-      }
-      R[r] = fmaf(-of_k[r], ks[r], v);
-      // zeros take no part in the sums over tokens, but 0 times NaN would: the column's rows from here on are NaN at the end
-      if (!(fabsf(R[r]) < INFINITY)) bad = t0 + r, R[r] = 0.f;
+    for (int r = 0; r < 4; ++r) {
+      const float v = t0 + r < left ? (BF ? bits_f32((uint32_t)vals[r] << 16) : (float)__builtin_bit_cast(_Float16, vals[r])) : 0.f;
+      R[r] = fmaf(-of_k[r], R[r], v);
+      wrong |= !(fabsf(R[r]) < INFINITY);
     }
-    bad = min(bad, __shfl_xor(bad, 16, 64));
-    bad = min(bad, __shfl_xor(bad, 32, 64));
-    if (g == 0) first_bad[m][wave] = bad;
+    const bool any = __any(wrong);
+    if (any) {
+      // NaN would reach earlier tokens by the zeros it is multiplied with: it is taken out, and the column's tokens from here
+      // on are NaN at the end
+      int bad = kChunk;
+#pragma unroll
+      for (int r = 3; r >= 0; --r)
+        if (!(fabsf(R[r]) < INFINITY)) bad = t0 + r, R[r] = 0.f;
+      bad = min(bad, __shfl_xor(bad, 16, 64));
+      bad = min(bad, __shfl_xor(bad, 32, 64));
+      if (g == 0) first_bad[wave][m] = bad;
+    }
+    if (lane == 0) any_bad[wave] = any;
     const int half = lane * 16 + 8 * (wave & 1);  // the tile's half of its step
     {
       u32x2 part[3];
@@ -484,19 +539,28 @@ __global__ __launch_bounds__(256) void k_delta_chunks(ChunkArgs c, uint32_t slic
       for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x2*>(&rest[wave >> 1][p][half]) = part[p];
     }
     __syncthreads();
-    const i32x4 bads = *reinterpret_cast<const i32x4*>(first_bad[m]);
-    const int first = min(min(bads.x, bads.y), min(bads.z, bads.w));
-    f32x4 V = {};
+    const i32x4 bads = *reinterpret_cast<const i32x4*>(any_bad);
+    int first = kChunk;
+    if (__builtin_amdgcn_readfirstlane(bads.x | bads.y | bads.z | bads.w)) {
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      if (x > wave / 2) break;
-      Operand T[3], y[3];
+      for (int w = 0; w < 4; ++w)
+        if (bads[w]) first = min(first, first_bad[w][m]);
+    }
+    f32x4 V;
+    {
+      f32x4 sum[3] = {};
 #pragma unroll
-      for (int p = 0; p < 3; ++p) T[p] = operand(image + I::kT + (I::lower(wave, x) * 3 + p) * 1024), y[p] = operand(rest[x][p]);
+      for (int x = 0; x < 2; ++x) {
+        if (x > wave / 2) break;
+        Operand y[3];
 #pragma unroll
-      for (int p = 2; p >= 0; --p)
+        for (int p = 0; p < 3; ++p) y[p] = operand(rest[x][p]);
 #pragma unroll
-        for (int z = 2 - p; z >= 0; --z) V = mfma_bf16(T[p], y[z], V);
+        for (int p = 0; p < 3; ++p)
+#pragma unroll
+          for (int z = 0; z + p < 3; ++z) sum[z + p] = mfma_bf16(T[x][p], y[z], sum[z + p]);
+      }
+      V = (sum[2] + sum[1]) + sum[0];
     }
     {
       u32x2 part[2], faint[3];
@@ -506,36 +570,42 @@ __global__ __launch_bounds__(256) void k_delta_chunks(ChunkArgs c, uint32_t slic
 #pragma unroll
       for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x2*>(&faded[wave >> 1][p][half]) = faint[p];
     }
+    image += value_next;
+    load_rest(row + (more ? kChunk : 0));
     __syncthreads();
-    f32x4 o = qs * of_q;
+    const float keep = first < kChunk ? NAN : fade;
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      if (x > wave / 2) break;
-      const Operand p0 = operand(image + I::kP + I::lower(wave, x) * 2048), p1 = operand(image + I::kP + I::lower(wave, x) * 2048 + 1024);
-      const Operand v0 = operand(fresh[x][0]), v1 = operand(fresh[x][1]);
-      o = mfma_bf16(p1, v0, o), o = mfma_bf16(p0, v1, o), o = mfma_bf16(p0, v0, o);
+    for (int t = 0; t < NT; ++t) {
+      f32x4 sum[3] = {};
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+#pragma unroll
+          for (int z = 0; z + p < 3; ++z) sum[z + p] = mfma_bf16(KT[t][x][p], operand(faded[x][z]), sum[z + p]);
+      S[t] = S[t] * keep + ((sum[2] + sum[1]) + sum[0]);
     }
+    publish();
+    {
+      f32x4 sum[2] = {};
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        if (x > wave / 2) break;
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+#pragma unroll
+          for (int z = 0; z + p < 2; ++z) sum[z + p] = mfma_bf16(P[x][p], operand(fresh[x][z]), sum[z + p]);
+      }
+      o += sum[1] + sum[0];
+    }
+    load_mix();
+    uint8_t* out = static_cast<uint8_t*>(a.out.p) + ((uint64_t)row * a.out.ts + (uint64_t)h * a.out.hs + 16 * slice) * 2;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       if (t0 + r >= left) continue;
       const float v = t0 + r >= first ? NAN : o[r];
-      static_cast<uint16_t*>(a.out.p)[(uint64_t)(row + t0 + r) * a.out.ts + (uint64_t)h * a.out.hs + col] =
-          (uint16_t)(kType == MR_BF16 ? pack_bf16(v, 0.f) : pack_f16(v, 0.f));
+      *reinterpret_cast<uint16_t*>(out + (uint32_t)((t0 + r) * o_ld + 2 * m)) = (uint16_t)(kType == MR_BF16 ? pack_bf16(v, 0.f) : pack_f16(v, 0.f));
     }
-    const float fade = first < kChunk ? NAN : vec[192];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      S[t] *= fade;
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int p = NP - 1; p >= 0; --p) {
-          const Operand k = operand(key_image + I::kKT + (((wave * NT + t) * 2 + x) * NP + p) * 1024);
-#pragma unroll
-          for (int z = 2 - p; z >= 0; --z) S[t] = mfma_bf16(k, operand(faded[x][z]), S[t]);
-        }
-    }
-    publish();
     __syncthreads();
   }
   float* to = end > c.last ? carry : target >= 0 ? q.states + ((uint64_t)target * a.d.value_heads + h) * state_size : nullptr;
@@ -573,7 +643,7 @@ hipError_t launch_chunks(const Launch& K, const DeltaArgs& a, int least, uint8_t
       hipLaunchKernelGGL((k_delta_prepare<DK, BF>), dim3(vh, c.last - c.first), dim3(256), 0, K.s, c);
     }
     ProfScope ps(K, "delta_chunks");
-    hipLaunchKernelGGL((k_delta_chunks<DK, BF ? 1 : 2, BF>), dim3(vh * (dv / 16), a.s.n_seqs), dim3(256), 0, K.s, c, dv / 16, parity);
+    hipLaunchKernelGGL((k_delta_chunks<DK, BF ? 1 : 2, BF>), dim3((vh * (dv / 16) + 7) / 8 * 8, a.s.n_seqs), dim3(256), 0, K.s, c, dv / 16, parity);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }

@@ -137,6 +137,8 @@ int mr_delta_rule(mr_ctx* c, const mr_delta* r, const mr_heads* q, const mr_head
   if (hq.n != d.n_key_heads || hk.n != d.n_key_heads || hv.n != d.n_value_heads || ho.n != d.n_value_heads)
     return fail(c, MR_E_INVAL, "heads of q, k, v and out are %u, %u, %u, %u, not %u, %u, %u, %u", hq.n, hk.n, hv.n, ho.n,
                 d.n_key_heads, d.n_key_heads, d.n_value_heads, d.n_value_heads);
+  for (const mr::Heads* x : {&hq, &hk, &hv, &ho})  // 64 rows within 32-bit offsets
+    if (x->ts >= 1ull << 24) return fail(c, MR_E_INVAL, "q, k, v or out has a token stride of 2^24 elements or more");
   if (!decay || !beta || misaligned(decay, 4) || misaligned(beta, 4))
     return fail(c, MR_E_INVAL, "decay or beta is NULL or not 4-byte aligned");
   if ((rc = take_sequences(c, n_tokens, n_seqs, cu, states, n_slots, source, target, &s))) return rc;

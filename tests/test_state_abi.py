@@ -141,7 +141,8 @@ def test_delta_refusals(hctx):  # noqa: F811
             (dict(out=None), M.MR_E_INVAL, "out is NULL"), (dict(q=M.Heads(X, 2)), M.MR_E_UNSUPPORTED, "F16"),
             (dict(k=M.Heads(X, 2, M.BF16)), M.MR_E_UNSUPPORTED, "F16"), (dict(out=M.Heads(X, 4, M.BF16)), M.MR_E_UNSUPPORTED, "F16"),
             (dict(q=M.Heads(X, 4, M.F16)), M.MR_E_INVAL, "heads"), (dict(v=M.Heads(X, 2, M.F16)), M.MR_E_INVAL, "heads"),
-            (dict(v=M.Heads(X, 4, M.F16, token_stride=4)), M.MR_E_INVAL, "stride"), (dict(decay=None), M.MR_E_INVAL, "decay"),
+            (dict(v=M.Heads(X, 4, M.F16, token_stride=4)), M.MR_E_INVAL, "stride"),
+            (dict(k=M.Heads(X, 2, M.F16, token_stride=1 << 24)), M.MR_E_INVAL, "2^24"), (dict(decay=None), M.MR_E_INVAL, "decay"),
             (dict(beta=X + 2), M.MR_E_INVAL, "beta"), (dict(cu=None), M.MR_E_INVAL, "cu"), (dict(n=1 << 24), M.MR_E_INVAL, "n_tokens"),
             (dict(seqs=65536), M.MR_E_INVAL, "n_seqs"), (dict(states=None), M.MR_E_INVAL, "states"),
             (dict(source=X + 2), M.MR_E_INVAL, "source"), (dict(n_slots=1 << 31), M.MR_E_INVAL, "slots")):
