@@ -3,6 +3,8 @@
 //   S' = exp(g) S,  S = S' + beta k (v - S'^T k)^T,  out = scale S^T q
 //
 // One token at a time, a workgroup for each sequence and head, its state in registers.
+#include <type_traits>
+
 #include "mr_state_device.h"
 
 namespace mr {
@@ -128,6 +130,10 @@ typedef u32x4 Operand;  // 8 numbers of 16 bits of a lane: lane (m, g), row (or 
 
 __device__ __forceinline__ f32x4 mfma_bf16(Operand a, Operand b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+typedef short bf16x4_bits __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ f32x4 mfma_bf16(u32x2 a, u32x2 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(bf16x4_bits, a), __builtin_bit_cast(bf16x4_bits, b), c, 0, 0, 0);
 }
 __device__ __forceinline__ f32x4 mfma_f16(Operand a, Operand b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -382,22 +388,25 @@ __global__ __launch_bounds__(256) void k_delta_prepare(ChunkArgs c) {
   }
 }
 
-// A sequence's chunks for 16 columns of a head's state. Wave w has the tokens 16 w .. of a chunk, and of the state its tiles of 16
-// rows from w * (DK / 64) on. The state, V - K S and V' go round through LDS as operands.
+// A sequence's chunks for 16 columns of a head's state. What the next chunk waits for is the state alone, through three steps:
+// V - K S, V', S. Four waves take them, each result going from one wave's registers through LDS to all: wave w has the state's
+// tiles of 16 rows from w * (DK / 64) on, whose part of K S it works out for the whole chunk, and the chunk's tokens from 16 w on
+// after that. Four others work out the tokens' outputs beside them, a step behind.
 template <int DK, int NP, bool BF>
-__global__ __launch_bounds__(256, 2) void k_delta_chunks(ChunkArgs c, uint32_t slices, int parity) {
+__global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs c, uint32_t slices, int parity) {
   constexpr int NS = DK / 32, NT = DK / 64;
-  constexpr uint32_t kType = BF ? MR_BF16 : MR_F16;
   using I = DeltaImage<DK, NP>;
-  __shared__ __attribute__((aligned(16))) uint8_t state[NS][3][1024], rest[2][3][1024], fresh[2][2][1024], faded[2][3][1024];
+  __shared__ __attribute__((aligned(16))) uint8_t state[NS][2][1024], rest[2][3][1024], faded[2][3][1024];
+  __shared__ f32x4 fresh[4][64], sums[4][4][64];
   __shared__ __attribute__((aligned(16))) int first_bad[4][16], any_bad[4];
   const DeltaArgs& a = c.a;
   const Sequences& q = a.s;
   // Workgroups go to the 8 XCDs in turn: the slices of a head, which read the same operands, to one of them.
   const uint32_t unit = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3), h = unit / slices, slice = unit % slices, s = blockIdx.y;
-  if (h >= c.a.d.value_heads) return;
+  if (h >= a.d.value_heads) return;
   const uint32_t hk = h / (a.d.value_heads / a.d.key_heads), DV = a.d.value_dim;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+  const int wave = (threadIdx.x >> 6) & 3, lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+  const bool outputs = __builtin_amdgcn_readfirstlane(threadIdx.x) >= 256;
   int q0, q1;
   rows_of(q.cu, q.n_rows, s, q0, q1);
   const int n = q1 - q0;
@@ -406,209 +415,255 @@ __global__ __launch_bounds__(256, 2) void k_delta_chunks(ChunkArgs c, uint32_t s
   const uint32_t start = first_tile(q.cu, q.n_rows, s, 1, 6), count = (n + kChunk - 1) / kChunk;
   const uint32_t end = start + max(count, 1u);  // a sequence without tokens takes part in one launch
   if (end <= c.first || start >= c.last) return;
-  const int source = slot_of(q, q.source, s), target = slot_of(q, q.target, s);
-  const uint32_t col = 16 * slice + m;
-  // this lane's numbers of a state: rows 4 g + r of each of the wave's tiles, one column
-  auto at = [&](float* base, int t, int r) {
-    const int x = wave * NT + t;
-    return base + (uint64_t)(32 * (x >> 1) + 8 * g + 4 * (x & 1) + r) * DV + col;
-  };
-  const uint64_t state_size = (uint64_t)DK * DV;
-  float* carried = c.carry + ((uint64_t)(parity ^ 1) * a.d.value_heads + h) * state_size;
-  float* carry = c.carry + ((uint64_t)parity * a.d.value_heads + h) * state_size;
-  f32x4 S[NT] = {};
-  {
-    float* from = start < c.first ? carried : source >= 0 ? q.states + ((uint64_t)source * a.d.value_heads + h) * state_size : nullptr;
-    if (from)
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) S[t][r] = *at(from, t, r);
-  }
-  // The state's tiles 2 s and 2 s + 1 are step s of the sums over a key's elements.
-  auto publish = [&] {
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      u32x2 part[3];
-      split(S[t], part);
-      const int x = wave * NT + t;
-#pragma unroll
-      for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x2*>(&state[x >> 1][p][lane * 16 + 8 * (x & 1)]) = part[p];
-    }
-  };
-  publish();
+  const uint32_t begin = max(start, c.first), stop = min(start + count, c.last);
+
   auto operand = [&](const uint8_t* p) { return *reinterpret_cast<const Operand*>(p + lane * 16); };
   // The operands of a chunk are on their way while the chunk before is worked on: each part is asked for as soon as its
-  // registers have been read.
-  const uint32_t begin = max(start, c.first), stop = min(start + count, c.last);
+  // registers have been read. The last chunk loads itself again: a wait for one load must know how many others there
+  // are behind it.
   const uint64_t value_step = (uint64_t)a.d.value_heads * I::kValue, key_step = (uint64_t)a.d.key_heads * I::kKey;
   const uint8_t* image = c.values + (uint64_t)(begin - c.first) * value_step + (uint64_t)h * I::kValue;
   const uint8_t* key_image = c.keys + (uint64_t)(begin - c.first) * key_step + (uint64_t)hk * I::kKey;
   const int t0 = 16 * wave + 4 * g;
-  Operand K[NS][NP], Q[NS][NP], T[2][3], P[2][2], KT[NT][2][NP];
-  f32x4 of_k, of_q, of_v;
-  float fade;
-  uint16_t vals[4];
-  auto load_keys = [&] {
-#pragma unroll
-    for (int x = 0; x < NS; ++x)
-#pragma unroll
-      for (int p = 0; p < NP; ++p) {
-        K[x][p] = operand(key_image + I::kK + ((wave * NS + x) * NP + p) * 1024);
-        Q[x][p] = operand(key_image + I::kQ + ((wave * NS + x) * NP + p) * 1024);
-      }
-  };
-  const int t_ld = (int)a.v.ts * 2, o_ld = (int)a.out.ts * 2;  // bytes from a token to the next
-  auto load_rest = [&](int row) {
-    const float* vec = reinterpret_cast<const float*>(image + I::kVec) + t0;
-    of_k = *reinterpret_cast<const f32x4*>(vec), of_q = *reinterpret_cast<const f32x4*>(vec + 64);
-    of_v = *reinterpret_cast<const f32x4*>(vec + 128);
-    const uint8_t* v = static_cast<const uint8_t*>(a.v.p) + ((uint64_t)row * a.v.ts + (uint64_t)h * a.v.hs + 16 * slice) * 2;
-    const int last = q1 - 1 - row;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) vals[r] = *reinterpret_cast<const uint16_t*>(v + (uint32_t)(min(t0 + r, last) * t_ld + 2 * m));
-#pragma unroll
-    for (int x = 0; x < 2; ++x)
-#pragma unroll
-      for (int p = 0; p < 3; ++p) T[x][p] = operand(image + I::kT + (I::lower(wave, min(x, wave / 2)) * 3 + p) * 1024);
-  };
-  auto load_mix = [&] {
-    fade = reinterpret_cast<const float*>(image + I::kVec)[192];
-#pragma unroll
-    for (int x = 0; x < 2; ++x)
-#pragma unroll
-      for (int p = 0; p < 2; ++p) P[x][p] = operand(image + I::kP + (I::lower(wave, min(x, wave / 2)) * 2 + p) * 1024);
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int p = 0; p < NP; ++p) KT[t][x][p] = operand(key_image + I::kKT + (((wave * NT + t) * 2 + x) * NP + p) * 1024);
-  };
   int row = q0 + (int)(begin - start) * kChunk;
-  if (begin < stop) load_keys(), load_rest(row), load_mix();
-  __syncthreads();
-  for (uint32_t chunk = begin; chunk < stop; ++chunk, row += kChunk) {
-    const int left = min(kChunk, q1 - row);
-    // The last chunk loads itself again: a wait for one load must know how many others there are behind it.
-    const bool more = chunk + 1 < stop;
-    const uint64_t value_next = more ? value_step : 0, key_next = more ? key_step : 0;
-    // K S and Q S of this wave's tokens; sums of products of like size, so that they do not wait for each other
-    f32x4 ks[3] = {}, qs[2] = {};
+
+  if (outputs) {
+    if (begin >= stop) return;
+    Operand Q[NS][NP], P[2][2];
+    f32x4 of_q;
+    auto load = [&] {
 #pragma unroll
-    for (int x = 0; x < NS; ++x) {
-      Operand S3[3];
+      for (int x = 0; x < NS; ++x)
 #pragma unroll
-      for (int p = 0; p < 3; ++p) S3[p] = operand(state[x][p]);
-#pragma unroll
-      for (int p = 0; p < NP; ++p) {
-#pragma unroll
-        for (int z = 0; z + p < 3; ++z) ks[z + p] = mfma_bf16(K[x][p], S3[z], ks[z + p]);
-#pragma unroll
-        for (int z = 0; z + p < 2; ++z) qs[z + p] = mfma_bf16(Q[x][p], S3[z], qs[z + p]);
-      }
-    }
-    key_image += key_next;
-    load_keys();
-    f32x4 R = (ks[2] + ks[1]) + ks[0], o = (qs[1] + qs[0]) * of_q;
-    bool wrong = false;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const float v = t0 + r < left ? (BF ? bits_f32((uint32_t)vals[r] << 16) : (float)__builtin_bit_cast(_Float16, vals[r])) : 0.f;
-      R[r] = fmaf(-of_k[r], R[r], v);
-      wrong |= !(fabsf(R[r]) < INFINITY);
-    }
-    const bool any = __any(wrong);
-    if (any) {
-      // NaN would reach earlier tokens by the zeros it is multiplied with: it is taken out, and the column's tokens from here
-      // on are NaN at the end
-      int bad = kChunk;
-#pragma unroll
-      for (int r = 3; r >= 0; --r)
-        if (!(fabsf(R[r]) < INFINITY)) bad = t0 + r, R[r] = 0.f;
-      bad = min(bad, __shfl_xor(bad, 16, 64));
-      bad = min(bad, __shfl_xor(bad, 32, 64));
-      if (g == 0) first_bad[wave][m] = bad;
-    }
-    if (lane == 0) any_bad[wave] = any;
-    const int half = lane * 16 + 8 * (wave & 1);  // the tile's half of its step
-    {
-      u32x2 part[3];
-      split(R, part);
-#pragma unroll
-      for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x2*>(&rest[wave >> 1][p][half]) = part[p];
-    }
-    __syncthreads();
-    const i32x4 bads = *reinterpret_cast<const i32x4*>(any_bad);
-    int first = kChunk;
-    if (__builtin_amdgcn_readfirstlane(bads.x | bads.y | bads.z | bads.w)) {
-#pragma unroll
-      for (int w = 0; w < 4; ++w)
-        if (bads[w]) first = min(first, first_bad[w][m]);
-    }
-    f32x4 V;
-    {
-      f32x4 sum[3] = {};
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        if (x > wave / 2) break;
-        Operand y[3];
-#pragma unroll
-        for (int p = 0; p < 3; ++p) y[p] = operand(rest[x][p]);
-#pragma unroll
-        for (int p = 0; p < 3; ++p)
-#pragma unroll
-          for (int z = 0; z + p < 3; ++z) sum[z + p] = mfma_bf16(T[x][p], y[z], sum[z + p]);
-      }
-      V = (sum[2] + sum[1]) + sum[0];
-    }
-    {
-      u32x2 part[2], faint[3];
-      split(V, part), split(V * of_v, faint);
-#pragma unroll
-      for (int p = 0; p < 2; ++p) *reinterpret_cast<u32x2*>(&fresh[wave >> 1][p][half]) = part[p];
-#pragma unroll
-      for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x2*>(&faded[wave >> 1][p][half]) = faint[p];
-    }
-    image += value_next;
-    load_rest(row + (more ? kChunk : 0));
-    __syncthreads();
-    const float keep = first < kChunk ? NAN : fade;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      f32x4 sum[3] = {};
+        for (int p = 0; p < NP; ++p) Q[x][p] = operand(key_image + I::kQ + ((wave * NS + x) * NP + p) * 1024);
+      of_q = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(image + I::kVec) + 64 + t0);
+    };
+    auto load_mix = [&] {
 #pragma unroll
       for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) P[x][p] = operand(image + I::kP + (I::lower(wave, min(x, wave / 2)) * 2 + p) * 1024);
+    };
+    const int step = (int)a.out.ts * 2;  // bytes from a token to the next
+    f32x4 o = {};
+    auto store = [&](int row) {
+      uint8_t* out = static_cast<uint8_t*>(a.out.p) + ((uint64_t)row * a.out.ts + (uint64_t)h * a.out.hs + 16 * slice) * 2;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (row + t0 + r < q1)
+          *reinterpret_cast<uint16_t*>(out + (uint32_t)((t0 + r) * step + 2 * m)) = (uint16_t)(BF ? pack_bf16(o[r], 0.f) : pack_f16(o[r], 0.f));
+    };
+    load(), load_mix();
+    __syncthreads();
+    for (uint32_t chunk = begin; chunk < stop; ++chunk, row += kChunk) {
+      const bool more = chunk + 1 < stop;
+      f32x4 qs[2] = {};  // sums of products of like size, so that they do not wait for each other
+#pragma unroll
+      for (int x = 0; x < NS; ++x) {
+        const Operand S2[2] = {operand(state[x][0]), operand(state[x][1])};
 #pragma unroll
         for (int p = 0; p < NP; ++p)
 #pragma unroll
-          for (int z = 0; z + p < 3; ++z) sum[z + p] = mfma_bf16(KT[t][x][p], operand(faded[x][z]), sum[z + p]);
-      S[t] = S[t] * keep + ((sum[2] + sum[1]) + sum[0]);
-    }
-    publish();
-    {
+          for (int z = 0; z + p < 2; ++z) qs[z + p] = mfma_bf16(Q[x][p], S2[z], qs[z + p]);
+      }
+      const f32x4 before = (qs[1] + qs[0]) * of_q;
+      image += more ? value_step : 0, key_image += more ? key_step : 0;
+      load();
+      __syncthreads();
+      if (chunk > begin) store(row - kChunk);
+      __syncthreads();
+      const i32x4 bads = *reinterpret_cast<const i32x4*>(any_bad);
       f32x4 sum[2] = {};
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         if (x > wave / 2) break;
+        u32x2 lo[2], hi[2];
+        split(fresh[2 * x][lane], lo), split(fresh[2 * x + 1][lane], hi);
+        const Operand v[2] = {{lo[0].x, lo[0].y, hi[0].x, hi[0].y}, {lo[1].x, lo[1].y, hi[1].x, hi[1].y}};
 #pragma unroll
         for (int p = 0; p < 2; ++p)
 #pragma unroll
-          for (int z = 0; z + p < 2; ++z) sum[z + p] = mfma_bf16(P[x][p], operand(fresh[x][z]), sum[z + p]);
+          for (int z = 0; z + p < 2; ++z) sum[z + p] = mfma_bf16(P[x][p], v[z], sum[z + p]);
       }
-      o += sum[1] + sum[0];
-    }
-    load_mix();
-    uint8_t* out = static_cast<uint8_t*>(a.out.p) + ((uint64_t)row * a.out.ts + (uint64_t)h * a.out.hs + 16 * slice) * 2;
+      load_mix();
+      o = before + (sum[1] + sum[0]);
+      if (__builtin_amdgcn_readfirstlane(bads.x | bads.y | bads.z | bads.w)) {
+        int first = kChunk;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      if (t0 + r >= left) continue;
-      const float v = t0 + r >= first ? NAN : o[r];
-      *reinterpret_cast<uint16_t*>(out + (uint32_t)((t0 + r) * o_ld + 2 * m)) = (uint16_t)(kType == MR_BF16 ? pack_bf16(v, 0.f) : pack_f16(v, 0.f));
+        for (int w = 0; w < 4; ++w)
+          if (bads[w]) first = min(first, first_bad[w][m]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (t0 + r >= first) o[r] = NAN;
+      }
+      __syncthreads();
     }
-    __syncthreads();
+    store(row - kChunk);
+    return;
   }
-  float* to = end > c.last ? carry : target >= 0 ? q.states + ((uint64_t)target * a.d.value_heads + h) * state_size : nullptr;
+
+  const int source = slot_of(q, q.source, s), target = slot_of(q, q.target, s);
+  const uint64_t state_size = (uint64_t)DK * DV;
+  // this lane's numbers of a state: rows 4 g + r of each of the wave's tiles, one column
+  auto at = [&](float* base, int t, int r) {
+    const int x = wave * NT + t;
+    return base + (uint64_t)(32 * (x >> 1) + 8 * g + 4 * (x & 1) + r) * DV + 16 * slice + m;
+  };
+  auto in_slot = [&](int slot) { return q.states + ((uint64_t)slot * a.d.value_heads + h) * state_size; };
+  auto carry = [&](int parity) { return c.carry + ((uint64_t)parity * a.d.value_heads + h) * state_size; };
+  f32x4 S[NT] = {};
+  if (float* from = start < c.first ? carry(parity ^ 1) : source >= 0 ? in_slot(source) : nullptr) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) S[t][r] = *at(from, t, r);
+  }
+  if (begin < stop) {
+    using Part = std::conditional_t<NT == 2, Operand, u32x2>;  // the wave's rows of the state as an operand
+    Operand T[2][3], KT[NT][2][NP];
+    Part K[4][NP];
+    f32x4 of_k, of_v;
+    float fade;
+    uint16_t vals[4];
+    const int step = (int)a.v.ts * 2;
+    auto load_keys = [&] {
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+          K[t][p] = *reinterpret_cast<const Part*>(key_image + I::kK + ((t * NS + wave * NT / 2) * NP + p) * 1024 + lane * 16 + (NT == 1 ? 8 * (wave & 1) : 0));
+    };
+    auto load_rest = [&](int row) {
+      const float* vec = reinterpret_cast<const float*>(image + I::kVec) + t0;
+      of_k = *reinterpret_cast<const f32x4*>(vec), of_v = *reinterpret_cast<const f32x4*>(vec + 128);
+      const uint8_t* v = static_cast<const uint8_t*>(a.v.p) + ((uint64_t)row * a.v.ts + (uint64_t)h * a.v.hs + 16 * slice) * 2;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) vals[r] = *reinterpret_cast<const uint16_t*>(v + (uint32_t)(min(t0 + r, q1 - 1 - row) * step + 2 * m));
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int p = 0; p < 3; ++p) T[x][p] = operand(image + I::kT + (I::lower(wave, min(x, wave / 2)) * 3 + p) * 1024);
+    };
+    auto load_fade = [&] {
+      fade = reinterpret_cast<const float*>(image + I::kVec)[192];
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int p = 0; p < NP; ++p) KT[t][x][p] = operand(key_image + I::kKT + (((wave * NT + t) * 2 + x) * NP + p) * 1024);
+    };
+    // The wave's part of K S for the next chunk. The state's tiles 2 s and 2 s + 1 are step s of the sums over a key's elements: as
+    // an operand they are what their lanes hold.
+    auto look = [&] {
+      u32x2 part[NT][3];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        split(S[t], part[t]);
+        const int x = wave * NT + t;
+#pragma unroll
+        for (int p = 0; p < 2; ++p) *reinterpret_cast<u32x2*>(&state[x >> 1][p][lane * 16 + 8 * (x & 1)]) = part[t][p];
+      }
+      f32x4 sum[4] = {};
+#pragma unroll
+      for (int p = NP - 1; p >= 0; --p)
+#pragma unroll
+        for (int z = 2 - p; z >= 0; --z) {
+          Part y;
+          if constexpr (NT == 2) y = Operand{part[0][z].x, part[0][z].y, part[1][z].x, part[1][z].y};
+          else y = part[0][z];
+#pragma unroll
+          for (int t = 0; t < 4; ++t) sum[t] = mfma_bf16(K[t][p], y, sum[t]);
+        }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) sums[wave][t][lane] = sum[t];
+    };
+    load_keys(), load_rest(row), load_fade();
+    look();
+    key_image += begin + 1 < stop ? key_step : 0;
+    load_keys();
+    __syncthreads();
+    for (uint32_t chunk = begin; chunk < stop; ++chunk, row += kChunk) {
+      const bool more = chunk + 1 < stop;
+      const int half = lane * 16 + 8 * (wave & 1);  // of the step that the wave's tokens are in
+      f32x4 R = (sums[0][wave][lane] + sums[1][wave][lane]) + (sums[2][wave][lane] + sums[3][wave][lane]);
+      bool wrong = false;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float v = row + t0 + r < q1 ? (BF ? bits_f32((uint32_t)vals[r] << 16) : (float)__builtin_bit_cast(_Float16, vals[r])) : 0.f;
+        R[r] = fmaf(-of_k[r], R[r], v);
+        wrong |= !(fabsf(R[r]) < INFINITY);
+      }
+      const bool any = __any(wrong);
+      if (any) {
+        // NaN would reach earlier tokens by the zeros it is multiplied with: it is taken out, and the column's tokens from here
+        // on are NaN at the end
+        int bad = kChunk;
+#pragma unroll
+        for (int r = 3; r >= 0; --r)
+          if (!(fabsf(R[r]) < INFINITY)) bad = t0 + r, R[r] = 0.f;
+        bad = min(bad, __shfl_xor(bad, 16, 64));
+        bad = min(bad, __shfl_xor(bad, 32, 64));
+        if (g == 0) first_bad[wave][m] = bad;
+      }
+      if (lane == 0) any_bad[wave] = any;
+      {
+        u32x2 part[3];
+        split(R, part);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x2*>(&rest[wave >> 1][p][half]) = part[p];
+      }
+      __syncthreads();
+      const i32x4 bads = *reinterpret_cast<const i32x4*>(any_bad);
+      f32x4 V;
+      {
+        f32x4 sum[3] = {};  // sums of products of like size, so that they do not wait for each other
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          if (x > wave / 2) break;
+          const Operand y[3] = {operand(rest[x][0]), operand(rest[x][1]), operand(rest[x][2])};
+#pragma unroll
+          for (int p = 0; p < 3; ++p)
+#pragma unroll
+            for (int z = 0; z + p < 3; ++z) sum[z + p] = mfma_bf16(T[x][p], y[z], sum[z + p]);
+        }
+        V = (sum[2] + sum[1]) + sum[0];
+      }
+      fresh[wave][lane] = V;
+      {
+        u32x2 part[3];
+        split(V * of_v, part);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x2*>(&faded[wave >> 1][p][half]) = part[p];
+      }
+      image += more ? value_step : 0;
+      load_rest(row + (more ? kChunk : 0));
+      float keep = fade;
+      if (__builtin_amdgcn_readfirstlane(bads.x | bads.y | bads.z | bads.w)) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          if (bads[w] && first_bad[w][m] < kChunk) keep = NAN;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        f32x4 sum[3] = {};
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int p = 0; p < NP; ++p)
+#pragma unroll
+            for (int z = 0; z + p < 3; ++z) sum[z + p] = mfma_bf16(KT[t][x][p], operand(faded[x][z]), sum[z + p]);
+        S[t] = S[t] * keep + ((sum[2] + sum[1]) + sum[0]);
+      }
+      load_fade();
+      look();
+      key_image += chunk + 2 < stop ? key_step : 0;
+      load_keys();
+      __syncthreads();
+    }
+  }
+  float* to = end > c.last ? carry(parity) : target >= 0 ? in_slot(target) : nullptr;
   if (!to || (n == 0 && target == source)) return;
 #pragma unroll
   for (int t = 0; t < NT; ++t)
@@ -643,7 +698,7 @@ hipError_t launch_chunks(const Launch& K, const DeltaArgs& a, int least, uint8_t
       hipLaunchKernelGGL((k_delta_prepare<DK, BF>), dim3(vh, c.last - c.first), dim3(256), 0, K.s, c);
     }
     ProfScope ps(K, "delta_chunks");
-    hipLaunchKernelGGL((k_delta_chunks<DK, BF ? 1 : 2, BF>), dim3((vh * (dv / 16) + 7) / 8 * 8, a.s.n_seqs), dim3(256), 0, K.s, c, dv / 16, parity);
+    hipLaunchKernelGGL((k_delta_chunks<DK, BF ? 1 : 2, BF>), dim3((vh * (dv / 16) + 7) / 8 * 8, a.s.n_seqs), dim3(512), 0, K.s, c, dv / 16, parity);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
