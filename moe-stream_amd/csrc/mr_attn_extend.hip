@@ -127,6 +127,13 @@ __device__ __forceinline__ Reach reach_of(const ExtendArgs& a, const Unit& u) {
   return t;
 }
 
+// Reports offsets and lengths out of range; by every thread of one workgroup.
+__device__ __forceinline__ void check_entries(const ExtendArgs& a) {
+  check_offsets(a.cu, a.n_seqs, a.nq, a.err, kErrOffset);
+  for (uint32_t s = threadIdx.x; s < a.n_seqs; s += blockDim.x)
+    if (a.len[s] < 0 || (int64_t)a.len[s] > (int64_t)a.max_pages << a.kv.page_shift) note_error(a.err, kErrLength);
+}
+
 template <int NT, int FMT, int D>
 constexpr int kPerSimd = NT * D >= 256 ? 1 : 2;
 
@@ -139,11 +146,7 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<NT, FMT, D>)) void k_attn_ex
   __shared__ float stats[kWaves / 2][16][2];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const uint32_t hk = blockIdx.y;
-  if (blockIdx.x == 0 && hk == 0) {
-    check_offsets(a.cu, a.n_seqs, a.nq, a.err, kErrOffset);
-    for (uint32_t s = threadIdx.x; s < a.n_seqs; s += blockDim.x)
-      if (a.len[s] < 0 || (int64_t)a.len[s] > (int64_t)a.max_pages << a.kv.page_shift) note_error(a.err, kErrLength);
-  }
+  if (blockIdx.x == 0 && hk == 0) check_entries(a);
   Unit u;
   if (!find_unit(a, blockIdx.x, false, u)) return;
   const Reach t = reach_of(a, u);
@@ -324,6 +327,303 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<NT, FMT, D>)) void k_attn_ex
   }
 }
 
+// ---- many rows ------------------------------------------------------------------------------
+// A tile of 128 rows, 32 to a wave, all waves at the same chunk of 64 tokens. Its codes are turned into operands once, by the
+// four waves together, and lie in LDS as the pages have them, so that writes and reads are whole rows of 16-byte pieces.
+// Both products are 32x32x16 matrix instructions, keys (then the values' elements) down and rows across: a lane has the scores
+// of one row. Of each 32 keys the result's row 16 c + 8 x + 4 h + r stands for key 16 x + 8 c + 4 h + r: lane half h then holds,
+// 8 numbers after the other, what the second product's right operand wants for the values of lane group 2 c + h.
+constexpr float kWideSlack = 4.f, kWideLift = 11.f;  // weights up to 2^15: the maximum is followed when it has moved by 2^4
+
+// A wave's quarter of a chunk on its way from the pages to LDS.
+template <int FMT, int D>
+struct Quarter {
+  static constexpr int NK = D / 32, NV = D / 64;   // operands of keys, pairs of operands of values
+  static constexpr int KW = D * FMT / 128, VW = FMT / 2;  // words of a lane's keys (16 of them), of a pair's values
+  uint32_t k[KW], v[NV][VW], ks[FMT == MR_KV_F16 ? 1 : D == 256 ? 2 : 1];
+  u32x2 vs[NV];
+
+  template <int N>
+  static __device__ __forceinline__ void words(const uint8_t* p, uint32_t (&to)[N]) {
+    if constexpr (N == 2) {
+      const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+      to[0] = x.x, to[1] = x.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N / 4; ++i) {
+        const u32x4 x = *reinterpret_cast<const u32x4*>(p + 1024 * i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) to[4 * i + j] = x[j];
+      }
+    }
+  }
+  // Keys 16 wave + m; pairs of values NV * wave and on.
+  __device__ __forceinline__ void load(const uint8_t* p, int wave, int lane) {
+    using L = KvLayout<FMT, D>;
+    const int m = lane & 15, g = lane >> 4;
+    const int kb = wave * KW * 4;  // byte of a lane's keys: pieces of 16 bytes are 1 KB apart
+    words(p + (kb >> 4) * 1024 + lane * 16 + (kb & 15), k);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int vb = (wave * NV + i) * VW * 4;
+      words(p + L::kV + (vb >> 4) * 1024 + lane * 16 + (vb & 15), v[i]);
+    }
+    if constexpr (FMT != MR_KV_F16) {
+#pragma unroll
+      for (int i = 0; i < (D == 256 ? 2 : 1); ++i) {
+        const int blk = D == 64 ? g >> 1 : D == 128 ? g : 2 * g + i;
+        ks[i] = *reinterpret_cast<const uint32_t*>(p + L::kKs + (blk * 16 + m) * 4);
+      }
+#pragma unroll
+      for (int i = 0; i < NV; ++i) vs[i] = *reinterpret_cast<const u32x2*>(p + L::kVs + g * (D / 2) + (wave * NV + i) * 8);
+    }
+  }
+  // To the chunk's keys and values in LDS, as operands.
+  __device__ __forceinline__ void store(uint8_t* keys, uint8_t* values, int wave, int lane) const {
+#pragma unroll
+    for (int i = 0; i < NK; ++i) {
+      u32x4 x;
+      const uint32_t s = ks[D == 256 ? i >> 2 : 0];
+      if constexpr (FMT == MR_KV_MXFP4) {
+        const uint32_t e = exp_bits_of(s, wave), c = k[i];
+        x = u32x4{fp4_pair<0>(c, e), fp4_pair<1>(c, e), fp4_pair<2>(c, e), fp4_pair<3>(c, e)};
+      } else {
+        const uint32_t b = s >> (8 * wave) & 0xFFu;
+        const f16x2 e = __builtin_bit_cast(f16x2, b << 8 | b << 24);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = __builtin_bit_cast(uint32_t, int8_pair(k[2 * i + (j >> 1)], j & 1) * e);
+      }
+      *reinterpret_cast<u32x4*>(keys + (wave * NK + i) * 1024 + lane * 16) = x;
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      u32x4 lo, hi;
+      value_pair<FMT>(v[i], vs[i].x, vs[i].y, lo, hi);
+      uint8_t* to = values + (wave * NV + i) * 2048 + lane * 16;
+      *reinterpret_cast<u32x4*>(to) = lo, *reinterpret_cast<u32x4*>(to + 1024) = hi;
+    }
+  }
+  static __device__ __forceinline__ uint32_t exp_bits_of(uint32_t s, int wave) { return s >> (8 * wave) << 23; }
+};
+
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+template <int FMT, int D>
+constexpr int kWidePerSimd = D == 256 ? 1 : D == 128 ? 2 : 3;
+
+template <int FMT, int D>
+__global__ __launch_bounds__(256, (kWidePerSimd<FMT, D>)) void k_attn_extend_wide(ExtendArgs a) {
+  constexpr int ND = D / 32, NI = D / 16, kTile = 64 * D * 2;  // bytes of a chunk's keys as operands
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2][2][kTile];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 31, half = lane >> 5;
+  const uint32_t hk = blockIdx.y;
+  if (blockIdx.x == 0 && hk == 0) check_entries(a);
+  Unit u;
+  if (!find_unit(a, blockIdx.x, false, u)) return;
+  const Reach t = reach_of(a, u);
+  const int mine = 32 * wave + n;  // this lane's row of the tile
+  const bool any_rows = 32 * wave < t.rows;
+
+  auto place = [&](uint64_t& row, uint32_t& head) {
+    const uint32_t r = (uint32_t)(t.r0 + min(mine, t.rows - 1)), i = a.group.of(r);
+    row = (uint64_t)(u.sp.q0 + (int)i), head = hk * a.group.d + (r - i * a.group.d);
+    return u.sp.len - u.sp.n + (int)i;
+  };
+  uint64_t row;
+  uint32_t head;
+  const int pos = place(row, head), from = first_seen(a, pos);
+  // of the wave's rows: the first one's position, and the last one's first key
+  const int wave_pos0 = __builtin_amdgcn_readfirstlane(pos), wave_pos1 = __builtin_amdgcn_readlane(pos, 31);
+  const int wave_first = first_seen(a, wave_pos0), wave_last_first = first_seen(a, wave_pos1);
+
+  // The query as f16 times a power of two, its largest element in [2^14, 2^15).
+  u32x4 qf[NI];
+  float c;
+  {
+    const uint16_t* qp = static_cast<const uint16_t*>(a.q.p) + row * a.q.ts + (uint64_t)head * a.q.hs;
+    const bool bf = a.q.dtype == MR_BF16;
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      // step (e, gp) of the sums has the elements 8 e .. of the quarters 2 gp and 2 gp + 1
+      qf[i] = *reinterpret_cast<const u32x4*>(qp + (2 * (i & 1) + half) * (D / 4) + 8 * (i >> 1));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const f32x2 x = bf ? unpack_bf16(qf[i][j]) : unpack_f16(qf[i][j]);
+        top = fmaxf(fmaxf(top, fabsf(x.x)), fabsf(x.y));
+      }
+    }
+    top = max_xor32(top);
+    const int e = top > 0.f ? ilogbf(fminf(top, 3.0e38f)) - 14 : 0;
+    const float sign = a.o.scale < 0.f ? -1.f : 1.f;
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const f32x2 x = bf ? unpack_bf16(qf[i][j]) : unpack_f16(qf[i][j]);
+        qf[i][j] = pack_f16(ldexpf(x.x, -e) * sign, ldexpf(x.y, -e) * sign);
+      }
+    c = fminf(fmaxf(ldexpf(fabsf(a.o.scale) * 1.44269504088896340736f, e), 0x1p-126f), kLargest);
+  }
+
+  const int cpp = 1 << (a.kv.page_shift - 6);
+  auto page_of = [&](int chunk) -> int {
+    if (chunk >= t.end) return -1;
+    const int p = a.table[(uint64_t)u.b * a.max_pages + (uint32_t)(chunk >> (a.kv.page_shift - 6))];
+    if (p >= 0 && (uint32_t)p < a.kv.n_pages) return p;
+    note_error(a.err, kErrPage);
+    return -1;
+  };
+  // lane i has the page of the i-th of 64 chunks
+  int pages = -1;
+  auto next_page = [&](int i) {
+    if ((i & 63) == 0) pages = page_of(t.begin + i + lane);
+    return __builtin_amdgcn_readlane(pages, i & 63);
+  };
+  Quarter<FMT, D> quarter;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)&lds[0][0][0];
+  auto fetch = [&](int page, int chunk, int b) {
+    const uint8_t* p = a.kv.at(page < 0 ? 0 : page, hk, chunk & (cpp - 1));
+    if constexpr (FMT == MR_KV_F16) {
+#pragma unroll
+      for (int i = 0; i < 2 * kTile / 4096; ++i)
+        load_lds16((uint64_t)p, 2 * kTile, (uint32_t)((i * 4 + wave) * 1024 + lane * 16), lds0 + b * 2 * kTile + (i * 4 + wave) * 1024);
+    } else {
+      quarter.load(p, wave, lane);
+    }
+  };
+  // behind the last chunk's work: the fetched one into buffer b
+  auto arrive = [&](int b) {
+    if constexpr (FMT == MR_KV_F16) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    else quarter.store(lds[b][0], lds[b][1], wave, lane);
+  };
+
+  f32x16 acc[ND];
+#pragma unroll
+  for (int x = 0; x < ND; ++x) acc[x] = f32x16{};
+  float ref = 0.f, l = 0.f;  // scores are relative to ref: the largest so far, or up to kWideSlack below it
+  bool seen = false;
+  // addresses of operands: keys 32 T + .., elements of step i; values' elements 32 x + n of 16 keys
+  const uint32_t k_at = lds0 + (uint32_t)(((n >> 3) & 1) * (D / 32) * 1024 + (16 * half + ((n >> 4) << 3 | (n & 7))) * 16);
+  const uint32_t v_at = lds0 + kTile + (uint32_t)((n >> 4) * 1024 + (16 * half + (n & 15)) * 16);
+  auto key_part = [&](uint32_t base, int T, int i) {
+    return *(const __attribute__((address_space(3))) u32x4*)(uintptr_t)(base + T * (D / 16) * 1024 + (i >> 1) * 1024 + (i & 1) * 512);
+  };
+  auto value_part = [&](uint32_t base, int cc, int x) {  // keys 16 cc and on
+    return *(const __attribute__((address_space(3))) u32x4*)(uintptr_t)(base + (cc >> 1) * (D / 16) * 1024 + x * 2048 + (cc & 1) * 512);
+  };
+
+  int page = -1;
+  if (t.begin < t.end) {
+    page = next_page(0);
+    fetch(page, t.begin, 0);
+    arrive(0);
+    __syncthreads();
+  }
+  for (int i = 0, cidx = t.begin, b = 0; cidx < t.end; ++i, ++cidx, b ^= 1) {
+    const bool there = page >= 0, more = cidx + 1 < t.end;
+    if (more) {
+      page = next_page(i + 1);
+      fetch(page, cidx + 1, b ^ 1);
+    }
+    const int k0 = cidx << 6;
+    if (any_rows && k0 <= wave_pos1 && k0 + 63 >= wave_first) {
+      uint32_t kb = k_at + b * 2 * kTile, vb = v_at + b * 2 * kTile;
+      asm("" : "+v"(kb), "+v"(vb));  // the parts' addresses are worked out from here, not kept
+      f32x16 s0, s1;
+#pragma unroll
+      for (int x = 0; x < 16; ++x) s0[x] = s1[x] = -ref;
+      __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+      for (int x = 0; x < NI; ++x) {
+        s0 = mfma32(key_part(kb, 0, x), qf[x], s0);
+        s1 = mfma32(key_part(kb, 1, x), qf[x], s1);
+      }
+      __builtin_amdgcn_s_setprio(0);
+      if (!there || k0 + 63 > wave_pos0 || k0 < wave_last_first) {
+        // bit i: the row sees key k0 + i
+        int most = pos - k0, least = from - k0;
+        asm volatile("" : "+v"(most));  // a branch: the compiler would do this in every step
+        uint64_t sees = (most < 0 ? 0 : ~0ull >> (63 - min(most, 63))) & (least > 63 ? 0 : ~0ull << max(least, 0));
+        if (!there) sees = 0;
+        sees >>= 4 * half;
+        const uint32_t sees0 = (uint32_t)sees, sees1 = (uint32_t)(sees >> 32);
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+          const int at = 16 * ((x >> 2) & 1) + 8 * (x >> 3) + (x & 3);
+          s0[x] = seen_or_least(s0[x], sees0, at);
+          s1[x] = seen_or_least(s1[x], sees1, at);
+        }
+      }
+      float top = s0[0];
+#pragma unroll
+      for (int x = 0; x < 16; ++x) top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, s0[x]), s1[x]);
+      top = max_xor32(top);
+      const bool move = top * c > kWideSlack || (!seen && top > -INFINITY);
+      if (__any(move)) {
+        const float by = move ? top : 0.f, f = !seen ? 0.f : __builtin_amdgcn_exp2f(-by * c);
+        if (move) {
+          l *= f;
+#pragma unroll
+          for (int x = 0; x < ND; ++x) acc[x] *= f;
+#pragma unroll
+          for (int x = 0; x < 16; ++x) s0[x] -= by, s1[x] -= by;
+          ref += by;
+          seen = true;
+        }
+      }
+      u32x4 pf[4];
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {
+        const f32x16& s = x < 8 ? s0 : s1;
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[2 * (x & 7)], c, kWideLift)), p1 = __builtin_amdgcn_exp2f(fmaf(s[2 * (x & 7) + 1], c, kWideLift));
+        const uint32_t w = pack_f16(p0, p1);
+        pf[x >> 2][x & 3] = w;
+        l = add_f16(w, l);
+      }
+      __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+      for (int cc = 0; cc < 4; ++cc)
+#pragma unroll
+        for (int x = 0; x < ND; ++x) acc[x] = mfma32(value_part(vb, cc, x), pf[cc], acc[x]);
+      __builtin_amdgcn_s_setprio(0);
+    }
+    if (more) arrive(b ^ 1);
+    __syncthreads();
+  }
+
+  if (mine >= t.rows) return;
+  l = add_xor32(l);
+  const float m = !seen ? -INFINITY : fminf(fmaxf(ref * c, -kLargest), kLargest) - kWideLift;
+  // this lane's elements: 32 x + 8 (i / 4) + 4 half + i % 4
+  if (u.parts > 1) {
+    const uint64_t unit = (((uint64_t)(u.slot + u.part) * a.kv.n_heads + hk) << a.bits) + mine;
+    float* dst = a.part + unit * D + 4 * half;
+#pragma unroll
+    for (int x = 0; x < ND; ++x)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) *reinterpret_cast<f32x4*>(dst + 32 * x + 2 * i) = f32x4{acc[x][i], acc[x][i + 1], acc[x][i + 2], acc[x][i + 3]};
+    float* st = a.part + (uint64_t)kScratchRows * D + unit * 2;
+    if (half == 0) st[0] = m, st[1] = l;
+    return;
+  }
+  float f = 1.f;
+  if (a.o.sinks) {
+    const float sink = sink_of(a.o.sinks, head), m1 = fmaxf(m, sink);
+    f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m1);
+    l = l * f + (sink == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sink - m1));
+  }
+  f = l == 0.f ? 0.f : f / l;
+#pragma unroll
+  for (int x = 0; x < ND; ++x)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4)
+      store4(a.out.p, a.out.dtype, row * a.out.ts + (uint64_t)head * a.out.hs + 32 * x + 2 * i + 4 * half,
+             f32x4{acc[x][i], acc[x][i + 1], acc[x][i + 2], acc[x][i + 3]} * f);
+}
+
 // Joins the parts of split tile blockIdx.x, a wave for each row: first all parts' weights, then the weighted sums.
 template <int D>
 __global__ __launch_bounds__(64 * kWaves) void k_extend_join(ExtendArgs a) {
@@ -365,21 +665,23 @@ __global__ __launch_bounds__(64 * kWaves) void k_extend_join(ExtendArgs a) {
 using ExtendKernel = void (*)(ExtendArgs);
 template <int NT, int FMT, int D>
 ExtendKernel pick(int& per_cu) {
+  constexpr ExtendKernel kernel = [] {
+    if constexpr (NT == 8) return k_attn_extend_wide<FMT, D>;
+    else return k_attn_extend<NT, FMT, D>;
+  }();
   static const int n = [] {
     int v = 0;
-    return hipOccupancyMaxActiveBlocksPerMultiprocessor(&v, k_attn_extend<NT, FMT, D>, 64 * kWaves, 0) == hipSuccess && v > 0 ? v : 1;
+    return hipOccupancyMaxActiveBlocksPerMultiprocessor(&v, kernel, 64 * kWaves, 0) == hipSuccess && v > 0 ? v : 1;
   }();
   per_cu = n;
-  return k_attn_extend<NT, FMT, D>;
+  return kernel;
 }
 template <int FMT, int D>
-ExtendKernel pick(int& bits, int& per_cu) {
-  if (bits == 4) return pick<1, FMT, D>(per_cu);
-  if (bits == 5 || D == 256) return bits = 5, pick<2, FMT, D>(per_cu);
-  return pick<4, FMT, D == 256 ? 128 : D>(per_cu);
+ExtendKernel pick(int bits, int& per_cu) {
+  return bits == 4 ? pick<1, FMT, D>(per_cu) : bits == 5 ? pick<2, FMT, D>(per_cu) : pick<8, FMT, D>(per_cu);
 }
 template <int FMT>
-ExtendKernel pick(uint32_t D, int& bits, int& per_cu) {
+ExtendKernel pick(uint32_t D, int bits, int& per_cu) {
   return D == 64 ? pick<FMT, 64>(bits, per_cu) : D == 128 ? pick<FMT, 128>(bits, per_cu) : pick<FMT, 256>(bits, per_cu);
 }
 
@@ -393,7 +695,7 @@ hipError_t launch_attn_extend(const Launch& K, const KvPages& kv, uint32_t forma
                               int n_cu) {
   const uint32_t group = q.n / kv.n_heads;
   const uint64_t rows = (uint64_t)nq * group;
-  int bits = rows <= 16ull * n_seqs ? 4 : rows <= 32ull * n_seqs ? 5 : 6, per_cu = 1;
+  int bits = rows <= 16ull * n_seqs ? 4 : rows <= 32ull * n_seqs ? 5 : 7, per_cu = 1;
   const ExtendKernel kernel = format == MR_KV_F16      ? pick<MR_KV_F16>(D, bits, per_cu)
                               : format == MR_KV_MXINT8 ? pick<MR_KV_MXINT8>(D, bits, per_cu)
                                                        : pick<MR_KV_MXFP4>(D, bits, per_cu);

@@ -24,7 +24,6 @@ namespace mr {
 
 namespace {
 
-typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kKeys = 64;   // keys of a step
@@ -62,22 +61,6 @@ __device__ __forceinline__ int k_piece(int row, int c) {
 template <int D>
 __device__ __forceinline__ int v_piece(int row, int c) {
   return D == 64 ? c ^ (((row >> 1) & 1) * 4) : c ^ ((row & 3) * 4);
-}
-
-// 16 bytes a lane from base + offset (a lane's own) straight to LDS, lane i's to dst + 16 i (the same dst for all
-// lanes); zeros for lanes whose offset is `bytes` or more. Not the compiler's builtin: after that it waits for
-// all of them before each LDS read that it cannot tell apart, here for the next step's tile in the middle of
-// this one. The caller waits (vmcnt) and synchronises.
-__device__ __forceinline__ void load_lds16(uint64_t base, uint32_t bytes, uint32_t offset, uint32_t dst) {
-  const u32x4 rsrc = {(uint32_t)base, (uint32_t)(base >> 32), bytes, 0x00020000u};
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane(dst)), "v"(offset), "s"(rsrc)
-               : "memory", "m0");
-}
-
-// x where bit `at` of `seen` is set, else -infinity.
-__device__ __forceinline__ float seen_or_least(float x, uint32_t seen, int at) {
-  const uint32_t keep = (uint32_t)__builtin_amdgcn_sbfe((int)seen, (uint32_t)at, 1u);
-  return bits_f32((keep & __float_as_uint(x)) | (~keep & 0xFF800000u));
 }
 
 struct PrefillArgs {

@@ -44,6 +44,34 @@ __device__ __forceinline__ f16x2 int8_pair(uint32_t codes, int pair) {
   return __builtin_bit_cast(f16x2, w) - f16x2{(_Float16)1152.f, (_Float16)1152.f};
 }
 
+// Two tiles of 16 elements of 8 tokens from their codes (MXFP4: a word for 4 tokens of both; MXINT8: two words for each tile) and the
+// tokens' scale bytes.
+template <int FMT>
+__device__ __forceinline__ void value_pair(const uint32_t (&c)[FMT / 2], uint32_t s0, uint32_t s1, u32x4& lo, u32x4& hi) {
+  if constexpr (FMT == MR_KV_MXFP4) {
+    const uint32_t p[8] = {fp4_pair<0>(c[0], exp_bits(s0, 0)), fp4_pair<1>(c[0], exp_bits(s0, 1)),
+                           fp4_pair<2>(c[0], exp_bits(s0, 2)), fp4_pair<3>(c[0], exp_bits(s0, 3)),
+                           fp4_pair<0>(c[1], exp_bits(s1, 0)), fp4_pair<1>(c[1], exp_bits(s1, 1)),
+                           fp4_pair<2>(c[1], exp_bits(s1, 2)), fp4_pair<3>(c[1], exp_bits(s1, 3))};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      lo[j] = __builtin_amdgcn_perm(p[2 * j + 1], p[2 * j], 0x05040100u);
+      hi[j] = __builtin_amdgcn_perm(p[2 * j + 1], p[2 * j], 0x07060302u);
+    }
+  } else if constexpr (FMT == MR_KV_MXINT8) {
+    // scale bytes j, j + 1 as the high bytes of two f16
+    const f16x2 e[4] = {__builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0u, s0, 0x010C000Cu)),
+                        __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0u, s0, 0x030C020Cu)),
+                        __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0u, s1, 0x010C000Cu)),
+                        __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0u, s1, 0x030C020Cu))};
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        (x ? hi : lo)[j] = __builtin_bit_cast(uint32_t, int8_pair(c[2 * x + (j >> 1)], j & 1) * e[j]);
+  }
+}
+
 template <int FMT, int D>
 struct Chunk {
   static constexpr int NP = D * FMT / 128;  // 16-byte pieces a lane has of the keys, and of the values
@@ -98,33 +126,11 @@ struct Chunk {
       lo = v[G * (D / 16) + 2 * b], hi = v[G * (D / 16) + 2 * b + 1];
       return;
     }
-    const int sw = 2 * (G * (D / 32) + b);
-    const uint32_t s0 = vs[sw >> 2][sw & 3], s1 = vs[sw >> 2][(sw & 3) + 1];
-    if constexpr (FMT == MR_KV_MXFP4) {
-      const uint32_t c0 = v[sw >> 2][sw & 3], c1 = v[sw >> 2][(sw & 3) + 1];
-      const uint32_t p[8] = {fp4_pair<0>(c0, exp_bits(s0, 0)), fp4_pair<1>(c0, exp_bits(s0, 1)),
-                             fp4_pair<2>(c0, exp_bits(s0, 2)), fp4_pair<3>(c0, exp_bits(s0, 3)),
-                             fp4_pair<0>(c1, exp_bits(s1, 0)), fp4_pair<1>(c1, exp_bits(s1, 1)),
-                             fp4_pair<2>(c1, exp_bits(s1, 2)), fp4_pair<3>(c1, exp_bits(s1, 3))};
+    const int sw = 2 * (G * (D / 32) + b), w = FMT == MR_KV_MXFP4 ? sw : 2 * sw;
+    uint32_t codes[FMT / 2];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        lo[j] = __builtin_amdgcn_perm(p[2 * j + 1], p[2 * j], 0x05040100u);
-        hi[j] = __builtin_amdgcn_perm(p[2 * j + 1], p[2 * j], 0x07060302u);
-      }
-    } else {
-      // scale bytes j, j + 1 as the high bytes of two f16
-      const f16x2 e[4] = {__builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0u, s0, 0x010C000Cu)),
-                          __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0u, s0, 0x030C020Cu)),
-                          __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0u, s1, 0x010C000Cu)),
-                          __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0u, s1, 0x030C020Cu))};
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int w = 2 * (G * (D / 16) + 2 * b + x);
-        const uint32_t c0 = v[w >> 2][w & 3], c1 = v[w >> 2][(w & 3) + 1];
-        (x ? hi : lo) = u32x4{__builtin_bit_cast(uint32_t, int8_pair(c0, 0) * e[0]), __builtin_bit_cast(uint32_t, int8_pair(c0, 1) * e[1]),
-                              __builtin_bit_cast(uint32_t, int8_pair(c1, 0) * e[2]), __builtin_bit_cast(uint32_t, int8_pair(c1, 1) * e[3])};
-      }
-    }
+    for (int i = 0; i < FMT / 2; ++i) codes[i] = v[(w + i) >> 2][(w + i) & 3];
+    value_pair<FMT>(codes, vs[sw >> 2][sw & 3], vs[sw >> 2][(sw & 3) + 1], lo, hi);
   }
 };
 
