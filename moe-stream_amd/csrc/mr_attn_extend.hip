@@ -343,66 +343,72 @@ struct Quarter {
   uint32_t k[KW], v[NV][VW], ks[FMT == MR_KV_F16 ? 1 : D == 256 ? 2 : 1];
   u32x2 vs[NV];
 
-  template <int N>
-  static __device__ __forceinline__ void words(const uint8_t* p, uint32_t (&to)[N]) {
-    if constexpr (N == 2) {
-      const u32x2 x = *reinterpret_cast<const u32x2*>(p);
-      to[0] = x.x, to[1] = x.y;
-    } else {
-#pragma unroll
-      for (int i = 0; i < N / 4; ++i) {
-        const u32x4 x = *reinterpret_cast<const u32x4*>(p + 1024 * i);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) to[4 * i + j] = x[j];
-      }
-    }
-  }
-  // Keys 16 wave + m; pairs of values NV * wave and on.
-  __device__ __forceinline__ void load(const uint8_t* p, int wave, int lane) {
+  // Load i of the keys 16 wave + m: 16 bytes of codes (or 8), then the scales.
+  static constexpr int kKeyLoads = (KW + 3) / 4 + 1, kValueLoads = NV;
+  __device__ __forceinline__ void load_keys(int i, const uint8_t* p, int wave, int lane) {
     using L = KvLayout<FMT, D>;
     const int m = lane & 15, g = lane >> 4;
     const int kb = wave * KW * 4;  // byte of a lane's keys: pieces of 16 bytes are 1 KB apart
-    words(p + (kb >> 4) * 1024 + lane * 16 + (kb & 15), k);
+    p += (uint32_t)((kb >> 4) * 1024 + (kb & 15));
+    if (i + 1 < kKeyLoads) {
+      if constexpr (KW == 2) {
+        const u32x2 x = *reinterpret_cast<const u32x2*>(p + lane * 16);
+        k[0] = x.x, k[1] = x.y;
+      } else {
+        const u32x4 x = *reinterpret_cast<const u32x4*>(p + 1024 * i + lane * 16);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int vb = (wave * NV + i) * VW * 4;
-      words(p + L::kV + (vb >> 4) * 1024 + lane * 16 + (vb & 15), v[i]);
-    }
-    if constexpr (FMT != MR_KV_F16) {
-#pragma unroll
-      for (int i = 0; i < (D == 256 ? 2 : 1); ++i) {
-        const int blk = D == 64 ? g >> 1 : D == 128 ? g : 2 * g + i;
-        ks[i] = *reinterpret_cast<const uint32_t*>(p + L::kKs + (blk * 16 + m) * 4);
+        for (int j = 0; j < 4; ++j) k[4 * i + j] = x[j];
       }
+    } else if (i < kKeyLoads) {
+      p -= (uint32_t)((kb >> 4) * 1024 + (kb & 15));
 #pragma unroll
-      for (int i = 0; i < NV; ++i) vs[i] = *reinterpret_cast<const u32x2*>(p + L::kVs + g * (D / 2) + (wave * NV + i) * 8);
+      for (int j = 0; j < (D == 256 ? 2 : 1); ++j) {
+        const int blk = D == 64 ? g >> 1 : D == 128 ? g : 2 * g + j;
+        ks[j] = *reinterpret_cast<const uint32_t*>(p + L::kKs + (blk * 16 + m) * 4);
+      }
     }
   }
-  // To the chunk's keys and values in LDS, as operands.
-  __device__ __forceinline__ void store(uint8_t* keys, uint8_t* values, int wave, int lane) const {
+  // Load i of the pairs of values NV * wave and on.
+  __device__ __forceinline__ void load_values(int i, const uint8_t* p, int wave, int lane) {
+    using L = KvLayout<FMT, D>;
+    if (i >= NV) return;
+    const int vb = (wave * NV + i) * VW * 4;
+    const uint8_t* at = p + L::kV + (vb >> 4) * 1024 + (vb & 15) + lane * 16;
+    if constexpr (VW == 2) {
+      const u32x2 x = *reinterpret_cast<const u32x2*>(at);
+      v[i][0] = x.x, v[i][1] = x.y;
+    } else {
+      const u32x4 x = *reinterpret_cast<const u32x4*>(at);
 #pragma unroll
-    for (int i = 0; i < NK; ++i) {
+      for (int j = 0; j < VW; ++j) v[i][j] = x[j & 3];
+    }
+    vs[i] = *reinterpret_cast<const u32x2*>(p + L::kVs + (lane >> 4) * (D / 2) + (wave * NV + i) * 8);
+  }
+  // Item i of the quarter as operands to the chunk's keys and values in LDS (a lane's addresses): first the keys', then the pairs
+  // of values.
+  static constexpr int kItems = NK + NV;
+  __device__ __forceinline__ void store(int i, uint32_t keys, uint32_t values, int wave) const {
+    if (i < NK) {
       u32x4 x;
       const uint32_t s = ks[D == 256 ? i >> 2 : 0];
       if constexpr (FMT == MR_KV_MXFP4) {
         const uint32_t e = exp_bits_of(s, wave), c = k[i];
         x = u32x4{fp4_pair<0>(c, e), fp4_pair<1>(c, e), fp4_pair<2>(c, e), fp4_pair<3>(c, e)};
-      } else {
+      } else if constexpr (FMT == MR_KV_MXINT8) {
         const uint32_t b = s >> (8 * wave) & 0xFFu;
         const f16x2 e = __builtin_bit_cast(f16x2, b << 8 | b << 24);
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[j] = __builtin_bit_cast(uint32_t, int8_pair(k[2 * i + (j >> 1)], j & 1) * e);
       }
-      *reinterpret_cast<u32x4*>(keys + (wave * NK + i) * 1024 + lane * 16) = x;
-    }
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
+      put16(keys + (wave * NK + i) * 1024, x);
+    } else if (i < kItems) {
+      const int j = i - NK;
       u32x4 lo, hi;
-      value_pair<FMT>(v[i], vs[i].x, vs[i].y, lo, hi);
-      uint8_t* to = values + (wave * NV + i) * 2048 + lane * 16;
-      *reinterpret_cast<u32x4*>(to) = lo, *reinterpret_cast<u32x4*>(to + 1024) = hi;
+      value_pair<FMT>(v[j], vs[j].x, vs[j].y, lo, hi);
+      put16(values + (wave * NV + j) * 2048, lo), put16(values + (wave * NV + j) * 2048 + 1024, hi);
     }
   }
+  static __device__ __forceinline__ void put16(uint32_t at, u32x4 x) { *(__attribute__((address_space(3))) u32x4*)(uintptr_t)at = x; }
   static __device__ __forceinline__ uint32_t exp_bits_of(uint32_t s, int wave) { return s >> (8 * wave) << 23; }
 };
 
@@ -424,19 +430,18 @@ __global__ __launch_bounds__(256, (kWidePerSimd<FMT, D>)) void k_attn_extend_wid
   if (!find_unit(a, blockIdx.x, false, u)) return;
   const Reach t = reach_of(a, u);
   const int mine = 32 * wave + n;  // this lane's row of the tile
-  const bool any_rows = 32 * wave < t.rows;
 
-  auto place = [&](uint64_t& row, uint32_t& head) {
+  auto place = [&](int mine, uint64_t& row, uint32_t& head) {
     const uint32_t r = (uint32_t)(t.r0 + min(mine, t.rows - 1)), i = a.group.of(r);
     row = (uint64_t)(u.sp.q0 + (int)i), head = hk * a.group.d + (r - i * a.group.d);
     return u.sp.len - u.sp.n + (int)i;
   };
   uint64_t row;
   uint32_t head;
-  const int pos = place(row, head), from = first_seen(a, pos);
+  const int pos = place(mine, row, head), from = first_seen(a, pos);
   // of the wave's rows: the first one's position, and the last one's first key
   const int wave_pos0 = __builtin_amdgcn_readfirstlane(pos), wave_pos1 = __builtin_amdgcn_readlane(pos, 31);
-  const int wave_first = first_seen(a, wave_pos0), wave_last_first = first_seen(a, wave_pos1);
+  const int wave_last_first = first_seen(a, wave_pos1);
 
   // The query as f16 times a power of two, its largest element in [2^14, 2^15).
   u32x4 qf[NI];
@@ -484,26 +489,26 @@ __global__ __launch_bounds__(256, (kWidePerSimd<FMT, D>)) void k_attn_extend_wid
   };
   Quarter<FMT, D> quarter;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)&lds[0][0][0];
-  auto fetch = [&](int page, int chunk, int b) {
-    const uint8_t* p = a.kv.at(page < 0 ? 0 : page, hk, chunk & (cpp - 1));
-    if constexpr (FMT == MR_KV_F16) {
-#pragma unroll
-      for (int i = 0; i < 2 * kTile / 4096; ++i)
-        load_lds16((uint64_t)p, 2 * kTile, (uint32_t)((i * 4 + wave) * 1024 + lane * 16), lds0 + b * 2 * kTile + (i * 4 + wave) * 1024);
-    } else {
-      quarter.load(p, wave, lane);
-    }
+  const uint64_t page_bytes = ((uint64_t)a.kv.n_heads << (a.kv.page_shift - 6)) * a.kv.chunk;
+  const uint8_t* head_base = a.kv.base + ((uint64_t)hk << (a.kv.page_shift - 6)) * a.kv.chunk;
+  auto address = [&](int page, int chunk) { return head_base + (uint32_t)max(page, 0) * page_bytes + (uint32_t)(chunk & (cpp - 1)) * (uint32_t)a.kv.chunk; };
+  // Loads 4 i + wave of a chunk of f16, straight to buffer b.
+  constexpr int kWhole = 2 * kTile / 4096;
+  auto fetch_whole = [&](int i, const uint8_t* p, int b) {
+    load_lds16((uint64_t)p, 2 * kTile, (uint32_t)((i * 4 + wave) * 1024 + lane * 16), lds0 + b * 2 * kTile + (i * 4 + wave) * 1024);
   };
-  // behind the last chunk's work: the fetched one into buffer b
-  auto arrive = [&](int b) {
-    if constexpr (FMT == MR_KV_F16) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    else quarter.store(lds[b][0], lds[b][1], wave, lane);
+  // Item i of what was fetched, to a lane's address in a buffer: the keys' first, then the values'.
+  constexpr bool kCodes = FMT != MR_KV_F16;
+  constexpr int kKeyItems = kCodes ? Quarter<FMT, D>::NK : 0, kItems = kCodes ? Quarter<FMT, D>::kItems : 0;
+  auto put = [&](int i, uint32_t to) {
+    if constexpr (FMT != MR_KV_F16) quarter.store(i, to, to + kTile, wave);
   };
+  const uint32_t to_at = lds0 + lane * 16;
 
   f32x16 acc[ND];
 #pragma unroll
   for (int x = 0; x < ND; ++x) acc[x] = f32x16{};
-  float ref = 0.f, l = 0.f;  // scores are relative to ref: the largest so far, or up to kWideSlack below it
+  float ref = 0.f, l = 0.f;  // weights are relative to ref, the largest score so far or up to kWideSlack below it
   bool seen = false;
   // addresses of operands: keys 32 T + .., elements of step i; values' elements 32 x + n of 16 keys
   const uint32_t k_at = lds0 + (uint32_t)(((n >> 3) & 1) * (D / 32) * 1024 + (16 * half + ((n >> 4) << 3 | (n & 7))) * 16);
@@ -515,91 +520,165 @@ __global__ __launch_bounds__(256, (kWidePerSimd<FMT, D>)) void k_attn_extend_wid
     return *(const __attribute__((address_space(3))) u32x4*)(uintptr_t)(base + (cc >> 1) * (D / 16) * 1024 + x * 2048 + (cc & 1) * 512);
   };
 
-  int page = -1;
+  // Codes are turned into operands a chunk ahead, between the matrix instructions: keys, fetched two chunks ahead, between those
+  // of the scores, values, one ahead, between those of the sums. f16 goes straight to LDS.
+  int page = -1, page1 = -1, page2 = -1;  // of this chunk and the next two
   if (t.begin < t.end) {
     page = next_page(0);
-    fetch(page, t.begin, 0);
-    arrive(0);
+    const uint8_t* p = address(page, t.begin);
+    if (t.begin + 1 < t.end) page1 = next_page(1);
+    if constexpr (kCodes) {
+      auto load_keys = [&](const uint8_t* p) {
+#pragma unroll
+        for (int x = 0; x < Quarter<FMT, D>::kKeyLoads; ++x) quarter.load_keys(x, p, wave, lane);
+      };
+      load_keys(p);
+#pragma unroll
+      for (int x = 0; x < Quarter<FMT, D>::kValueLoads; ++x) quarter.load_values(x, p, wave, lane);
+#pragma unroll
+      for (int x = 0; x < kItems; ++x) put(x, to_at);
+      load_keys(t.begin + 1 < t.end ? address(page1, t.begin + 1) : p);
+    } else {
+#pragma unroll
+      for (int x = 0; x < kWhole; ++x) fetch_whole(x, p, 0);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
     __syncthreads();
+  }
+  // Where the next chunks' codes come from. Behind the last chunks too, of some chunk that is there: a wait for one load must
+  // know how many others there are behind it.
+  const uint8_t *next = nullptr, *next_keys = nullptr;
+  auto look_ahead = [&](int i, int cidx) {
+    const bool more = cidx + 1 < t.end, far = cidx + 2 < t.end;
+    if (far) page2 = next_page(i + 2);
+    next = address(more ? page1 : page, cidx + more);
+    next_keys = address(far ? page2 : page, far ? cidx + 2 : cidx);
+  };
+  // Load i of the next chunk's values, or of all of it.
+  auto load = [&](int i, int b) {
+    if constexpr (kCodes) quarter.load_values(i, next, wave, lane);
+    else if (i < kWhole) fetch_whole(i, next, b ^ 1);
+  };
+  auto end_step = [&] {
+    if (!kCodes) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    page = page1, page1 = page2;
+  };
+  if (32 * wave >= t.rows) {
+    // a wave without rows has its quarter of the chunks alone
+    for (int i = 0, cidx = t.begin, b = 0; cidx < t.end; ++i, ++cidx, b ^= 1) {
+      look_ahead(i, cidx);
+#pragma unroll
+      for (int x = 0; x < NI; ++x) load(x, b);
+#pragma unroll
+      for (int x = 0; x < kItems; ++x) put(x, to_at + (b ^ 1) * 2 * kTile);
+      if constexpr (kCodes) {
+#pragma unroll
+        for (int x = 0; x < Quarter<FMT, D>::kKeyLoads; ++x) quarter.load_keys(x, next_keys, wave, lane);
+      }
+      end_step();
+    }
+    return;
   }
   for (int i = 0, cidx = t.begin, b = 0; cidx < t.end; ++i, ++cidx, b ^= 1) {
-    const bool there = page >= 0, more = cidx + 1 < t.end;
-    if (more) {
-      page = next_page(i + 1);
-      fetch(page, cidx + 1, b ^ 1);
-    }
+    const bool there = page >= 0;
     const int k0 = cidx << 6;
-    if (any_rows && k0 <= wave_pos1 && k0 + 63 >= wave_first) {
-      uint32_t kb = k_at + b * 2 * kTile, vb = v_at + b * 2 * kTile;
-      asm("" : "+v"(kb), "+v"(vb));  // the parts' addresses are worked out from here, not kept
-      f32x16 s0, s1;
+    look_ahead(i, cidx);
+    uint32_t kb = k_at + b * 2 * kTile, vb = v_at + b * 2 * kTile, to = to_at + (b ^ 1) * 2 * kTile;
+    asm("" : "+v"(kb), "+v"(vb), "+v"(to));  // the parts' addresses are worked out from here, not kept
+    constexpr int kAhead = D == 64 ? 1 : 2;  // operands are read so many pairs of products ahead
+    u32x4 kf[kAhead + 1][2], vf[3], pf[4];
 #pragma unroll
-      for (int x = 0; x < 16; ++x) s0[x] = s1[x] = -ref;
-      __builtin_amdgcn_s_setprio(1);
+    for (int x = 0; x < kAhead; ++x) kf[x][0] = key_part(kb, 0, x), kf[x][1] = key_part(kb, 1, x);
+    f32x16 s0 = {}, s1 = {};
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-      for (int x = 0; x < NI; ++x) {
-        s0 = mfma32(key_part(kb, 0, x), qf[x], s0);
-        s1 = mfma32(key_part(kb, 1, x), qf[x], s1);
+    for (int x = 0; x < NI; ++x) {
+      if (x + kAhead < NI) {
+        kf[(x + kAhead) % (kAhead + 1)][0] = key_part(kb, 0, x + kAhead);
+        kf[(x + kAhead) % (kAhead + 1)][1] = key_part(kb, 1, x + kAhead);
       }
-      __builtin_amdgcn_s_setprio(0);
-      if (!there || k0 + 63 > wave_pos0 || k0 < wave_last_first) {
-        // bit i: the row sees key k0 + i
-        int most = pos - k0, least = from - k0;
-        asm volatile("" : "+v"(most));  // a branch: the compiler would do this in every step
-        uint64_t sees = (most < 0 ? 0 : ~0ull >> (63 - min(most, 63))) & (least > 63 ? 0 : ~0ull << max(least, 0));
-        if (!there) sees = 0;
-        sees >>= 4 * half;
-        const uint32_t sees0 = (uint32_t)sees, sees1 = (uint32_t)(sees >> 32);
-#pragma unroll
-        for (int x = 0; x < 16; ++x) {
-          const int at = 16 * ((x >> 2) & 1) + 8 * (x >> 3) + (x & 3);
-          s0[x] = seen_or_least(s0[x], sees0, at);
-          s1[x] = seen_or_least(s1[x], sees1, at);
-        }
-      }
-      float top = s0[0];
-#pragma unroll
-      for (int x = 0; x < 16; ++x) top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, s0[x]), s1[x]);
-      top = max_xor32(top);
-      const bool move = top * c > kWideSlack || (!seen && top > -INFINITY);
-      if (__any(move)) {
-        const float by = move ? top : 0.f, f = !seen ? 0.f : __builtin_amdgcn_exp2f(-by * c);
-        if (move) {
-          l *= f;
-#pragma unroll
-          for (int x = 0; x < ND; ++x) acc[x] *= f;
-#pragma unroll
-          for (int x = 0; x < 16; ++x) s0[x] -= by, s1[x] -= by;
-          ref += by;
-          seen = true;
-        }
-      }
-      u32x4 pf[4];
+      if (x >= NI - 2) vf[x - (NI - 2)] = value_part(vb, 0, x - (NI - 2));
+      s0 = mfma32(kf[x % (kAhead + 1)][0], qf[x], s0);
+      load(x, b);  // between the matrix instructions: waves that wait for their turn to load would keep them waiting
+      s1 = mfma32(kf[x % (kAhead + 1)][1], qf[x], s1);
+      if (x < kKeyItems) put(x, to);  // behind the last chunk too, of what was fetched last: nobody reads it
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    __builtin_amdgcn_s_setprio(0);
+    if (!there || k0 + 63 > wave_pos0 || k0 < wave_last_first) {
+      // bit i: the row sees key k0 + i
+      int most = pos - k0, least = from - k0;
+      asm volatile("" : "+v"(most));  // a branch: the compiler would do this in every step
+      uint64_t sees = (most < 0 ? 0 : ~0ull >> (63 - min(most, 63))) & (least > 63 ? 0 : ~0ull << max(least, 0));
+      if (!there) sees = 0;
+      sees >>= 4 * half;
+      const uint32_t sees0 = (uint32_t)sees, sees1 = (uint32_t)(sees >> 32);
 #pragma unroll
       for (int x = 0; x < 16; ++x) {
-        const f32x16& s = x < 8 ? s0 : s1;
-        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[2 * (x & 7)], c, kWideLift)), p1 = __builtin_amdgcn_exp2f(fmaf(s[2 * (x & 7) + 1], c, kWideLift));
-        const uint32_t w = pack_f16(p0, p1);
-        pf[x >> 2][x & 3] = w;
-        l = add_f16(w, l);
+        const int at = 16 * ((x >> 2) & 1) + 8 * (x >> 3) + (x & 3);
+        s0[x] = seen_or_least(s0[x], sees0, at);
+        s1[x] = seen_or_least(s1[x], sees1, at);
       }
-      __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-      for (int cc = 0; cc < 4; ++cc)
-#pragma unroll
-        for (int x = 0; x < ND; ++x) acc[x] = mfma32(value_part(vb, cc, x), pf[cc], acc[x]);
-      __builtin_amdgcn_s_setprio(0);
     }
-    if (more) arrive(b ^ 1);
-    __syncthreads();
+    float top = s0[0];
+#pragma unroll
+    for (int x = 0; x < 16; ++x) top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, s0[x]), s1[x]);
+    top = max_xor32(top);
+    const bool move = (top - ref) * c > kWideSlack || (!seen && top > -INFINITY);
+    if (__any(move)) {
+      const float f = !move ? 1.f : !seen ? 0.f : __builtin_amdgcn_exp2f((ref - top) * c);
+      l *= f;
+#pragma unroll
+      for (int x = 0; x < ND; ++x) {
+        acc[x] *= f;
+        if (D == 256) __builtin_amdgcn_sched_barrier(0);
+      }
+      ref = move ? top : ref;
+      seen |= move;
+    }
+    auto weigh = [&](int x) {
+      const f32x16& s = x < 8 ? s0 : s1;
+      const float p0 = __builtin_amdgcn_exp2f(fmaf(s[2 * (x & 7)] - ref, c, kWideLift));
+      const float p1 = __builtin_amdgcn_exp2f(fmaf(s[2 * (x & 7) + 1] - ref, c, kWideLift));
+      const uint32_t w = pack_f16(p0, p1);
+      pf[x >> 2][x & 3] = w;
+      l = add_f16(w, l);
+    };
+#pragma unroll
+    for (int x = 0; x < 4; ++x) weigh(x);
+    constexpr int NV = 4 * ND;
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int q = 0; q < NV; ++q) {
+      if (q + 2 < NV) vf[(q + 2) % 3] = value_part(vb, (q + 2) / ND, (q + 2) % ND);
+      acc[q % ND] = mfma32(vf[q % 3], pf[q / ND], acc[q % ND]);
+      // the next 16 keys' weights
+      if (q / ND < 3) {
+#pragma unroll
+        for (int x = 4 * (q / ND + 1) + q % ND * 4 / ND; x < 4 * (q / ND + 1) + (q % ND + 1) * 4 / ND; ++x) weigh(x);
+      }
+      if constexpr (kCodes) {
+        if (q < Quarter<FMT, D>::kKeyLoads) quarter.load_keys(q, next_keys, wave, lane);
+      }
+      // the values in the second half, when their codes have come
+      constexpr int kEach = NV / 2 / (kItems - kKeyItems + !kCodes);
+      if (kCodes && q >= NV / 2 && (q - NV / 2) % kEach == 0) put(kKeyItems + (q - NV / 2) / kEach, to);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    __builtin_amdgcn_s_setprio(0);
+    end_step();
   }
 
-  if (mine >= t.rows) return;
   l = add_xor32(l);
+  int after = mine;
+  asm volatile("" : "+v"(after));  // the row's place is worked out again here, not kept through the steps
+  if (after >= t.rows) return;
+  place(after, row, head);
   const float m = !seen ? -INFINITY : fminf(fmaxf(ref * c, -kLargest), kLargest) - kWideLift;
   // this lane's elements: 32 x + 8 (i / 4) + 4 half + i % 4
   if (u.parts > 1) {
-    const uint64_t unit = (((uint64_t)(u.slot + u.part) * a.kv.n_heads + hk) << a.bits) + mine;
+    const uint64_t unit = (((uint64_t)(u.slot + u.part) * a.kv.n_heads + hk) << a.bits) + after;
     float* dst = a.part + unit * D + 4 * half;
 #pragma unroll
     for (int x = 0; x < ND; ++x)
