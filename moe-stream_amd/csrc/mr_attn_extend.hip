@@ -417,7 +417,7 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
 }
 
 template <int FMT, int D>
-constexpr int kWidePerSimd = D == 256 ? 1 : D == 128 ? 2 : 3;
+constexpr int kWidePerSimd = D == 256 ? 1 : D == 128 ? 2 : FMT == MR_KV_MXINT8 ? 3 : 4;
 
 template <int FMT, int D>
 __global__ __launch_bounds__(256, (kWidePerSimd<FMT, D>)) void k_attn_extend_wide(ExtendArgs a) {
@@ -508,7 +508,11 @@ __global__ __launch_bounds__(256, (kWidePerSimd<FMT, D>)) void k_attn_extend_wid
   f32x16 acc[ND];
 #pragma unroll
   for (int x = 0; x < ND; ++x) acc[x] = f32x16{};
-  float ref = 0.f, l = 0.f;  // weights are relative to ref, the largest score so far or up to kWideSlack below it
+  // Weights are 2^(s c - base): relative to ref, the largest score so far or up to kWideSlack below it, base = ref c - kWideLift. With one
+  // rounding of s c - base they are right to their own size, however base was rounded; that rounding is the same factor for
+  // all of a row's. Where it could be 2^-12 or more, ref is taken from the scores first.
+  constexpr float kNear = 0x1p12f;
+  float ref = 0.f, base = -kWideLift, l = 0.f;
   bool seen = false;
   // addresses of operands: keys 32 T + .., elements of step i; values' elements 32 x + n of 16 keys
   const uint32_t k_at = lds0 + (uint32_t)(((n >> 3) & 1) * (D / 32) * 1024 + (16 * half + ((n >> 4) << 3 | (n & 7))) * 16);
@@ -606,6 +610,7 @@ __global__ __launch_bounds__(256, (kWidePerSimd<FMT, D>)) void k_attn_extend_wid
       __builtin_amdgcn_sched_barrier(0);
     }
     __builtin_amdgcn_s_setprio(0);
+    if constexpr (D == 256) asm("" : "+v"(s0), "+v"(s1));  // moved out of the accumulators' registers once
     if (!there || k0 + 63 > wave_pos0 || k0 < wave_last_first) {
       // bit i: the row sees key k0 + i
       int most = pos - k0, least = from - k0;
@@ -627,20 +632,28 @@ __global__ __launch_bounds__(256, (kWidePerSimd<FMT, D>)) void k_attn_extend_wid
     top = max_xor32(top);
     const bool move = (top - ref) * c > kWideSlack || (!seen && top > -INFINITY);
     if (__any(move)) {
-      const float f = !move ? 1.f : !seen ? 0.f : __builtin_amdgcn_exp2f((ref - top) * c);
+      const float next_base = fabsf(top * c) < kNear ? fmaf(top, c, -kWideLift) : -kWideLift;
+      const bool near = fabsf(top * c) < kNear && fabsf(ref * c) < kNear;
+      const float f = !move ? 1.f : !seen ? 0.f : __builtin_amdgcn_exp2f(near ? base - next_base : (ref - top) * c);
       l *= f;
 #pragma unroll
       for (int x = 0; x < ND; ++x) {
+        if constexpr (D == 256) asm volatile("" : "+a"(acc[x]));  // read here, not in every step
         acc[x] *= f;
-        if (D == 256) __builtin_amdgcn_sched_barrier(0);
       }
-      ref = move ? top : ref;
+      ref = move ? top : ref, base = move ? next_base : base;
       seen |= move;
+    }
+    const bool far_off = fabsf(ref * c) >= kNear;
+    if (__any(far_off)) {
+      const float off = far_off ? ref : 0.f;
+#pragma unroll
+      for (int x = 0; x < 16; ++x) s0[x] -= off, s1[x] -= off;
     }
     auto weigh = [&](int x) {
       const f32x16& s = x < 8 ? s0 : s1;
-      const float p0 = __builtin_amdgcn_exp2f(fmaf(s[2 * (x & 7)] - ref, c, kWideLift));
-      const float p1 = __builtin_amdgcn_exp2f(fmaf(s[2 * (x & 7) + 1] - ref, c, kWideLift));
+      const float p0 = __builtin_amdgcn_exp2f(fmaf(s[2 * (x & 7)], c, -base));
+      const float p1 = __builtin_amdgcn_exp2f(fmaf(s[2 * (x & 7) + 1], c, -base));
       const uint32_t w = pack_f16(p0, p1);
       pf[x >> 2][x & 3] = w;
       l = add_f16(w, l);
@@ -675,7 +688,7 @@ __global__ __launch_bounds__(256, (kWidePerSimd<FMT, D>)) void k_attn_extend_wid
   asm volatile("" : "+v"(after));  // the row's place is worked out again here, not kept through the steps
   if (after >= t.rows) return;
   place(after, row, head);
-  const float m = !seen ? -INFINITY : fminf(fmaxf(ref * c, -kLargest), kLargest) - kWideLift;
+  const float m = !seen ? -INFINITY : fabsf(ref * c) < kNear ? base : fminf(fmaxf(ref * c, -kLargest), kLargest) - kWideLift;
   // this lane's elements: 32 x + 8 (i / 4) + 4 half + i % 4
   if (u.parts > 1) {
     const uint64_t unit = (((uint64_t)(u.slot + u.part) * a.kv.n_heads + hk) << a.bits) + after;
