@@ -419,7 +419,9 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
 template <int FMT, int D>
 constexpr int kWidePerSimd = D == 256 ? 1 : D == 128 ? 2 : FMT == MR_KV_MXINT8 ? 3 : 4;
 
-template <int FMT, int D>
+// KH: how many of a chunk's halves of 32 keys a wave has: both, or, in tiles of 64 rows, two waves one each of the same rows, whose
+// results are joined at the end.
+template <int FMT, int D, int KH>
 __global__ __launch_bounds__(256, (kWidePerSimd<FMT, D>)) void k_attn_extend_wide(ExtendArgs a) {
   constexpr int ND = D / 32, NI = D / 16, kTile = 64 * D * 2;  // bytes of a chunk's keys as operands
   __shared__ __attribute__((aligned(16))) uint8_t lds[2][2][kTile];
@@ -429,7 +431,8 @@ __global__ __launch_bounds__(256, (kWidePerSimd<FMT, D>)) void k_attn_extend_wid
   Unit u;
   if (!find_unit(a, blockIdx.x, false, u)) return;
   const Reach t = reach_of(a, u);
-  const int mine = 32 * wave + n;  // this lane's row of the tile
+  const int block = KH == 2 ? wave : wave & 1, first_half = KH == 2 ? 0 : wave >> 1;
+  const int mine = 32 * block + n;  // this lane's row of the tile
 
   auto place = [&](int mine, uint64_t& row, uint32_t& head) {
     const uint32_t r = (uint32_t)(t.r0 + min(mine, t.rows - 1)), i = a.group.of(r);
@@ -515,8 +518,8 @@ __global__ __launch_bounds__(256, (kWidePerSimd<FMT, D>)) void k_attn_extend_wid
   float ref = 0.f, base = -kWideLift, l = 0.f;
   bool seen = false;
   // addresses of operands: keys 32 T + .., elements of step i; values' elements 32 x + n of 16 keys
-  const uint32_t k_at = lds0 + (uint32_t)(((n >> 3) & 1) * (D / 32) * 1024 + (16 * half + ((n >> 4) << 3 | (n & 7))) * 16);
-  const uint32_t v_at = lds0 + kTile + (uint32_t)((n >> 4) * 1024 + (16 * half + (n & 15)) * 16);
+  const uint32_t k_at = lds0 + first_half * (D / 16) * 1024 + (uint32_t)(((n >> 3) & 1) * (D / 32) * 1024 + (16 * half + ((n >> 4) << 3 | (n & 7))) * 16);
+  const uint32_t v_at = lds0 + kTile + first_half * (D / 16) * 1024 + (uint32_t)((n >> 4) * 1024 + (16 * half + (n & 15)) * 16);
   auto key_part = [&](uint32_t base, int T, int i) {
     return *(const __attribute__((address_space(3))) u32x4*)(uintptr_t)(base + T * (D / 16) * 1024 + (i >> 1) * 1024 + (i & 1) * 512);
   };
@@ -568,7 +571,7 @@ __global__ __launch_bounds__(256, (kWidePerSimd<FMT, D>)) void k_attn_extend_wid
     __syncthreads();
     page = page1, page1 = page2;
   };
-  if (32 * wave >= t.rows) {
+  if (32 * block >= t.rows) {
     // a wave without rows has its quarter of the chunks alone
     for (int i = 0, cidx = t.begin, b = 0; cidx < t.end; ++i, ++cidx, b ^= 1) {
       look_ahead(i, cidx);
@@ -582,6 +585,7 @@ __global__ __launch_bounds__(256, (kWidePerSimd<FMT, D>)) void k_attn_extend_wid
       }
       end_step();
     }
+    if (KH == 1) __syncthreads();
     return;
   }
   for (int i = 0, cidx = t.begin, b = 0; cidx < t.end; ++i, ++cidx, b ^= 1) {
@@ -591,29 +595,34 @@ __global__ __launch_bounds__(256, (kWidePerSimd<FMT, D>)) void k_attn_extend_wid
     uint32_t kb = k_at + b * 2 * kTile, vb = v_at + b * 2 * kTile, to = to_at + (b ^ 1) * 2 * kTile;
     asm("" : "+v"(kb), "+v"(vb), "+v"(to));  // the parts' addresses are worked out from here, not kept
     constexpr int kAhead = D == 64 ? 1 : 2;  // operands are read so many pairs of products ahead
-    u32x4 kf[kAhead + 1][2], vf[3], pf[4];
+    u32x4 kf[kAhead + 1][KH], vf[3], pf[2 * KH];
 #pragma unroll
-    for (int x = 0; x < kAhead; ++x) kf[x][0] = key_part(kb, 0, x), kf[x][1] = key_part(kb, 1, x);
-    f32x16 s0 = {}, s1 = {};
+    for (int x = 0; x < kAhead; ++x)
+#pragma unroll
+      for (int y = 0; y < KH; ++y) kf[x][y] = key_part(kb, y, x);
+    f32x16 s[KH] = {};
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int x = 0; x < NI; ++x) {
       if (x + kAhead < NI) {
-        kf[(x + kAhead) % (kAhead + 1)][0] = key_part(kb, 0, x + kAhead);
-        kf[(x + kAhead) % (kAhead + 1)][1] = key_part(kb, 1, x + kAhead);
+#pragma unroll
+        for (int y = 0; y < KH; ++y) kf[(x + kAhead) % (kAhead + 1)][y] = key_part(kb, y, x + kAhead);
       }
       if (x >= NI - 2) vf[x - (NI - 2)] = value_part(vb, 0, x - (NI - 2));
-      s0 = mfma32(kf[x % (kAhead + 1)][0], qf[x], s0);
+      s[0] = mfma32(kf[x % (kAhead + 1)][0], qf[x], s[0]);
       load(x, b);  // between the matrix instructions: waves that wait for their turn to load would keep them waiting
-      s1 = mfma32(kf[x % (kAhead + 1)][1], qf[x], s1);
+      if constexpr (KH == 2) s[1] = mfma32(kf[x % (kAhead + 1)][1], qf[x], s[1]);
       if (x < kKeyItems) put(x, to);  // behind the last chunk too, of what was fetched last: nobody reads it
       __builtin_amdgcn_sched_barrier(0);
     }
     __builtin_amdgcn_s_setprio(0);
-    if constexpr (D == 256) asm("" : "+v"(s0), "+v"(s1));  // moved out of the accumulators' registers once
+    if constexpr (D == 256) {  // moved out of the accumulators' registers once
+#pragma unroll
+      for (int y = 0; y < KH; ++y) asm("" : "+v"(s[y]));
+    }
     if (!there || k0 + 63 > wave_pos0 || k0 < wave_last_first) {
-      // bit i: the row sees key k0 + i
-      int most = pos - k0, least = from - k0;
+      // bit i: the row sees the i-th key of the wave's
+      int most = pos - k0 - 32 * first_half, least = from - k0 - 32 * first_half;
       asm volatile("" : "+v"(most));  // a branch: the compiler would do this in every step
       uint64_t sees = (most < 0 ? 0 : ~0ull >> (63 - min(most, 63))) & (least > 63 ? 0 : ~0ull << max(least, 0));
       if (!there) sees = 0;
@@ -622,13 +631,19 @@ __global__ __launch_bounds__(256, (kWidePerSimd<FMT, D>)) void k_attn_extend_wid
 #pragma unroll
       for (int x = 0; x < 16; ++x) {
         const int at = 16 * ((x >> 2) & 1) + 8 * (x >> 3) + (x & 3);
-        s0[x] = seen_or_least(s0[x], sees0, at);
-        s1[x] = seen_or_least(s1[x], sees1, at);
+        s[0][x] = seen_or_least(s[0][x], sees0, at);
+        if (KH == 2) s[KH - 1][x] = seen_or_least(s[KH - 1][x], sees1, at);
       }
     }
-    float top = s0[0];
+    // two chains, so that one does not wait for itself
+    float top = s[0][0], top2 = s[0][1];
 #pragma unroll
-    for (int x = 0; x < 16; ++x) top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, s0[x]), s1[x]);
+    for (int x = 0; x < 16 * KH; x += 4) {
+      const f32x16& y = s[x / 16];
+      top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, y[x % 16]), y[x % 16 + 2]);
+      top2 = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top2, y[x % 16 + 1]), y[x % 16 + 3]);
+    }
+    top = __builtin_elementwise_maximum(top, top2);
     top = max_xor32(top);
     const bool move = (top - ref) * c > kWideSlack || (!seen && top > -INFINITY);
     if (__any(move)) {
@@ -648,26 +663,26 @@ __global__ __launch_bounds__(256, (kWidePerSimd<FMT, D>)) void k_attn_extend_wid
     if (__any(far_off)) {
       const float off = far_off ? ref : 0.f;
 #pragma unroll
-      for (int x = 0; x < 16; ++x) s0[x] -= off, s1[x] -= off;
+      for (int x = 0; x < 16 * KH; ++x) s[x / 16][x % 16] -= off;
     }
     auto weigh = [&](int x) {
-      const f32x16& s = x < 8 ? s0 : s1;
-      const float p0 = __builtin_amdgcn_exp2f(fmaf(s[2 * (x & 7)], c, -base));
-      const float p1 = __builtin_amdgcn_exp2f(fmaf(s[2 * (x & 7) + 1], c, -base));
+      const f32x16& y = s[x / 8];
+      const float p0 = __builtin_amdgcn_exp2f(fmaf(y[2 * (x & 7)], c, -base));
+      const float p1 = __builtin_amdgcn_exp2f(fmaf(y[2 * (x & 7) + 1], c, -base));
       const uint32_t w = pack_f16(p0, p1);
       pf[x >> 2][x & 3] = w;
       l = add_f16(w, l);
     };
 #pragma unroll
     for (int x = 0; x < 4; ++x) weigh(x);
-    constexpr int NV = 4 * ND;
+    constexpr int NV = 2 * KH * ND;
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int q = 0; q < NV; ++q) {
       if (q + 2 < NV) vf[(q + 2) % 3] = value_part(vb, (q + 2) / ND, (q + 2) % ND);
       acc[q % ND] = mfma32(vf[q % 3], pf[q / ND], acc[q % ND]);
       // the next 16 keys' weights
-      if (q / ND < 3) {
+      if (q / ND < 2 * KH - 1) {
 #pragma unroll
         for (int x = 4 * (q / ND + 1) + q % ND * 4 / ND; x < 4 * (q / ND + 1) + (q % ND + 1) * 4 / ND; ++x) weigh(x);
       }
@@ -684,11 +699,27 @@ __global__ __launch_bounds__(256, (kWidePerSimd<FMT, D>)) void k_attn_extend_wid
   }
 
   l = add_xor32(l);
+  float m = !seen ? -INFINITY : fabsf(ref * c) < kNear ? base : fminf(fmaxf(ref * c, -kLargest), kLargest) - kWideLift;
+  if constexpr (KH == 1) {
+    // the second halves' results through LDS: number x of lane i at 64 x + i
+    float* other = reinterpret_cast<float*>(&lds[0][0][0]) + block * (ND * 16 + 2) * 64 + lane;
+    if (first_half) {
+#pragma unroll
+      for (int x = 0; x < 16 * ND; ++x) other[64 * x] = acc[x / 16][x % 16];
+      other[64 * 16 * ND] = m, other[64 * (16 * ND + 1)] = l;
+    }
+    __syncthreads();
+    if (first_half) return;
+    const float m2 = other[64 * 16 * ND], l2 = other[64 * (16 * ND + 1)], m1 = fmaxf(m, m2);
+    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m1), f2 = m2 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m2 - m1);
+#pragma unroll
+    for (int x = 0; x < 16 * ND; ++x) acc[x / 16][x % 16] = acc[x / 16][x % 16] * f + other[64 * x] * f2;
+    l = l * f + l2 * f2, m = m1;
+  }
   int after = mine;
   asm volatile("" : "+v"(after));  // the row's place is worked out again here, not kept through the steps
   if (after >= t.rows) return;
   place(after, row, head);
-  const float m = !seen ? -INFINITY : fabsf(ref * c) < kNear ? base : fminf(fmaxf(ref * c, -kLargest), kLargest) - kWideLift;
   // this lane's elements: 32 x + 8 (i / 4) + 4 half + i % 4
   if (u.parts > 1) {
     const uint64_t unit = (((uint64_t)(u.slot + u.part) * a.kv.n_heads + hk) << a.bits) + after;
@@ -758,7 +789,8 @@ using ExtendKernel = void (*)(ExtendArgs);
 template <int NT, int FMT, int D>
 ExtendKernel pick(int& per_cu) {
   constexpr ExtendKernel kernel = [] {
-    if constexpr (NT == 8) return k_attn_extend_wide<FMT, D>;
+    if constexpr (NT == 8) return k_attn_extend_wide<FMT, D, 2>;
+    else if constexpr (NT == 4) return k_attn_extend_wide<FMT, D, 1>;
     else return k_attn_extend<NT, FMT, D>;
   }();
   static const int n = [] {
@@ -770,7 +802,10 @@ ExtendKernel pick(int& per_cu) {
 }
 template <int FMT, int D>
 ExtendKernel pick(int bits, int& per_cu) {
-  return bits == 4 ? pick<1, FMT, D>(per_cu) : bits == 5 ? pick<2, FMT, D>(per_cu) : pick<8, FMT, D>(per_cu);
+  return bits == 4   ? pick<1, FMT, D>(per_cu)
+         : bits == 5 ? pick<2, FMT, D>(per_cu)
+         : bits == 6 ? pick<4, FMT, D>(per_cu)
+                     : pick<8, FMT, D>(per_cu);
 }
 template <int FMT>
 ExtendKernel pick(uint32_t D, int bits, int& per_cu) {
@@ -787,12 +822,15 @@ hipError_t launch_attn_extend(const Launch& K, const KvPages& kv, uint32_t forma
                               int n_cu) {
   const uint32_t group = q.n / kv.n_heads;
   const uint64_t rows = (uint64_t)nq * group;
-  int bits = rows <= 16ull * n_seqs ? 4 : rows <= 32ull * n_seqs ? 5 : 7, per_cu = 1;
+  const int bits = rows <= 16ull * n_seqs ? 4 : rows <= 32ull * n_seqs ? 5 : rows <= 64ull * n_seqs ? 6 : 7;
+  int per_cu = 1;
   const ExtendKernel kernel = format == MR_KV_F16      ? pick<MR_KV_F16>(D, bits, per_cu)
                               : format == MR_KV_MXINT8 ? pick<MR_KV_MXINT8>(D, bits, per_cu)
                                                        : pick<MR_KV_MXFP4>(D, bits, per_cu);
   ExtendArgs a{kv, q, out, cu, len, table, max_pages, n_seqs, (int)nq, Divisor(group), bits, 0, o, err, scratch};
-  const uint64_t cap = (uint64_t)max_pages << (kv.page_shift - 6);
+  // chunks that a tile sees at most
+  const uint64_t pages = (uint64_t)max_pages << (kv.page_shift - 6);
+  const uint64_t cap = o.window ? std::min<uint64_t>(pages, (o.window + ((1ull << bits) / group + 1) + 62) / 64 + 1) : pages;
   const uint64_t tiles = (rows >> bits) + n_seqs;  // at most
   const uint32_t room = std::min<uint32_t>(kScratchRows >> bits, per_cu * n_cu);
   // the chunks of all tiles are counted in 32 bits

@@ -86,6 +86,11 @@ CASES = [
     (256, 1, 8, 64, [33, 1], [40, 200], 0, False),
     (64, 1, 2, 64, [130], [1300], 1, False),      # only itself
     (128, 1, 4, 64, [200, 3], [264, 320], 200, True),
+    (64, 1, 8, 64, [6, 5], [500, 64], 0, True),
+    (64, 2, 4, 128, [9, 13, 0, 16], [2000, 13, 5, 700], 0, False),
+    (128, 1, 8, 64, [6, 8, 5], [3000, 40, 5], 0, True),
+    (256, 1, 8, 64, [5, 6, 7], [400, 130, 7], 0, True),
+    (256, 2, 8, 64, [3], [1500], 100, False),
 ]
 
 
