@@ -51,14 +51,16 @@ __device__ __forceinline__ Span span_of(const ExtendArgs& a, uint32_t b) {
   return s;
 }
 
-// Unit `i`: a tile of a sequence and a part of its keys. split_only: tile i of the sequences of several parts, whose
-// part is then 0. slot: parts of split sequences in front of the tile's.
+// A workgroup's unit: a tile of a sequence, a part of its keys and a key head. split_only: tile blockIdx.x of the sequences of several
+// parts and key head blockIdx.y; the part is then 0. slot: parts of split sequences in front of the tile's.
 struct Unit {
-  uint32_t b, tile, part, parts, slot;
+  uint32_t b, hk, tile, part, parts, slot;
   Span sp;
 };
-__device__ __forceinline__ bool find_unit(const ExtendArgs& a, uint32_t i, bool split_only, Unit& r) {
+__device__ __forceinline__ bool find_unit(const ExtendArgs& a, bool split_only, Unit& r) {
   const uint32_t lane = threadIdx.x & 63;
+  uint32_t i = blockIdx.x;
+  r.hk = blockIdx.y;
   if (a.parts == 1) {
     if (split_only) return false;
     r.b = find_seq(a.cu, a.n_seqs, a.nq, a.group.d, a.bits, i);
@@ -83,6 +85,16 @@ __device__ __forceinline__ bool find_unit(const ExtendArgs& a, uint32_t i, bool 
   const uint32_t most = max(a.parts, tiles + a.parts / 2);
   uint32_t size = max(kMinPart, (all + a.parts - 1) / a.parts);
   while (size < all && sum_of([&](uint32_t t, uint32_t c) { return t * max(1u, (c + size - 1) / size); }) > most) size += (size + 7) / 8;
+  if (!split_only) {
+    // Workgroups go to the 8 XCDs in turn: each gets an eighth of the units, in their order, so that the tiles that read the same keys
+    // find them in one L2 (four prompts' parts, f16, 32 heads on 4: 184 us without, XX so).
+    const uint32_t units = __builtin_amdgcn_readfirstlane(sum_of([&](uint32_t t, uint32_t c) { return t * max(1u, (c + size - 1) / size); }));
+    const uint32_t per = (units * a.kv.n_heads + 7) / 8, at = blockIdx.y * gridDim.x + blockIdx.x;
+    if (at >> 3 >= per) return false;
+    i = (at & 7) * per + (at >> 3);
+    r.hk = __builtin_amdgcn_readfirstlane(i / units), i -= r.hk * units;
+    if (r.hk >= a.kv.n_heads) return false;
+  }
   uint32_t before = 0, slots = 0;
   for (uint32_t b0 = 0; b0 < a.n_seqs; b0 += 64) {
     if (b0) s = b0 + lane < a.n_seqs ? span_of(a, b0 + lane) : Span{};
@@ -95,8 +107,9 @@ __device__ __forceinline__ bool find_unit(const ExtendArgs& a, uint32_t i, bool 
       r.b = b0 + l;
       r.parts = __builtin_amdgcn_readlane(parts, l);
       const uint32_t in = i - before - __builtin_amdgcn_readlane(sum - count, l);
-      r.tile = split_only ? in : in / r.parts;
-      r.part = split_only ? 0 : in - r.tile * r.parts;
+      const uint32_t tiles = (uint32_t)__builtin_amdgcn_readlane(s.tiles, l);
+      r.part = split_only ? 0 : in / tiles;  // the tiles of a part one after the other
+      r.tile = in - r.part * tiles;
       r.slot = slots + __builtin_amdgcn_readlane(ssum - split, l) + r.tile * r.parts;
       r.sp = Span{__builtin_amdgcn_readlane(s.q0, l), __builtin_amdgcn_readlane(s.n, l), __builtin_amdgcn_readlane(s.len, l),
                   __builtin_amdgcn_readlane(s.c0, l), __builtin_amdgcn_readlane(s.chunks, l),
@@ -145,10 +158,10 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<NT, FMT, D>)) void k_attn_ex
   __shared__ __attribute__((aligned(16))) float sums[kWaves / 2][16 * D];
   __shared__ float stats[kWaves / 2][16][2];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-  const uint32_t hk = blockIdx.y;
-  if (blockIdx.x == 0 && hk == 0) check_entries(a);
+  if (blockIdx.x == 0 && blockIdx.y == 0) check_entries(a);
   Unit u;
-  if (!find_unit(a, blockIdx.x, false, u)) return;
+  if (!find_unit(a, false, u)) return;
+  const uint32_t hk = u.hk;
   const Reach t = reach_of(a, u);
 
   // This lane's row of each 16: its place in q and out, and which keys it sees. The query as f16 times a power of
@@ -426,10 +439,10 @@ __global__ __launch_bounds__(256, (kWidePerSimd<FMT, D>)) void k_attn_extend_wid
   constexpr int ND = D / 32, NI = D / 16, kTile = 64 * D * 2;  // bytes of a chunk's keys as operands
   __shared__ __attribute__((aligned(16))) uint8_t lds[2][2][kTile];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 31, half = lane >> 5;
-  const uint32_t hk = blockIdx.y;
-  if (blockIdx.x == 0 && hk == 0) check_entries(a);
+  if (blockIdx.x == 0 && blockIdx.y == 0) check_entries(a);
   Unit u;
-  if (!find_unit(a, blockIdx.x, false, u)) return;
+  if (!find_unit(a, false, u)) return;
+  const uint32_t hk = u.hk;
   const Reach t = reach_of(a, u);
   const int block = KH == 2 ? wave : wave & 1, first_half = KH == 2 ? 0 : wave >> 1;
   const int mine = 32 * block + n;  // this lane's row of the tile
@@ -527,8 +540,8 @@ __global__ __launch_bounds__(256, (kWidePerSimd<FMT, D>)) void k_attn_extend_wid
     return *(const __attribute__((address_space(3))) u32x4*)(uintptr_t)(base + (cc >> 1) * (D / 16) * 1024 + x * 2048 + (cc & 1) * 512);
   };
 
-  // Codes are turned into operands a chunk ahead, between the matrix instructions: keys, fetched two chunks ahead, between those
-  // of the scores, values, one ahead, between those of the sums. f16 goes straight to LDS.
+  // Codes are fetched two chunks ahead and turned into operands one ahead, between the matrix instructions: keys between those of
+  // the scores, values between those of the sums. f16 goes straight to LDS, one ahead.
   int page = -1, page1 = -1, page2 = -1;  // of this chunk and the next two
   if (t.begin < t.end) {
     page = next_page(0);
@@ -544,7 +557,10 @@ __global__ __launch_bounds__(256, (kWidePerSimd<FMT, D>)) void k_attn_extend_wid
       for (int x = 0; x < Quarter<FMT, D>::kValueLoads; ++x) quarter.load_values(x, p, wave, lane);
 #pragma unroll
       for (int x = 0; x < kItems; ++x) put(x, to_at);
-      load_keys(t.begin + 1 < t.end ? address(page1, t.begin + 1) : p);
+      p = t.begin + 1 < t.end ? address(page1, t.begin + 1) : p;
+      load_keys(p);
+#pragma unroll
+      for (int x = 0; x < Quarter<FMT, D>::kValueLoads; ++x) quarter.load_values(x, p, wave, lane);
     } else {
 #pragma unroll
       for (int x = 0; x < kWhole; ++x) fetch_whole(x, p, 0);
@@ -554,20 +570,32 @@ __global__ __launch_bounds__(256, (kWidePerSimd<FMT, D>)) void k_attn_extend_wid
   }
   // Where the next chunks' codes come from. Behind the last chunks too, of some chunk that is there: a wait for one load must
   // know how many others there are behind it.
-  const uint8_t *next = nullptr, *next_keys = nullptr;
+  const uint8_t *next = nullptr, *far = nullptr;  // of the next chunk, of the one after it
+  uint32_t warm[2] = {};
   auto look_ahead = [&](int i, int cidx) {
-    const bool more = cidx + 1 < t.end, far = cidx + 2 < t.end;
-    if (far) page2 = next_page(i + 2);
+    const bool more = cidx + 1 < t.end, more2 = cidx + 2 < t.end;
+    if (more2) page2 = next_page(i + 2);
     next = address(more ? page1 : page, cidx + more);
-    next_keys = address(far ? page2 : page, far ? cidx + 2 : cidx);
+    far = address(more2 ? page2 : page, more2 ? cidx + 2 : cidx);
+    if constexpr (!kCodes) asm volatile("" ::"v"(warm[0]), "v"(warm[1]));
   };
-  // Load i of the next chunk's values, or of all of it.
+  // f16: a word of each line of the chunk after the next, which is then in the L2 when its turn comes. Behind the next chunk's own
+  // loads, so that these alone are waited for.
+  constexpr int kWarm = D == 256 ? 2 : 1;
+  auto warm_up = [&] {
+    if constexpr (!kCodes) {
+#pragma unroll
+      for (int x = 0; x < kWarm; ++x)
+        warm[x] = *reinterpret_cast<const volatile uint32_t*>(far + min((uint32_t)(x * 256 + wave * 64 + lane) * 128, 2u * kTile - 4));
+    }
+  };
+  // Load i of the next chunk of f16.
   auto load = [&](int i, int b) {
-    if constexpr (kCodes) quarter.load_values(i, next, wave, lane);
-    else if (i < kWhole) fetch_whole(i, next, b ^ 1);
+    if constexpr (!kCodes)
+      if (i < kWhole) fetch_whole(i, next, b ^ 1);
   };
   auto end_step = [&] {
-    if (!kCodes) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (!kCodes) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(kWarm) : "memory");
     __syncthreads();
     page = page1, page1 = page2;
   };
@@ -577,11 +605,14 @@ __global__ __launch_bounds__(256, (kWidePerSimd<FMT, D>)) void k_attn_extend_wid
       look_ahead(i, cidx);
 #pragma unroll
       for (int x = 0; x < NI; ++x) load(x, b);
+      warm_up();
 #pragma unroll
       for (int x = 0; x < kItems; ++x) put(x, to_at + (b ^ 1) * 2 * kTile);
       if constexpr (kCodes) {
 #pragma unroll
-        for (int x = 0; x < Quarter<FMT, D>::kKeyLoads; ++x) quarter.load_keys(x, next_keys, wave, lane);
+        for (int x = 0; x < Quarter<FMT, D>::kKeyLoads; ++x) quarter.load_keys(x, far, wave, lane);
+#pragma unroll
+        for (int x = 0; x < Quarter<FMT, D>::kValueLoads; ++x) quarter.load_values(x, far, wave, lane);
       }
       end_step();
     }
@@ -616,6 +647,7 @@ __global__ __launch_bounds__(256, (kWidePerSimd<FMT, D>)) void k_attn_extend_wid
       __builtin_amdgcn_sched_barrier(0);
     }
     __builtin_amdgcn_s_setprio(0);
+    warm_up();
     if constexpr (D == 256) {  // moved out of the accumulators' registers once
 #pragma unroll
       for (int y = 0; y < KH; ++y) asm("" : "+v"(s[y]));
@@ -687,11 +719,11 @@ __global__ __launch_bounds__(256, (kWidePerSimd<FMT, D>)) void k_attn_extend_wid
         for (int x = 4 * (q / ND + 1) + q % ND * 4 / ND; x < 4 * (q / ND + 1) + (q % ND + 1) * 4 / ND; ++x) weigh(x);
       }
       if constexpr (kCodes) {
-        if (q < Quarter<FMT, D>::kKeyLoads) quarter.load_keys(q, next_keys, wave, lane);
+        // the keys' next codes, then the values as operands, each followed by its next codes
+        constexpr int kItem = kItems - kKeyItems, kEach = (NV - 1) / kItem;
+        if (q < Quarter<FMT, D>::kKeyLoads) quarter.load_keys(q, far, wave, lane);
+        if (q % kEach == kEach - 1 && q / kEach < kItem) put(kKeyItems + q / kEach, to), quarter.load_values(q / kEach, far, wave, lane);
       }
-      // the values in the second half, when their codes have come
-      constexpr int kEach = NV / 2 / (kItems - kKeyItems + !kCodes);
-      if (kCodes && q >= NV / 2 && (q - NV / 2) % kEach == 0) put(kKeyItems + (q - NV / 2) / kEach, to);
       __builtin_amdgcn_sched_barrier(0);
     }
     __builtin_amdgcn_s_setprio(0);
@@ -752,7 +784,7 @@ template <int D>
 __global__ __launch_bounds__(64 * kWaves) void k_extend_join(ExtendArgs a) {
   constexpr int L = D / 4, G = 64 / L;  // lanes of a row, parts at a time
   Unit u;
-  if (!find_unit(a, blockIdx.x, true, u)) return;
+  if (!find_unit(a, true, u)) return;
   const Reach t = reach_of(a, u);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const uint32_t hk = blockIdx.y;
@@ -839,7 +871,7 @@ hipError_t launch_attn_extend(const Launch& K, const KvPages& kv, uint32_t forma
   hipError_t e;
   {
     ProfScope ps(K, "attn_extend");
-    const uint64_t units = a.parts > 1 ? std::max<uint64_t>(a.parts, tiles + a.parts / 2) : tiles;
+    const uint64_t units = a.parts > 1 ? (std::max<uint64_t>(a.parts, tiles + a.parts / 2) + 7) / 8 * 8 : tiles;
     hipLaunchKernelGGL(kernel, dim3((unsigned)units, kv.n_heads), dim3(64 * kWaves), 0, K.s, a);
     e = hipGetLastError();
     if (e != hipSuccess || a.parts == 1) return e;
