@@ -38,7 +38,8 @@ extern "C" {
  * at position seq_len[s] - n + i and sees the keys at its own and at earlier positions, with a window the last of
  * those; a row before position 0, of more new tokens than cached ones, sees nothing and is zero. Lengths, pages,
  * window, sinks and numerics are mr_attn_decode's. n_seqs: up to 65535. opts NULL: defaults.
- * n_q times the query heads of a key head: below 2^24. Shares its scratch with mr_attn_decode: one call of a context
+ * n_q times the query heads of a key head: below 2^24; a sixteenth of that, n_seqs and 2048, times the key heads: below 2^24
+ * (more is refused). Shares its scratch with mr_attn_decode: one call of a context
  * at a time. */
 int mr_attn_extend(mr_ctx* ctx, const mr_kv* kv, const mr_heads* q, uint32_t n_q, uint32_t n_seqs, const int32_t* cu_q,
                    const int32_t* seq_len, const int32_t* block_table, uint32_t max_pages, const mr_attn_opts* opts,

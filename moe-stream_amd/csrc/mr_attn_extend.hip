@@ -51,16 +51,18 @@ __device__ __forceinline__ Span span_of(const ExtendArgs& a, uint32_t b) {
   return s;
 }
 
-// A workgroup's unit: a tile of a sequence, a part of its keys and a key head. split_only: tile blockIdx.x of the sequences of several
-// parts and key head blockIdx.y; the part is then 0. slot: parts of split sequences in front of the tile's.
+// A workgroup's unit: a tile of a sequence, a part of its keys and a key head, heads in turn: workgroups go to the 8 XCDs in turn, so that
+// the tiles of a head, a part after the other, are on few of them and find the keys that they share in one L2 (a prompt's part among 32
+// tokens, 8 heads: 208 us with units in turn, 195 so). split_only: tile blockIdx.x of the sequences of several parts and key head
+// blockIdx.y; the part is then 0. slot: parts of split sequences in front of the tile's.
 struct Unit {
   uint32_t b, hk, tile, part, parts, slot;
   Span sp;
 };
 __device__ __forceinline__ bool find_unit(const ExtendArgs& a, bool split_only, Unit& r) {
   const uint32_t lane = threadIdx.x & 63;
-  uint32_t i = blockIdx.x;
-  r.hk = blockIdx.y;
+  uint32_t i = split_only ? blockIdx.x : blockIdx.x / a.kv.n_heads;
+  r.hk = split_only ? blockIdx.y : blockIdx.x - i * a.kv.n_heads;
   if (a.parts == 1) {
     if (split_only) return false;
     r.b = find_seq(a.cu, a.n_seqs, a.nq, a.group.d, a.bits, i);
@@ -85,16 +87,6 @@ __device__ __forceinline__ bool find_unit(const ExtendArgs& a, bool split_only, 
   const uint32_t most = max(a.parts, tiles + a.parts / 2);
   uint32_t size = max(kMinPart, (all + a.parts - 1) / a.parts);
   while (size < all && sum_of([&](uint32_t t, uint32_t c) { return t * max(1u, (c + size - 1) / size); }) > most) size += (size + 7) / 8;
-  if (!split_only) {
-    // Workgroups go to the 8 XCDs in turn: each gets an eighth of the units, in their order, so that the tiles that read the same keys
-    // find them in one L2 (four prompts' parts, f16, 32 heads on 4: 184 us without, XX so).
-    const uint32_t units = __builtin_amdgcn_readfirstlane(sum_of([&](uint32_t t, uint32_t c) { return t * max(1u, (c + size - 1) / size); }));
-    const uint32_t per = (units * a.kv.n_heads + 7) / 8, at = blockIdx.y * gridDim.x + blockIdx.x;
-    if (at >> 3 >= per) return false;
-    i = (at & 7) * per + (at >> 3);
-    r.hk = __builtin_amdgcn_readfirstlane(i / units), i -= r.hk * units;
-    if (r.hk >= a.kv.n_heads) return false;
-  }
   uint32_t before = 0, slots = 0;
   for (uint32_t b0 = 0; b0 < a.n_seqs; b0 += 64) {
     if (b0) s = b0 + lane < a.n_seqs ? span_of(a, b0 + lane) : Span{};
@@ -158,7 +150,7 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<NT, FMT, D>)) void k_attn_ex
   __shared__ __attribute__((aligned(16))) float sums[kWaves / 2][16 * D];
   __shared__ float stats[kWaves / 2][16][2];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-  if (blockIdx.x == 0 && blockIdx.y == 0) check_entries(a);
+  if (blockIdx.x == 0) check_entries(a);
   Unit u;
   if (!find_unit(a, false, u)) return;
   const uint32_t hk = u.hk;
@@ -439,7 +431,7 @@ __global__ __launch_bounds__(256, (kWidePerSimd<FMT, D>)) void k_attn_extend_wid
   constexpr int ND = D / 32, NI = D / 16, kTile = 64 * D * 2;  // bytes of a chunk's keys as operands
   __shared__ __attribute__((aligned(16))) uint8_t lds[2][2][kTile];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 31, half = lane >> 5;
-  if (blockIdx.x == 0 && blockIdx.y == 0) check_entries(a);
+  if (blockIdx.x == 0) check_entries(a);
   Unit u;
   if (!find_unit(a, false, u)) return;
   const uint32_t hk = u.hk;
@@ -571,23 +563,11 @@ __global__ __launch_bounds__(256, (kWidePerSimd<FMT, D>)) void k_attn_extend_wid
   // Where the next chunks' codes come from. Behind the last chunks too, of some chunk that is there: a wait for one load must
   // know how many others there are behind it.
   const uint8_t *next = nullptr, *far = nullptr;  // of the next chunk, of the one after it
-  uint32_t warm[2] = {};
   auto look_ahead = [&](int i, int cidx) {
     const bool more = cidx + 1 < t.end, more2 = cidx + 2 < t.end;
     if (more2) page2 = next_page(i + 2);
     next = address(more ? page1 : page, cidx + more);
     far = address(more2 ? page2 : page, more2 ? cidx + 2 : cidx);
-    if constexpr (!kCodes) asm volatile("" ::"v"(warm[0]), "v"(warm[1]));
-  };
-  // f16: a word of each line of the chunk after the next, which is then in the L2 when its turn comes. Behind the next chunk's own
-  // loads, so that these alone are waited for.
-  constexpr int kWarm = D == 256 ? 2 : 1;
-  auto warm_up = [&] {
-    if constexpr (!kCodes) {
-#pragma unroll
-      for (int x = 0; x < kWarm; ++x)
-        warm[x] = *reinterpret_cast<const volatile uint32_t*>(far + min((uint32_t)(x * 256 + wave * 64 + lane) * 128, 2u * kTile - 4));
-    }
   };
   // Load i of the next chunk of f16.
   auto load = [&](int i, int b) {
@@ -595,7 +575,7 @@ __global__ __launch_bounds__(256, (kWidePerSimd<FMT, D>)) void k_attn_extend_wid
       if (i < kWhole) fetch_whole(i, next, b ^ 1);
   };
   auto end_step = [&] {
-    if (!kCodes) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(kWarm) : "memory");
+    if (!kCodes) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     page = page1, page1 = page2;
   };
@@ -605,7 +585,6 @@ __global__ __launch_bounds__(256, (kWidePerSimd<FMT, D>)) void k_attn_extend_wid
       look_ahead(i, cidx);
 #pragma unroll
       for (int x = 0; x < NI; ++x) load(x, b);
-      warm_up();
 #pragma unroll
       for (int x = 0; x < kItems; ++x) put(x, to_at + (b ^ 1) * 2 * kTile);
       if constexpr (kCodes) {
@@ -647,7 +626,6 @@ __global__ __launch_bounds__(256, (kWidePerSimd<FMT, D>)) void k_attn_extend_wid
       __builtin_amdgcn_sched_barrier(0);
     }
     __builtin_amdgcn_s_setprio(0);
-    warm_up();
     if constexpr (D == 256) {  // moved out of the accumulators' registers once
 #pragma unroll
       for (int y = 0; y < KH; ++y) asm("" : "+v"(s[y]));
@@ -871,13 +849,13 @@ hipError_t launch_attn_extend(const Launch& K, const KvPages& kv, uint32_t forma
   hipError_t e;
   {
     ProfScope ps(K, "attn_extend");
-    const uint64_t units = a.parts > 1 ? (std::max<uint64_t>(a.parts, tiles + a.parts / 2) + 7) / 8 * 8 : tiles;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)units, kv.n_heads), dim3(64 * kWaves), 0, K.s, a);
+    const uint64_t units = a.parts > 1 ? std::max<uint64_t>(a.parts, tiles + a.parts / 2) : tiles;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(units * kv.n_heads)), dim3(64 * kWaves), 0, K.s, a);
     e = hipGetLastError();
     if (e != hipSuccess || a.parts == 1) return e;
   }
   ProfScope ps(K, "extend_join");
-  const dim3 j((unsigned)std::min<uint64_t>(tiles, a.parts / 2 + 1), kv.n_heads, 4), blk(64 * kWaves);
+  const dim3 j((unsigned)std::min<uint64_t>(tiles, a.parts / 2 + 1), kv.n_heads, bits <= 5 ? 4 : 1 << (bits - 3)), blk(64 * kWaves);
   if (D == 64) hipLaunchKernelGGL((k_extend_join<64>), j, blk, 0, K.s, a);
   if (D == 128) hipLaunchKernelGGL((k_extend_join<128>), j, blk, 0, K.s, a);
   if (D == 256) hipLaunchKernelGGL((k_extend_join<256>), j, blk, 0, K.s, a);

@@ -59,6 +59,8 @@ int mr_attn_extend(mr_ctx* c, const mr_kv* kv, const mr_heads* q, uint32_t nq, u
   if ((rc = check_lengths(c, kv, seq_len, block_table, max_pages, n_seqs))) return rc;
   if ((uint64_t)nq * (hq.n / kv->d.n_heads) > kMaxRows)
     return fail(c, MR_E_INVAL, "%u rows of %u heads that share keys are 2^24 or more", nq, hq.n / kv->d.n_heads);
+  if (((uint64_t)nq * (hq.n / kv->d.n_heads) / 16 + n_seqs + 2048) * kv->d.n_heads >= 1u << 24)  // 2^32 threads of a launch
+    return fail(c, MR_E_INVAL, "%u rows in %u sequences are too many tiles for %u key heads", nq, n_seqs, kv->d.n_heads);
   if (nq == 0 || n_seqs == 0) return MR_OK;
   if ((rc = bind(c))) return rc;
   const hipError_t e = mr::launch_attn_extend(c->launch(), pages(kv), kv->d.format, D, hq, nq, n_seqs, cu_q, seq_len,
