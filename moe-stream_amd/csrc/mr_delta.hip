@@ -178,26 +178,77 @@ struct ChunkArgs {
   float* carry;            // [2][value head][state]: of the sequences that go on in the next launch
   uint32_t first, last;    // chunks of this launch, by their numbers
   int least;               // sequences of fewer tokens are not this path's
+  int dense;               // chunks and sequences are numbered among those that are
 };
 
-// Chunk number `at`: its sequence, and which of the sequence's chunks.
-__device__ __forceinline__ bool find_chunk(const ChunkArgs& c, uint32_t at, int& row, int& n) {
-  const Sequences& q = c.a.s;
-  const uint32_t s = find_seq(q.cu, q.n_seqs, q.n_rows, 1, 6, at);
+constexpr uint32_t kDenseSeqs = 1024;  // each workgroup looks through so many
+
+// Sequence number i of this path (chunk: the one that chunk number i is in), the number of its first chunk, its rows.
+struct Chunked {
+  uint32_t s, start;
   int q0, q1;
-  rows_of(q.cu, q.n_rows, s, q0, q1);
-  const int64_t i = (int64_t)at - first_tile(q.cu, q.n_rows, s, 1, 6);
-  if (i < 0 || i * kChunk >= q1 - q0 || q1 - q0 < c.least) return false;
-  row = q0 + (int)i * kChunk, n = min(kChunk, q1 - row);
+};
+__device__ __forceinline__ bool find_sequence(const ChunkArgs& c, uint32_t i, bool chunk, Chunked& r) {
+  const Sequences& q = c.a.s;
+  if (!c.dense) {
+    r.s = chunk ? find_seq(q.cu, q.n_seqs, q.n_rows, 1, 6, i) : i;
+    r.start = first_tile(q.cu, q.n_rows, r.s, 1, 6);
+    rows_of(q.cu, q.n_rows, r.s, r.q0, r.q1);
+    return r.q1 - r.q0 >= c.least;
+  }
+  uint32_t seqs = 0, chunks = 0;
+  for (uint32_t s0 = 0; s0 < q.n_seqs; s0 += 64) {
+    const uint32_t s = s0 + (threadIdx.x & 63);
+    int q0 = 0, q1 = 0;
+    if (s < q.n_seqs) rows_of(q.cu, q.n_rows, s, q0, q1);
+    const uint32_t here = s < q.n_seqs && q1 - q0 >= c.least, n = here ? (uint32_t)(q1 - q0 + kChunk - 1) / kChunk : 0;
+    const uint32_t at = wave_prefix(here), sum = wave_prefix(n);
+    const uint64_t past = __ballot(chunk ? chunks + sum > i : seqs + at > i);
+    if (past) {
+      const int l = __ffsll((unsigned long long)past) - 1;
+      r.s = s0 + l, r.start = chunks + __builtin_amdgcn_readlane(sum - n, l);
+      r.q0 = __builtin_amdgcn_readlane(q0, l), r.q1 = __builtin_amdgcn_readlane(q1, l);
+      return true;
+    }
+    seqs += __builtin_amdgcn_readlane(at, 63), chunks += __builtin_amdgcn_readlane(sum, 63);
+  }
+  return false;
+}
+
+// Chunk number `at`: its first row and its rows.
+__device__ __forceinline__ bool find_chunk(const ChunkArgs& c, uint32_t at, int& row, int& n) {
+  Chunked r;
+  if (!find_sequence(c, at, true, r)) return false;
+  const int64_t i = (int64_t)at - r.start;
+  if (i < 0 || i * kChunk >= r.q1 - r.q0) return false;
+  row = r.q0 + (int)i * kChunk, n = min(kChunk, r.q1 - row);
   return true;
 }
 
+// The sum of lanes 0 .. l in lane l, by wave_prefix's moves.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double add_moved(double v) {
+  const u32x2 w = __builtin_bit_cast(u32x2, v);
+  const u32x2 x = {(uint32_t)__builtin_amdgcn_update_dpp(0, (int)w.x, CTRL, ROWS, 0xF, false),
+                   (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w.y, CTRL, ROWS, 0xF, false)};
+  return v + __builtin_bit_cast(double, x);
+}
+__device__ __forceinline__ double wave_prefix(double v) {
+  v = add_moved<0x111, 0xF>(v), v = add_moved<0x112, 0xF>(v), v = add_moved<0x114, 0xF>(v), v = add_moved<0x118, 0xF>(v);
+  return add_moved<0x143, 0xC>(add_moved<0x142, 0xA>(v));
+}
+
+// A chunk of a value head; the first head that shares a key head also lays out that one's operands.
+//
+// A^T and T lie in one square: A^T above the diagonal, T = (I + A)^-1 on it and below.
 template <int DK, bool BF>
-__global__ __launch_bounds__(256) void k_delta_prepare(ChunkArgs c) {
+__global__ __launch_bounds__(256, 4) void k_delta_prepare(ChunkArgs c) {
   constexpr int NP = BF ? 1 : 2, NS = DK / 32, kPad = 68;
   using I = DeltaImage<DK, NP>;
-  __shared__ __attribute__((aligned(16))) float B[kChunk][kPad], W[kChunk][kPad];  // A^T and T^T
-  __shared__ __attribute__((aligned(16))) uint16_t kst[kChunk][DK + 8];
+  __shared__ union {
+    float m[kChunk][kPad];
+    uint16_t keys[kChunk][DK + 8];
+  } lds __attribute__((aligned(16)));
   __shared__ float hi[kChunk], lo[kChunk], beta[kChunk], unit_k[kChunk], unit_q[kChunk];
   __shared__ int bad[kChunk];
   const DeltaArgs& a = c.a;
@@ -229,32 +280,74 @@ __global__ __launch_bounds__(256) void k_delta_prepare(ChunkArgs c) {
   Operand kw[NS], qw[NS];
 #pragma unroll
   for (int s = 0; s < NS; ++s) kw[s] = rows16(a.k, wave, s), qw[s] = rows16(a.q, wave, s);
+  float lg = 0.f, b = 0.f;
+  if (wave == 0 && lane < n) gates(a, (uint64_t)(row + lane), h, lg, b);  // the wave with the fewest products below
+  // Products of this wave's 16 tokens with the earlier ones: rows are the earlier tokens, this wave's the columns.
+  f32x4 kk[4] = {}, pt[4] = {};
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    if (t > wave) break;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      const Operand k = t == wave ? kw[s] : rows16(a.k, t, s);
+      kk[t] = dot(k, kw[s], kk[t]), pt[t] = dot(k, qw[s], pt[t]);
+    }
+  }
   {
-    const float kk = squares(kw), qq = squares(qw);
+    const float k2 = squares(kw), q2 = squares(qw);
     if (g == 0) {
-      unit_k[16 * wave + m] = a.d.unit_eps > 0.f ? 1.f / sqrtf(kk + a.d.unit_eps) : 1.f;
-      unit_q[16 * wave + m] = a.d.scale * (a.d.unit_eps > 0.f ? 1.f / sqrtf(qq + a.d.unit_eps) : 1.f);
-      bad[16 * wave + m] = !(kk < INFINITY);
+      unit_k[16 * wave + m] = a.d.unit_eps > 0.f ? 1.f / sqrtf(k2 + a.d.unit_eps) : 1.f;
+      unit_q[16 * wave + m] = a.d.scale * (a.d.unit_eps > 0.f ? 1.f / sqrtf(q2 + a.d.unit_eps) : 1.f);
+      bad[16 * wave + m] = !(k2 < INFINITY);
     }
     if (h % group == 0) {
 #pragma unroll
-      for (int s = 0; s < NS; ++s) *reinterpret_cast<Operand*>(&kst[16 * wave + m][32 * s + 8 * g]) = kw[s];
+      for (int s = 0; s < NS; ++s) *reinterpret_cast<Operand*>(&lds.keys[16 * wave + m][32 * s + 8 * g]) = kw[s];
     }
   }
   __syncthreads();
+  if (h % group == 0) {
+    // A key head's operands: f16 numbers as two bf16 ones.
+    auto put = [&](uint8_t* to, Operand x) {
+      if constexpr (BF) {
+        *reinterpret_cast<Operand*>(to + lane * 16) = x;
+      } else {
+        u32x2 part[2][2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const f32x2 y = unpack_f16(x[2 * e]), z = unpack_f16(x[2 * e + 1]);
+          split(f32x4{y.x, y.y, z.x, z.y}, part[e]);
+        }
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+          *reinterpret_cast<Operand*>(to + p * 1024 + lane * 16) = Operand{part[0][p].x, part[0][p].y, part[1][p].x, part[1][p].y};
+      }
+    };
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      put(key_image + I::kK + (wave * NS + s) * NP * 1024, kw[s]);
+      put(key_image + I::kQ + (wave * NS + s) * NP * 1024, qw[s]);
+    }
+    for (int t = wave; t < DK / 16; t += 4) {
+      const int e = 32 * (t >> 1) + 8 * (m >> 2) + 4 * (t & 1) + (m & 3);
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        Operand x;
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const int j = 32 * s + 16 * (y >> 1) + 4 * g + 2 * (y & 1);
+          x[y] = (uint32_t)lds.keys[j][e] | (uint32_t)lds.keys[j + 1][e] << 16;
+        }
+        put(key_image + I::kKT + (t * 2 + s) * NP * 1024, x);
+      }
+    }
+  }
   if (wave == 0) {
     // Sums of the decays in powers of two and 64 bits, kept as two numbers of 32: what two sums differ by is what counts. A token whose
     // key, decay or beta is not finite counts as none here, and as NaN for all that comes after it.
-    float lg = 0.f, b = 0.f;
-    if (lane < n) gates(a, (uint64_t)(row + lane), h, lg, b);
     const bool wrong = bad[lane] || !(lg < INFINITY) || !(fabsf(b) < INFINITY);
     if (wrong) lg = 0.f, b = 0.f;
-    double sum = fmax((double)lg, -1e4) * 1.4426950408889634;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const double x = __shfl_up(sum, o, 64);
-      if (lane >= o) sum += x;
-    }
+    const double sum = wave_prefix(fmax((double)lg, -1e4) * 1.4426950408889634);
     hi[lane] = (float)sum, lo[lane] = (float)(sum - (double)(float)sum), beta[lane] = b, bad[lane] = wrong;
     const double end = __shfl(sum, 63, 64);
     const float rise = __builtin_amdgcn_exp2f((float)sum), fall = __builtin_amdgcn_exp2f((float)(end - sum));
@@ -265,25 +358,16 @@ __global__ __launch_bounds__(256) void k_delta_prepare(ChunkArgs c) {
     if (lane == 0) vec[192] = __builtin_amdgcn_exp2f((float)end);
   }
   __syncthreads();
-  // Tiles of A^T and P^T: rows are the earlier tokens j, this wave's 16 tokens i the columns.
   const int i = 16 * wave + m;
-  f32x4 pt[4] = {};
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
     if (t > wave) break;
-    f32x4 kk = {}, qk = {};
-#pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      const Operand k = t == wave ? kw[s] : rows16(a.k, t, s);
-      kk = dot(k, kw[s], kk), qk = dot(k, qw[s], qk);
-    }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int j = 16 * t + 4 * g + r;
       const float decay = __builtin_amdgcn_exp2f((hi[i] - hi[j]) + (lo[i] - lo[j]));
-      const bool none = bad[i] || bad[j];
-      B[j][i] = j < i && !none ? kk[r] * unit_k[j] * unit_k[i] * beta[i] * decay : 0.f;
-      pt[t][r] = j <= i && !bad[j] ? qk[r] * unit_k[j] * unit_q[i] * decay : 0.f;
+      if (j < i) lds.m[j][i] = bad[i] || bad[j] ? 0.f : kk[t][r] * unit_k[j] * unit_k[i] * beta[i] * decay;
+      pt[t][r] = j <= i && !bad[j] ? pt[t][r] * unit_k[j] * unit_q[i] * decay : 0.f;
     }
   }
 #pragma unroll
@@ -296,20 +380,20 @@ __global__ __launch_bounds__(256) void k_delta_prepare(ChunkArgs c) {
       *reinterpret_cast<Operand*>(image + I::kP + (I::lower(wave, s) * 2 + p) * 1024 + lane * 16) = Operand{x[p].x, x[p].y, y[p].x, y[p].y};
   }
   __syncthreads();
-  // W = T^T = (I + B)^-1, B strictly upper: blocks of 16 on the diagonal column by column, from the last row up; then
-  // W_ji = -W_jj sum_(k = j + 1 .. i) B_jk W_ki, a diagonal of blocks after the other, in products of 32 bits.
+  // Blocks of 16 on the diagonal, column m of the transposed one from its last row up; then, a diagonal of blocks after the
+  // other and in products of 32 bits, T^T_je = -T^T_jj sum_(k = j + 1 .. e) A^T_jk T^T_ke.
   {
     float w[16];
 #pragma unroll
     for (int r = 15; r >= 0; --r) {
       float v = r == m ? 1.f : 0.f;
 #pragma unroll
-      for (int k = r + 1; k < 16; ++k) v = fmaf(-B[16 * wave + r][16 * wave + k], w[k], v);
+      for (int k = r + 1; k < 16; ++k) v = fmaf(-lds.m[16 * wave + r][16 * wave + k], w[k], v);
       w[r] = v;
     }
 #pragma unroll
     for (int r = 0; r < 16; ++r)
-      if (g == r >> 2) W[16 * wave + r][i] = w[r];
+      if (g == r >> 2 && r <= m) lds.m[i][16 * wave + r] = w[r];
   }
   __syncthreads();
 #pragma unroll
@@ -318,15 +402,20 @@ __global__ __launch_bounds__(256) void k_delta_prepare(ChunkArgs c) {
     if (e < 4) {
       f32x4 y = {}, z = {};
       for (int k = j + 1; k <= e; ++k) {
-        const f32x4 b = *reinterpret_cast<const f32x4*>(&B[16 * j + m][16 * k + 4 * g]);
+        const f32x4 x = *reinterpret_cast<const f32x4*>(&lds.m[16 * j + m][16 * k + 4 * g]);
+        f32x4 w = *reinterpret_cast<const f32x4*>(&lds.m[16 * e + m][16 * k + 4 * g]);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) y = __builtin_amdgcn_mfma_f32_16x16x4f32(b[r], W[16 * k + 4 * g + r][16 * e + m], y, 0, 0, 0);
+        for (int r = 0; r < 4; ++r) {
+          if (k == e && 4 * g + r > m) w[r] = 0.f;  // the other matrix's side of the diagonal
+          y = __builtin_amdgcn_mfma_f32_16x16x4f32(x[r], w[r], y, 0, 0, 0);
+        }
       }
-      const f32x4 b = *reinterpret_cast<const f32x4*>(&W[16 * j + m][16 * j + 4 * g]);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) z = __builtin_amdgcn_mfma_f32_16x16x4f32(b[r], y[r], z, 0, 0, 0);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) W[16 * j + 4 * g + r][16 * e + m] = -z[r];
+      for (int r = 0; r < 4; ++r) {
+        const float x = 4 * g + r >= m ? lds.m[16 * j + 4 * g + r][16 * j + m] : 0.f;
+        z = __builtin_amdgcn_mfma_f32_16x16x4f32(x, y[r], z, 0, 0, 0);
+      }
+      *reinterpret_cast<f32x4*>(&lds.m[16 * e + m][16 * j + 4 * g]) = -z;
     }
     __syncthreads();
   }
@@ -338,11 +427,10 @@ __global__ __launch_bounds__(256) void k_delta_prepare(ChunkArgs c) {
     for (int x = 0; x < 2; ++x) {
       f32x4 v = {};
       if (2 * s + x <= wave) {
+        const int j = 32 * s + 16 * x + 4 * g;
+        v = *reinterpret_cast<const f32x4*>(&lds.m[i][j]);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int j = 32 * s + 16 * x + 4 * g + r;
-          v[r] = W[j][i] * beta[j];
-        }
+        for (int r = 0; r < 4; ++r) v[r] = j + r <= i ? v[r] * beta[j + r] : 0.f;
       }
       split(v, part[x]);
     }
@@ -350,41 +438,6 @@ __global__ __launch_bounds__(256) void k_delta_prepare(ChunkArgs c) {
     for (int p = 0; p < 3; ++p)
       *reinterpret_cast<Operand*>(image + I::kT + (I::lower(wave, s) * 3 + p) * 1024 + lane * 16) =
           Operand{part[0][p].x, part[0][p].y, part[1][p].x, part[1][p].y};
-  }
-  if (h % group) return;
-  // A key head's operands: f16 numbers as two bf16 ones.
-  auto put = [&](uint8_t* to, Operand x) {
-    if constexpr (BF) {
-      *reinterpret_cast<Operand*>(to + lane * 16) = x;
-    } else {
-      u32x2 part[2][2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const f32x2 y = unpack_f16(x[2 * e]), z = unpack_f16(x[2 * e + 1]);
-        split(f32x4{y.x, y.y, z.x, z.y}, part[e]);
-      }
-#pragma unroll
-      for (int p = 0; p < 2; ++p)
-        *reinterpret_cast<Operand*>(to + p * 1024 + lane * 16) = Operand{part[0][p].x, part[0][p].y, part[1][p].x, part[1][p].y};
-    }
-  };
-#pragma unroll
-  for (int s = 0; s < NS; ++s) {
-    put(key_image + I::kK + (wave * NS + s) * NP * 1024, kw[s]);
-    put(key_image + I::kQ + (wave * NS + s) * NP * 1024, qw[s]);
-  }
-  for (int t = wave; t < DK / 16; t += 4) {
-    const int e = 32 * (t >> 1) + 8 * (m >> 2) + 4 * (t & 1) + (m & 3);
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      Operand x;
-#pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        const int j = 32 * s + 16 * (y >> 1) + 4 * g + 2 * (y & 1);
-        x[y] = (uint32_t)kst[j][e] | (uint32_t)kst[j + 1][e] << 16;
-      }
-      put(key_image + I::kKT + (t * 2 + s) * NP * 1024, x);
-    }
   }
 }
 
@@ -402,17 +455,16 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs c, uint32_t s
   const DeltaArgs& a = c.a;
   const Sequences& q = a.s;
   // Workgroups go to the 8 XCDs in turn: the slices of a head, which read the same operands, to one of them.
-  const uint32_t unit = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3), h = unit / slices, slice = unit % slices, s = blockIdx.y;
-  if (h >= a.d.value_heads) return;
+  const uint32_t unit = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3), h = unit / slices, slice = unit % slices;
+  if (c.least == 0 && blockIdx.x == 0 && blockIdx.y == 0) check_offsets(q.cu, q.n_seqs, q.n_rows, q.err, kErrPacked);  // else k_delta_step has
+  Chunked seq;
+  if (h >= a.d.value_heads || !find_sequence(c, blockIdx.y, false, seq)) return;
   const uint32_t hk = h / (a.d.value_heads / a.d.key_heads), DV = a.d.value_dim;
   const int wave = (threadIdx.x >> 6) & 3, lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
   const bool outputs = __builtin_amdgcn_readfirstlane(threadIdx.x) >= 256;
-  int q0, q1;
-  rows_of(q.cu, q.n_rows, s, q0, q1);
-  const int n = q1 - q0;
-  if (c.least == 0 && blockIdx.x == 0 && s == 0) check_offsets(q.cu, q.n_seqs, q.n_rows, q.err, kErrPacked);  // else k_delta_step has
-  if (n < c.least) return;
-  const uint32_t start = first_tile(q.cu, q.n_rows, s, 1, 6), count = (n + kChunk - 1) / kChunk;
+  const uint32_t s = seq.s, start = seq.start;
+  const int q0 = seq.q0, q1 = seq.q1, n = q1 - q0;
+  const uint32_t count = (n + kChunk - 1) / kChunk;
   const uint32_t end = start + max(count, 1u);  // a sequence without tokens takes part in one launch
   if (end <= c.first || start >= c.last) return;
   const uint32_t begin = max(start, c.first), stop = min(start + count, c.last);
@@ -686,8 +738,11 @@ hipError_t launch_chunks(const Launch& K, const DeltaArgs& a, int least, uint8_t
   using I = DeltaImage<DK, BF ? 1 : 2>;
   const uint32_t vh = a.d.value_heads, kh = a.d.key_heads, dv = a.d.value_dim;
   const uint64_t carry = 2ull * vh * DK * dv * sizeof(float), chunk = (uint64_t)vh * I::kValue + (uint64_t)kh * I::kKey;
-  const uint32_t all = ((uint32_t)a.s.n_rows >> 6) + a.s.n_seqs, room = (uint32_t)std::min<uint64_t>((kScratch - carry) / chunk, 65535);
-  ChunkArgs c{a, nullptr, nullptr, reinterpret_cast<float*>(scratch), 0, 0, least};
+  const uint32_t longest = least ? (uint32_t)a.s.n_rows / (uint32_t)least : a.s.n_seqs;  // sequences of so many tokens at most
+  const bool dense = least && a.s.n_seqs <= kDenseSeqs;
+  const uint32_t seqs = dense ? std::min(a.s.n_seqs, longest) : a.s.n_seqs;
+  const uint32_t all = ((uint32_t)a.s.n_rows >> 6) + seqs, room = (uint32_t)std::min<uint64_t>((kScratch - carry) / chunk, 65535);
+  ChunkArgs c{a, nullptr, nullptr, reinterpret_cast<float*>(scratch), 0, 0, least, dense};
   int parity = 0;
   for (c.first = 0; c.first < all; c.first = c.last, parity ^= 1) {
     c.last = std::min(all, c.first + room);
@@ -698,7 +753,7 @@ hipError_t launch_chunks(const Launch& K, const DeltaArgs& a, int least, uint8_t
       hipLaunchKernelGGL((k_delta_prepare<DK, BF>), dim3(vh, c.last - c.first), dim3(256), 0, K.s, c);
     }
     ProfScope ps(K, "delta_chunks");
-    hipLaunchKernelGGL((k_delta_chunks<DK, BF ? 1 : 2, BF>), dim3((vh * (dv / 16) + 7) / 8 * 8, a.s.n_seqs), dim3(512), 0, K.s, c, dv / 16, parity);
+    hipLaunchKernelGGL((k_delta_chunks<DK, BF ? 1 : 2, BF>), dim3((vh * (dv / 16) + 7) / 8 * 8, seqs), dim3(512), 0, K.s, c, dv / 16, parity);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
@@ -713,7 +768,8 @@ hipError_t launch_delta_rule(const Launch& K, const DeltaShape& d, const Heads& 
                              const float* decay, const float* beta, const Sequences& s, const Heads& out, void* scratch) {
   const DeltaArgs a{d, q, k, v, out, decay, beta, s};
   const bool bf = q.dtype == MR_BF16;
-  const bool chunks = s.n_rows > kStepTokens, steps = !chunks || s.n_seqs > 1;  // one sequence takes one path
+  // One sequence takes one path, and so do sequences that are all short if none is without tokens; else one may be long.
+  const bool chunks = (int64_t)s.n_rows - s.n_seqs + 1 > kStepTokens, steps = !chunks || s.n_seqs > 1;
   if (steps) {
     ProfScope ps(K, "delta_step");
     if (d.key_dim == 64 && d.value_dim == 64) launch_step<64, 64>(K, bf, a, kStepTokens);
