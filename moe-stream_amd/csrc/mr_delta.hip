@@ -585,25 +585,28 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs c, uint32_t s
         for (int p = 0; p < NP; ++p)
           K[t][p] = *reinterpret_cast<const Part*>(key_image + I::kK + ((t * NS + wave * NT / 2) * NP + p) * 1024 + lane * 16 + (NT == 1 ? 8 * (wave & 1) : 0));
     };
-    auto load_rest = [&](int row) {
-      const float* vec = reinterpret_cast<const float*>(image + I::kVec) + t0;
-      of_k = *reinterpret_cast<const f32x4*>(vec), of_v = *reinterpret_cast<const f32x4*>(vec + 128);
+    auto vec = [&] { return reinterpret_cast<const float*>(image + I::kVec) + t0; };
+    auto load_values = [&](int row) {
+      of_k = *reinterpret_cast<const f32x4*>(vec());
       const uint8_t* v = static_cast<const uint8_t*>(a.v.p) + ((uint64_t)row * a.v.ts + (uint64_t)h * a.v.hs + 16 * slice) * 2;
 #pragma unroll
       for (int r = 0; r < 4; ++r) vals[r] = *reinterpret_cast<const uint16_t*>(v + (uint32_t)(min(t0 + r, q1 - 1 - row) * step + 2 * m));
+    };
+    auto load_solution = [&] {
+      of_v = *reinterpret_cast<const f32x4*>(vec() + 128);
 #pragma unroll
       for (int x = 0; x < 2; ++x)
 #pragma unroll
         for (int p = 0; p < 3; ++p) T[x][p] = operand(image + I::kT + (I::lower(wave, min(x, wave / 2)) * 3 + p) * 1024);
     };
-    auto load_fade = [&] {
+    auto load_fade = [&](const uint8_t* keys) {
       fade = reinterpret_cast<const float*>(image + I::kVec)[192];
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int x = 0; x < 2; ++x)
 #pragma unroll
-          for (int p = 0; p < NP; ++p) KT[t][x][p] = operand(key_image + I::kKT + (((wave * NT + t) * 2 + x) * NP + p) * 1024);
+          for (int p = 0; p < NP; ++p) KT[t][x][p] = operand(keys + I::kKT + (((wave * NT + t) * 2 + x) * NP + p) * 1024);
     };
     // The wave's part of K S for the next chunk. The state's tiles 2 s and 2 s + 1 are step s of the sums over a key's elements: as
     // an operand they are what their lanes hold.
@@ -630,15 +633,19 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs c, uint32_t s
 #pragma unroll
       for (int t = 0; t < 4; ++t) sums[wave][t][lane] = sum[t];
     };
-    load_keys(), load_rest(row), load_fade();
+    load_keys(), load_values(row), load_solution(), load_fade(key_image);
     look();
-    key_image += begin + 1 < stop ? key_step : 0;
-    load_keys();
     __syncthreads();
     for (uint32_t chunk = begin; chunk < stop; ++chunk, row += kChunk) {
       const bool more = chunk + 1 < stop;
       const int half = lane * 16 + 8 * (wave & 1);  // of the step that the wave's tokens are in
-      f32x4 R = (sums[0][wave][lane] + sums[1][wave][lane]) + (sums[2][wave][lane] + sums[3][wave][lane]);
+      // Loads are asked for behind a step's reads of LDS, while these are on their way.
+      const f32x4 part0 = sums[0][wave][lane], part1 = sums[1][wave][lane], part2 = sums[2][wave][lane], part3 = sums[3][wave][lane];
+      __builtin_amdgcn_sched_barrier(0);
+      key_image += more ? key_step : 0, image += more ? value_step : 0;
+      load_keys();
+      __builtin_amdgcn_sched_barrier(0);
+      f32x4 R = (part0 + part1) + (part2 + part3);
       bool wrong = false;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -670,14 +677,19 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs c, uint32_t s
       f32x4 V;
       {
         f32x4 sum[3] = {};  // sums of products of like size, so that they do not wait for each other
+        Operand y[2][3];
+#pragma unroll
+        for (int p = 0; p < 3; ++p) y[0][p] = operand(rest[0][p]), y[1][p] = operand(rest[1][p]);
+        __builtin_amdgcn_sched_barrier(0);
+        load_values(row + (more ? kChunk : 0));
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           if (x > wave / 2) break;
-          const Operand y[3] = {operand(rest[x][0]), operand(rest[x][1]), operand(rest[x][2])};
 #pragma unroll
           for (int p = 0; p < 3; ++p)
 #pragma unroll
-            for (int z = 0; z + p < 3; ++z) sum[z + p] = mfma_bf16(T[x][p], y[z], sum[z + p]);
+            for (int z = 0; z + p < 3; ++z) sum[z + p] = mfma_bf16(T[x][p], y[x][z], sum[z + p]);
         }
         V = (sum[2] + sum[1]) + sum[0];
       }
@@ -688,30 +700,35 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs c, uint32_t s
 #pragma unroll
         for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x2*>(&faded[wave >> 1][p][half]) = part[p];
       }
-      image += more ? value_step : 0;
-      load_rest(row + (more ? kChunk : 0));
-      float keep = fade;
+      bool lost = false;
       if (__builtin_amdgcn_readfirstlane(bads.x | bads.y | bads.z | bads.w)) {
 #pragma unroll
         for (int w = 0; w < 4; ++w)
-          if (bads[w] && first_bad[w][m] < kChunk) keep = NAN;
+          lost |= bads[w] && first_bad[w][m] < kChunk;
       }
       __syncthreads();
+      {
+        Operand y[2][3];
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        f32x4 sum[3] = {};
+        for (int p = 0; p < 3; ++p) y[0][p] = operand(faded[0][p]), y[1][p] = operand(faded[1][p]);
+        __builtin_amdgcn_sched_barrier(0);
+        load_solution();
+        __builtin_amdgcn_sched_barrier(0);
+        const float keep = lost ? NAN : fade;
+        f32x4 sum[NT][3] = {};
 #pragma unroll
         for (int x = 0; x < 2; ++x)
 #pragma unroll
           for (int p = 0; p < NP; ++p)
 #pragma unroll
-            for (int z = 0; z + p < 3; ++z) sum[z + p] = mfma_bf16(KT[t][x][p], operand(faded[x][z]), sum[z + p]);
-        S[t] = S[t] * keep + ((sum[2] + sum[1]) + sum[0]);
+            for (int z = 0; z + p < 3; ++z)
+#pragma unroll
+              for (int t = 0; t < NT; ++t) sum[t][z + p] = mfma_bf16(KT[t][x][p], y[x][z], sum[t][z + p]);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) S[t] = S[t] * keep + ((sum[t][2] + sum[t][1]) + sum[t][0]);
       }
-      load_fade();
+      load_fade(key_image);
       look();
-      key_image += chunk + 2 < stop ? key_step : 0;
-      load_keys();
       __syncthreads();
     }
   }
