@@ -249,8 +249,8 @@ __global__ __launch_bounds__(256, 4) void k_delta_prepare(ChunkArgs c) {
     float m[kChunk][kPad];
     uint16_t keys[kChunk][DK + 8];
   } lds __attribute__((aligned(16)));
-  __shared__ float hi[kChunk], lo[kChunk], beta[kChunk], unit_k[kChunk], unit_q[kChunk];
-  __shared__ int bad[kChunk];
+  __shared__ __attribute__((aligned(16))) float hi[kChunk], lo[kChunk], beta[kChunk], unit_k[kChunk], unit_q[kChunk];
+  __shared__ __attribute__((aligned(16))) int bad[kChunk];
   const DeltaArgs& a = c.a;
   const uint32_t h = blockIdx.x, group = a.d.value_heads / a.d.key_heads, hk = h / group;
   int row, n;
@@ -359,15 +359,23 @@ __global__ __launch_bounds__(256, 4) void k_delta_prepare(ChunkArgs c) {
   }
   __syncthreads();
   const int i = 16 * wave + m;
+  {
+    const float hi_i = hi[i], lo_i = lo[i], gain = unit_k[i] * beta[i], of_q = unit_q[i];
+    const bool bad_i = bad[i];
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    if (t > wave) break;
+    for (int t = 0; t < 4; ++t) {
+      if (t > wave) break;
+      const int j0 = 16 * t + 4 * g;
+      const f32x4 hi_j = *reinterpret_cast<const f32x4*>(hi + j0), lo_j = *reinterpret_cast<const f32x4*>(lo + j0);
+      const f32x4 unit_j = *reinterpret_cast<const f32x4*>(unit_k + j0);
+      const i32x4 bad_j = *reinterpret_cast<const i32x4*>(bad + j0);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int j = 16 * t + 4 * g + r;
-      const float decay = __builtin_amdgcn_exp2f((hi[i] - hi[j]) + (lo[i] - lo[j]));
-      if (j < i) lds.m[j][i] = bad[i] || bad[j] ? 0.f : kk[t][r] * unit_k[j] * unit_k[i] * beta[i] * decay;
-      pt[t][r] = j <= i && !bad[j] ? pt[t][r] * unit_k[j] * unit_q[i] * decay : 0.f;
+      for (int r = 0; r < 4; ++r) {
+        const float f = unit_j[r] * __builtin_amdgcn_exp2f((hi_i - hi_j[r]) + (lo_i - lo_j[r]));
+        const float x = bad_i || bad_j[r] ? 0.f : kk[t][r] * f * gain;
+        if (t < wave || 4 * g + r < m) lds.m[j0 + r][i] = x;
+        pt[t][r] = (t < wave || 4 * g + r <= m) && !bad_j[r] ? pt[t][r] * f * of_q : 0.f;
+      }
     }
   }
 #pragma unroll
@@ -383,12 +391,14 @@ __global__ __launch_bounds__(256, 4) void k_delta_prepare(ChunkArgs c) {
   // Blocks of 16 on the diagonal, column m of the transposed one from its last row up; then, a diagonal of blocks after the
   // other and in products of 32 bits, T^T_je = -T^T_jj sum_(k = j + 1 .. e) A^T_jk T^T_ke.
   {
-    float w[16];
+    float w[16], column[16];  // lane m has the block's column m: row r's numbers come from the lanes
+#pragma unroll
+    for (int r = 0; r < 15; ++r) column[r] = lds.m[16 * wave + r][i];
 #pragma unroll
     for (int r = 15; r >= 0; --r) {
       float v = r == m ? 1.f : 0.f;
 #pragma unroll
-      for (int k = r + 1; k < 16; ++k) v = fmaf(-lds.m[16 * wave + r][16 * wave + k], w[k], v);
+      for (int k = r + 1; k < 16; ++k) v = fmaf(-bits_f32(__builtin_amdgcn_readlane(__float_as_uint(column[r]), k)), w[k], v);
       w[r] = v;
     }
 #pragma unroll
