@@ -262,8 +262,9 @@ __global__ __launch_bounds__(256, 4) void k_delta_prepare(ChunkArgs c) {
   // rows of keys and queries as operands, zeros behind the last
   auto rows16 = [&](const Heads& x, int t, int s) {
     const int i = 16 * t + m;
-    if (i >= n) return Operand{0, 0, 0, 0};
-    return *reinterpret_cast<const Operand*>(static_cast<const uint16_t*>(x.p) + (uint64_t)(row + i) * x.ts + (uint64_t)hk * x.hs + 32 * s + 8 * g);
+    const uint8_t* p = static_cast<const uint8_t*>(x.p) + ((uint64_t)row * x.ts + (uint64_t)hk * x.hs) * 2;
+    const Operand v = *reinterpret_cast<const Operand*>(p + (uint32_t)(min(i, n - 1) * (int)x.ts * 2 + 64 * s + 16 * g));
+    return i < n ? v : Operand{0, 0, 0, 0};
   };
   auto squares = [&](const Operand (&x)[NS]) {
     float v = 0.f;
