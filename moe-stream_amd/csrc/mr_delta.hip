@@ -800,10 +800,11 @@ hipError_t launch_delta_rule(const Launch& K, const DeltaShape& d, const Heads& 
   const bool chunks = (int64_t)s.n_rows - s.n_seqs + 1 > kStepTokens, steps = !chunks || s.n_seqs > 1;
   if (steps) {
     ProfScope ps(K, "delta_step");
-    if (d.key_dim == 64 && d.value_dim == 64) launch_step<64, 64>(K, bf, a, kStepTokens);
-    if (d.key_dim == 64 && d.value_dim == 128) launch_step<64, 128>(K, bf, a, kStepTokens);
-    if (d.key_dim == 128 && d.value_dim == 64) launch_step<128, 64>(K, bf, a, kStepTokens);
-    if (d.key_dim == 128 && d.value_dim == 128) launch_step<128, 128>(K, bf, a, kStepTokens);
+    const int most = chunks ? kStepTokens : s.n_rows;
+    if (d.key_dim == 64 && d.value_dim == 64) launch_step<64, 64>(K, bf, a, most);
+    if (d.key_dim == 64 && d.value_dim == 128) launch_step<64, 128>(K, bf, a, most);
+    if (d.key_dim == 128 && d.value_dim == 64) launch_step<128, 64>(K, bf, a, most);
+    if (d.key_dim == 128 && d.value_dim == 128) launch_step<128, 128>(K, bf, a, most);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || !chunks) return e;
   }
