@@ -37,10 +37,11 @@ extern "C" {
  * cache, its new ones (the last of them) among them, placed as for mr_attn_decode. Its i-th of n rows stands
  * at position seq_len[s] - n + i and sees the keys at its own and at earlier positions, with a window the last of
  * those; a row before position 0, of more new tokens than cached ones, sees nothing and is zero. Lengths, pages,
- * window, sinks and numerics are mr_attn_decode's. n_seqs: up to 65535. opts NULL: defaults.
- * n_q times the query heads of a key head: below 2^24; a sixteenth of that, n_seqs and 2048, times the key heads: below 2^24
- * (more is refused). Shares its scratch with mr_attn_decode: one call of a context
- * at a time. */
+ * window, sinks and numerics are mr_attn_decode's; where sequences have more than 32 rows (new tokens times the
+ * query heads of a key head) on average, weights keep their 11 bits down to 2^-25 of the largest only. n_seqs: up to
+ * 65535; n_q times the query heads of a key head: below 2^24; a sixteenth of that, n_seqs and 2048, times the key
+ * heads: below 2^24 (more is refused). opts NULL: defaults. Shares its scratch with mr_attn_decode: one call of a
+ * context at a time. */
 int mr_attn_extend(mr_ctx* ctx, const mr_kv* kv, const mr_heads* q, uint32_t n_q, uint32_t n_seqs, const int32_t* cu_q,
                    const int32_t* seq_len, const int32_t* block_table, uint32_t max_pages, const mr_attn_opts* opts,
                    const mr_heads* out);
@@ -78,17 +79,20 @@ typedef struct mr_delta_desc {
 
 typedef struct mr_delta mr_delta;
 
-/* One layer's rule. Allocates the context's workspace for long sequences (of one size for all calls) with the
+/* One layer's rule. Allocates the context's workspace for long sequences (256 MiB, all rules' calls in turn) with the
  * first one. */
 int mr_delta_create(mr_ctx* ctx, const mr_delta_desc* desc, mr_delta** out);
 void mr_delta_destroy(mr_delta* delta);
 /* For each value head, a state S [key_dim, value_dim] (f32, a slot is [n_value_heads, key_dim, value_dim]) and token t
  * with its key k, query q, value v, g = decay (a log: 0 or less, -infinity among them) and beta:
  *   S' = exp(g) S, S = S' + beta k (v - S'^T k)^T, out = scale S^T q.
- * q, k, v and out: F16 or BF16, all the same, token strides below 2^24 elements; decay, beta: f32 [tokens, value heads] with gate_stride. States, sums,
- * and all that the next state comes from are held to 32 bits or the like: products of more than a few tokens run on
- * 16-bit matrix instructions in three parts of 8 bits a number. out is rounded once. Decays above 0 (growth) are taken
- * as they are. n_tokens: up to 2^24 - 1; n_seqs: up to 65535. */
+ * q, k, v and out: F16 or BF16, all the same, token strides below 2^24 elements; decay, beta: f32 [tokens, value
+ * heads] with gate_stride. States, sums, and all that the next state comes from are held to 32 bits or the like:
+ * products of more than a few tokens run on 16-bit matrix instructions in three parts of 8 bits a number. out is
+ * rounded once. Decays above 0 (growth) are taken as they are, -infinity forgets. What is not finite reaches no
+ * earlier token: a value makes its column NaN or infinite from its token on; a key, another decay or a beta all
+ * columns; a query its own row. Squares of keys stay within 32 bits: elements below 10^18. n_tokens: up to
+ * 2^24 - 1; n_seqs: up to 65535. */
 int mr_delta_rule(mr_ctx* ctx, const mr_delta* delta, const mr_heads* q, const mr_heads* k, const mr_heads* v,
                   const float* decay, const float* beta, uint32_t n_tokens, uint32_t n_seqs, const int32_t* cu,
                   float* states, uint32_t n_slots, const int32_t* source, const int32_t* target, const mr_heads* out);

@@ -412,3 +412,333 @@ def test_delta_of_more_chunks_than_the_workspace_holds(gpu_ctx):
             assert (np.abs(c.out[i, h] - y) <= off * 1.01 + 2.0 ** -8 * np.abs(y)).all(), (s, h)
             assert (np.abs(c.kept[c.target[s], h] - last) <= e + 1e-37).all(), (s, h)
         at += n
+
+
+@pytest.mark.parametrize("cu", [[0, 2, 400], [-3, 4, 160], [100, 0, 120], [160, 160, 0], [2 ** 30, -2 ** 31, 2 ** 31 - 1]])
+@pytest.mark.parametrize("most", [20, 160])
+def test_offsets_out_of_range(gpu_ctx, cu, most):
+    """They end in an error, whichever path takes them, and what is right in them has its result."""
+    rng = np.random.default_rng(11)
+    cu = np.array([min(x, x * most // 160) if abs(x) < 1000 else x for x in cu], np.int32)
+    c = Delta(gpu_ctx, 1, 1, 64, 64, [most - 3], M.BF16, False, rng)
+    c.new, c.source, c.target = [0, 0], np.array([-1, -1], np.int32), np.array([0, 1], np.int32)
+    c.run(cu=cu, error="cu")
+    x = R.rounded(rng.normal(size=(most, 1, 64)), M.BF16)
+    w, bx, out = gpu_ctx.to_device(np.ones((64, 4), np.float32)), R.Rows(gpu_ctx, x, M.BF16), R.Rows(gpu_ctx, None, M.F32, most, 1, 64)
+    dev = R.i32(gpu_ctx, cu)
+    M.causal_conv(gpu_ctx, M.Rows(bx.buf, 64, M.BF16), w, 4, most, 2, dev, M.Rows(out.buf, 64))
+    sync_error(gpu_ctx, "cu")
+    got = out.get()[:, 0]
+    first, last = np.clip(cu[:2], 0, most)
+    if first == 0 and last > 0:
+        y, off, _ = S.conv(x[:last, 0], np.ones((64, 4)), None, False, np.zeros((3, 64)))
+        assert (np.abs(got[:last] - y) <= off).all()
+    for b in (w, bx, out, dev):
+        b.free()
+
+
+def test_kernel_names(gpu_ctx):
+    """The documented names count launches."""
+    rng = np.random.default_rng(13)
+    l = Layer(gpu_ctx, rng, 2, 130, [3000, 2])
+    l.set([100, 2], [3000, 2])
+    gpu_ctx.set_option(M.OPT_PROFILE, 1)
+    gpu_ctx.profile_reset()
+    l.call()
+    gpu_ctx.sync()
+    counts = {k: gpu_ctx.profile_read(k)[0] for k in ("attn_extend", "extend_join", "causal_conv", "delta_step", "delta_prepare", "delta_chunks")}
+    gpu_ctx.set_option(M.OPT_PROFILE, 0)
+    assert all(n == 1 for n in counts.values()), counts
+    l.close()
+
+
+def test_delta_of_one_long_sequence_among_empty_ones(gpu_ctx):
+    rng = np.random.default_rng(12)
+    c = Delta(gpu_ctx, 1, 1, 64, 64, [0] * 20 + [70] + [0] * 19, M.BF16, False, rng)
+    c.run()
+    c.check()
+
+
+@pytest.mark.parametrize("n_seqs", [70, 1100])
+def test_many_sequences(gpu_ctx, n_seqs):
+    """More sequences than a wave has lanes, and than are looked through one by one: some long, most short."""
+    rng = np.random.default_rng(n_seqs)
+    new = rng.integers(0, 4, n_seqs)
+    new[[3, n_seqs // 2, n_seqs - 1]] = [80, 40, 130]
+    new = new.tolist()
+    c = Delta(gpu_ctx, 1, 1, 64, 64, new, M.F16, False, rng)
+    c.run()
+    c.check()
+
+    T, P, C_ = sum(new), 3, 64
+    x = R.rounded(rng.normal(size=(T, 1, C_)), M.BF16)
+    w = rng.normal(size=(C_, 4)).astype(np.float32)
+    states = rng.normal(size=(n_seqs, P, C_)).astype(np.float32)
+    bx, out = R.Rows(gpu_ctx, x, M.BF16), R.Rows(gpu_ctx, None, M.F32, T, 1, C_)
+    dev = [gpu_ctx.to_device(w), gpu_ctx.to_device(states), R.i32(gpu_ctx, offsets(new)), R.i32(gpu_ctx, np.arange(n_seqs))]
+    M.causal_conv(gpu_ctx, M.Rows(bx.buf, C_, M.BF16), dev[0], 4, T, n_seqs, dev[2], M.Rows(out.buf, C_), states=dev[1],
+                  n_slots=n_seqs, source=dev[3], target=dev[3])
+    gpu_ctx.sync()
+    got, kept, at = out.get()[:, 0], dev[1].download(np.float32).reshape(states.shape), 0
+    for s, m in enumerate(new):
+        y, off, last = S.conv(x[at:at + m, 0], w, None, False, states[s])
+        assert (np.abs(got[at:at + m] - y) <= off).all() and (kept[s] == last).all()
+        at += m
+    for b in (bx, out, *dev):
+        b.free()
+
+    lens = [n + int(k) for n, k in zip(new, rng.integers(0, 100, n_seqs))]
+    lens[3] = 900
+    cache = Cached(gpu_ctx, M.KV_MXFP4, 64, 1, 64, lens, rng)
+    q = R.rounded(rng.normal(size=(T, 2, 64)), M.BF16)
+    bq, o = R.Rows(gpu_ctx, q, M.BF16), R.Rows(gpu_ctx, None, M.BF16, T, 2, 64)
+    idx = [R.i32(gpu_ctx, a) for a in (offsets(new), lens, cache.table)]
+    cache.kv.extend(bq.heads, T, n_seqs, *idx, cache.table.shape[1], o.heads)
+    gpu_ctx.sync()
+    y, tol = extend_ref(q, cache, new, lens, 0.125, 0, None, M.BF16)
+    assert (np.abs(o.get() - y) <= tol).all()
+    for b in (bq, o, *idx):
+        b.free()
+    cache.kv.close()
+
+
+def test_extend_of_a_page_behind_4_gib(gpu_ctx):
+    rng = np.random.default_rng(14)
+    hk, D, pages = 8, 256, 8400  # pages of 512 KiB
+    assert M.KvCache.nbytes(M.KV_F16, pages, 64, hk, D) > 2 ** 32
+    kv = M.KvCache(gpu_ctx, M.KV_F16, pages, 64, hk, D)
+    n, table = 130, np.array([[pages - 1, 3, pages - 2]], np.int32)
+    k, v = (rng.normal(size=(n, hk, D)).astype(np.float32) for _ in range(2))
+    t = np.arange(n)
+    bk, bv, slots = R.Rows(gpu_ctx, k, M.F32), R.Rows(gpu_ctx, v, M.F32), R.i32(gpu_ctx, table[0][t // 64] * 64 + t % 64)
+    kv.write(bk.heads, bv.heads, n, slots)
+    for new in (1, 5, 90):
+        q = R.rounded(rng.normal(size=(new, hk * 2, D)), M.BF16)
+        bq, out = R.Rows(gpu_ctx, q, M.BF16), R.Rows(gpu_ctx, None, M.BF16, new, hk * 2, D)
+        dev = [R.i32(gpu_ctx, a) for a in ([0, new], [n], table)]
+        kv.extend(bq.heads, new, 1, *dev, 3, out.heads)
+        gpu_ctx.sync()
+        c = type("C", (), {"k": [R.stored(k, M.KV_F16)], "v": [R.stored(v, M.KV_F16)]})
+        y, tol = extend_ref(q, c, [new], [n], D ** -0.5, 0, None, M.BF16)
+        assert (np.abs(out.get() - y) <= tol).all()
+        for b in (bq, out, *dev):
+            b.free()
+    for b in (bk, bv, slots):
+        b.free()
+    kv.close()
+
+
+# scores that 16 bits do not hold, scores far apart, sinks and queries that are not finite
+@pytest.mark.parametrize("new", [1, 3, 12, 40])  # each form of the kernel
+@pytest.mark.parametrize("D", [64, 256])
+def test_extend_extremes(gpu_ctx, new, D):
+    rng = np.random.default_rng(new)
+    n, group = 300, 4
+    cache = Cached(gpu_ctx, M.KV_F16, 64, 1, D, [n], rng)
+    q = rng.normal(size=(new, group, D))
+    q[:, 1] *= 1e6      # scores of 10^6 and more: nearly one key each
+    q[:, 2] *= 1e-30    # all keys alike
+    q = R.rounded(q, M.BF16)
+    q[0, 3, 5] = np.nan
+    sinks = np.array([-np.inf, 3.0, 1.0, 0.0], np.float32)
+    bq, out = R.Rows(gpu_ctx, q, M.BF16), R.Rows(gpu_ctx, None, M.BF16, new, group, D)
+    dev = [R.i32(gpu_ctx, a) for a in ([0, new], [n], cache.table)]
+    for s, scale in ((sinks, 0.0), (None, 0.0), (sinks, -0.3), (None, 1e-30)):
+        ds = gpu_ctx.to_device(s) if s is not None else None
+        cache.kv.extend(bq.heads, new, 1, *dev, cache.table.shape[1], out.heads, scale=scale, sinks=ds)
+        gpu_ctx.sync()
+        got = out.get()
+        assert np.isnan(got[0, 3]).all()
+        q1 = np.where(np.isnan(q), 0, q)
+        y, tol = extend_ref(q1, cache, [new], [n], scale or D ** -0.5, 0, s, M.BF16)
+        ok = np.abs(got - y) <= tol
+        ok[0, 3] = True
+        assert ok.all(), np.argwhere(~ok)[:4]
+        if ds is not None:
+            ds.free()
+    for bad in (np.inf, np.nan):
+        s = np.array([1.0, bad, 0.0, 0.0], np.float32)
+        ds = gpu_ctx.to_device(s)
+        cache.kv.extend(bq.heads, new, 1, *dev, cache.table.shape[1], out.heads, sinks=ds)
+        gpu_ctx.sync()
+        got = out.get()
+        assert np.isnan(got[:, 1]).all() and np.isfinite(got[:, 0]).all() and np.isfinite(got[:, 2]).all()
+        ds.free()
+    for b in (bq, out, *dev):
+        b.free()
+    cache.kv.close()
+
+
+@pytest.mark.parametrize("new", [1, 12, 40])
+def test_extend_weights_far_below_the_largest(gpu_ctx, new):
+    """A first key 17 above the rest that has no value: the rest's weights, 2^-24.5 of the largest, keep their bits."""
+    n, D, group = 2000, 64, 4
+    rng = np.random.default_rng(1)
+    cache = Cached(gpu_ctx, M.KV_F16, 64, 1, D, [n], rng, scale=0.0)
+    k, v = np.zeros((1, 1, D), np.float32), np.zeros((1, 1, D), np.float32)
+    k[0, 0, 0] = 17.0
+    bk, bv, slot = R.Rows(gpu_ctx, k, M.F32), R.Rows(gpu_ctx, v, M.F32), R.i32(gpu_ctx, [cache.table[0, 0] * 64])
+    cache.kv.write(bk.heads, bv.heads, 1, slot)
+    cache.k[0][0], cache.v[0][0] = k[0], 0.0
+    q = np.zeros((new, group, D))
+    q[..., 0] = 1.0
+    bq, out = R.Rows(gpu_ctx, q, M.BF16), R.Rows(gpu_ctx, None, M.BF16, new, group, D)
+    dev = [R.i32(gpu_ctx, a) for a in ([0, new], [n], cache.table)]
+    cache.kv.extend(bq.heads, new, 1, *dev, cache.table.shape[1], out.heads, scale=1.0)
+    gpu_ctx.sync()
+    y, _ = extend_ref(q, cache, [new], [n], 1.0, 0, None, M.BF16)
+    # a weight is off by 2^-11 of itself (its sum too), the output by its own rounding
+    w = np.abs(cache.v[0]).mean() * n * np.exp(-17.0)
+    assert (np.abs(out.get() - y) <= 2.0 ** -8 * np.abs(y) + 2.0 ** -10 * w).all()
+    for b in (bk, bv, slot, bq, out, *dev):
+        b.free()
+    cache.kv.close()
+
+
+# ---- graphs, streams, as they are used ----------------------------------------------------------------
+class Layer:
+    """A linear layer's convolution and rule, and an attention layer's cache, over the same new tokens."""
+
+    def __init__(self, ctx, rng, n_seqs, most, lens):
+        self.ctx, self.n, self.T, self.kh, self.vh, self.D = ctx, n_seqs, most, 2, 4, 64
+        C_ = self.C = (2 * self.kh + self.vh) * self.D
+        self.w = (rng.normal(size=(C_, 4)) / 2).astype(np.float32)
+        self.x = R.rounded(rng.normal(size=(most, 1, C_)), M.BF16)
+        self.g, self.b = -np.abs(rng.normal(size=(most, self.vh))).astype(np.float32), rng.uniform(0.1, 0.9, (most, self.vh)).astype(np.float32)
+        self.conv_states = rng.normal(size=(2 * n_seqs, 3, C_)).astype(np.float32)
+        self.states = (rng.normal(size=(2 * n_seqs, self.vh, self.D, self.D)) * 0.1).astype(np.float32)
+        self.q = R.rounded(rng.normal(size=(most, 8, 64)), M.BF16)
+        self.cache = Cached(ctx, M.KV_MXINT8, 64, 2, 64, lens, rng)
+        self.rule = M.DeltaRule(ctx, self.kh, self.vh, self.D, self.D, unit_eps=1e-6)
+        up = ctx.to_device
+        self.d = dict(w=up(self.w), x=R.Rows(ctx, self.x, M.BF16), y=R.Rows(ctx, None, M.BF16, most, 1, C_), g=up(self.g), b=up(self.b),
+                      cs=up(self.conv_states), s=up(self.states), o=R.Rows(ctx, None, M.BF16, most, self.vh, self.D),
+                      q=R.Rows(ctx, self.q, M.BF16), a=R.Rows(ctx, None, M.BF16, most, 8, 64), cu=R.i32(ctx, np.zeros(n_seqs + 1)),
+                      len=R.i32(ctx, np.zeros(n_seqs)), table=R.i32(ctx, self.cache.table), src=R.i32(ctx, np.arange(n_seqs)),
+                      dst=R.i32(ctx, np.arange(n_seqs) + n_seqs))
+
+    def call(self):
+        d, D, s = self.d, self.D, 2
+        M.causal_conv(self.ctx, M.Rows(d["x"].buf, self.C, M.BF16), d["w"], 4, self.T, self.n, d["cu"], M.Rows(d["y"].buf, self.C, M.BF16),
+                      silu=True, states=d["cs"], n_slots=2 * self.n, source=d["src"], target=d["dst"])
+        at = lambda first, heads: M.Heads(d["y"].buf.ptr + first * D * s, heads, M.BF16, self.C, D)  # noqa: E731
+        self.rule.forward(at(0, self.kh), at(self.kh, self.kh), at(2 * self.kh, self.vh), d["g"], d["b"], self.T, self.n, d["cu"],
+                          d["o"].heads, states=d["s"], n_slots=2 * self.n, source=d["src"], target=d["dst"])
+        self.cache.kv.extend(d["q"].heads, self.T, self.n, d["cu"], d["len"], d["table"], self.cache.table.shape[1], d["a"].heads)
+
+    def set(self, new, lens):
+        self.ctx.sync()
+        for name, x in (("cu", offsets(new)), ("len", lens)):
+            self.d[name].upload(np.asarray(x, np.int32))
+        for name in ("y", "o", "a"):
+            self.d[name].buf.upload(np.full(self.d[name].buf.nbytes // 2, self.d[name].mark, np.uint16))
+        self.d["cs"].upload(self.conv_states), self.d["s"].upload(self.states)
+
+    def results(self):
+        self.ctx.sync()
+        return [self.d[n].all().copy() for n in ("y", "o", "a")] + [self.d[n].download(np.float32).copy() for n in ("cs", "s")]
+
+    def close(self):
+        self.rule.close(), self.cache.kv.close()
+        for x in self.d.values():
+            x.free()
+
+
+def test_graphs_see_present_offsets_and_share_their_scratch(gpu_ctx):
+    """Two captured graphs of all three calls, replayed in turn with other offsets and lengths, and eager calls between: the same bits."""
+    rng = np.random.default_rng(20)
+    layers = [Layer(gpu_ctx, rng, 3, 160, [900, 400, 64]), Layer(gpu_ctx, rng, 2, 90, [1500, 200])]
+    plans = [[([1, 1, 1], [900, 300, 1]), ([100, 0, 60], [500, 7, 60]), ([40, 33, 2], [41, 400, 64])],
+             [([90, 0], [1500, 0]), ([1, 5], [1300, 200]), ([33, 57], [33, 199])]]
+    want = []
+    for l, plan in zip(layers, plans):
+        want.append([])
+        for new, lens in plan:
+            l.set(new, lens)
+            l.call()
+            want[-1].append(l.results())
+    graphs = []
+    for l in layers:
+        gpu_ctx.graph_begin()
+        l.call()
+        graphs.append(gpu_ctx.graph_end())
+    for step in (0, 2, 1, 0, 1):
+        for l, plan in zip(layers, plans):
+            l.set(*plan[step])
+        for g in graphs:
+            g.launch()
+        for l, w in zip(layers, want):
+            for a, b in zip(l.results(), w[step]):
+                assert np.array_equal(a, b, equal_nan=True)
+        layers[0].set(*plans[0][step])
+        layers[0].call()  # eager, on the same scratch
+        for a, b in zip(layers[0].results(), want[0][step]):
+            assert np.array_equal(a, b, equal_nan=True)
+    for g in graphs:
+        g.close()
+    for l in layers:
+        l.close()
+
+
+def test_parts_of_a_prompt_follow_each_other(gpu_ctx):
+    """A prompt in one call and in parts, states and cache carried on: the same to the rounding of what is carried, which is none (conv)
+    or that of 32-bit sums (rule); attention over the cache does not carry at all."""
+    rng = np.random.default_rng(21)
+    n = 150
+    l = Layer(gpu_ctx, rng, 1, n, [n])
+    l.conv_states[:], l.states[:] = 0, 0
+    l.set([n], [n])
+    l.call()
+    whole = l.results()
+    l.set([n], [n])
+    d, at = l.d, 0
+    d["src"].upload(np.array([-1], np.int32))
+    for part in (1, 64, 3, 40, 33, 9):
+        x, y, o = (l.d[k].buf.ptr + at * w for k, w in (("x", l.C * 2), ("y", l.C * 2), ("o", l.vh * l.D * 2)))
+        cu, ln = R.i32(gpu_ctx, [0, part]), R.i32(gpu_ctx, [at + part])
+        kw = dict(n_slots=2, source=d["src"], target=d["dst"])
+        M.causal_conv(gpu_ctx, M.Rows(x, l.C, M.BF16), d["w"], 4, part, 1, cu, M.Rows(y, l.C, M.BF16), silu=True, states=d["cs"], **kw)
+        h = lambda first, heads: M.Heads(y + first * l.D * 2, heads, M.BF16, l.C, l.D)  # noqa: E731, B023
+        l.rule.forward(h(0, 2), h(2, 2), h(4, 4), d["g"].ptr + at * 16, d["b"].ptr + at * 16, part, 1, cu, M.Heads(o, 4, M.BF16), states=d["s"], **kw)
+        l.cache.kv.extend(M.Heads(d["q"].buf.ptr + at * 1024, 8, M.BF16), part, 1, cu, ln, d["table"], l.cache.table.shape[1],
+                          M.Heads(d["a"].buf.ptr + at * 1024, 8, M.BF16))
+        gpu_ctx.sync()
+        d["src"].upload(np.array([1], np.int32))
+        cu.free(), ln.free()
+        at += part
+    parts = l.results()
+    assert (parts[0] == whole[0]).all() and (parts[3][l.C * 3:] == whole[3][l.C * 3:]).all()
+    o1, o2 = (R.from_bits(x[1], M.BF16).reshape(n, -1) for x in (whole, parts))
+    # each token adds (2 * 64 + 32) half steps to a column at most (stateref.delta), and does not let it grow; both sides' outputs are rounded
+    near = 2 * 160 * n * S.U
+    s1, s2 = (x[4].reshape(2, l.vh, l.D, l.D)[1].astype(np.float64) for x in (whole, parts))
+    norm = np.sqrt((s1 * s1).sum(1)).max()
+    assert np.sqrt(((s1 - s2) ** 2).sum(1)).max() <= near * norm
+    assert (np.abs(o1 - o2) <= 2.0 ** -7 * np.abs(o1) + near * max(np.abs(o1).max(), norm)).all()
+    a1, a2 = (R.from_bits(x[2], M.BF16) for x in (whole, parts))
+    # two forms of the kernel: weights and their sum off by 2^-11 each, the outputs by their rounding
+    assert (np.abs(a1 - a2) <= 2.0 ** -7 * np.abs(a1) + 4 * 2.0 ** -11 * np.abs(l.cache.v[0]).max()).all()
+    l.close()
+
+
+def test_another_stream(gpu_ctx):
+    """The calls run on the context's stream, whichever that is, behind what is on it."""
+    import ctypes as C
+
+    hip = C.CDLL("libamdhip64.so")
+    stream = C.c_void_p()
+    assert hip.hipStreamCreateWithFlags(C.byref(stream), 1) == 0
+    got = []
+    for own in (True, False):
+        with M.Context() as ctx:
+            if not own:
+                ctx.set_stream(stream.value)
+            l = Layer(ctx, np.random.default_rng(22), 2, 100, [300, 90])
+            l.set([60, 40], [300, 90])
+            l.call()
+            l.call()  # from the same states again
+            got.append(l.results())
+            l.close()
+    assert hip.hipStreamDestroy(stream) == 0
+    for a, b in zip(*got):
+        assert np.array_equal(a, b)

@@ -78,7 +78,14 @@ def test_extend_refusals(hctx):  # noqa: F811
             (dict(scale=math.inf), M.MR_E_INVAL, "scale"), (dict(sinks=X + 1), M.MR_E_INVAL, "sinks"),
             (dict(q=M.Heads(X + 2, 16, M.BF16)), M.MR_E_INVAL, "aligned")):
         refused(status, text, call, **kw)
+    many = M.KvCache(hctx, M.KV_MXFP4, 4, 64, 64, 64)
+    q64 = M.Heads(X, 64, M.BF16)
+    for nq, n in ((16 * ((1 << 18) - 2048 - 2), 1), (16, (1 << 16) - 1), (16 * ((1 << 18) - 2048 - 60000 - 1), 60000)):
+        refused(M.MR_E_NODEV, "host-only", many.extend, q64, nq, n, X, X, X, 2, q64)
+    for nq, n in ((16 * ((1 << 18) - 2048), 1), (16 * ((1 << 18) - 2048 - 60000), 60000)):
+        refused(M.MR_E_INVAL, "too many tiles", many.extend, q64, nq, n, X, X, X, 2, q64)
     other = M.Context(M.DEVICE_NONE)
+    many.close()
     assert M.lib.mr_attn_extend(other.h, kv.h, C.byref(q.c), 1, 1, X, X, X, 1, None, C.byref(q.c)) == M.MR_E_INVAL
     assert M.lib.mr_attn_extend(None, kv.h, C.byref(q.c), 1, 1, X, X, X, 1, None, C.byref(q.c)) == M.MR_E_INVAL
     other.close(), kv.close()
