@@ -13,7 +13,8 @@ namespace {
 constexpr int kWaves = 4;
 constexpr uint32_t kSplitSeqs = 1024;      // with more sequences none is split: each workgroup looks through them all
 constexpr uint32_t kScratchRows = 65536;   // rows of partial results
-constexpr uint32_t kMinPart = kWaves;      // chunks of a part at least
+constexpr uint32_t kMinPart = kWaves;      // steps of a part at least
+constexpr int kFewRows = 16;               // up to so many rows are a wave's of its own chunks in every kernel
 
 struct ExtendArgs {
   KvPages kv;
@@ -33,7 +34,7 @@ struct ExtendArgs {
 struct Span {
   int q0, n, len;       // first row (token) of the call, new tokens, cached tokens
   int c0, chunks;       // chunks that some row sees
-  uint32_t tiles;
+  uint32_t tiles, steps;  // steps of a workgroup through the chunks
 };
 __device__ __forceinline__ int first_seen(const ExtendArgs& a, int pos) {
   return a.o.window && pos >= 0 && (uint32_t)pos >= a.o.window ? pos - (int)a.o.window + 1 : 0;
@@ -47,7 +48,9 @@ __device__ __forceinline__ Span span_of(const ExtendArgs& a, uint32_t b) {
   s.len = (int)min(max((int64_t)a.len[b], (int64_t)0), cap);
   s.c0 = first_seen(a, s.len - s.n) >> 6;
   s.chunks = s.n && s.len ? ((s.len - 1) >> 6) + 1 - s.c0 : 0;
-  s.tiles = ((uint32_t)s.n * a.group.d + (1u << a.bits) - 1) >> a.bits;
+  const uint32_t rows = (uint32_t)s.n * a.group.d;
+  s.tiles = (rows + (1u << a.bits) - 1) >> a.bits;
+  s.steps = a.bits > 5 && rows <= kFewRows ? (uint32_t)(s.chunks + kWaves - 1) / kWaves : (uint32_t)s.chunks;
   return s;
 }
 
@@ -72,13 +75,13 @@ __device__ __forceinline__ bool find_unit(const ExtendArgs& a, bool split_only, 
     return tile >= 0 && tile < (int64_t)r.sp.tiles;
   }
   Span s = lane < a.n_seqs ? span_of(a, lane) : Span{};
-  // f(tiles, chunks) of every sequence, summed
+  // f(tiles, steps) of every sequence, summed
   auto sum_of = [&](auto f) {
-    uint32_t v = lane < a.n_seqs ? f(s.tiles, (uint32_t)s.chunks) : 0;
+    uint32_t v = lane < a.n_seqs ? f(s.tiles, s.steps) : 0;
     for (uint32_t b0 = 64; b0 < a.n_seqs; b0 += 64)
       if (b0 + lane < a.n_seqs) {
         const Span x = span_of(a, b0 + lane);
-        v += f(x.tiles, (uint32_t)x.chunks);
+        v += f(x.tiles, x.steps);
       }
     return wave_total(v);
   };
@@ -90,7 +93,7 @@ __device__ __forceinline__ bool find_unit(const ExtendArgs& a, bool split_only, 
   uint32_t before = 0, slots = 0;
   for (uint32_t b0 = 0; b0 < a.n_seqs; b0 += 64) {
     if (b0) s = b0 + lane < a.n_seqs ? span_of(a, b0 + lane) : Span{};
-    const uint32_t parts = max(1u, ((uint32_t)s.chunks + size - 1) / size), n = s.tiles * parts;
+    const uint32_t parts = max(1u, (s.steps + size - 1) / size), n = s.tiles * parts;
     const uint32_t split = parts > 1 ? n : 0, count = split_only ? (parts > 1 ? s.tiles : 0) : n;
     const uint32_t sum = wave_prefix(count), ssum = wave_prefix(split);
     const uint64_t past = __ballot(before + sum > i);
@@ -105,7 +108,7 @@ __device__ __forceinline__ bool find_unit(const ExtendArgs& a, bool split_only, 
       r.slot = slots + __builtin_amdgcn_readlane(ssum - split, l) + r.tile * r.parts;
       r.sp = Span{__builtin_amdgcn_readlane(s.q0, l), __builtin_amdgcn_readlane(s.n, l), __builtin_amdgcn_readlane(s.len, l),
                   __builtin_amdgcn_readlane(s.c0, l), __builtin_amdgcn_readlane(s.chunks, l),
-                  (uint32_t)__builtin_amdgcn_readlane(s.tiles, l)};
+                  (uint32_t)__builtin_amdgcn_readlane(s.tiles, l), 0};
       return true;
     }
     before += __builtin_amdgcn_readlane(sum, 63);
@@ -145,16 +148,10 @@ constexpr int kPerSimd = NT * D >= 256 ? 1 : 2;
 // A tile of NT times 16 rows, the columns of the matrix products S = K Q^T and O = V^T P. A wave takes chunks of 64 tokens by
 // itself, operands straight from the pages.
 template <int NT, int FMT, int D>
-__global__ __launch_bounds__(64 * kWaves, (kPerSimd<NT, FMT, D>)) void k_attn_extend(ExtendArgs a) {
+__device__ __forceinline__ void attend_few(const ExtendArgs& a, const Unit& u, const Reach& t, float (*sums)[16 * D], float (*stats)[16][2]) {
   constexpr int ND = D / 16;
-  __shared__ __attribute__((aligned(16))) float sums[kWaves / 2][16 * D];
-  __shared__ float stats[kWaves / 2][16][2];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-  if (blockIdx.x == 0) check_entries(a);
-  Unit u;
-  if (!find_unit(a, false, u)) return;
   const uint32_t hk = u.hk;
-  const Reach t = reach_of(a, u);
 
   // This lane's row of each 16: its place in q and out, and which keys it sees. The query as f16 times a power of
   // two, its largest element in [2^14, 2^15): exact for f16, for bf16 all but what lies 2^-30 below the largest.
@@ -332,6 +329,15 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<NT, FMT, D>)) void k_attn_ex
   }
 }
 
+template <int NT, int FMT, int D>
+__global__ __launch_bounds__(64 * kWaves, (kPerSimd<NT, FMT, D>)) void k_attn_extend(ExtendArgs a) {
+  __shared__ __attribute__((aligned(16))) float sums[kWaves / 2][16 * D];
+  __shared__ float stats[kWaves / 2][16][2];
+  if (blockIdx.x == 0) check_entries(a);
+  Unit u;
+  if (find_unit(a, false, u)) attend_few<NT, FMT, D>(a, u, reach_of(a, u), sums, stats);
+}
+
 // ---- many rows ------------------------------------------------------------------------------
 // A tile of 128 rows, 32 to a wave, all waves at the same chunk of 64 tokens. Its codes are turned into operands once, by the
 // four waves together, and lie in LDS as the pages have them, so that writes and reads are whole rows of 16-byte pieces.
@@ -436,6 +442,11 @@ __global__ __launch_bounds__(256, (kWidePerSimd<FMT, D>)) void k_attn_extend_wid
   if (!find_unit(a, false, u)) return;
   const uint32_t hk = u.hk;
   const Reach t = reach_of(a, u);
+  if (__builtin_expect(t.rows <= kFewRows, 0)) {
+    // single tokens beside a prompt's part
+    attend_few<1, FMT, D>(a, u, t, reinterpret_cast<float(*)[16 * D]>(&lds[0][0][0]), reinterpret_cast<float(*)[16][2]>(&lds[1][0][0]));
+    return;
+  }
   const int block = KH == 2 ? wave : wave & 1, first_half = KH == 2 ? 0 : wave >> 1;
   const int mine = 32 * block + n;  // this lane's row of the tile
 
