@@ -806,6 +806,13 @@ __global__ __launch_bounds__(64 * kWaves) void k_extend_join(ExtendArgs a) {
   }
 }
 
+// Whether tiles of 17 to 32 rows are a wave's of its own chunks: where its operands, turned into f16 for two products of 16 rows,
+// leave it registers. Else they are a tile of 64 rows of k_attn_extend_wide. 32 sequences of 3 new tokens behind up to 24000, 8 heads
+// on each key head, D 64, 128, 256 (8, 4, 2 key heads), this : that (us): MXFP4 80 : 91, 95 : 83, 87 : 107; MXINT8 110 : 117,
+// 150 : 108, 135 : 125; F16 161 : 152, 184 : 153, 191 : 157.
+template <int FMT, int D>
+constexpr bool kTwo = FMT != MR_KV_F16 && (D == 64 || (D == 256 && FMT == MR_KV_MXFP4));
+
 using ExtendKernel = void (*)(ExtendArgs);
 template <int NT, int FMT, int D>
 ExtendKernel pick(int& per_cu) {
@@ -822,14 +829,16 @@ ExtendKernel pick(int& per_cu) {
   return kernel;
 }
 template <int FMT, int D>
-ExtendKernel pick(int bits, int& per_cu) {
-  return bits == 4   ? pick<1, FMT, D>(per_cu)
-         : bits == 5 ? pick<2, FMT, D>(per_cu)
-         : bits == 6 ? pick<4, FMT, D>(per_cu)
-                     : pick<8, FMT, D>(per_cu);
+ExtendKernel pick(int& bits, int& per_cu) {
+  if (bits == 4) return pick<1, FMT, D>(per_cu);
+  if constexpr (kTwo<FMT, D>) {
+    if (bits == 5) return pick<2, FMT, D>(per_cu);
+  }
+  bits = std::max(bits, 6);
+  return bits == 6 ? pick<4, FMT, D>(per_cu) : pick<8, FMT, D>(per_cu);
 }
 template <int FMT>
-ExtendKernel pick(uint32_t D, int bits, int& per_cu) {
+ExtendKernel pick(uint32_t D, int& bits, int& per_cu) {
   return D == 64 ? pick<FMT, 64>(bits, per_cu) : D == 128 ? pick<FMT, 128>(bits, per_cu) : pick<FMT, 256>(bits, per_cu);
 }
 
@@ -843,7 +852,7 @@ hipError_t launch_attn_extend(const Launch& K, const KvPages& kv, uint32_t forma
                               int n_cu) {
   const uint32_t group = q.n / kv.n_heads;
   const uint64_t rows = (uint64_t)nq * group;
-  const int bits = rows <= 16ull * n_seqs ? 4 : rows <= 32ull * n_seqs ? 5 : rows <= 64ull * n_seqs ? 6 : 7;
+  int bits = rows <= 16ull * n_seqs ? 4 : rows <= 32ull * n_seqs ? 5 : rows <= 64ull * n_seqs ? 6 : 7;
   int per_cu = 1;
   const ExtendKernel kernel = format == MR_KV_F16      ? pick<MR_KV_F16>(D, bits, per_cu)
                               : format == MR_KV_MXINT8 ? pick<MR_KV_MXINT8>(D, bits, per_cu)
