@@ -457,8 +457,9 @@ __global__ __launch_bounds__(256, 4) void k_delta_prepare(ChunkArgs c) {
 // tiles of 16 rows from w * (DK / 64) on, whose part of K S it works out for the whole chunk, and the chunk's tokens from 16 w on
 // after that. Four others work out the tokens' outputs beside them, a step behind.
 template <int DK, int NP, bool BF>
-__global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs c, uint32_t slices, int parity) {
+__global__ __launch_bounds__(512, (DK == 64 || NP == 1 ? 4 : 2)) void k_delta_chunks(ChunkArgs c, uint32_t slices, int parity) {
   constexpr int NS = DK / 32, NT = DK / 64;
+  constexpr bool kLate = DK == 128 && NP == 1;  // T is asked for a step later: there is no room for it before
   using I = DeltaImage<DK, NP>;
   __shared__ __attribute__((aligned(16))) uint8_t state[NS][2][1024], rest[2][3][1024], faded[2][3][1024];
   __shared__ f32x4 fresh[4][64], sums[4][4][64];
@@ -471,8 +472,9 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs c, uint32_t s
   Chunked seq;
   if (h >= a.d.value_heads || !find_sequence(c, blockIdx.y, false, seq)) return;
   const uint32_t hk = h / (a.d.value_heads / a.d.key_heads), DV = a.d.value_dim;
-  const int wave = (threadIdx.x >> 6) & 3, lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
-  const bool outputs = __builtin_amdgcn_readfirstlane(threadIdx.x) >= 256;
+  const int number = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = number & 3;
+  const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+  const bool outputs = number >= 4;
   const uint32_t s = seq.s, start = seq.start;
   const int q0 = seq.q0, q1 = seq.q1, n = q1 - q0;
   const uint32_t count = (n + kChunk - 1) / kChunk;
@@ -499,7 +501,7 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs c, uint32_t s
       for (int x = 0; x < NS; ++x)
 #pragma unroll
         for (int p = 0; p < NP; ++p) Q[x][p] = operand(key_image + I::kQ + ((wave * NS + x) * NP + p) * 1024);
-      of_q = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(image + I::kVec) + 64 + t0);
+      of_q = *reinterpret_cast<const f32x4*>(image + I::kVec + 256 + (uint32_t)(4 * t0));
     };
     auto load_mix = [&] {
 #pragma unroll
@@ -596,15 +598,15 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs c, uint32_t s
         for (int p = 0; p < NP; ++p)
           K[t][p] = *reinterpret_cast<const Part*>(key_image + I::kK + ((t * NS + wave * NT / 2) * NP + p) * 1024 + lane * 16 + (NT == 1 ? 8 * (wave & 1) : 0));
     };
-    auto vec = [&] { return reinterpret_cast<const float*>(image + I::kVec) + t0; };
+    auto vec = [&](int i) { return *reinterpret_cast<const f32x4*>(image + I::kVec + 256 * i + (uint32_t)(4 * t0)); };
     auto load_values = [&](int row) {
-      of_k = *reinterpret_cast<const f32x4*>(vec());
+      of_k = vec(0);
       const uint8_t* v = static_cast<const uint8_t*>(a.v.p) + ((uint64_t)row * a.v.ts + (uint64_t)h * a.v.hs + 16 * slice) * 2;
 #pragma unroll
       for (int r = 0; r < 4; ++r) vals[r] = *reinterpret_cast<const uint16_t*>(v + (uint32_t)(min(t0 + r, q1 - 1 - row) * step + 2 * m));
     };
     auto load_solution = [&] {
-      of_v = *reinterpret_cast<const f32x4*>(vec() + 128);
+      of_v = vec(2);
 #pragma unroll
       for (int x = 0; x < 2; ++x)
 #pragma unroll
@@ -723,8 +725,7 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs c, uint32_t s
 #pragma unroll
         for (int p = 0; p < 3; ++p) y[0][p] = operand(faded[0][p]), y[1][p] = operand(faded[1][p]);
         __builtin_amdgcn_sched_barrier(0);
-        load_solution();
-        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (!kLate) { load_solution(); __builtin_amdgcn_sched_barrier(0); }
         const float keep = lost ? NAN : fade;
         f32x4 sum[NT][3] = {};
 #pragma unroll
@@ -738,8 +739,13 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs c, uint32_t s
 #pragma unroll
         for (int t = 0; t < NT; ++t) S[t] = S[t] * keep + ((sum[t][2] + sum[t][1]) + sum[t][0]);
       }
+      __builtin_amdgcn_sched_barrier(0);
       load_fade(key_image);
+      __builtin_amdgcn_sched_barrier(0);
       look();
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (kLate) load_solution();
+      __builtin_amdgcn_sched_barrier(0);
       __syncthreads();
     }
   }
