@@ -255,7 +255,7 @@ __global__ __launch_bounds__(256, 4) void k_delta_prepare(ChunkArgs c) {
   const uint32_t h = blockIdx.x, group = a.d.value_heads / a.d.key_heads, hk = h / group;
   int row, n;
   if (!find_chunk(c, c.first + blockIdx.y, row, n)) return;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
   uint8_t* image = c.values + ((uint64_t)blockIdx.y * a.d.value_heads + h) * I::kValue;
   uint8_t* key_image = c.keys + ((uint64_t)blockIdx.y * a.d.key_heads + hk) * I::kKey;
 
