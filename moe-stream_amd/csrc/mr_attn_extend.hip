@@ -54,10 +54,10 @@ __device__ __forceinline__ Span span_of(const ExtendArgs& a, uint32_t b) {
   return s;
 }
 
-// A workgroup's unit: a tile of a sequence, a part of its keys and a key head, heads in turn: workgroups go to the 8 XCDs in turn, so that
-// the tiles of a head, a part after the other, are on few of them and find the keys that they share in one L2 (a prompt's part among 32
-// tokens, 8 heads: 208 us with units in turn, 195 so). split_only: tile blockIdx.x of the sequences of several parts and key head
-// blockIdx.y; the part is then 0. slot: parts of split sequences in front of the tile's.
+// A workgroup's unit: a tile of a sequence, a part of its keys and a key head, heads in turn: workgroups go to the 8 XCDs in turn, so
+// that the tiles of a head, a part after the other, are on few of them and find the keys that they share in one L2 (a prompt's part
+// among 32 tokens, 8 heads: 208 us with units in turn, 195 so). split_only: tile blockIdx.x of the sequences of several parts and key
+// head blockIdx.y; the part is then 0. slot: parts of split sequences in front of the tile's.
 struct Unit {
   uint32_t b, hk, tile, part, parts, slot;
   Span sp;
@@ -146,11 +146,13 @@ template <int NT, int FMT, int D>
 constexpr int kPerSimd = NT * D >= 256 ? 1 : 2;
 
 // A tile of NT times 16 rows, the columns of the matrix products S = K Q^T and O = V^T P. A wave takes chunks of 64 tokens by
-// itself, operands straight from the pages.
+// itself, operands straight from the pages, and the waves' results are joined at the end. The cache's bytes bound it while a tile has
+// 16 rows: two new tokens of 32 sequences behind up to 24000, 32 heads on 4 of 128: MXFP4 52 us (4.2 TB/s), F16 154 us (5.3 TB/s);
+// turning codes into operands for more rows than that is then most of it.
 template <int NT, int FMT, int D>
 __device__ __forceinline__ void attend_few(const ExtendArgs& a, const Unit& u, const Reach& t, float (*sums)[16 * D], float (*stats)[16][2]) {
   constexpr int ND = D / 16;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const uint32_t hk = u.hk;
 
   // This lane's row of each 16: its place in q and out, and which keys it sees. The query as f16 times a power of
@@ -342,7 +344,10 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<NT, FMT, D>)) void k_attn_ex
 // A tile of 128 rows, 32 to a wave, all waves at the same chunk of 64 tokens. Its codes are turned into operands once, by the
 // four waves together, and lie in LDS as the pages have them, so that writes and reads are whole rows of 16-byte pieces.
 // Both products are 32x32x16 matrix instructions, keys (then the values' elements) down and rows across: a lane has the scores
-// of one row. Of each 32 keys the result's row 16 c + 8 x + 4 h + r stands for key 16 x + 8 c + 4 h + r: lane half h then holds,
+// of one row. Each chunk's codes are turned once for 128 rows, not for 32. Bounds: heads of 256, matrix and vector instructions of the
+// one wave of a SIMD, which hardly overlap (2048 tokens behind 30001, 16 heads on 2, MXINT8: 1170 us, 890 TFLOP/s); heads of 128,
+// loads and the last round of units (four parts of prompts in F16, 167 us, 760 TFLOP/s); heads of 64, vector instructions (a part of
+// 1000 tokens and 32 single ones, MXINT8: 174 us, 670 TFLOP/s). Of each 32 keys the result's row 16 c + 8 x + 4 h + r stands for key 16 x + 8 c + 4 h + r: lane half h then holds,
 // 8 numbers after the other, what the second product's right operand wants for the values of lane group 2 c + h.
 constexpr float kWideSlack = 4.f, kWideLift = 11.f;  // weights up to 2^15: the maximum is followed when it has moved by 2^4
 
@@ -443,7 +448,8 @@ __global__ __launch_bounds__(256, (kWidePerSimd<FMT, D>)) void k_attn_extend_wid
   const uint32_t hk = u.hk;
   const Reach t = reach_of(a, u);
   if (__builtin_expect(t.rows <= kFewRows, 0)) {
-    // single tokens beside a prompt's part
+    // single tokens beside a prompt's part: of 32, 194 us as tiles like the others, 174 us so; expected to be the rarer, which
+    // leaves the others' loop where it is (1170 us for heads of 256, else 1212 us)
     attend_few<1, FMT, D>(a, u, t, reinterpret_cast<float(*)[16 * D]>(&lds[0][0][0]), reinterpret_cast<float(*)[16][2]>(&lds[1][0][0]));
     return;
   }
@@ -768,7 +774,8 @@ __global__ __launch_bounds__(256, (kWidePerSimd<FMT, D>)) void k_attn_extend_wid
              f32x4{acc[x][i], acc[x][i + 1], acc[x][i + 2], acc[x][i + 3]} * f);
 }
 
-// Joins the parts of split tile blockIdx.x, a wave for each row: first all parts' weights, then the weighted sums.
+// Joins the parts of split tile blockIdx.x, a wave for each row: first all parts' weights, then the weighted sums. Memory and the look
+// for the tile bound it: 5 to 19 us (51200 rows of 128 in two or three parts).
 template <int D>
 __global__ __launch_bounds__(64 * kWaves) void k_extend_join(ExtendArgs a) {
   constexpr int L = D / 4, G = 64 / L;  // lanes of a row, parts at a time

@@ -3,7 +3,8 @@
 // out_t = act(bias + sum_j w_j x_(t - taps + 1 + j)): each input is used `taps` times, so memory bounds it. A lane has 8
 // adjacent channels of a run of rows of one sequence, the last inputs in registers; only a run's first rows read
 // inputs of the run before again. A sequence's first run has no fewer than taps - 1 rows, or all of them: it alone
-// reads the old state, and the same lane writes the new one after that, so that both may be one slot.
+// reads the old state, and the same lane writes the new one after that, so that both may be one slot. Seven prompts, 8192 channels,
+// f32 to bf16, 253 MB: 64 us, 4.0 TB/s; 48 sequences of one token: 6.5 us, launch and three loads in turn.
 #include "mr_state_device.h"
 
 namespace mr {
