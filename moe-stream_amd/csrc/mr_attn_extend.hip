@@ -344,11 +344,13 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<NT, FMT, D>)) void k_attn_ex
 // A tile of 128 rows, 32 to a wave, all waves at the same chunk of 64 tokens. Its codes are turned into operands once, by the
 // four waves together, and lie in LDS as the pages have them, so that writes and reads are whole rows of 16-byte pieces.
 // Both products are 32x32x16 matrix instructions, keys (then the values' elements) down and rows across: a lane has the scores
-// of one row. Each chunk's codes are turned once for 128 rows, not for 32. Bounds: heads of 256, matrix and vector instructions of the
-// one wave of a SIMD, which hardly overlap (2048 tokens behind 30001, 16 heads on 2, MXINT8: 1170 us, 890 TFLOP/s); heads of 128,
-// loads and the last round of units (four parts of prompts in F16, 167 us, 760 TFLOP/s); heads of 64, vector instructions (a part of
-// 1000 tokens and 32 single ones, MXINT8: 174 us, 670 TFLOP/s). Of each 32 keys the result's row 16 c + 8 x + 4 h + r stands for key 16 x + 8 c + 4 h + r: lane half h then holds,
+// of one row. Of each 32 keys the result's row 16 c + 8 x + 4 h + r stands for key 16 x + 8 c + 4 h + r: lane half h then holds,
 // 8 numbers after the other, what the second product's right operand wants for the values of lane group 2 c + h.
+//
+// Bounds: heads of 256, matrix and vector instructions of the one wave of a SIMD, which hardly overlap (2048 tokens behind 30001,
+// 16 heads on 2, MXINT8: 1170 us, 890 TFLOP/s); heads of 128, loads and the last round of units (four parts of prompts, 32 heads
+// on 4, F16: 167 us, 760 TFLOP/s); heads of 64, vector instructions (a part of 1000 tokens and 32 single ones, 64 heads on 8,
+// MXINT8: 174 us, 620 TFLOP/s).
 constexpr float kWideSlack = 4.f, kWideLift = 11.f;  // weights up to 2^15: the maximum is followed when it has moved by 2^4
 
 // A wave's quarter of a chunk on its way from the pages to LDS.
@@ -449,7 +451,7 @@ __global__ __launch_bounds__(256, (kWidePerSimd<FMT, D>)) void k_attn_extend_wid
   const Reach t = reach_of(a, u);
   if (__builtin_expect(t.rows <= kFewRows, 0)) {
     // single tokens beside a prompt's part: of 32, 194 us as tiles like the others, 174 us so; expected to be the rarer, which
-    // leaves the others' loop where it is (1170 us for heads of 256, else 1212 us)
+    // leaves the others' code where it is (a part of 2048 tokens, heads of 256: 1175 us, else 1212 us)
     attend_few<1, FMT, D>(a, u, t, reinterpret_cast<float(*)[16 * D]>(&lds[0][0][0]), reinterpret_cast<float(*)[16][2]>(&lds[1][0][0]));
     return;
   }

@@ -28,16 +28,16 @@ __device__ __forceinline__ void gates(const DeltaArgs& a, uint64_t t, uint32_t h
   beta = 1.f / (1.f + expf(-beta));
 }
 
-// A state's rows lie across the lanes, four columns each; a thread has every G-th row. S'^T k and S'^T q are taken
+// A state's rows lie across the lanes, four columns each; a thread has N adjacent rows. S'^T k and S'^T q are taken
 // together, as out = scale (S'^T q + (k . q) correction): one exchange between the lanes for each token. For one token the states'
-// bytes bound it (48 sequences, 32 heads of 128 by 128, 202 MB: 48 us, 4.2 TB/s; one sequence 6.3 us, launch and loads in turn),
-// for a few the exchanges (16 sequences of 5 tokens, 69 MB: 23 us).
+// bytes bound it (48 sequences, 32 heads of 128 by 128, 202 MB: 48 us, 4.2 TB/s; one sequence 6.2 us, launch and loads in turn),
+// for a few the products and exchanges of each token in turn (16 sequences of 5 tokens, 69 MB: 22 us).
 template <int DK, int DV, bool BF>
 __global__ __launch_bounds__(256) void k_delta_step(DeltaArgs a, int most) {
-  constexpr int L = DV / 4, G = 256 / L, N = DK / G, E = DK / 64;
+  constexpr int L = DV / 4, G = 256 / L, N = DK / G, E = DK / 64, F = DV / 64;
   constexpr int kT = 8;  // tokens staged at once
   constexpr uint32_t kType = BF ? MR_BF16 : MR_F16;
-  __shared__ __attribute__((aligned(16))) float key[kT][DK], query[kT][DK], red[2][4][2][DV];
+  __shared__ __attribute__((aligned(16))) float key[kT][DK], query[kT][DK], value[kT][DV], red[2][4][2][DV];
   __shared__ float fade[kT], gain[kT], both[kT];
   const Sequences& sq = a.s;
   const uint32_t h = blockIdx.x, s = blockIdx.y, hk = h / (a.d.value_heads / a.d.key_heads);
@@ -47,28 +47,41 @@ __global__ __launch_bounds__(256) void k_delta_step(DeltaArgs a, int most) {
   const int n = q1 - q0;
   const int source = slot_of(sq, sq.source, s), target = slot_of(sq, sq.target, s);
   if (n > most || (n == 0 && (target < 0 || target == source))) return;
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = tid / L, col = 4 * (tid % L);
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = tid / L, col = 4 * (tid % L);
 
   f32x4 S[N] = {};
   if (source >= 0) {
     const float* p = sq.states + ((uint64_t)source * a.d.value_heads + h) * (DK * DV) + col;
 #pragma unroll
-    for (int i = 0; i < N; ++i) S[i] = *reinterpret_cast<const f32x4*>(p + (g + G * i) * DV);
+    for (int i = 0; i < N; ++i) S[i] = *reinterpret_cast<const f32x4*>(p + (N * g + i) * DV);
   }
   for (int t0 = 0; t0 < n; t0 += kT) {
     const int m = min(kT, n - t0);
     __syncthreads();
-    for (int t = wave; t < m; t += 4) {
-      const uint64_t row = (uint64_t)(q0 + t0 + t);
-      float x[E], y[E], xx = 0.f, yy = 0.f, xy = 0.f;
+    // Tokens wave and wave + 4: all their loads first.
+    float x[2][E], y[2][E], v[2][F], lg[2], b[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint64_t row = (uint64_t)(q0 + t0 + min(wave + 4 * j, m - 1));
       const uint16_t* qp = static_cast<const uint16_t*>(a.q.p) + row * a.q.ts + (uint64_t)hk * a.q.hs + E * lane;
       const uint16_t* kp = static_cast<const uint16_t*>(a.k.p) + row * a.k.ts + (uint64_t)hk * a.k.hs + E * lane;
+      const uint16_t* vp = static_cast<const uint16_t*>(a.v.p) + row * a.v.ts + (uint64_t)h * a.v.hs + F * lane;
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        x[e] = BF ? bits_f32((uint32_t)qp[e] << 16) : h2f(qp[e]);
-        y[e] = BF ? bits_f32((uint32_t)kp[e] << 16) : h2f(kp[e]);
-        xx = fmaf(x[e], x[e], xx), yy = fmaf(y[e], y[e], yy), xy = fmaf(x[e], y[e], xy);
+        x[j][e] = BF ? bits_f32((uint32_t)qp[e] << 16) : h2f(qp[e]);
+        y[j][e] = BF ? bits_f32((uint32_t)kp[e] << 16) : h2f(kp[e]);
       }
+#pragma unroll
+      for (int e = 0; e < F; ++e) v[j][e] = BF ? bits_f32((uint32_t)vp[e] << 16) : h2f(vp[e]);
+      gates(a, row, h, lg[j], b[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int t = wave + 4 * j;
+      if (t >= m) break;
+      float xx = 0.f, yy = 0.f, xy = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) xx = fmaf(x[j][e], x[j][e], xx), yy = fmaf(y[j][e], y[j][e], yy), xy = fmaf(x[j][e], y[j][e], xy);
       float fx = a.d.scale, fy = 1.f;
       if (a.d.unit_eps > 0.f) {
         fx /= sqrtf(wave_sum_fast(xx) + a.d.unit_eps);
@@ -76,20 +89,22 @@ __global__ __launch_bounds__(256) void k_delta_step(DeltaArgs a, int most) {
       }
       xy = wave_sum_fast(xy);
 #pragma unroll
-      for (int e = 0; e < E; ++e) query[t][E * lane + e] = x[e] * fx, key[t][E * lane + e] = y[e] * fy;
-      if (lane == 0) {
-        float lg, b;
-        gates(a, row, h, lg, b);
-        fade[t] = expf(lg), gain[t] = b, both[t] = xy * fx * fy;
-      }
+      for (int e = 0; e < E; ++e) query[t][E * lane + e] = x[j][e] * fx, key[t][E * lane + e] = y[j][e] * fy;
+#pragma unroll
+      for (int e = 0; e < F; ++e) value[t][F * lane + e] = v[j][e];
+      if (lane == 0) fade[t] = expf(lg[j]), gain[t] = b[j], both[t] = xy * fx * fy;
     }
     __syncthreads();
     for (int t = 0; t < m; ++t) {
       const uint64_t row = (uint64_t)(q0 + t0 + t);
-      const f32x4 v = load4(a.v.p, kType, row * a.v.ts + (uint64_t)h * a.v.hs + col);
-      f32x4 sk = {}, sq4 = {};
+      f32x4 sk = {}, sq4 = {}, k[N / 4];
 #pragma unroll
-      for (int i = 0; i < N; ++i) sk += S[i] * key[t][g + G * i], sq4 += S[i] * query[t][g + G * i];
+      for (int i = 0; i < N / 4; ++i) {
+        k[i] = *reinterpret_cast<const f32x4*>(&key[t][N * g + 4 * i]);
+        const f32x4 x = *reinterpret_cast<const f32x4*>(&query[t][N * g + 4 * i]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sk += S[4 * i + j] * k[i][j], sq4 += S[4 * i + j] * x[j];
+      }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         sk[j] = add_xor32(sk[j]), sq4[j] = add_xor32(sq4[j]);
@@ -103,16 +118,16 @@ __global__ __launch_bounds__(256) void k_delta_step(DeltaArgs a, int most) {
       for (int w = 0; w < 4; ++w)
         sk += *reinterpret_cast<const f32x4*>(&r[w][0][col]), sq4 += *reinterpret_cast<const f32x4*>(&r[w][1][col]);
       const float f = fade[t];
-      const f32x4 d = (v - sk * f) * gain[t];
+      const f32x4 d = (*reinterpret_cast<const f32x4*>(&value[t][col]) - sk * f) * gain[t];
       if (tid < L) store4(a.out.p, kType, row * a.out.ts + (uint64_t)h * a.out.hs + col, sq4 * f + d * both[t]);
 #pragma unroll
-      for (int i = 0; i < N; ++i) S[i] = S[i] * f + d * key[t][g + G * i];
+      for (int i = 0; i < N; ++i) S[i] = S[i] * f + d * k[i / 4][i % 4];
     }
   }
   if (target >= 0) {
     float* p = sq.states + ((uint64_t)target * a.d.value_heads + h) * (DK * DV) + col;
 #pragma unroll
-    for (int i = 0; i < N; ++i) *reinterpret_cast<f32x4*>(p + (g + G * i) * DV) = S[i];
+    for (int i = 0; i < N; ++i) *reinterpret_cast<f32x4*>(p + (N * g + i) * DV) = S[i];
   }
 }
 
@@ -772,9 +787,10 @@ void launch_step(const Launch& K, bool bf, const DeltaArgs& a, int most) {
   hipLaunchKernelGGL((bf ? k_delta_step<DK, DV, true> : k_delta_step<DK, DV, false>), g, b, 0, K.s, a, most);
 }
 
-// Sequences of up to so many tokens go through k_delta_step: a token takes it 0.5 us, the other two kernels' launches and first
-// chunk 16 us.
-constexpr int kStepTokens = 32;
+// Sequences of up to so many tokens go through k_delta_step, whose workgroups of one sequence take 1.1 us a token; the other two
+// kernels take 19 us for a sequence's first chunk, each further sequence about 3.5 us of all CUs. 32 heads of 128, step : chunks (us):
+// one sequence of 16 tokens 22 : 19, of 32, 40 : 19; 4 sequences of 32, 44 : 30; 16 of 16, 38 : 72, of 32, 63 : 72.
+int step_tokens(uint32_t n_seqs, uint32_t value_heads) { return (int)std::min<uint64_t>(32, 12 + (uint64_t)n_seqs * value_heads / 16); }
 constexpr uint64_t kScratch = 256ull << 20;
 
 template <int DK, bool BF>
@@ -812,11 +828,13 @@ hipError_t launch_delta_rule(const Launch& K, const DeltaShape& d, const Heads& 
                              const float* decay, const float* beta, const Sequences& s, const Heads& out, void* scratch) {
   const DeltaArgs a{d, q, k, v, out, decay, beta, s};
   const bool bf = q.dtype == MR_BF16;
-  // One sequence takes one path, and so do sequences that are all short if none is without tokens; else one may be long.
-  const bool chunks = (int64_t)s.n_rows - s.n_seqs + 1 > kStepTokens, steps = !chunks || s.n_seqs > 1;
+  // One sequence takes one path, and so do sequences that are all short if none is without tokens. Where so few rows are one long
+  // sequence's among empty ones, it goes token by token too: two more launches for every batch of single tokens would cost 7 us of 48.
+  const int few = step_tokens(s.n_seqs, d.value_heads);
+  const bool chunks = (int64_t)s.n_rows - s.n_seqs + 1 > few, steps = !chunks || s.n_seqs > 1;
   if (steps) {
     ProfScope ps(K, "delta_step");
-    const int most = chunks ? kStepTokens : s.n_rows;
+    const int most = chunks ? few : s.n_rows;
     if (d.key_dim == 64 && d.value_dim == 64) launch_step<64, 64>(K, bf, a, most);
     if (d.key_dim == 64 && d.value_dim == 128) launch_step<64, 128>(K, bf, a, most);
     if (d.key_dim == 128 && d.value_dim == 64) launch_step<128, 64>(K, bf, a, most);
@@ -824,7 +842,7 @@ hipError_t launch_delta_rule(const Launch& K, const DeltaShape& d, const Heads& 
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || !chunks) return e;
   }
-  const int least = steps ? kStepTokens + 1 : 0;
+  const int least = steps ? few + 1 : 0;
   uint8_t* w = static_cast<uint8_t*>(scratch);
   if (d.key_dim == 64) return bf ? launch_chunks<64, true>(K, a, least, w) : launch_chunks<64, false>(K, a, least, w);
   return bf ? launch_chunks<128, true>(K, a, least, w) : launch_chunks<128, false>(K, a, least, w);
