@@ -309,6 +309,15 @@ def test_delta(gpu_ctx, new, kh, vh, dk, dv, kind, raw, in_place):
     c.check()
 
 
+# lengths about the one up to which sequences go token by token: 12 and more, by the number of sequences and heads
+@pytest.mark.parametrize("new", [[11], [12], [13], [14], [12, 13, 14], [32, 33, 31], [13] * 9])
+@pytest.mark.parametrize("kh,vh,dk,dv,kind", [(1, 2, 128, 128, "bf16"), (1, 2, 64, 128, "f16"), (4, 16, 64, 64, "bf16")])
+def test_delta_at_the_border_of_its_paths(gpu_ctx, new, kh, vh, dk, dv, kind):
+    c = Delta(gpu_ctx, kh, vh, dk, dv, new, TYPES[kind], False, np.random.default_rng(sum(new) + vh))
+    c.run()
+    c.check()
+
+
 @pytest.mark.parametrize("new", [[1, 3], [150, 70]])
 def test_delta_decays_of_any_size(gpu_ctx, new):
     rng = np.random.default_rng(8)
