@@ -109,7 +109,8 @@ __device__ __forceinline__ bool find_unit(const ExtendArgs& a, bool split_only, 
       r.sp = Span{__builtin_amdgcn_readlane(s.q0, l), __builtin_amdgcn_readlane(s.n, l), __builtin_amdgcn_readlane(s.len, l),
                   __builtin_amdgcn_readlane(s.c0, l), __builtin_amdgcn_readlane(s.chunks, l),
                   (uint32_t)__builtin_amdgcn_readlane(s.tiles, l), 0};
-      return true;
+      // Offsets in order leave room: parts beyond the first are half of a.parts at most, or all of them. Overlapping ones may not.
+      return r.parts == 1 || r.slot + r.parts <= a.parts;
     }
     before += __builtin_amdgcn_readlane(sum, 63);
     slots += __builtin_amdgcn_readlane(ssum, 63);
@@ -871,9 +872,11 @@ hipError_t launch_attn_extend(const Launch& K, const KvPages& kv, uint32_t forma
   const uint64_t pages = (uint64_t)max_pages << (kv.page_shift - 6);
   const uint64_t cap = o.window ? std::min<uint64_t>(pages, (o.window + ((1ull << bits) / group + 1) + 62) / 64 + 1) : pages;
   const uint64_t tiles = (rows >> bits) + n_seqs;  // at most
+  // chunks that a sequence's tiles see together, at most
+  const uint64_t span = o.window ? std::min<uint64_t>(pages, ((uint64_t)o.window + nq + 62) / 64 + 1) : pages;
   const uint32_t room = std::min<uint32_t>(kScratchRows >> bits, per_cu * n_cu);
   // the chunks of all tiles are counted in 32 bits
-  const bool whole = cap <= 2 * kWaves || n_seqs > kSplitSeqs || tiles * cap >= 1ull << 31;
+  const bool whole = cap <= 2 * kWaves || n_seqs > kSplitSeqs || tiles * span >= 1ull << 31;
   a.parts = whole ? 1 : std::max<uint32_t>(1, room / kv.n_heads);
   hipError_t e;
   {

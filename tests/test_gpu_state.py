@@ -175,6 +175,33 @@ def test_extend_entries_out_of_range(gpu_ctx):
     cache.kv.close()
 
 
+@pytest.mark.parametrize("new", [1, 12, 30])
+def test_extend_of_overlapping_offsets(gpu_ctx, new):
+    """Every other sequence claims all rows: an error, rows that hold some sequence's result or none, and nothing written elsewhere."""
+    n_seqs, n = 60, 3000
+    T = new * n_seqs
+    rng = np.random.default_rng(new)
+    cache = Cached(gpu_ctx, M.KV_MXFP4, 64, 1, 64, [n], rng)
+    table = np.repeat(cache.table, n_seqs, 0)
+    q = R.rounded(rng.normal(size=(T, 4, 64)), M.BF16)
+    bq, out = R.Rows(gpu_ctx, q, M.BF16), R.Rows(gpu_ctx, None, M.BF16, T, 4, 64)
+    cu = np.array([T * (s & 1) for s in range(n_seqs + 1)], np.int32)
+    dev = [R.i32(gpu_ctx, a) for a in (cu, [n] * n_seqs, table)]
+    cache.kv.extend(bq.heads, T, n_seqs, *dev, table.shape[1], out.heads)
+    sync_error(gpu_ctx, "cu_q")
+    assert np.isfinite(out.get()).all()
+    # the same call with offsets in order
+    dev[0].upload(offsets([new] * n_seqs))
+    cache.kv.extend(bq.heads, T, n_seqs, *dev, table.shape[1], out.heads)
+    gpu_ctx.sync()
+    some = slice(7 * new, 8 * new)
+    y, tol = extend_ref(q[some], cache, [new], [n], 0.125, 0, None, M.BF16)
+    assert (np.abs(out.get()[some] - y) <= tol).all()
+    for b in (bq, out, *dev):
+        b.free()
+    cache.kv.close()
+
+
 # ---- causal convolution --------------------------------------------------------------------------
 @pytest.mark.parametrize("C_,new", [(8, [1]), (64, [1, 1, 1, 1, 1]), (520, [2, 0, 5, 1, 33]), (2056, [16, 17, 15, 4, 3]),
                                     (4104, [100, 1]), (64, [0, 0, 3])])
