@@ -789,7 +789,7 @@ void launch_step(const Launch& K, bool bf, const DeltaArgs& a, int most) {
 
 // Sequences of up to so many tokens go through k_delta_step, whose workgroups of one sequence take 1.1 us a token; the other two
 // kernels take 19 us for a sequence's first chunk, each further sequence about 3.5 us of all CUs. 32 heads of 128, step : chunks (us):
-// one sequence of 16 tokens 22 : 19, of 32, 40 : 19; 4 sequences of 32, 44 : 30; 16 of 16, 38 : 72, of 32, 63 : 72.
+// one sequence of 16 tokens 22 : 18, of 32, 40 : 19 (of 33); 4 sequences of 32, 44 : 30 (of 33); 16 of 16, 38, of 32, 63 : 72 (of 40).
 int step_tokens(uint32_t n_seqs, uint32_t value_heads) { return (int)std::min<uint64_t>(32, 12 + (uint64_t)n_seqs * value_heads / 16); }
 constexpr uint64_t kScratch = 256ull << 20;
 
