@@ -828,10 +828,11 @@ hipError_t launch_delta_rule(const Launch& K, const DeltaShape& d, const Heads& 
                              const float* decay, const float* beta, const Sequences& s, const Heads& out, void* scratch) {
   const DeltaArgs a{d, q, k, v, out, decay, beta, s};
   const bool bf = q.dtype == MR_BF16;
-  // One sequence takes one path, and so do sequences that are all short if none is without tokens. Where so few rows are one long
-  // sequence's among empty ones, it goes token by token too: two more launches for every batch of single tokens would cost 7 us of 48.
+  // One sequence takes one path, and so do a few rows of sequences that are all short if none is without tokens: two more launches
+  // would cost batches of single tokens 7 us (48 sequences: of 47; 160: of 131). If some are, one long sequence of so few rows, 1.1 us a
+  // token, goes token by token.
   const int few = step_tokens(s.n_seqs, d.value_heads);
-  const bool chunks = (int64_t)s.n_rows - s.n_seqs + 1 > few, steps = !chunks || s.n_seqs > 1;
+  const bool chunks = (int64_t)s.n_rows - s.n_seqs + 1 > few || s.n_rows > 8 * few, steps = !chunks || s.n_seqs > 1;
   if (steps) {
     ProfScope ps(K, "delta_step");
     const int most = chunks ? few : s.n_rows;

@@ -488,9 +488,10 @@ def test_kernel_names(gpu_ctx):
     l.close()
 
 
-def test_delta_of_one_long_sequence_among_empty_ones(gpu_ctx):
+@pytest.mark.parametrize("n", [40, 70, 108, 109, 110, 130])  # 14 * 8 rows, 3 of them in no sequence, are the most that all go token by token
+def test_delta_of_one_long_sequence_among_empty_ones(gpu_ctx, n):
     rng = np.random.default_rng(12)
-    c = Delta(gpu_ctx, 1, 1, 64, 64, [0] * 20 + [70] + [0] * 19, M.BF16, False, rng)
+    c = Delta(gpu_ctx, 1, 1, 64, 64, [0] * 20 + [n] + [0] * 19, M.BF16, False, rng)
     c.run()
     c.check()
 
