@@ -89,7 +89,8 @@ void mr_delta_destroy(mr_delta* delta);
  * q, k, v and out: F16 or BF16, all the same, token strides below 2^24 elements; decay, beta: f32 [tokens, value
  * heads] with gate_stride. States, sums, and all that the next state comes from are held to 32 bits or the like:
  * products of more than a few tokens run on 16-bit matrix instructions in three parts of 8 bits a number. out is
- * rounded once. Decays above 0 (growth) are taken as they are, -infinity forgets. What is not finite reaches no
+ * rounded once. Decays above 0 (growth) are taken as they are (64 tokens whose add up to more than ln 2 go one by one, about
+ * 0.7 us each), -infinity forgets. What is not finite, of the inputs or because 32 bits do not hold it, reaches no
  * earlier token: a value makes its column NaN or infinite from its token on; a key, another decay or a beta all
  * columns; a query its own row. Squares of keys stay within 32 bits: elements below 10^18. n_tokens: up to
  * 2^24 - 1; n_seqs: up to 65535. */

@@ -139,6 +139,10 @@ __global__ __launch_bounds__(256) void k_delta_step(DeltaArgs a, int most) {
 // T and P do not need the state: k_delta_prepare works them out for all chunks at once; k_delta_chunks then goes
 // through a sequence's chunks, a workgroup for 16 columns of a head's state.
 //
+// Where decays above 0 add up to more than a factor of two within a chunk, A, T and the powers above could leave 32 bits though
+// the rule itself does not (64 tokens of g = 2, beta 0 but for the last one's): such a chunk of a head goes token by token through
+// k_delta_chunks, as k_delta_step would take it (1024 tokens, 32 heads of 128, all growing: 680 us, else 50 us).
+//
 // States are held to 32 bits: S, T, V - K S and V' enter the 16-bit matrix instructions as sums of three bf16 parts (8 bits each),
 // in as many products as reach 2^-24; P, and S and V' for the outputs alone, as two. k and q are exact: themselves in bf16, or,
 // for f16, two bf16 parts.
@@ -181,7 +185,8 @@ struct DeltaImage {
   static constexpr int kT = 0;                // [tile and step][3 parts]: T beta
   static constexpr int kP = 18 * 1024;        // [tile and step][2 parts]: scale P
   static constexpr int kVec = 30 * 1024;      // f32: [64] of K S, [64] of Q S, [64] of V', [0] of S
-  static constexpr int kValue = 31 * 1024;    // bytes of a value head's chunk
+  static constexpr int kSlow = 31 * 1024;     // of a chunk token by token: kVec has [64] -1, [64] of a query, [64] beta, here are [64] of a key, [64] exp(g)
+  static constexpr int kValue = kSlow + 512;  // bytes of a value head's chunk
   static constexpr int kK = 0;                // [tile of tokens][step][NP]
   static constexpr int kQ = DK / 8 * NP * 1024;
   static constexpr int kKT = 2 * kQ;          // [tile of the state's rows][step][NP]
@@ -270,7 +275,7 @@ __global__ __launch_bounds__(256, 4) void k_delta_prepare(ChunkArgs c) {
     uint16_t keys[kChunk][DK + 8];
   } lds __attribute__((aligned(16)));
   __shared__ __attribute__((aligned(16))) float hi[kChunk], lo[kChunk], beta[kChunk], unit_k[kChunk], unit_q[kChunk];
-  __shared__ __attribute__((aligned(16))) int bad[kChunk];
+  __shared__ __attribute__((aligned(16))) int bad[kChunk], slow;
   const DeltaArgs& a = c.a;
   const uint32_t h = blockIdx.x, group = a.d.value_heads / a.d.key_heads, hk = h / group;
   int row, n;
@@ -368,6 +373,8 @@ __global__ __launch_bounds__(256, 4) void k_delta_prepare(ChunkArgs c) {
     // key, decay or beta is not finite counts as none here, and as NaN for all that comes after it.
     const bool wrong = bad[lane] || !(lg < INFINITY) || !(fabsf(b) < INFINITY);
     if (wrong) lg = 0.f, b = 0.f;
+    const bool grows = __any(lg > 0.f) && wave_sum_fast(fmaxf(lg, 0.f)) > 0.6931f;
+    if (lane == 0) slow = grows;
     const double sum = wave_prefix(fmax((double)lg, -1e4) * 1.4426950408889634);
     hi[lane] = (float)sum, lo[lane] = (float)(sum - (double)(float)sum), beta[lane] = b, bad[lane] = wrong;
     const double end = __shfl(sum, 63, 64);
@@ -379,6 +386,16 @@ __global__ __launch_bounds__(256, 4) void k_delta_prepare(ChunkArgs c) {
     if (lane == 0) vec[192] = __builtin_amdgcn_exp2f((float)end);
   }
   __syncthreads();
+  if (slow) {
+    // What a token needs by itself; NaN and infinities as they are.
+    if (wave > 0) return;
+    float g1 = 0.f, b1 = 0.f;
+    if (lane < n) gates(a, (uint64_t)(row + lane), h, g1, b1);
+    float *vec = reinterpret_cast<float*>(image + I::kVec), *more = reinterpret_cast<float*>(image + I::kSlow);
+    vec[lane] = -1.f, vec[64 + lane] = unit_q[lane], vec[128 + lane] = b1;
+    more[lane] = unit_k[lane], more[64 + lane] = expf(g1);
+    return;
+  }
   const int i = 16 * wave + m;
   {
     const float hi_i = hi[i], lo_i = lo[i], gain = unit_k[i] * beta[i], of_q = unit_q[i];
@@ -520,7 +537,9 @@ __global__ __launch_bounds__(512, (DK == 64 || NP == 1 ? 4 : 2)) void k_delta_ch
     if (begin >= stop) return;
     Operand Q[NS][NP], P[2][2];
     f32x4 of_q;
+    float slow;
     auto load = [&] {
+      slow = *reinterpret_cast<const float*>(image + I::kVec);
 #pragma unroll
       for (int x = 0; x < NS; ++x)
 #pragma unroll
@@ -544,8 +563,19 @@ __global__ __launch_bounds__(512, (DK == 64 || NP == 1 ? 4 : 2)) void k_delta_ch
     };
     load(), load_mix();
     __syncthreads();
+    bool left = false;  // outputs of the chunk before to be stored
     for (uint32_t chunk = begin; chunk < stop; ++chunk, row += kChunk) {
       const bool more = chunk + 1 < stop;
+      if (__builtin_expect(slow < 0.f, 0)) {
+        // the other waves take this chunk, with a barrier for each token
+        if (left) store(row - kChunk);
+        left = false;
+        image += more ? value_step : 0, key_image += more ? key_step : 0;
+        load(), load_mix();
+        for (int t = min(kChunk, q1 - row); t > 0; --t) __syncthreads();
+        __syncthreads();
+        continue;
+      }
       f32x4 qs[2] = {};  // sums of products of like size, so that they do not wait for each other
 #pragma unroll
       for (int x = 0; x < NS; ++x) {
@@ -559,7 +589,7 @@ __global__ __launch_bounds__(512, (DK == 64 || NP == 1 ? 4 : 2)) void k_delta_ch
       image += more ? value_step : 0, key_image += more ? key_step : 0;
       load();
       __syncthreads();
-      if (chunk > begin) store(row - kChunk);
+      if (left) store(row - kChunk);
       __syncthreads();
       const i32x4 bads = *reinterpret_cast<const i32x4*>(any_bad);
       f32x4 sum[2] = {};
@@ -585,9 +615,10 @@ __global__ __launch_bounds__(512, (DK == 64 || NP == 1 ? 4 : 2)) void k_delta_ch
         for (int r = 0; r < 4; ++r)
           if (t0 + r >= first) o[r] = NAN;
       }
+      left = true;
       __syncthreads();
     }
-    store(row - kChunk);
+    if (left) store(row - kChunk);
     return;
   }
 
@@ -670,6 +701,50 @@ __global__ __launch_bounds__(512, (DK == 64 || NP == 1 ? 4 : 2)) void k_delta_ch
 #pragma unroll
       for (int t = 0; t < 4; ++t) sums[wave][t][lane] = sum[t];
     };
+    // A chunk token by token: each wave's rows of the state, sums over the lanes and, through LDS, over the waves. The call's
+    // arguments are read and the lane's places worked out here: kept through the other chunks they would push those's registers out.
+    auto go_by_tokens = [&] {
+      const __attribute__((address_space(4))) auto* c2 = (const __attribute__((address_space(4))) ChunkArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+      int lane2 = lane;
+      asm volatile("" : "+s"(c2), "+v"(lane2));
+      constexpr uint32_t kType = BF ? MR_BF16 : MR_F16;
+      const uint32_t m = lane2 & 15, g = lane2 >> 4;
+      const uint16_t* kp = static_cast<const uint16_t*>(c2->a.k.p) + (uint64_t)row * c2->a.k.ts + (uint64_t)hk * c2->a.k.hs;
+      const uint16_t* qp = static_cast<const uint16_t*>(c2->a.q.p) + (uint64_t)row * c2->a.q.ts + (uint64_t)hk * c2->a.q.hs;
+      const uint16_t* vp = static_cast<const uint16_t*>(c2->a.v.p) + (uint64_t)row * c2->a.v.ts + (uint64_t)h * c2->a.v.hs + 16 * slice;
+      uint16_t* op = static_cast<uint16_t*>(c2->a.out.p) + (uint64_t)row * c2->a.out.ts + (uint64_t)h * c2->a.out.hs + 16 * slice;
+      float(*red)[4][3][16] = reinterpret_cast<float(*)[4][3][16]>(&rest[0][0][0]);
+      const float *vec = reinterpret_cast<const float*>(image + I::kVec), *of_key = reinterpret_cast<const float*>(image + I::kSlow);
+      const int tokens = min(kChunk, q1 - row);
+#pragma unroll 1
+      for (int t = 0; t < tokens; ++t, kp += c2->a.k.ts, qp += c2->a.q.ts, vp += c2->a.v.ts, op += c2->a.out.ts) {
+        f32x4 k[NT];
+        float sum[3] = {};  // of S k, S q, k q
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          const int x = wave * NT + i;
+          const uint32_t e = 32 * (x >> 1) + 8 * g + 4 * (x & 1);
+          k[i] = load4(kp, kType, e) * of_key[t];
+          const f32x4 y = load4(qp, kType, e) * vec[64 + t];
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            sum[0] = fmaf(S[i][r], k[i][r], sum[0]), sum[1] = fmaf(S[i][r], y[r], sum[1]), sum[2] = fmaf(k[i][r], y[r], sum[2]);
+        }
+        const float v = BF ? bits_f32((uint32_t)vp[m] << 16) : (float)__builtin_bit_cast(_Float16, vp[m]);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+          sum[i] = add_xor16(add_xor32(sum[i]));
+          if (g == 0) red[t & 1][wave][i][m] = sum[i];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 3; ++i) sum[i] = (red[t & 1][0][i][m] + red[t & 1][1][i][m]) + (red[t & 1][2][i][m] + red[t & 1][3][i][m]);
+        const float f = of_key[64 + t], d = (v - sum[0] * f) * vec[128 + t], o = fmaf(d, sum[2], sum[1] * f);
+        if (wave == 0 && g == 0) op[m] = (uint16_t)(BF ? pack_bf16(o, 0.f) : pack_f16(o, 0.f));
+#pragma unroll
+        for (int i = 0; i < NT; ++i) S[i] = S[i] * f + k[i] * d;
+      }
+    };
     load_keys(), load_values(row), load_solution(), load_fade(key_image);
     look();
     __syncthreads();
@@ -679,6 +754,14 @@ __global__ __launch_bounds__(512, (DK == 64 || NP == 1 ? 4 : 2)) void k_delta_ch
       // Loads are asked for behind a step's reads of LDS, while these are on their way.
       const f32x4 part0 = sums[0][wave][lane], part1 = sums[1][wave][lane], part2 = sums[2][wave][lane], part3 = sums[3][wave][lane];
       __builtin_amdgcn_sched_barrier(0);
+      if (__builtin_expect(__builtin_amdgcn_readfirstlane(__float_as_int(of_k[0])) == __float_as_int(-1.f), 0)) {
+        go_by_tokens();
+        key_image += more ? key_step : 0, image += more ? value_step : 0;
+        load_keys(), load_values(row + (more ? kChunk : 0)), load_solution(), load_fade(key_image);
+        look();
+        __syncthreads();
+        continue;
+      }
       key_image += more ? key_step : 0, image += more ? value_step : 0;
       load_keys();
       __builtin_amdgcn_sched_barrier(0);

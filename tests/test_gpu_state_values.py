@@ -1,0 +1,110 @@
+"""The gated delta rule where numbers grow, pass 32 bits or are not finite, on each of its paths and types, against plain 64-bit
+forms (stateref.py)."""
+import numpy as np
+import pytest
+
+import moe_rocm as M
+
+import attnref as R
+import stateref as S
+from test_gpu_attn import TYPES
+from test_gpu_state import Delta
+
+pytestmark = pytest.mark.gpu
+
+LARGE = 1e37  # states below it are compared; what 32 bits do not hold may be anything from its token on
+
+
+def unit(x):
+    return x / np.sqrt((x * x).sum(-1, keepdims=True))
+
+
+def check_what_32_bits_hold(c, compare_states=True):
+    """Each row up to the first one at which the 64-bit state, or what makes it, has passed LARGE, column by column; and the last state
+    of columns that never do. -> how many rows were compared, how many not."""
+    g, beta, g_off, b_off = S.gates(c.a[:, :c.vh], c.b[:, :c.vh], c.a_log, c.dt_bias)
+    at, half, seen, unseen = c.start, R.HALF[c.kind], 0, 0
+    for s, n in enumerate(c.new):
+        for h in range(c.vh):
+            hk, i = h // (c.vh // c.kh), slice(at, at + n)
+            state = c.states[c.source[s], h] if c.source[s] >= 0 else np.zeros((c.dk, c.dv))
+            sizes = np.zeros((n, c.dv))
+            x = state.astype(np.float64).copy()
+            for t in range(n):  # how large the column is, and its correction
+                k = c.k[at + t, hk].astype(np.float64)
+                k = k / np.sqrt(k @ k + c.eps) if c.eps else k
+                x = x * np.exp(g[at + t, h])
+                look = k @ x
+                d = beta[at + t, h] * (c.v[at + t, h] - look)
+                sizes[t] = np.maximum(np.maximum(np.abs(x).max(0), np.abs(look)), np.maximum(np.abs(d), np.abs(c.v[at + t, h])))
+                x = np.clip(x + np.outer(k, d), -1e60, 1e60)
+            fits = np.maximum.accumulate(sizes, 0) < LARGE
+            y, off, last, e = S.delta(c.q[i, hk], c.k[i, hk], c.v[i, h], g[i, h], beta[i, h], state, c.dk ** -0.5, c.eps, g_off[i, h], b_off[i, h])
+            tol = off * (1 + half) + half * np.abs(y) * 1.01 + 2.0 ** -25 * (c.kind == M.F16)
+            if c.kind == M.F16:
+                fits = fits & (np.abs(y) < 65000)
+            d = np.abs(c.out[i, h] - y)
+            assert (d[fits] <= tol[fits]).all(), (s, h, np.argwhere(fits & ~(d <= tol))[:4])
+            seen, unseen = seen + fits.sum(), unseen + (~fits).sum()
+            if compare_states and c.target[s] >= 0 and n:
+                whole = np.abs(x).max(0) < LARGE
+                whole &= sizes.max(0) < LARGE
+                d = np.abs(c.kept[c.target[s], h] - last)[:, whole]
+                assert (d <= e[whole] + 1e-37).all(), (s, h, float((d / (e[whole] + 1e-37)).max()))
+        at += n
+    return int(seen), int(unseen)
+
+
+def grow(c, how, rng):
+    """Decays above 0 in c, and what keeps the result within 32 bits."""
+    T = c.T
+    if how == "until the last token":  # nothing is kept until a sequence's last token
+        c.a[:], c.b[:] = 2.0, 0.0
+        c.source[:] = -1
+        at = 1
+        for n in c.new:
+            at += n
+            c.b[at - 1] = 0.5
+    if how == "by steps":  # up and down again, a hundred times and more within a chunk
+        c.a[:] = np.where(np.arange(T) // 16 % 2, -0.35, 0.35)[:, None]
+    if how == "a little":  # less than a factor of two in 64 tokens
+        c.a[:] = 0.01
+    if how == "one token":
+        c.a[:] = -np.abs(c.a)
+        c.a[c.T // 2] = 60.0
+        c.a[c.T // 2 + 1] = -58.0
+    if how == "beyond":  # out of 32 bits after 40 tokens or so
+        c.a[:] = 2.0
+
+
+@pytest.mark.parametrize("how", ["until the last token", "by steps", "a little", "one token", "beyond"])
+@pytest.mark.parametrize("new", [[8], [64], [140], [6, 90, 0, 33]])
+@pytest.mark.parametrize("kh,vh,dk,dv,kind", [(1, 2, 64, 64, "bf16"), (1, 1, 64, 128, "f16"), (2, 2, 128, 64, "bf16"), (1, 2, 128, 128, "f16")])
+def test_growth(gpu_ctx, how, new, kh, vh, dk, dv, kind):
+    """Decays above 0 are taken as they are, whichever path a sequence takes; what leaves 32 bits reaches no earlier token."""
+    rng = np.random.default_rng(sum(new) + dk)
+    c = Delta(gpu_ctx, kh, vh, dk, dv, new, TYPES[kind], False, rng)
+    grow(c, how, rng)
+    c.run()
+    seen, unseen = check_what_32_bits_hold(c)
+    assert seen > 0 and (unseen > 0 or how != "beyond" or max(new) < 60 or kind == "f16")
+
+
+def test_growth_across_launches(gpu_ctx):
+    """256 heads of 128: about seven chunks to a launch; chunks that grow among ones that do not, at the borders too."""
+    rng = np.random.default_rng(31)
+    new = [40, 700, 3, 500]
+    c = Delta(gpu_ctx, 256, 256, 128, 128, new, M.BF16, False, rng, states=np.zeros((9, 256, 128, 128)))
+    c.source[:] = -1
+    up = np.arange(c.T) // 64 % 3 == 1
+    c.a[:] = np.where(up, 0.05, -np.abs(rng.normal(size=c.T)) * 0.3)[:, None]
+    c.run()
+    at = 1
+    for s, n in enumerate(new):
+        for h in (0, 255):
+            i = slice(at, at + n)
+            y, off, last, e = S.delta(c.q[i, h], c.k[i, h], c.v[i, h], c.a[i, h].astype(np.float64), c.b[i, h].astype(np.float64),
+                                      np.zeros((128, 128)), 128 ** -0.5, 0.0, np.zeros(n), np.zeros(n))
+            assert (np.abs(c.out[i, h] - y) <= off * 1.01 + 2.0 ** -8 * np.abs(y) * 1.01).all(), (s, h)
+            assert (np.abs(c.kept[c.target[s], h] - last) <= e + 1e-37).all(), (s, h)
+        at += n
