@@ -386,14 +386,15 @@ __global__ __launch_bounds__(256, 4) void k_delta_prepare(ChunkArgs c) {
     if (lane == 0) vec[192] = __builtin_amdgcn_exp2f((float)end);
   }
   __syncthreads();
-  if (slow) {
-    // What a token needs by itself; NaN and infinities as they are.
-    if (wave > 0) return;
+  auto go_by_tokens = [&] {  // what a token needs by itself; NaN and infinities as they are
     float g1 = 0.f, b1 = 0.f;
     if (lane < n) gates(a, (uint64_t)(row + lane), h, g1, b1);
     float *vec = reinterpret_cast<float*>(image + I::kVec), *more = reinterpret_cast<float*>(image + I::kSlow);
     vec[lane] = -1.f, vec[64 + lane] = unit_q[lane], vec[128 + lane] = b1;
     more[lane] = unit_k[lane], more[64 + lane] = expf(g1);
+  };
+  if (slow) {
+    if (wave == 0) go_by_tokens();
     return;
   }
   const int i = 16 * wave + m;
@@ -467,6 +468,7 @@ __global__ __launch_bounds__(256, 4) void k_delta_prepare(ChunkArgs c) {
     }
     __syncthreads();
   }
+  bool over = false;
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
     if (s > wave / 2) break;
@@ -478,7 +480,10 @@ __global__ __launch_bounds__(256, 4) void k_delta_prepare(ChunkArgs c) {
         const int j = 32 * s + 16 * x + 4 * g;
         v = *reinterpret_cast<const f32x4*>(&lds.m[i][j]);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = j + r <= i ? v[r] * beta[j + r] : 0.f;
+        for (int r = 0; r < 4; ++r) {
+          v[r] = j + r <= i ? v[r] * beta[j + r] : 0.f;
+          over |= !(fabsf(v[r]) < INFINITY);
+        }
       }
       split(v, part[x]);
     }
@@ -487,6 +492,10 @@ __global__ __launch_bounds__(256, 4) void k_delta_prepare(ChunkArgs c) {
       *reinterpret_cast<Operand*>(image + I::kT + (I::lower(wave, s) * 3 + p) * 1024 + lane * 16) =
           Operand{part[0][p].x, part[0][p].y, part[1][p].x, part[1][p].y};
   }
+  // What two tokens do to each other, long keys or a large beta, can leave 32 bits too, and would be multiplied with zeros then.
+  if (__any(over) && lane == 0) slow = 1;
+  __syncthreads();
+  if (slow && wave == 0) go_by_tokens();
 }
 
 // A sequence's chunks for 16 columns of a head's state. What the next chunk waits for is the state alone, through three steps:

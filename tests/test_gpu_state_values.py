@@ -38,6 +38,7 @@ def check_what_32_bits_hold(c, compare_states=True):
                 d = beta[at + t, h] * (c.v[at + t, h] - look)
                 sizes[t] = np.maximum(np.maximum(np.abs(x).max(0), np.abs(look)), np.maximum(np.abs(d), np.abs(c.v[at + t, h])))
                 x = np.clip(x + np.outer(k, d), -1e60, 1e60)
+                sizes[t] = np.maximum(sizes[t], np.abs(x).max(0))
             fits = np.maximum.accumulate(sizes, 0) < LARGE
             y, off, last, e = S.delta(c.q[i, hk], c.k[i, hk], c.v[i, h], g[i, h], beta[i, h], state, c.dk ** -0.5, c.eps, g_off[i, h], b_off[i, h])
             tol = off * (1 + half) + half * np.abs(y) * 1.01 + 2.0 ** -25 * (c.kind == M.F16)
@@ -108,3 +109,32 @@ def test_growth_across_launches(gpu_ctx):
             assert (np.abs(c.out[i, h] - y) <= off * 1.01 + 2.0 ** -8 * np.abs(y) * 1.01).all(), (s, h)
             assert (np.abs(c.kept[c.target[s], h] - last) <= e + 1e-37).all(), (s, h)
         at += n
+
+
+@pytest.mark.parametrize("new", [[8], [64], [140], [40, 0, 70]])
+@pytest.mark.parametrize("kh,vh,dk,dv,kind", [(1, 2, 64, 64, "bf16"), (1, 1, 64, 128, "f16"), (1, 2, 128, 64, "bf16"), (1, 2, 128, 128, "f16")])
+def test_long_keys_without_values(gpu_ctx, new, kh, vh, dk, dv, kind):
+    """What tokens would do to each other passes 32 bits, but they do nothing: only a sequence's last one has a value."""
+    rng = np.random.default_rng(sum(new) + dv)
+    c = Delta(gpu_ctx, kh, vh, dk, dv, new, TYPES[kind], False, rng)
+    c.k = R.rounded(rng.normal(size=c.k.shape) * 3, c.kind)
+    c.a[:], c.b[:], c.source[:] = 0.0, 1.0, -1
+    last = 1 + np.cumsum(new) - 1
+    v = np.zeros_like(c.v)
+    v[last] = c.v[last]
+    c.v = v
+    c.run()
+    seen, unseen = check_what_32_bits_hold(c)
+    assert unseen == 0
+
+
+@pytest.mark.parametrize("at", [0, 5, 40, 63, 64, 100])
+@pytest.mark.parametrize("dk,dv,kind", [(64, 64, "bf16"), (128, 128, "bf16")])
+def test_beta_beyond_32_bits_reaches_no_earlier_token(gpu_ctx, at, dk, dv, kind):
+    rng = np.random.default_rng(at)
+    c = Delta(gpu_ctx, 1, 2, dk, dv, [140], TYPES[kind], False, rng)
+    c.k[at + 1] = R.rounded(c.k[at + 1] * 1e10, c.kind)
+    c.b[at + 1, 1] = 1e30  # head 0 has only the long key
+    c.run()
+    seen, unseen = check_what_32_bits_hold(c, compare_states=False)
+    assert seen >= at * dv * 2 and unseen > 0
