@@ -175,6 +175,8 @@ __device__ __forceinline__ void split(f32x4 x, u32x2 (&part)[N]) {
   }
 }
 
+constexpr float kFits = 0x1.ffp127f;  // from here on a first part of 8 bits is infinite
+
 // What k_delta_prepare leaves, in the order of the lanes that read it: operands of 1 KB.
 // A chunk's tokens 32 s + 4 g + r and 32 s + 16 + 4 g + r (r = 0..3) are, in turn, the 8 numbers of lane group g in step s of a sum
 // over tokens: what the lanes of a product's result hold of two tiles of 16.
@@ -482,7 +484,7 @@ __global__ __launch_bounds__(256, 4) void k_delta_prepare(ChunkArgs c) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           v[r] = j + r <= i ? v[r] * beta[j + r] : 0.f;
-          over |= !(fabsf(v[r]) < INFINITY);
+          over |= !(fabsf(v[r]) < kFits);
         }
       }
       split(v, part[x]);
@@ -602,24 +604,43 @@ __global__ __launch_bounds__(512, (DK == 64 || NP == 1 ? 4 : 2)) void k_delta_ch
       __syncthreads();
       const i32x4 bads = *reinterpret_cast<const i32x4*>(any_bad);
       f32x4 sum[2] = {};
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        if (x > wave / 2) break;
+      auto mix = [&](int x, f32x4 v0, f32x4 v1) {
         u32x2 lo[2], hi[2];
-        split(fresh[2 * x][lane], lo), split(fresh[2 * x + 1][lane], hi);
+        split(v0, lo), split(v1, hi);
         const Operand v[2] = {{lo[0].x, lo[0].y, hi[0].x, hi[0].y}, {lo[1].x, lo[1].y, hi[1].x, hi[1].y}};
 #pragma unroll
         for (int p = 0; p < 2; ++p)
 #pragma unroll
           for (int z = 0; z + p < 2; ++z) sum[z + p] = mfma_bf16(P[x][p], v[z], sum[z + p]);
+      };
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        if (x > wave / 2) break;
+        mix(x, fresh[2 * x][lane], fresh[2 * x + 1][lane]);
+      }
+      int first = kChunk;  // the column's first token that is not finite
+      if (__builtin_expect(__any(!(fabsf(sum[0].x) + fabsf(sum[0].y) + fabsf(sum[0].z) + fabsf(sum[0].w) < INFINITY)), 0)) {
+        // Corrections that are sums beyond 32 bits, as with V - K S below; all products again without them.
+        sum[0] = f32x4{}, sum[1] = f32x4{};
+#pragma unroll 1
+        for (int x = 0; x <= wave / 2; ++x) {
+          f32x4 now[2] = {fresh[2 * x][lane], fresh[2 * x + 1][lane]};
+#pragma unroll
+          for (int r = 7; r >= 0; --r)
+            if (!(fabsf(now[r / 4][r % 4]) < kFits)) first = min(first, 32 * x + 16 * (r / 4) + 4 * g + r % 4), now[r / 4][r % 4] = 0.f;
+          x ? mix(1, now[0], now[1]) : mix(0, now[0], now[1]);
+        }
+        first = min(first, __shfl_xor(first, 16, 64));
+        first = min(first, __shfl_xor(first, 32, 64));
       }
       load_mix();
       o = before + (sum[1] + sum[0]);
       if (__builtin_amdgcn_readfirstlane(bads.x | bads.y | bads.z | bads.w)) {
-        int first = kChunk;
 #pragma unroll
         for (int w = 0; w < 4; ++w)
           if (bads[w]) first = min(first, first_bad[w][m]);
+      }
+      if (__any(first < kChunk)) {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
           if (t0 + r >= first) o[r] = NAN;
@@ -780,7 +801,7 @@ __global__ __launch_bounds__(512, (DK == 64 || NP == 1 ? 4 : 2)) void k_delta_ch
       for (int r = 0; r < 4; ++r) {
         const float v = row + t0 + r < q1 ? (BF ? bits_f32((uint32_t)vals[r] << 16) : (float)__builtin_bit_cast(_Float16, vals[r])) : 0.f;
         R[r] = fmaf(-of_k[r], R[r], v);
-        wrong |= !(fabsf(R[r]) < INFINITY);
+        wrong |= !(fabsf(R[r]) < kFits);
       }
       const bool any = __any(wrong);
       if (any) {
@@ -789,7 +810,7 @@ __global__ __launch_bounds__(512, (DK == 64 || NP == 1 ? 4 : 2)) void k_delta_ch
         int bad = kChunk;
 #pragma unroll
         for (int r = 3; r >= 0; --r)
-          if (!(fabsf(R[r]) < INFINITY)) bad = t0 + r, R[r] = 0.f;
+          if (!(fabsf(R[r]) < kFits)) bad = t0 + r, R[r] = 0.f;
         bad = min(bad, __shfl_xor(bad, 16, 64));
         bad = min(bad, __shfl_xor(bad, 32, 64));
         if (g == 0) first_bad[wave][m] = bad;

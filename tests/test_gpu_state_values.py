@@ -138,3 +138,28 @@ def test_beta_beyond_32_bits_reaches_no_earlier_token(gpu_ctx, at, dk, dv, kind)
     c.run()
     seen, unseen = check_what_32_bits_hold(c, compare_states=False)
     assert seen >= at * dv * 2 and unseen > 0
+
+
+@pytest.mark.parametrize("at", [3, 21, 40, 62, 80, 120])
+@pytest.mark.parametrize("dk,dv", [(64, 64), (128, 128)])
+@pytest.mark.parametrize("how", ["sum", "difference"])
+def test_corrections_beyond_32_bits_reach_no_earlier_token(gpu_ctx, at, dk, dv, how):
+    """Values near the largest that two tokens add up beyond it, or that a state takes to the last step of 32 bits."""
+    rng = np.random.default_rng(at)
+    c = Delta(gpu_ctx, 1, 2, dk, dv, [140], M.BF16, False, rng)
+    big = R.rounded(np.array([3.38e38]), M.BF16)[0]
+    i = at + 1
+    c.a[i - 1:i + 2, 1] = 0.0
+    if how == "sum":  # the second one's key is the first one's turned round: its correction is twice as large
+        c.k[i] = -c.k[i - 1]
+        c.v[i - 1, 1, 5] = c.v[i, 1, 5] = big
+        c.b[i - 1:i + 1, 1] = 1.0
+    else:  # within 32 bits, but not in parts of 8
+        c.states[c.source[0], 1, :, 5] = 0.0
+        c.k[i - 1] = np.eye(dk)[7]
+        c.k[i] = np.eye(dk)[7]
+        c.v[i - 1, 1, 5], c.v[i, 1, 5] = R.rounded(np.array([-0.8e36]), M.BF16)[0], R.rounded(np.array([3.3895e38]), M.BF16)[0]
+        c.b[i - 1:i + 1, 1] = 1.0
+    c.run()
+    seen, unseen = check_what_32_bits_hold(c, compare_states=False)
+    assert unseen > 0 and seen >= 140 * dv * 2 - 141
