@@ -24,6 +24,7 @@ struct ExtendArgs {
   int nq;
   Divisor group;       // query heads of a key head
   int bits;            // log2 of a tile's rows
+  float slack;         // of k_attn_extend_wide, in powers of two
   uint32_t parts;      // parts that the CUs hold at once; 1: none is split
   AttnOpts o;
   uint32_t* err;
@@ -352,7 +353,11 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<NT, FMT, D>)) void k_attn_ex
 // 16 heads on 2, MXINT8: 1170 us, 890 TFLOP/s); heads of 128, loads and the last round of units (four parts of prompts, 32 heads
 // on 4, F16: 167 us, 760 TFLOP/s); heads of 64, vector instructions (a part of 1000 tokens and 32 single ones, 64 heads on 8,
 // MXINT8: 174 us, 620 TFLOP/s).
-constexpr float kWideSlack = 4.f, kWideLift = 11.f;  // weights up to 2^15: the maximum is followed when it has moved by 2^4
+// Weights go up to 2^15, and the maximum is followed when it has moved by 2^slack: the largest weight lies between 2^(15 - slack) and
+// 2^15, and ones down to 2^(slack - 29) of it keep all bits of f16. Where sequences have up to 32 rows, the slack is one, and the bits are
+// those of attend_few: 3 new tokens of 32 sequences, 32 heads on 4 of 128, MXFP4 76.5 us with four and 79 us with one. For more rows it
+// is four: 5 new tokens of the same 91.5 and 95 us, four prompts' parts 175 and 181 us.
+constexpr float kTopWeight = 15.f, kSlackFew = 1.f, kSlackMany = 4.f;
 
 // A wave's quarter of a chunk on its way from the pages to LDS.
 template <int FMT, int D>
@@ -536,11 +541,12 @@ __global__ __launch_bounds__(256, (kWidePerSimd<FMT, D>)) void k_attn_extend_wid
   f32x16 acc[ND];
 #pragma unroll
   for (int x = 0; x < ND; ++x) acc[x] = f32x16{};
-  // Weights are 2^(s c - base): relative to ref, the largest score so far or up to kWideSlack below it, base = ref c - kWideLift. With one
+  // Weights are 2^(s c - base): relative to ref, the largest score so far or up to the slack below it, base = ref c - lift. With one
   // rounding of s c - base they are right to their own size, however base was rounded; that rounding is the same factor for
   // all of a row's. Where it could be 2^-12 or more, ref is taken from the scores first.
   constexpr float kNear = 0x1p12f;
-  float ref = 0.f, base = -kWideLift, l = 0.f;
+  const float slack = KH == 2 ? kSlackMany : a.slack, lift = kTopWeight - slack;  // tiles of 128 rows have more than 64 on average
+  float ref = 0.f, base = -lift, l = 0.f;
   bool seen = false;
   // addresses of operands: keys 32 T + .., elements of step i; values' elements 32 x + n of 16 keys
   const uint32_t k_at = lds0 + first_half * (D / 16) * 1024 + (uint32_t)(((n >> 3) & 1) * (D / 32) * 1024 + (16 * half + ((n >> 4) << 3 | (n & 7))) * 16);
@@ -675,9 +681,9 @@ __global__ __launch_bounds__(256, (kWidePerSimd<FMT, D>)) void k_attn_extend_wid
     }
     top = __builtin_elementwise_maximum(top, top2);
     top = max_xor32(top);
-    const bool move = (top - ref) * c > kWideSlack || (!seen && top > -INFINITY);
+    const bool move = (top - ref) * c > slack || (!seen && top > -INFINITY);
     if (__any(move)) {
-      const float next_base = fabsf(top * c) < kNear ? fmaf(top, c, -kWideLift) : -kWideLift;
+      const float next_base = fabsf(top * c) < kNear ? fmaf(top, c, -lift) : -lift;
       const bool near = fabsf(top * c) < kNear && fabsf(ref * c) < kNear;
       const float f = !move ? 1.f : !seen ? 0.f : __builtin_amdgcn_exp2f(near ? base - next_base : (ref - top) * c);
       l *= f;
@@ -729,7 +735,7 @@ __global__ __launch_bounds__(256, (kWidePerSimd<FMT, D>)) void k_attn_extend_wid
   }
 
   l = add_xor32(l);
-  float m = !seen ? -INFINITY : fabsf(ref * c) < kNear ? base : fminf(fmaxf(ref * c, -kLargest), kLargest) - kWideLift;
+  float m = !seen ? -INFINITY : fabsf(ref * c) < kNear ? base : fminf(fmaxf(ref * c, -kLargest), kLargest) - lift;
   if constexpr (KH == 1) {
     // the second halves' results through LDS: number x of lane i at 64 x + i
     float* other = reinterpret_cast<float*>(&lds[0][0][0]) + block * (ND * 16 + 2) * 64 + lane;
@@ -867,7 +873,7 @@ hipError_t launch_attn_extend(const Launch& K, const KvPages& kv, uint32_t forma
   const ExtendKernel kernel = format == MR_KV_F16      ? pick<MR_KV_F16>(D, bits, per_cu)
                               : format == MR_KV_MXINT8 ? pick<MR_KV_MXINT8>(D, bits, per_cu)
                                                        : pick<MR_KV_MXFP4>(D, bits, per_cu);
-  ExtendArgs a{kv, q, out, cu, len, table, max_pages, n_seqs, (int)nq, Divisor(group), bits, 0, o, err, scratch};
+  ExtendArgs a{kv, q, out, cu, len, table, max_pages, n_seqs, (int)nq, Divisor(group), bits, rows <= 32ull * n_seqs ? kSlackFew : kSlackMany, 0, o, err, scratch};
   // chunks that a tile sees at most
   const uint64_t pages = (uint64_t)max_pages << (kv.page_shift - 6);
   const uint64_t cap = o.window ? std::min<uint64_t>(pages, (o.window + ((1ull << bits) / group + 1) + 62) / 64 + 1) : pages;

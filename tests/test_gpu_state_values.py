@@ -1,5 +1,5 @@
-"""The gated delta rule where numbers grow, pass 32 bits or are not finite, on each of its paths and types, against plain 64-bit
-forms (stateref.py)."""
+"""Operators over kept states where values decide: weights of attention far below the largest; the gated delta rule where numbers
+grow, pass 32 bits or are not finite, on each of its paths and types; against plain 64-bit forms (attnref.py, stateref.py)."""
 import numpy as np
 import pytest
 
@@ -7,16 +7,12 @@ import moe_rocm as M
 
 import attnref as R
 import stateref as S
-from test_gpu_attn import TYPES
-from test_gpu_state import Delta
+from test_gpu_attn import FORMATS, TYPES
+from test_gpu_state import Cached, Delta, extend_ref
 
 pytestmark = pytest.mark.gpu
 
 LARGE = 1e37  # states below it are compared; what 32 bits do not hold may be anything from its token on
-
-
-def unit(x):
-    return x / np.sqrt((x * x).sum(-1, keepdims=True))
 
 
 def check_what_32_bits_hold(c, compare_states=True):
@@ -163,3 +159,36 @@ def test_corrections_beyond_32_bits_reach_no_earlier_token(gpu_ctx, at, dk, dv, 
     c.run()
     seen, unseen = check_what_32_bits_hold(c, compare_states=False)
     assert unseen > 0 and seen >= 140 * dv * 2 - 141
+
+
+@pytest.mark.parametrize("new,deep", [(1, True), (4, True), (5, True), (6, True), (8, True), (9, False), (16, False), (40, False)])
+@pytest.mark.parametrize("D,fmt", [(64, "f16"), (64, "mxint8"), (128, "f16"), (128, "mxfp4"), (256, "mxint8")])
+def test_extend_weights_keep_the_bits_that_they_are_said_to(gpu_ctx, new, deep, D, fmt):
+    """A first key far above the rest that has no value: up to 32 rows on average (4 heads) the rest's weights keep 11 bits down to
+    2^-28 of the largest, with more rows down to 2^-25."""
+    # Of the rest's weight e^-gap, in steps of 2^-24 below a largest one of 2^11 (2^8), the fraction is near a half: 0.3% of it
+    # would be lost with three bits fewer than said.
+    gap = 19.34375 if deep else 17.25
+    n, group = 500, 4  # not cut into parts
+    rng = np.random.default_rng(1)
+    cache = Cached(gpu_ctx, FORMATS[fmt], 64, 1, D, [n], rng, scale=0.0)
+    k, v = np.zeros((n, 1, D), np.float32), np.full((n, 1, D), 49152.0, np.float32)  # the same in each format
+    k[0, 0, 0], v[0] = 16.0, 0.0
+    t = np.arange(n)
+    bk, bv, slots = R.Rows(gpu_ctx, k, M.F32), R.Rows(gpu_ctx, v, M.F32), R.i32(gpu_ctx, cache.table[0][t // 64] * 64 + t % 64)
+    cache.kv.write(bk.heads, bv.heads, n, slots)
+    cache.k[0], cache.v[0] = R.stored(k, FORMATS[fmt]), R.stored(v, FORMATS[fmt])
+    assert (cache.v[0][1:] == 49152.0).all() and cache.k[0][0, 0, 0] == 16.0
+    q = np.zeros((new, group, D))
+    q[..., 0] = 1.0
+    bq, out = R.Rows(gpu_ctx, q, M.F16), R.Rows(gpu_ctx, None, M.F16, new, group, D)
+    dev = [R.i32(gpu_ctx, a) for a in ([0, new], [n], cache.table)]
+    cache.kv.extend(bq.heads, new, 1, *dev, cache.table.shape[1], out.heads, scale=gap / 16.0)
+    gpu_ctx.sync()
+    y, _ = extend_ref(q, cache, [new], [n], gap / 16.0, 0, None, M.F16)
+    # half a step of 2^-11 for a weight, the same for the output; what 32 bits add (a score near 28 in powers of two, sums of 500) is
+    # less than 2^-17
+    assert (np.abs(out.get() - y) <= (2.0 ** -10 + 2.0 ** -17) * np.abs(y)).all()
+    for b in (bk, bv, slots, bq, out, *dev):
+        b.free()
+    cache.kv.close()
