@@ -20,8 +20,8 @@
  *    there. source and target may be NULL, for negative ones throughout, and states where both are. A slot past the
  *    last is taken as a negative one, with an error at mr_sync. No slot is another sequence's target in the
  *    same call: it would hold some mixture. A sequence without tokens takes its state from source to target.
- *  - Kernel names for mr_profile_read: "attn_extend", "extend_join", "causal_conv", "delta_step", "delta_prepare",
- *    "delta_chunks".
+ *  - Kernel names for mr_profile_read: "attn_extend", "extend_join", "causal_conv", "delta_step", "delta_list",
+ *    "delta_prepare", "delta_chunks".
  */
 #ifndef MOE_ROCM_STATE_H
 #define MOE_ROCM_STATE_H

@@ -197,6 +197,10 @@ struct DeltaImage {
   static __device__ __forceinline__ int lower(int w, int s) { return w < 2 ? w : 2 * (w - 1) + s; }
 };
 
+struct Long {
+  uint32_t s, start;  // a sequence of this path, the number of its first chunk
+};
+
 struct ChunkArgs {
   DeltaArgs a;
   uint8_t *values, *keys;  // images [chunk][value head], [chunk][key head]
@@ -204,17 +208,42 @@ struct ChunkArgs {
   uint32_t first, last;    // chunks of this launch, by their numbers
   int least;               // sequences of fewer tokens are not this path's
   int dense;               // chunks and sequences are numbered among those that are
+  Long* list;              // of many sequences: those of this path, n_long entries
+  uint32_t n_long;
 };
 
-constexpr uint32_t kDenseSeqs = 1024;  // each workgroup looks through so many
+// Each workgroup looks through so many; of more, k_delta_list lists the long ones first. Launches for as many as there are sequences
+// instead grew with the square of these (4000 single tokens, 32 heads of 128: 28 ms, with the list 0.48 ms).
+constexpr uint32_t kDenseSeqs = 1024;
+constexpr uint32_t kNone = 0xFFFFFFFFu;
 
-// Sequence number i of this path (chunk: the one that chunk number i is in), the number of its first chunk, its rows.
+// The list's last entry whose first chunk is `chunk` or before, 64 candidates at a time; all 64 lanes active.
+__device__ __forceinline__ uint32_t find_long(const ChunkArgs& c, uint32_t chunk) {
+  uint32_t lo = 0, n = c.n_long;
+  for (;;) {
+    const uint32_t step = (n + 63) / 64, at = (threadIdx.x & 63) * step;
+    const int k = __popcll(__ballot(at < n && c.list[lo + at].start <= chunk));
+    const uint32_t past = k > 0 ? (uint32_t)(k - 1) * step : 0;
+    lo += past, n = min(step, n - past);
+    if (step == 1) return __builtin_amdgcn_readfirstlane(lo);
+  }
+}
+
+// Sequence number i of this path (chunk: the one that chunk number i is in), the number of its first chunk, its rows. With a list,
+// sequences are numbered from the one that the launch's first chunk is in.
 struct Chunked {
   uint32_t s, start;
   int q0, q1;
 };
 __device__ __forceinline__ bool find_sequence(const ChunkArgs& c, uint32_t i, bool chunk, Chunked& r) {
   const Sequences& q = c.a.s;
+  if (c.list) {
+    const uint32_t at = chunk ? find_long(c, i) : find_long(c, c.first) + i;
+    if (at >= c.n_long || c.list[at].start == kNone) return false;
+    r.s = __builtin_amdgcn_readfirstlane(c.list[at].s), r.start = __builtin_amdgcn_readfirstlane(c.list[at].start);
+    rows_of(q.cu, q.n_rows, r.s, r.q0, r.q1);
+    return true;
+  }
   if (!c.dense) {
     r.s = chunk ? find_seq(q.cu, q.n_seqs, q.n_rows, 1, 6, i) : i;
     r.start = first_tile(q.cu, q.n_rows, r.s, 1, 6);
@@ -238,6 +267,40 @@ __device__ __forceinline__ bool find_sequence(const ChunkArgs& c, uint32_t i, bo
     seqs += __builtin_amdgcn_readlane(at, 63), chunks += __builtin_amdgcn_readlane(sum, 63);
   }
   return false;
+}
+
+// The long sequences of many, in order, by one workgroup: a thread counts those of a few adjacent ones, then writes them behind what
+// the threads before it have. Entries behind the last have no first chunk.
+__global__ __launch_bounds__(1024) void k_delta_list(ChunkArgs c) {
+  __shared__ uint32_t sums[16][2];
+  const Sequences& q = c.a.s;
+  const uint32_t each = (q.n_seqs + 1023) / 1024, s0 = min(threadIdx.x * each, q.n_seqs), s1 = min(s0 + each, q.n_seqs);
+  const int wave = threadIdx.x >> 6;
+  auto chunks_of = [&](uint32_t s) {
+    int q0, q1;
+    rows_of(q.cu, q.n_rows, s, q0, q1);
+    return q1 - q0 >= c.least ? (uint32_t)(q1 - q0 + kChunk - 1) / kChunk : 0;
+  };
+  uint32_t seqs = 0, chunks = 0;
+  for (uint32_t s = s0; s < s1; ++s) {
+    const uint32_t n = chunks_of(s);
+    seqs += n > 0, chunks += n;
+  }
+  const uint32_t at = wave_prefix(seqs), sum = wave_prefix(chunks);
+  if ((threadIdx.x & 63) == 63) sums[wave][0] = at, sums[wave][1] = sum;
+  __syncthreads();
+  uint32_t i = at - seqs, start = sum - chunks, all = 0;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) {
+    if (w < wave) i += sums[w][0], start += sums[w][1];
+    all += sums[w][0];
+  }
+  for (uint32_t s = s0; s < s1; ++s) {
+    const uint32_t n = chunks_of(s);
+    if (n && i < c.n_long) c.list[i] = Long{s, start};
+    i += n > 0, start += n;
+  }
+  for (uint32_t j = all + threadIdx.x; j < c.n_long; j += 1024) c.list[j] = Long{0, kNone};
 }
 
 // Chunk number `at`: its first row and its rows.
@@ -910,23 +973,29 @@ template <int DK, bool BF>
 hipError_t launch_chunks(const Launch& K, const DeltaArgs& a, int least, uint8_t* scratch) {
   using I = DeltaImage<DK, BF ? 1 : 2>;
   const uint32_t vh = a.d.value_heads, kh = a.d.key_heads, dv = a.d.value_dim;
-  const uint64_t carry = 2ull * vh * DK * dv * sizeof(float), chunk = (uint64_t)vh * I::kValue + (uint64_t)kh * I::kKey;
   const uint32_t longest = least ? (uint32_t)a.s.n_rows / (uint32_t)least : a.s.n_seqs;  // sequences of so many tokens at most
-  const bool dense = least && a.s.n_seqs <= kDenseSeqs;
-  const uint32_t seqs = dense ? std::min(a.s.n_seqs, longest) : a.s.n_seqs;
-  const uint32_t all = ((uint32_t)a.s.n_rows >> 6) + seqs, room = (uint32_t)std::min<uint64_t>((kScratch - carry) / chunk, 65535);
-  ChunkArgs c{a, nullptr, nullptr, reinterpret_cast<float*>(scratch), 0, 0, least, dense};
+  const uint32_t seqs = std::min(a.s.n_seqs, longest);
+  const bool listed = least && a.s.n_seqs > kDenseSeqs;
+  const uint64_t list = listed ? ((uint64_t)seqs * sizeof(Long) + 1023) / 1024 * 1024 : 0;
+  const uint64_t carry = 2ull * vh * DK * dv * sizeof(float), chunk = (uint64_t)vh * I::kValue + (uint64_t)kh * I::kKey;
+  const uint32_t all = ((uint32_t)a.s.n_rows >> 6) + seqs, room = (uint32_t)std::min<uint64_t>((kScratch - list - carry) / chunk, 65535);
+  ChunkArgs c{a, nullptr, nullptr, reinterpret_cast<float*>(scratch + list), 0, 0, least, least > 0, nullptr, 0};
+  if (listed) {
+    ProfScope ps(K, "delta_list");
+    c.list = reinterpret_cast<Long*>(scratch), c.n_long = seqs;
+    hipLaunchKernelGGL(k_delta_list, dim3(1), dim3(1024), 0, K.s, c);
+  }
   int parity = 0;
   for (c.first = 0; c.first < all; c.first = c.last, parity ^= 1) {
     c.last = std::min(all, c.first + room);
-    c.values = scratch + carry;
+    c.values = scratch + list + carry;
     c.keys = c.values + (uint64_t)(c.last - c.first) * vh * I::kValue;
     {
       ProfScope ps(K, "delta_prepare");
       hipLaunchKernelGGL((k_delta_prepare<DK, BF>), dim3(vh, c.last - c.first), dim3(256), 0, K.s, c);
     }
     ProfScope ps(K, "delta_chunks");
-    hipLaunchKernelGGL((k_delta_chunks<DK, BF ? 1 : 2, BF>), dim3((vh * (dv / 16) + 7) / 8 * 8, seqs), dim3(512), 0, K.s, c, dv / 16, parity);
+    hipLaunchKernelGGL((k_delta_chunks<DK, BF ? 1 : 2, BF>), dim3((vh * (dv / 16) + 7) / 8 * 8, listed ? std::min(seqs, c.last - c.first) : seqs), dim3(512), 0, K.s, c, dv / 16, parity);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }

@@ -1,4 +1,4 @@
-"""Operators over kept states where values decide: weights of attention far below the largest; the gated delta rule where numbers
+"""Operators over kept states where values and numbers of sequences decide: weights of attention far below the largest; the gated delta rule where numbers
 grow, pass 32 bits or are not finite, on each of its paths and types; against plain 64-bit forms (attnref.py, stateref.py)."""
 import numpy as np
 import pytest
@@ -192,3 +192,58 @@ def test_extend_weights_keep_the_bits_that_they_are_said_to(gpu_ctx, new, deep, 
     for b in (bk, bv, slots, bq, out, *dev):
         b.free()
     cache.kv.close()
+
+
+@pytest.mark.parametrize("n_seqs", [1024, 1025, 3000])
+def test_delta_launches_go_by_rows_not_by_sequences(gpu_ctx, n_seqs):
+    """A batch of single tokens has room for few long sequences, however many sequences it has."""
+    kh, vh, D = 16, 32, 128
+    rng = np.random.default_rng(1)
+    q, k = (R.rounded(rng.normal(size=(n_seqs, kh, D)) / D ** 0.5, M.BF16) for _ in range(2))
+    v = R.rounded(rng.normal(size=(n_seqs, vh, D)), M.BF16)
+    a, b = -np.abs(rng.normal(size=(n_seqs, vh))).astype(np.float32), rng.uniform(0.1, 0.9, (n_seqs, vh)).astype(np.float32)
+    rows = [R.Rows(gpu_ctx, x, M.BF16) for x in (q, k, v)] + [R.Rows(gpu_ctx, None, M.BF16, n_seqs, vh, D)]
+    dev = [gpu_ctx.to_device(a), gpu_ctx.to_device(b), R.i32(gpu_ctx, np.arange(n_seqs + 1))]
+    rule = M.DeltaRule(gpu_ctx, kh, vh, D, D)
+    gpu_ctx.set_option(M.OPT_PROFILE, 1)
+    gpu_ctx.profile_reset()
+    rule.forward(rows[0].heads, rows[1].heads, rows[2].heads, *dev[:2], n_seqs, n_seqs, dev[2], rows[3].heads)
+    gpu_ctx.sync()
+    launches = {x: gpu_ctx.profile_read(x)[0] for x in ("delta_step", "delta_prepare", "delta_chunks")}
+    gpu_ctx.set_option(M.OPT_PROFILE, 0)
+    assert launches == {"delta_step": 1, "delta_prepare": 1, "delta_chunks": 1}, launches
+    qk = np.repeat((q.astype(np.float64) * k).sum(-1), vh // kh, 1)
+    y = D ** -0.5 * (qk * b)[..., None] * v  # from a state of zeros
+    size = np.repeat(np.abs(q.astype(np.float64) * k).sum(-1), vh // kh, 1)
+    tol = 2.0 ** -8 * np.abs(y) * 1.01 + (D + 8) * S.U * D ** -0.5 * (size * b)[..., None] * np.abs(v)
+    assert (np.abs(rows[3].get() - y) <= tol).all()
+    rule.close()
+    for x in (*rows, *dev):
+        x.free()
+
+
+def test_delta_long_sequences_among_many_across_launches(gpu_ctx):
+    """More sequences than each workgroup looks through, some long, with more chunks than the workspace holds at once."""
+    n_seqs, kh, vh, D = 1500, 32, 128, 64
+    rng = np.random.default_rng(2)
+    new = rng.integers(0, 3, n_seqs)
+    long = {0: 700, 1: 33, 700: 32, 701: 1500, 1023: 64, 1024: 65, 1300: 1100, n_seqs - 1: 90}
+    for s, n in long.items():
+        new[s] = n
+    new = new.tolist()
+    c = Delta(gpu_ctx, kh, vh, D, D, new, M.BF16, False, rng, states=np.zeros((len(long), vh, D, D)))
+    c.source[:] = -1
+    c.target[:] = -1
+    for i, s in enumerate(long):
+        c.target[s] = i
+    c.run()
+    first = 1 + np.concatenate([[0], np.cumsum(new)])
+    for s in [*long, 2, 3, 699, 702, 1022, 1299]:
+        for h in (0, 77, 127):
+            i, n = slice(first[s], first[s] + new[s]), new[s]
+            y, off, last, e = S.delta(c.q[i, h // 4], c.k[i, h // 4], c.v[i, h], c.a[i, h].astype(np.float64), c.b[i, h].astype(np.float64),
+                                      np.zeros((D, D)), D ** -0.5, 0.0, np.zeros(n), np.zeros(n))
+            assert (np.abs(c.out[i, h] - y) <= off * 1.01 + 2.0 ** -8 * np.abs(y) * 1.01).all(), (s, h)
+            if c.target[s] >= 0:
+                assert (np.abs(c.kept[c.target[s], h] - last) <= e + 1e-37).all(), (s, h)
+    assert (c.out[:1] == c.mark).all() and (c.out[first[-1]:] == c.mark).all()
