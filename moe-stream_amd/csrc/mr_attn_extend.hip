@@ -110,8 +110,9 @@ __device__ __forceinline__ bool find_unit(const ExtendArgs& a, bool split_only, 
       r.sp = Span{__builtin_amdgcn_readlane(s.q0, l), __builtin_amdgcn_readlane(s.n, l), __builtin_amdgcn_readlane(s.len, l),
                   __builtin_amdgcn_readlane(s.c0, l), __builtin_amdgcn_readlane(s.chunks, l),
                   (uint32_t)__builtin_amdgcn_readlane(s.tiles, l), 0};
-      // Offsets in order leave room: parts beyond the first are half of a.parts at most, or all of them. Overlapping ones may not.
-      return r.parts == 1 || r.slot + r.parts <= a.parts;
+      // Offsets in order leave room: parts beyond the first are half of a.parts at most, or all of them. Overlapping ones may not: sums
+      // of their tiles and parts may pass 32 bits even, so that the slot is compared by itself.
+      return r.parts == 1 || (r.slot < a.parts && r.parts <= a.parts - r.slot);
     }
     before += __builtin_amdgcn_readlane(sum, 63);
     slots += __builtin_amdgcn_readlane(ssum, 63);
