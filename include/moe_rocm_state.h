@@ -11,9 +11,10 @@
  *
  * Further conventions
  *  - New tokens are packed: sequence s has rows cu[s] .. cu[s + 1] - 1 of the n rows of a call, one token or
- *    many, or none; cu holds n_seqs + 1 offsets that do not decrease. Offsets outside the rows are taken as the
- *    nearest inside and decreasing ones as empty sequences, both with an error at mr_sync; rows that two
- *    sequences claim then hold either's result or none. Rows of an output in no sequence are left as they are.
+ *    many, or none; cu holds n_seqs + 1 offsets that do not decrease. Rows of an output in no sequence are left as they
+ *    are. Offsets outside the rows are taken as the nearest inside, with an error at mr_sync. Decreasing ones end in an
+ *    error too, and the call's rows of output and target states then hold a result, some mixture of results, or what was there
+ *    before, those of sequences behind and before the offset among them; nothing else is written.
  *  - States are the caller's: n_slots of them, f32, dense, 16-byte aligned. Sequence s starts from the state of
  *    slot source[s], from zeros if that is negative, and leaves its last one in slot target[s], nowhere if that
  *    is negative. The two may be one slot, or two: the state before a draft that is not taken is then still

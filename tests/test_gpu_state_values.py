@@ -7,8 +7,8 @@ import moe_rocm as M
 
 import attnref as R
 import stateref as S
-from test_gpu_attn import FORMATS, TYPES
-from test_gpu_state import Cached, Delta, extend_ref
+from test_gpu_attn import FORMATS, TYPES, sync_error
+from test_gpu_state import Cached, Delta, extend_ref, offsets
 
 pytestmark = pytest.mark.gpu
 
@@ -247,3 +247,48 @@ def test_delta_long_sequences_among_many_across_launches(gpu_ctx):
             if c.target[s] >= 0:
                 assert (np.abs(c.kept[c.target[s], h] - last) <= e + 1e-37).all(), (s, h)
     assert (c.out[:1] == c.mark).all() and (c.out[first[-1]:] == c.mark).all()
+
+
+@pytest.mark.parametrize("cu,new", [([0, 60, 400], [60, 83]), ([-3, 4, 143], [4, 139]), ([-9, -2, 100], [0, 100]), ([0, 143, 500], [143, 0]),
+                                    ([5, 9, 2 ** 31 - 1], [4, 134])])
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+def test_delta_offsets_outside_the_rows(gpu_ctx, cu, new, kind):
+    """They are taken as the nearest inside: sequences, states and rows in no sequence as for those."""
+    rng = np.random.default_rng(7)
+    c = Delta(gpu_ctx, 1, 2, 64, 64, [140, 0], TYPES[kind], False, rng)  # 143 rows
+    c.new = new
+    c.run(cu=np.array(cu, np.int32), error="cu", start=max(cu[0], 0))
+    c.check()
+
+
+@pytest.mark.parametrize("per", [3, 40])
+def test_decreasing_offsets_write_rows_and_targets_only(gpu_ctx, per):
+    """All but the last sequence claim the same rows, by turns from the front: an error, and each row of the outputs and each target
+    state as it was or with numbers in it; the next call is right."""
+    n_seqs, rng = 9, np.random.default_rng(per)
+    T = per * n_seqs
+    cu = np.array([0, T - per] * 4 + [T - per, T], np.int32)[:n_seqs + 1]
+    cu[-2:] = T - per, T
+    c = Delta(gpu_ctx, 1, 2, 64, 64, [T - 3] + [0] * (n_seqs - 1), M.BF16, False, rng)
+    c.source[:], c.target[:] = -1, np.arange(n_seqs)
+    c.run(cu=cu, error="cu")
+    assert np.isfinite(c.out).all() and np.isfinite(c.kept).all()
+    assert (c.kept[n_seqs:] == c.states[n_seqs:]).all()
+    c.new = [per] * n_seqs
+    c.run(cu=offsets(c.new), start=0)
+    c.check()
+    x = R.rounded(rng.normal(size=(T, 1, 64)), M.BF16)
+    w, bx, out = gpu_ctx.to_device(np.ones((64, 4), np.float32)), R.Rows(gpu_ctx, x, M.BF16), R.Rows(gpu_ctx, None, M.F32, T, 1, 64)
+    states, dev = gpu_ctx.to_device(np.full((n_seqs + 1, 3, 64), 5.0, np.float32)), [R.i32(gpu_ctx, a) for a in (cu, np.arange(n_seqs))]
+    for order, error in ((cu, True), (offsets([per] * n_seqs), False)):
+        dev[0].upload(order)
+        M.causal_conv(gpu_ctx, M.Rows(bx.buf, 64, M.BF16), w, 4, T, n_seqs, dev[0], M.Rows(out.buf, 64), states=states, n_slots=n_seqs + 1,
+                      source=None, target=dev[1])
+        sync_error(gpu_ctx, "cu") if error else gpu_ctx.sync()
+        kept = states.download(np.float32).reshape(-1, 3, 64)
+        assert np.isfinite(out.get()).all() and np.isfinite(kept).all() and (kept[n_seqs:] == 5.0).all()
+    for s in range(n_seqs):
+        y, off, last = S.conv(x[s * per:(s + 1) * per, 0], np.ones((64, 4)), None, False, np.zeros((3, 64)))
+        assert (np.abs(out.get()[s * per:(s + 1) * per, 0] - y) <= off).all() and (kept[s] == last).all()
+    for b in (w, bx, out, states, *dev):
+        b.free()
