@@ -446,7 +446,7 @@ int mr_sync(mr_ctx* c) {
     *word = 0;
   }
   if (any)
-    return set_err(c, MR_E_INVAL, "attention: an entry was out of range in%s%s%s%s%s%s (what it names was left out)", kinds[0],
+    return set_err(c, MR_E_INVAL, "an index entry was out of range or order in%s%s%s%s%s%s (what it names was left out)", kinds[0],
                    kinds[1], kinds[2], kinds[3], kinds[4], kinds[5]);
   return MR_OK;
 }

@@ -292,3 +292,16 @@ def test_decreasing_offsets_write_rows_and_targets_only(gpu_ctx, per):
         assert (np.abs(out.get()[s * per:(s + 1) * per, 0] - y) <= off).all() and (kept[s] == last).all()
     for b in (w, bx, out, states, *dev):
         b.free()
+
+
+def test_errors_of_entries_speak_of_their_kind_alone(gpu_ctx):
+    """The convolution and the rule are no attention: their errors name the offsets or slots."""
+    rng = np.random.default_rng(3)
+    c = Delta(gpu_ctx, 1, 1, 64, 64, [3, 2], M.BF16, False, rng)
+    c.source[0] = 99
+    for change, kind, others in (({}, " source or target", (" cu", "attention", "slots")), ({"cu": np.array([0, 9, 4], np.int32)}, " cu", ("attention", "cu_q"))):
+        with pytest.raises(M.MoeRocmError) as e:
+            c.run(**change)
+        assert kind in e.value.message and not any(x in e.value.message for x in others), e.value.message
+        c.source[0] = 0
+    gpu_ctx.sync()
