@@ -64,3 +64,46 @@ def delta(q, k, v, g, beta, state, scale, unit_eps, g_off, b_off):
         nq = np.sqrt(q[t] @ q[t])
         off[t] = abs(scale) * nq * (e + c * U * (np.sqrt((S * S).sum(0)) + s + np.sqrt(kk) * np.abs(d)))
     return out, off, S, e
+
+
+def parts_of(x, n):
+    """x (32 bits) as n numbers of 8 bits, the largest first, each rounded to nearest even."""
+    out, x = [], np.asarray(x, np.float32)
+    for _ in range(n):
+        b = x.view(np.uint32).astype(np.uint64)
+        out.append((((b + 0x7FFF + ((b >> 16) & 1)) >> 16).astype(np.uint32) << 16).view(np.float32))
+        x = x - out[-1]
+    return out
+
+
+# The 2-norm of a head's state, relative to it, may be off by so much where decays let it live for a while: eight half steps of 32 bits.
+# About eight roundings meet a state's number on its way through a chunk (sums of K S over four parts, V - K S, three sums of V', of the
+# new state), each 2^-24 / sqrt(3) in the mean square of partial sums up to twice the result's size: sqrt(8) * 2 / sqrt(3) = 3.3 half
+# steps; the rest is left for the decays' powers. A number in two parts of 8 bits instead of three is off by 2^-17 at most, 2^-17.8 in the mean
+# square: 74 half steps.
+STATE_NORM = 8 * U
+STATE_VALUES, STATE_DECAY = 0.1, 0.005  # of the values and the log decays: what the state was counts for as much as what is added
+
+
+def chunked(k, v, g, beta, state, exact=True, parts=(3, 3, 3, 3), skip=()):
+    """The state after chunks of 64 tokens, the products of parts of 8 bits in 32-bit sums. parts: how many of the state, of V - K S, of
+    the inverse, of the corrections; skip: products (part of the inverse, part of V - K S) left out; exact: keys are one part, else two."""
+    f32, S = np.float32, np.asarray(state, np.float32).copy()
+
+    def product(a, b, skip=()):
+        return sum((a[p] @ b[z] for p in reversed(range(len(a))) for z in reversed(range(len(b))) if p + z < 3 and (p, z) not in skip),
+                   np.zeros((a[0].shape[0], b[0].shape[1]), f32))
+
+    for c in range(0, len(k), 64):
+        K, G, b = k[c:c + 64].astype(f32), np.cumsum(np.asarray(g[c:c + 64], np.float64)), beta[c:c + 64].astype(f32)
+        keys = [K] if exact else parts_of(K, 2)
+        A = np.tril((K @ K.T) * np.exp(np.minimum(G[:, None] - G, 0)).astype(f32) * b[:, None], -1)
+        T = (np.linalg.inv(np.eye(len(K)) + A.astype(np.float64)).astype(f32)) * b
+        R = v[c:c + 64].astype(f32) - np.exp(G).astype(f32)[:, None] * product(keys, parts_of(S, parts[0]))
+        V = product(parts_of(T, parts[2]), parts_of(R, parts[1]), skip)
+        S = S * f32(np.exp(G[-1])) + product([x.T for x in keys], parts_of(V * np.exp(G[-1] - G).astype(f32)[:, None], parts[3]))
+    return S
+
+
+def state_norm_error(got, want):
+    return float(np.sqrt(((got - want) ** 2).sum() / (want ** 2).sum()))

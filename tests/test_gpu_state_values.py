@@ -305,3 +305,65 @@ def test_errors_of_entries_speak_of_their_kind_alone(gpu_ctx):
         assert kind in e.value.message and not any(x in e.value.message for x in others), e.value.message
         c.source[0] = 0
     gpu_ctx.sync()
+
+
+@pytest.mark.parametrize("new", [[5], [64], [140], [7, 300, 33]])
+@pytest.mark.parametrize("dk,dv,kind", [(64, 64, "bf16"), (64, 128, "f16"), (128, 128, "bf16"), (128, 64, "f16")])
+def test_delta_states_to_32_bits(gpu_ctx, new, dk, dv, kind):
+    """A head's state is off by a few half steps of 32 bits of its norm: a lost part or product of the matrix instructions' operands is
+    twice the bound and more (tests/test_state_precision.py)."""
+    c = Delta(gpu_ctx, 1, 2, dk, dv, new, TYPES[kind], False, np.random.default_rng(sum(new) + dk))
+    c.a *= np.float32(S.STATE_DECAY / 0.3)
+    c.v = R.rounded(c.v * S.STATE_VALUES / 2, c.kind)
+    c.run()
+    c.check()
+    at = 1
+    for s, n in enumerate(new):
+        for h in range(2):
+            i = slice(at, at + n)
+            _, _, want, _ = S.delta(c.q[i, 0], c.k[i, 0], c.v[i, h], c.a[i, h].astype(np.float64), c.b[i, h], c.states[c.source[s], h], dk ** -0.5, 0.0, np.zeros(n), np.zeros(n))
+            e = S.state_norm_error(c.kept[c.target[s], h], want)
+            assert e <= S.STATE_NORM, (s, h, e / S.U)
+        at += n
+
+
+@pytest.mark.parametrize("what,x", [("value", np.inf), ("value", np.nan), ("key", np.inf), ("key", np.nan), ("beta", np.inf), ("beta", np.nan),
+                                    ("decay", np.inf), ("decay", np.nan), ("query", np.inf), ("query", np.nan)])
+@pytest.mark.parametrize("new,at", [([8], 0), ([8], 5), ([70], 3), ([70], 66), ([5, 140, 2], 6), ([5, 140, 2], 70), ([90, 4], 92)])
+@pytest.mark.parametrize("dk,dv,kind,raw", [(64, 64, "f16", False), (128, 128, "bf16", True), (128, 64, "f16", True)])
+def test_delta_what_is_not_finite_on_each_path(gpu_ctx, what, x, new, at, dk, dv, kind, raw):
+    """It reaches its own sequence from its token on: a value its column, a key all columns, a decay or a beta those of its head, a query its
+    own row and no state. Everything else has the bits of the call without it."""
+    c = Delta(gpu_ctx, 1, 2, dk, dv, new, TYPES[kind], raw, np.random.default_rng(at + dk))
+    row = at + 1
+    clean = c.v.copy(), c.k.copy(), c.b.copy(), c.a.copy(), c.q.copy()
+    if raw and what in ("beta", "decay"):
+        x = np.nan  # raw gates of infinity stand for a beta of one, a decay of minus infinity
+    if what == "value":
+        c.v[row, 1, 5] = x
+    if what == "key":
+        c.k[row, 0, 3] = x
+    if what == "beta":
+        c.b[row, 1] = x
+    if what == "decay":
+        c.a[row, 1] = x
+    if what == "query":
+        c.q[row, 0, 9] = x
+    c.run()
+    out, kept = c.out, c.kept
+    c.v, c.k, c.b, c.a, c.q = clean
+    c.run()
+    c.check()
+    ends = 1 + np.cumsum(new)
+    s = int((ends > row).argmax())
+    heads = [0, 1] if what in ("key", "query") else [1]
+    columns = [5] if what == "value" else slice(None)
+    hit, lost = np.zeros(out.shape, bool), np.zeros(kept.shape, bool)
+    for h in heads:
+        hit[row:ends[s] if what != "query" else row + 1, h, columns] = True
+        if what != "query":
+            lost[c.target[s], h][:, columns] = True
+    assert not np.isfinite(out[hit]).any() and (out[~hit] == c.out[~hit]).all()
+    # of a state's column that is lost some number is not finite: a zero of a later key keeps a row of it
+    assert (kept[~lost] == c.kept[~lost]).all()
+    assert not np.isfinite(kept[c.target[s]][heads][..., columns]).all(1).any() if what != "query" else True
