@@ -356,8 +356,8 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<NT, FMT, D>)) void k_attn_ex
 // MXINT8: 174 us, 620 TFLOP/s).
 // Weights go up to 2^15, and the maximum is followed when it has moved by 2^slack: the largest weight lies between 2^(15 - slack) and
 // 2^15, and ones down to 2^(slack - 29) of it keep all bits of f16. Where sequences have up to 32 rows, the slack is one, and the bits are
-// those of attend_few: 3 new tokens of 32 sequences, 32 heads on 4 of 128, MXFP4 76.5 us with four and 79 us with one. For more rows it
-// is four: 5 new tokens of the same 91.5 and 95 us, four prompts' parts 175 and 181 us.
+// those of attend_few: 3 new tokens of 32 sequences, 32 heads on 4 of 128, MXFP4 76.5 us with four and 79 us with one
+// (16 on 2 of 256, MXINT8: 123 and 139 us). For more rows it is four: 5 new tokens of the same 91.5 and 95 us, four prompts' parts 175 and 181 us.
 constexpr float kTopWeight = 15.f, kSlackFew = 1.f, kSlackMany = 4.f;
 
 // A wave's quarter of a chunk on its way from the pages to LDS.
@@ -825,8 +825,8 @@ __global__ __launch_bounds__(64 * kWaves) void k_extend_join(ExtendArgs a) {
 
 // Whether tiles of 17 to 32 rows are a wave's of its own chunks: where its operands, turned into f16 for two products of 16 rows,
 // leave it registers. Else they are a tile of 64 rows of k_attn_extend_wide. 32 sequences of 3 new tokens behind up to 24000, 8 heads
-// on each key head, D 64, 128, 256 (8, 4, 2 key heads), this : that (us): MXFP4 80 : 91, 95 : 83, 87 : 107; MXINT8 110 : 117,
-// 150 : 108, 135 : 125; F16 161 : 152, 184 : 153, 191 : 157.
+// on each key head, D 64, 128, 256 (8, 4, 2 key heads), this : that (us): MXFP4 81 : 95, 95 : 86, 88 : 125; MXINT8 109 : 116,
+// 150 : 106, 144 : 143 (a call: 150 : 139); F16 161 : 153, 184 : 152, 191 : 160.
 template <int FMT, int D>
 constexpr bool kTwo = FMT != MR_KV_F16 && (D == 64 || (D == 256 && FMT == MR_KV_MXFP4));
 

@@ -145,7 +145,8 @@ __global__ __launch_bounds__(256) void k_delta_step(DeltaArgs a, int most) {
 //
 // States are held to 32 bits: S, T, V - K S and V' enter the 16-bit matrix instructions as sums of three bf16 parts (8 bits each),
 // in as many products as reach 2^-24; P, and S and V' for the outputs alone, as two. k and q are exact: themselves in bf16, or,
-// for f16, two bf16 parts.
+// for f16, two bf16 parts. Two parts are 16 bits, which leave outputs of 8 or 11 bits as they would be: off from 64 bits by what the
+// plain 32-bit form is, 1.7e-3 and 2.1e-4 of their norm (4096 tokens in bf16, seven prompts in f16).
 constexpr int kChunk = 64;
 
 typedef u32x4 Operand;  // 8 numbers of 16 bits of a lane: lane (m, g), row (or column) m, the 8 at 8 g of 32
@@ -567,10 +568,10 @@ __global__ __launch_bounds__(256, 4) void k_delta_prepare(ChunkArgs c) {
 // V - K S, V', S. Four waves take them, each result going from one wave's registers through LDS to all: wave w has the state's
 // tiles of 16 rows from w * (DK / 64) on, whose part of K S it works out for the whole chunk, and the chunk's tokens from 16 w on
 // after that. Four others work out the tokens' outputs beside them, a step behind. A chunk takes 1.8 us (4096 tokens of one sequence,
-// 32 heads of 128, all 256 CUs: 113 us): three barriers, exchanges through LDS and 78 KB of operands by the CU's loads, 580 cycles
+// 32 heads of 128, all 256 CUs: 115 us): three barriers, exchanges through LDS and 78 KB of operands by the CU's loads, 580 cycles
 // of each wave's matrix instructions. In 128 registers two workgroups share a CU, where there are so many: seven prompts of 12 heads,
-// keys of 64, 70 us with one and 58 us with two; 32 heads of 128 in bf16, 153 and 127 us; f16 keys of 128, in two parts, would
-// spill (212 and 653 us).
+// f16 keys of 64, 73 us with one and 60 us with two; 32 heads of 128 in bf16, 156 and 132 us, though 3 and 5 registers are spilled for it. f16 keys
+// of 128, in two parts, would spill 96 (214 us with one, 524 us).
 template <int DK, int NP, bool BF>
 __global__ __launch_bounds__(512, (DK == 64 || NP == 1 ? 4 : 2)) void k_delta_chunks(ChunkArgs c, uint32_t slices, int parity) {
   constexpr int NS = DK / 32, NT = DK / 64;
