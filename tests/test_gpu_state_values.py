@@ -367,3 +367,55 @@ def test_delta_what_is_not_finite_on_each_path(gpu_ctx, what, x, new, at, dk, dv
     # of a state's column that is lost some number is not finite: a zero of a later key keeps a row of it
     assert (kept[~lost] == c.kept[~lost]).all()
     assert not np.isfinite(kept[c.target[s]][heads][..., columns]).all(1).any() if what != "query" else True
+
+
+def test_delta_graph_of_many_sequences_sees_present_offsets(gpu_ctx):
+    """A captured call of 1100 sequences, replayed with other offsets and decays, eager calls of other shapes on the same workspace between:
+    the same bits as eager calls."""
+    rng, n_seqs, T, D = np.random.default_rng(4), 1100, 1700, 64
+    q, k, v = (R.rounded(rng.normal(size=(T, 1, D)) / 8, M.BF16) for _ in range(3))
+    rows = [R.Rows(gpu_ctx, x, M.BF16) for x in (q, k, v)] + [R.Rows(gpu_ctx, None, M.BF16, T, 1, D)]
+    plans = []
+    for at, n, growth in ((3, 500, 0.0), (1099, 300, 0.05), (600, 40, 0.0)):
+        new = rng.integers(0, 2, n_seqs)
+        new[at], new[at // 2] = n, 70
+        a = -np.abs(rng.normal(size=T)).astype(np.float32) * 0.1
+        a[offsets(new)[at]:offsets(new)[at] + n // 2] += growth * 4
+        plans.append((offsets(new), a))
+    states = rng.normal(size=(n_seqs, 1, D, D)).astype(np.float32)
+    cu, a, b = R.i32(gpu_ctx, plans[0][0]), gpu_ctx.to_device(plans[0][1]), gpu_ctx.to_device(rng.uniform(0.1, 0.9, T).astype(np.float32))
+    ds, slots = gpu_ctx.to_device(states), R.i32(gpu_ctx, np.arange(n_seqs))
+    rule = M.DeltaRule(gpu_ctx, 1, 1, D, D)
+    mark = rows[3].all().copy()
+
+    def call(n=n_seqs, tokens=T):
+        rule.forward(rows[0].heads, rows[1].heads, rows[2].heads, a, b, tokens, n, cu, rows[3].heads, states=ds, n_slots=n_seqs, source=slots, target=slots)
+
+    def start(plan):
+        gpu_ctx.sync()
+        cu.upload(plan[0]), a.upload(plan[1]), ds.upload(states), rows[3].buf.upload(mark)
+
+    def results():
+        gpu_ctx.sync()
+        return rows[3].all().copy(), ds.download(np.float32).copy()
+
+    want = []
+    for plan in plans:
+        start(plan)
+        call()
+        want.append(results())
+    start(plans[0])
+    gpu_ctx.graph_begin()
+    call()
+    graph = gpu_ctx.graph_end()
+    for i in (0, 2, 1, 1, 0):
+        start(plans[i])
+        graph.launch()
+        for x, y in zip(results(), want[i]):
+            assert np.array_equal(x, y, equal_nan=True)
+        start((np.concatenate([[0], np.full(n_seqs, 200)]).astype(np.int32), plans[i][1]))
+        call(1, 200)
+        gpu_ctx.sync()
+    graph.close(), rule.close()
+    for x in (*rows, cu, a, b, ds, slots):
+        x.free()
